@@ -22,6 +22,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libgg_b200.so")
 DEBUG_LIB_PATH = os.path.join(HERE, "lib", "libgg_b200_debug.so")
 
 BF16, FP16 = 0, 1
+F32 = 2  # router logits only
 DTYPES = {"bf16": BF16, "fp16": FP16}
 
 GG_OK, GG_NOT_SUPPORTED, GG_ERR_ARG, GG_ERR_CUDA, GG_ERR_DEVICE = 0, 1, -1, -2, -3
@@ -62,6 +63,32 @@ class GGGradProblem(ctypes.Structure):
     ]
 
 
+# Token movement, by operation (enum gg_permute_op).
+OP_DISPATCH, OP_COMBINE, OP_COMBINE_GRAD = 3, 4, 5
+
+_i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+
+
+class GGRouteProblem(ctypes.Structure):
+    _fields_ = [("logits_type", _i32), ("experts", _i32), ("top_k", _i32), ("normalize", _i32), ("scale", _f32), ("tokens", _i64)] + [
+        (n, _vp) for n in ("logits", "mask", "ids", "weights", "lse", "counts", "offsets", "live", "dest", "src", "prob", "losses")]
+
+
+class GGRouteGradProblem(ctypes.Structure):
+    _fields_ = [("logits_type", _i32), ("experts", _i32), ("top_k", _i32), ("normalize", _i32), ("scale", _f32), ("tokens", _i64)] + [
+        (n, _vp) for n in ("logits", "mask", "ids", "lse", "counts", "live", "dweights", "dlosses", "dlogits")]
+
+
+class GGPermuteProblem(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("experts", _i32), ("top_k", _i32), ("tokens", _i64), ("hidden", _i64)] + [
+        (n, _vp) for n in ("x", "rows", "dy", "drows", "dest", "offsets", "weights", "dweights")]
+
+
+class GGW4Problem(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("experts", _i32), ("group_size", _i32), ("top_k", _i32), ("n", _i64), ("k", _i64), ("rows", _i64),
+                ("tokens", _i64)] + [(n, _vp) for n in ("x", "qweight", "scales", "zeros", "offsets", "src", "out")]
+
+
 # Every symbol include/gg_b200.h declares, with its ctypes signature.
 SIGNATURES = {
     "gg_abi_version": (ctypes.c_int, []),
@@ -71,6 +98,14 @@ SIGNATURES = {
                                   ctypes.c_char_p, ctypes.c_size_t]),
     "gg_prepare_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGGradProblem), ctypes.c_int32,
                                        ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
+    "gg_prepare_route": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGRouteProblem), ctypes.c_void_p, ctypes.c_char_p,
+                                        ctypes.c_size_t]),
+    "gg_prepare_route_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGRouteGradProblem), ctypes.c_void_p,
+                                             ctypes.c_char_p, ctypes.c_size_t]),
+    "gg_prepare_permute": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGPermuteProblem), ctypes.c_int32, ctypes.c_void_p,
+                                          ctypes.c_char_p, ctypes.c_size_t]),
+    "gg_prepare_w4": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGW4Problem), ctypes.c_void_p, ctypes.c_char_p,
+                                     ctypes.c_size_t]),
     "gg_run": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "gg_release": (None, [ctypes.c_void_p]),
     "gg_detail": (ctypes.c_char_p, [ctypes.c_void_p]),
@@ -177,6 +212,78 @@ class B200Backend:
         if rc == GG_NOT_SUPPORTED:
             return why.value.decode() or "not supported"
         raise GGError(rc, self.last_error())
+
+    def _prepared(self, rc: int, why) -> str:
+        if rc == GG_OK:
+            return ""
+        if rc == GG_NOT_SUPPORTED:
+            return why.value.decode() or "not supported"
+        raise GGError(rc, self.last_error())
+
+    def prepare_route(self, logits_type: int, tokens: int, experts: int, top_k: int, logits_ptr: int, ids_ptr: int,
+                      weights_ptr: int, counts_ptr: int, offsets_ptr: int, live_ptr: int, dest_ptr: int, src_ptr: int,
+                      lse_ptr: int = 0, prob_ptr: int = 0, losses_ptr: int = 0, mask_ptr: int = 0, normalize: bool = True,
+                      scale: float = 1.0, stream: int = 0) -> str:
+        """Prepare the router (gg_prepare_route): logits [tokens, experts] in BF16, FP16 or F32 -> ids, weights, counts, offsets,
+        live, dest, src and, where their pointers are given, lse, prob and losses. Then run() launches it. Returns "" or the N/A
+        reason; raises GGError on a CUDA or argument error (as every prepare_* below)."""
+        prob = GGRouteProblem(int(logits_type), int(experts), int(top_k), int(bool(normalize)), float(scale), int(tokens),
+                              logits_ptr or None, mask_ptr or None, ids_ptr or None, weights_ptr or None, lse_ptr or None,
+                              counts_ptr or None, offsets_ptr or None, live_ptr or None, dest_ptr or None, src_ptr or None,
+                              prob_ptr or None, losses_ptr or None)
+        why = ctypes.create_string_buffer(256)
+        return self._prepared(self._lib.gg_prepare_route(self._h, ctypes.byref(prob), ctypes.c_void_p(stream or None), why, 256), why)
+
+    def prepare_route_grad(self, logits_type: int, tokens: int, experts: int, top_k: int, logits_ptr: int, dlogits_ptr: int,
+                           ids_ptr: int, lse_ptr: int, counts_ptr: int, live_ptr: int, dweights_ptr: int = 0,
+                           dlosses_ptr: int = 0, mask_ptr: int = 0, normalize: bool = True, scale: float = 1.0,
+                           stream: int = 0) -> str:
+        """Prepare the router's backward pass (gg_prepare_route_grad): dweights [tokens, top_k] and dlosses [2] -> dlogits."""
+        prob = GGRouteGradProblem(int(logits_type), int(experts), int(top_k), int(bool(normalize)), float(scale), int(tokens),
+                                  logits_ptr or None, mask_ptr or None, ids_ptr or None, lse_ptr or None, counts_ptr or None,
+                                  live_ptr or None, dweights_ptr or None, dlosses_ptr or None, dlogits_ptr or None)
+        why = ctypes.create_string_buffer(256)
+        return self._prepared(self._lib.gg_prepare_route_grad(self._h, ctypes.byref(prob), ctypes.c_void_p(stream or None), why, 256),
+                              why)
+
+    def _prepare_permute(self, op: int, stream: int, dtype: int, experts: int, top_k: int, tokens: int, hidden: int, **ptrs) -> str:
+        prob = GGPermuteProblem(int(dtype), int(experts), int(top_k), int(tokens), int(hidden),
+                                *[ptrs.get(n, 0) or None for n in ("x", "rows", "dy", "drows", "dest", "offsets", "weights", "dweights")])
+        why = ctypes.create_string_buffer(256)
+        return self._prepared(self._lib.gg_prepare_permute(self._h, ctypes.byref(prob), int(op), ctypes.c_void_p(stream or None), why,
+                                                           256), why)
+
+    def prepare_dispatch(self, dtype: int, tokens: int, top_k: int, experts: int, hidden: int, x_ptr: int, dest_ptr: int,
+                         offsets_ptr: int, rows_ptr: int, stream: int = 0) -> str:
+        """Prepare dispatch (gg_prepare_permute): x [tokens, hidden] -> rows [tokens * top_k, hidden] in expert order."""
+        return self._prepare_permute(OP_DISPATCH, stream, dtype, experts, top_k, tokens, hidden, x=x_ptr, rows=rows_ptr,
+                                     dest=dest_ptr, offsets=offsets_ptr)
+
+    def prepare_combine(self, dtype: int, tokens: int, top_k: int, experts: int, hidden: int, rows_ptr: int, dest_ptr: int,
+                        y_ptr: int, weights_ptr: int = 0, stream: int = 0) -> str:
+        """Prepare combine: rows in expert order -> y [tokens, hidden], weighted, or a plain sum without weights (the gradient of
+        dispatch)."""
+        return self._prepare_permute(OP_COMBINE, stream, dtype, experts, top_k, tokens, hidden, x=y_ptr, rows=rows_ptr,
+                                     dest=dest_ptr, weights=weights_ptr)
+
+    def prepare_combine_grad(self, dtype: int, tokens: int, top_k: int, experts: int, hidden: int, dy_ptr: int, rows_ptr: int,
+                             dest_ptr: int, offsets_ptr: int, drows_ptr: int, weights_ptr: int = 0, dweights_ptr: int = 0,
+                             stream: int = 0) -> str:
+        """Prepare combine's backward pass: dy [tokens, hidden] -> drows [tokens * top_k, hidden] and, with dweights_ptr,
+        dweights [tokens, top_k] (rows are read for these only)."""
+        return self._prepare_permute(OP_COMBINE_GRAD, stream, dtype, experts, top_k, tokens, hidden, dy=dy_ptr, rows=rows_ptr,
+                                     dest=dest_ptr, offsets=offsets_ptr, drows=drows_ptr, weights=weights_ptr, dweights=dweights_ptr)
+
+    def prepare_w4(self, dtype: int, experts: int, n: int, k: int, group_size: int, rows: int, x_ptr: int, qweight_ptr: int,
+                   scales_ptr: int, offsets_ptr: int, out_ptr: int, zeros_ptr: int = 0, src_ptr: int = 0, tokens: int = 0,
+                   top_k: int = 1, stream: int = 0) -> str:
+        """Prepare the products with 4-bit weights (gg_prepare_w4): out [rows, n] of x [tokens, k] through src, or of x [rows, k]
+        without it, by the router's offsets in device memory."""
+        prob = GGW4Problem(int(dtype), int(experts), int(group_size), int(top_k), int(n), int(k), int(rows), int(tokens),
+                           x_ptr or None, qweight_ptr or None, scales_ptr or None, zeros_ptr or None, offsets_ptr or None,
+                           src_ptr or None, out_ptr or None)
+        why = ctypes.create_string_buffer(256)
+        return self._prepared(self._lib.gg_prepare_w4(self._h, ctypes.byref(prob), ctypes.c_void_p(stream or None), why, 256), why)
 
     def run(self, stream: int = 0) -> None:
         rc = self._lib.gg_run(self._h, ctypes.c_void_p(stream or None))

@@ -18,6 +18,7 @@ import re
 import subprocess
 import sys
 import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -29,25 +30,22 @@ NVCC = os.environ.get("NVCC", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-I" + INCLUDE, "-I" + CSRC]
 
+# Sources and the headers each is built from; compiled to lib/obj/*.o, so that an edit recompiles only
+# the sources that include it.
+GEMM_HEADERS = ["gg_kernel.cuh", "gg_ptx.cuh"]
+SOURCES = {
+    "gg_capi.cu": GEMM_HEADERS + ["gg_handle.h", "gg_sched.h"],
+    "gg_moe.cu": GEMM_HEADERS + ["gg_handle.h", "gg_moe.cuh", "gg_route.cuh", "gg_permute.cuh", "gg_w4.cuh"],
+    "gg_bench_main.cu": [os.path.join("..", "..", "include", "gg_backend.hpp")],
+    "gg_cublas_backends.cpp": [os.path.join("..", "..", "include", "gg_backend.hpp")],
+}
+
 TARGETS = {
-    "libgg_b200.so": {
-        "srcs": ["gg_capi.cu"],
-        "deps": ["gg_capi.cu", "gg_kernel.cuh", "gg_ptx.cuh", "gg_sched.h"],
-        "flags": ["-Xcompiler", "-fPIC", "-shared"],
-    },
+    "libgg_b200.so": {"srcs": ["gg_capi.cu", "gg_moe.cu"], "flags": ["-shared"]},
     # the same library with the kernel's bounds checks compiled in (-DGG_DEBUG): a failed check
     # records its site in the device status word and skips the access
-    "libgg_b200_debug.so": {
-        "srcs": ["gg_capi.cu"],
-        "deps": ["gg_capi.cu", "gg_kernel.cuh", "gg_ptx.cuh", "gg_sched.h"],
-        "flags": ["-Xcompiler", "-fPIC", "-shared", "-DGG_DEBUG"],
-    },
-    "gg_bench": {
-        "srcs": ["gg_bench_main.cu", "gg_cublas_backends.cpp", "gg_capi.cu"],
-        "deps": ["gg_bench_main.cu", "gg_cublas_backends.cpp", "gg_capi.cu", "gg_kernel.cuh", "gg_ptx.cuh", "gg_sched.h",
-                 os.path.join("..", "..", "include", "gg_backend.hpp")],
-        "flags": ["-lcublas"],
-    },
+    "libgg_b200_debug.so": {"srcs": ["gg_capi.cu", "gg_moe.cu"], "flags": ["-shared"], "debug": True},
+    "gg_bench": {"srcs": ["gg_bench_main.cu", "gg_cublas_backends.cpp", "gg_capi.cu", "gg_moe.cu"], "flags": ["-lcublas"]},
 }
 
 
@@ -60,19 +58,34 @@ def _stale(out: str, deps: list[str]) -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> list[str]:
-    os.makedirs(LIB, exist_ok=True)
-    built = []
-    for name, t in TARGETS.items():
-        srcs = [os.path.join(CSRC, s) for s in t["srcs"]]
-        if not all(os.path.exists(s) for s in srcs):
-            continue
-        out = os.path.join(LIB, name)
-        if not force and not _stale(out, t["deps"]):
-            continue
-        cmd = [NVCC] + COMMON + t["flags"] + ["-o", out] + srcs
+    obj = os.path.join(LIB, "obj")
+    os.makedirs(obj, exist_ok=True)
+
+    def run(cmd: list[str]) -> None:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+
+    def object_of(src: str, debug: bool) -> str:
+        return os.path.join(obj, src + (".debug.o" if debug else ".o"))
+
+    compile_cmds = {}
+    for t in TARGETS.values():
+        debug = t.get("debug", False)
+        for src in t["srcs"]:
+            out = object_of(src, debug)
+            if force or _stale(out, [src] + SOURCES[src]):
+                compile_cmds[out] = ([NVCC] + COMMON + ["-Xcompiler", "-fPIC", "-c"] + (["-DGG_DEBUG"] if debug else []) +
+                                     ["-o", out, os.path.join(CSRC, src)])
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        list(pool.map(run, compile_cmds.values()))
+    built = []
+    for name, t in TARGETS.items():
+        objects = [object_of(src, t.get("debug", False)) for src in t["srcs"]]
+        out = os.path.join(LIB, name)
+        if os.path.exists(out) and all(os.path.getmtime(o) <= os.path.getmtime(out) for o in objects):
+            continue
+        run([NVCC] + ARCH + ["-o", out] + objects + t["flags"])
         built.append(out)
     return built
 
@@ -92,9 +105,10 @@ def _kernel_name(mangled: str) -> str:
 def resource_usage() -> list[dict]:
     """Compile the library with -Xptxas -v into a scratch file; one row per kernel."""
     with tempfile.TemporaryDirectory() as d:
-        cmd = [NVCC] + COMMON + TARGETS["libgg_b200.so"]["flags"] + ["-Xptxas", "-v", "-o",
+        cmd = [NVCC] + COMMON + ["-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v", "-o",
                                                                      os.path.join(d, "libgg_b200.so"),
-                                                                     os.path.join(CSRC, "gg_capi.cu")]
+                                                                     os.path.join(CSRC, "gg_capi.cu"),
+                                                                     os.path.join(CSRC, "gg_moe.cu")]
         run = subprocess.run(cmd, check=True, capture_output=True, text=True)
     rows, cur = [], None
     for line in (run.stdout + run.stderr).splitlines():

@@ -9,7 +9,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -18,6 +17,7 @@
 #include <vector>
 
 #include "gg_b200.h"
+#include "gg_handle.h"
 #include "gg_kernel.cuh"
 #include "gg_sched.h"
 
@@ -93,98 +93,8 @@ const gg::TileShape *tile_shapes() {
 }
 
 using gg::Choice;
-
-}  // namespace
-
-struct gg_handle {
-    // options
-    int opt_variant = -1;
-    int opt_band = 0;
-    int opt_raster = -1;
-    int opt_bn = 0;
-    int opt_split = 0;
-    int opt_sk_tail = -1;
-    int opt_stream_k = 0;  // 0 off (default), -1 cost model decides, 1 / 2 stream-K over the partial
-                           // last wave (+ one wave)
-    int opt_max_ctas = 0;
-    int64_t opt_timeout_ms = 2000;
-    int opt_test_stall = 0;
-    int opt_test_bounds = 0;  // test only: declare the output one row short to the debug build's checks
-    int opt_pdl = 1;
-    int opt_store = -1;  // -1 auto, 0 = staging + TMA stores, 1 = direct stores
-    int opt_tail = -1;   // split launch for skewed routing: -1 auto, 0 off, 1 on
-    int opt_chunks = 1;  // wgrad: 3-D chunk views for the MN-major operand loads where the shape allows
-    int opt_order = 0;  // planned tile order (wgrad with store-bound and tensor-bound groups): -1 auto, 0 off, 1 on
-    int opt_half = 0;    // 1 on (half-height last tiles where a group allows), 0 off (default), -1 = on
-    int opt_sched = 0;  // -1 auto (dynamic for multi-wave launches of whole tiles), 0 static, 1 dynamic
-    int opt_l2_a = -1;  // L2 eviction priority of the A / B operand loads (forward):
-    int opt_l2_b = 0;   // 0 no hint, 1 evict_first, 2 evict_last; l2_a -1 = automatic
-
-    // prepared state
-    bool ready = false;
-    int device = -1;
-    int dtype = 0;
-    int variant = 0;
-    int64_t total_m = 0;
-    int32_t *d_meta = nullptr;  // tile_off[G+1] then row_off[G+1]
-    size_t meta_cap = 0;        // int32 entries
-    uint32_t *d_status = nullptr;
-    float *d_ws = nullptr;  // split-K partial sums
-    size_t ws_cap = 0;      // bytes
-    int32_t *d_counters = nullptr;
-    size_t counters_cap = 0;  // bytes
-    int32_t *d_tiles = nullptr;      // planned tile order: (group, mt << 16 | nt) per tile
-    size_t tiles_cap = 0;            // int32 entries
-    CUtensorMap *d_gmaps = nullptr;  // wgrad: per-group tensor maps
-    size_t gmaps_cap = 0;            // maps
-    int op = 0;                      // gg::kOpForward / kOpDgrad / kOpWgrad
-    CUtensorMap tmap_a{}, tmap_b{}, tmap_out{};
-    CUtensorMap tmap_a_half{};  // A in 64-row boxes, for half-height pair tiles
-    // Second launch of a split launch: the one-CTA kernel over the groups' remainders of at most
-    // 128 rows (tmap_a / tmap_out are shared with the first launch).
-    struct {
-        bool active = false;
-        const void *fn = nullptr;
-        int grid = 0, smem = 0;
-        CUtensorMap tmap_b{};
-        gg::KernelParams params{};
-    } tail;
-    gg::KernelParams params{};
-    int grid = 0;
-    const void *fn = nullptr;
-    int smem = 0;
-    int cg = 1;
-
-    std::string detail, last_error;
-};
-
-namespace {
-
-int fail(gg_handle *h, int code, const char *fmt, ...) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    std::vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    h->last_error = buf;
-    return code;
-}
-
-int refuse(gg_handle *h, char *why, size_t why_len, const char *msg) {
-    h->last_error = msg;
-    if (why && why_len > 0) {
-        std::strncpy(why, msg, why_len - 1);
-        why[why_len - 1] = '\0';
-    }
-    return GG_NOT_SUPPORTED;
-}
-
-#define GG_CUDA(h, expr)                                                                                  \
-    do {                                                                                                  \
-        cudaError_t e_ = (expr);                                                                          \
-        if (e_ != cudaSuccess)                                                                            \
-            return fail((h), GG_ERR_CUDA, "%s: %s (%s:%d)", #expr, cudaGetErrorString(e_), __FILE__, __LINE__); \
-    } while (0)
+using gg::fail;
+using gg::refuse;
 
 }  // namespace
 
@@ -316,6 +226,7 @@ void gg_release(gg_handle *h) {
     h->counters_cap = 0;
     h->meta_cap = 0;
     h->tail.active = false;
+    h->moe.launches = 0;
     h->ready = false;
     h->detail.clear();
 }
@@ -908,6 +819,7 @@ int gg_prepare(gg_handle *h, const gg_problem *p, gg_stream_t stream, char *why,
     if (!h)
         return GG_ERR_ARG;
     h->ready = false;
+    h->moe.launches = 0;
     h->last_error.clear();
     if (why && why_len)
         why[0] = '\0';
@@ -922,6 +834,7 @@ int gg_prepare_grad(gg_handle *h, const gg_grad_problem *p, int32_t op, gg_strea
     if (!h)
         return GG_ERR_ARG;
     h->ready = false;
+    h->moe.launches = 0;
     h->last_error.clear();
     if (why && why_len)
         why[0] = '\0';
@@ -943,6 +856,8 @@ int gg_run(gg_handle *h, gg_stream_t stream) {
         return GG_ERR_ARG;
     if (!h->ready)
         return fail(h, GG_ERR_ARG, "gg_run before a successful gg_prepare");
+    if (h->moe.launches > 0)
+        return gg::run_moe(h, stream);
     if (h->params.total_tiles == 0 && !h->tail.active)
         return GG_OK;  // every group empty: nothing to write
     cudaLaunchConfig_t cfg{};
@@ -994,7 +909,8 @@ int gg_device_status(gg_handle *h, gg_stream_t stream, uint32_t *status) {
         if (h->d_counters)
             GG_CUDA(h, cudaMemset(h->d_counters, 0, h->counters_cap));
         return fail(h, GG_ERR_DEVICE, "%s: status 0x%x",
-                    (*status & gg::kStatusBounds) ? "debug bounds check failed" : "kernel bounded wait timed out", *status);
+                    h->moe.launches > 0                ? "index out of range"
+                    : (*status & gg::kStatusBounds) ? "debug bounds check failed" : "kernel bounded wait timed out", *status);
     }
     return GG_OK;
 }

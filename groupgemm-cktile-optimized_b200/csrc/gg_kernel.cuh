@@ -448,7 +448,7 @@ __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, const Ab
 
 // Bounded wait by one thread until a global counter, written by other CTAs, reaches `want`.
 // Returns false if this or another role gave up.
-__device__ __noinline__ bool wait_count(const int32_t *ctr, int want, const Abort ab, uint32_t code) {
+__device__ __noinline__ inline bool wait_count(const int32_t *ctr, int want, const Abort ab, uint32_t code) {
     const uint64_t t0 = ptx::globaltimer();
     for (uint32_t it = 1;; ++it) {
         if (*reinterpret_cast<const volatile int32_t *>(ctr) >= want)

@@ -1,0 +1,426 @@
+// Host side of the layer operators around the grouped GEMM: argument checks, workspaces and launches
+// of the router, dispatch / combine and the 4-bit products (C ABI in include/gg_b200.h).
+//
+// As with the grouped GEMM, a prepare call validates the problem and allocates what the handle needs,
+// and gg_run enqueues the prepared operator's kernels without waiting.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+#include <new>
+
+#include "gg_b200.h"
+#include "gg_handle.h"
+#include "gg_permute.cuh"
+#include "gg_route.cuh"
+#include "gg_w4.cuh"
+
+namespace gg {
+
+int run_moe(gg_handle *h, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    // as in gg_run: every kernel waits for the one before it before it touches global memory
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = h->opt_pdl ? 1 : 0;
+    cfg.stream = stream;
+    void *args[1] = {h->moe.params};
+    for (int i = 0; i < h->moe.launches; ++i) {
+        const MoeLaunch &l = h->moe.launch[i];
+        if (!l.grid)
+            continue;  // nothing to do
+        cfg.gridDim = dim3(l.grid, 1, 1);
+        cfg.blockDim = dim3(l.block, 1, 1);
+        cfg.dynamicSmemBytes = l.smem;
+        GG_CUDA(h, cudaLaunchKernelExC(&cfg, l.fn, args));
+    }
+    return GG_OK;
+}
+
+}  // namespace gg
+
+namespace {
+
+using gg::fail;
+using gg::MoeLaunch;
+using gg::refuse;
+
+constexpr int64_t kMaxIndex = int64_t(1) << 31;  // rows and slots are int32 in device memory
+
+bool aligned16(std::initializer_list<const void *> ptrs) {
+    uintptr_t all = 0;
+    for (const void *p : ptrs)
+        all |= reinterpret_cast<uintptr_t>(p);
+    return (all & 15u) == 0;
+}
+
+bool aligned4(std::initializer_list<const void *> ptrs) {
+    uintptr_t all = 0;
+    for (const void *p : ptrs)
+        all |= reinterpret_cast<uintptr_t>(p);
+    return (all & 3u) == 0;
+}
+
+// What every prepare call of this file begins with.
+int begin(gg_handle *h, const void *p, char *why, size_t why_len) {
+    if (!h)
+        return GG_ERR_ARG;
+    h->ready = false;
+    h->moe.launches = 0;
+    h->last_error.clear();
+    if (why && why_len)
+        why[0] = '\0';
+    if (!p)
+        return fail(h, GG_ERR_ARG, "null problem");
+    return GG_OK;
+}
+
+// The device's checks and the handle's status word, once the arguments are accepted.
+int bind_device(gg_handle *h, gg_stream_t stream, int &num_sms, char *why, size_t why_len) {
+    int dev = 0, major = 0, minor = 0;
+    GG_CUDA(h, cudaGetDevice(&dev));
+    GG_CUDA(h, cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev));
+    GG_CUDA(h, cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+    GG_CUDA(h, cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev));
+    if (major != 10 || minor != 0)
+        return refuse(h, why, why_len, "needs an sm_100 GPU (B200/GB200)");
+    h->device = dev;
+    if (!h->d_status)
+        GG_CUDA(h, cudaMalloc(&h->d_status, 16));
+    GG_CUDA(h, cudaMemsetAsync(h->d_status, 0, 16, stream));
+    return GG_OK;
+}
+
+int reserve(gg_handle *h, size_t bytes) {
+    if (h->ws_cap >= bytes)
+        return GG_OK;
+    if (h->d_ws)
+        cudaFree(h->d_ws);
+    h->d_ws = nullptr;
+    h->ws_cap = 0;
+    GG_CUDA(h, cudaMalloc(&h->d_ws, bytes));
+    h->ws_cap = bytes;
+    return GG_OK;
+}
+
+template <class P> void set_params(gg_handle *h, const P &p) {
+    static_assert(sizeof(P) <= sizeof(h->moe.params), "parameter block too large");
+    std::memcpy(h->moe.params, &p, sizeof(P));
+}
+
+int finish(gg_handle *h, gg_stream_t stream, std::initializer_list<MoeLaunch> launches, const char *detail) {
+    int n = 0;
+    for (const MoeLaunch &l : launches)
+        h->moe.launch[n++] = l;
+    GG_CUDA(h, cudaStreamSynchronize(stream));  // as gg_prepare: the handle's own buffers are in place
+    h->detail = detail;
+    h->moe.launches = n;
+    h->ready = true;
+    return GG_OK;
+}
+
+// An entry of the C ABI lets no C++ exception out.
+template <class F> int guarded(gg_handle *h, F &&f) noexcept {
+    try {
+        return f();
+    } catch (...) {
+        if (h)
+            h->ready = false;
+        return GG_ERR_ARG;
+    }
+}
+
+const char *type_name(int t) { return t == GG_F32 ? "fp32" : t == GG_FP16 ? "fp16" : "bf16"; }
+
+// ---- router ----
+
+template <class T, int V> const void *route_fn(bool grad) {
+    return grad ? reinterpret_cast<const void *>(&gg::moe::route_grad<T, V>) : reinterpret_cast<const void *>(&gg::moe::route_topk<T, V>);
+}
+template <class T> const void *route_fn(int experts, bool grad) {
+    const int v = (experts + 31) / 32;
+    if (v <= 1)
+        return route_fn<T, 1>(grad);
+    if (v <= 2)
+        return route_fn<T, 2>(grad);
+    if (v <= 4)
+        return route_fn<T, 4>(grad);
+    if (v <= 8)
+        return route_fn<T, 8>(grad);
+    if (v <= 16)
+        return route_fn<T, 16>(grad);
+    return route_fn<T, 32>(grad);
+}
+const void *route_fn(int type, int experts, bool grad) {
+    return type == GG_F32 ? route_fn<float>(experts, grad)
+           : type == GG_FP16 ? route_fn<__half>(experts, grad) : route_fn<__nv_bfloat16>(experts, grad);
+}
+
+const char *route_bad(int32_t type, int64_t tokens, int32_t experts, int32_t top_k) {
+    if (type != GG_BF16 && type != GG_FP16 && type != GG_F32)
+        return "logits_type must be bf16 (0), fp16 (1) or fp32 (2)";
+    if (tokens < 0 || tokens >= kMaxIndex)
+        return "tokens must be 0..2^31 - 1";
+    if (experts < 1 || experts > gg::moe::kMaxExperts)
+        return "experts must be 1..1024";
+    if (top_k < 1 || top_k > gg::moe::kMaxTopK || top_k > experts)
+        return "top_k must be 1..32 and at most experts";
+    if (tokens * top_k >= kMaxIndex)
+        return "tokens * top_k must be below 2^31";
+    return nullptr;
+}
+
+int prepare_route(gg_handle *h, const gg_route_problem &q, gg_stream_t stream, char *why, size_t why_len) {
+    if (const char *bad = route_bad(q.logits_type, q.tokens, q.experts, q.top_k))
+        return refuse(h, why, why_len, bad);
+    if (!q.counts || !q.offsets || !q.live || (q.tokens > 0 && (!q.logits || !q.ids || !q.weights || !q.dest || !q.src)))
+        return refuse(h, why, why_len, "logits, ids, weights, counts, offsets, live, dest and src must be non-null device pointers");
+    if (!aligned16({q.logits}) ||
+        !aligned4({q.ids, q.weights, q.lse, q.counts, q.offsets, q.live, q.dest, q.src, q.prob, q.losses}))
+        return refuse(h, why, why_len, "logits must be 16-byte aligned, the outputs 4-byte aligned");
+    int num_sms = 0;
+    if (const int rc = bind_device(h, stream, num_sms, why, why_len))
+        return rc;
+    gg::moe::RouteParams p{};
+    p.logits = q.logits;
+    p.mask = q.mask;
+    p.ids = q.ids;
+    p.weights = q.weights;
+    p.lse = q.lse;
+    p.counts = q.counts;
+    p.offsets = q.offsets;
+    p.live = q.live;
+    p.dest = q.dest;
+    p.src = q.src;
+    p.prob = q.prob;
+    p.losses = q.losses;
+    p.tokens = q.tokens;
+    p.experts = q.experts;
+    p.top_k = q.top_k;
+    p.normalize = q.normalize != 0;
+    p.scale = q.scale;
+    const int64_t wanted = std::max<int64_t>(1, (q.tokens + gg::moe::kRouteWarps - 1) / gg::moe::kRouteWarps);
+    p.blocks = int(std::min<int64_t>(wanted, num_sms));
+    p.per_block = std::max<int64_t>(1, (q.tokens + p.blocks - 1) / p.blocks);
+    const size_t entries = size_t(p.blocks) * size_t(q.experts + 1);
+    if (const int rc = reserve(h, 2 * entries * 4))
+        return rc;
+    p.block_sums = h->d_ws;
+    p.block_counts = reinterpret_cast<int32_t *>(h->d_ws + entries);
+    set_params(h, p);
+    MoeLaunch topk{route_fn(q.logits_type, q.experts, false), unsigned(p.blocks), gg::moe::kRouteThreads,
+                   size_t(gg::moe::kRouteWarps) * size_t(q.experts) * 4};
+    MoeLaunch place{reinterpret_cast<const void *>(&gg::moe::route_place), unsigned(p.blocks), gg::moe::kRouteThreads, 0};
+    char detail[160];
+    std::snprintf(detail, sizeof(detail), "gg_route<%s> experts=%d top_k=%d blocks=%d", type_name(q.logits_type), q.experts, q.top_k, p.blocks);
+    return finish(h, stream, {topk, place}, detail);
+}
+
+int prepare_route_grad(gg_handle *h, const gg_route_grad_problem &q, gg_stream_t stream, char *why, size_t why_len) {
+    if (const char *bad = route_bad(q.logits_type, q.tokens, q.experts, q.top_k))
+        return refuse(h, why, why_len, bad);
+    if (!q.counts || !q.live || (q.tokens > 0 && (!q.logits || !q.ids || !q.lse || !q.dlogits)))
+        return refuse(h, why, why_len, "logits, ids, lse, counts, live and dlogits must be non-null device pointers");
+    if (!aligned16({q.logits, q.dlogits}) || !aligned4({q.ids, q.lse, q.counts, q.live, q.dweights, q.dlosses}))
+        return refuse(h, why, why_len, "logits and dlogits must be 16-byte aligned, the other operands 4-byte aligned");
+    int num_sms = 0;
+    if (const int rc = bind_device(h, stream, num_sms, why, why_len))
+        return rc;
+    gg::moe::RouteGradParams p{};
+    p.logits = q.logits;
+    p.mask = q.mask;
+    p.ids = q.ids;
+    p.lse = q.lse;
+    p.counts = q.counts;
+    p.live = q.live;
+    p.dweights = q.dweights;
+    p.dlosses = q.dlosses;
+    p.dlogits = q.dlogits;
+    p.status = h->d_status;
+    p.tokens = q.tokens;
+    p.experts = q.experts;
+    p.top_k = q.top_k;
+    p.normalize = q.normalize != 0;
+    p.scale = q.scale;
+    set_params(h, p);
+    const void *fn = route_fn(q.logits_type, q.experts, true);
+    const size_t smem = size_t(1 + gg::moe::kRouteWarps) * size_t(q.experts) * 4;
+    const int64_t blocks = std::min<int64_t>((q.tokens + gg::moe::kRouteWarps - 1) / gg::moe::kRouteWarps, int64_t(num_sms) * 8);
+    char detail[160];
+    std::snprintf(detail, sizeof(detail), "gg_route_grad<%s> experts=%d top_k=%d blocks=%d", type_name(q.logits_type), q.experts, q.top_k, int(blocks));
+    return finish(h, stream, {MoeLaunch{fn, unsigned(blocks), gg::moe::kRouteThreads, smem}}, detail);
+}
+
+// ---- dispatch / combine ----
+
+const char *permute_bad(int32_t dtype, int64_t tokens, int32_t top_k, int32_t experts, int64_t hidden) {
+    if (dtype != GG_BF16 && dtype != GG_FP16)
+        return "dtype must be bf16 (0) or fp16 (1)";
+    if (tokens < 0 || tokens >= kMaxIndex)
+        return "tokens must be 0..2^31 - 1";
+    if (top_k < 1 || top_k > gg::moe::kMaxTopK)
+        return "top_k must be 1..32";
+    if (experts < 1)
+        return "experts must be >= 1";
+    if (hidden < 8 || hidden % 8 != 0 || hidden > (int64_t(1) << 30))
+        return "hidden must be a multiple of 8 (16-byte rows) in 8..2^30";
+    if (tokens * top_k >= kMaxIndex)
+        return "tokens * top_k must be below 2^31";
+    return nullptr;
+}
+
+int prepare_permute(gg_handle *h, const gg_permute_problem &q, int32_t op, gg_stream_t stream, char *why, size_t why_len) {
+    if (const char *bad = permute_bad(q.dtype, q.tokens, q.top_k, q.experts, q.hidden))
+        return refuse(h, why, why_len, bad);
+    gg::moe::PermuteParams p{};
+    const bool some = q.tokens > 0;
+    if (op == GG_OP_DISPATCH) {
+        if (!q.offsets || (some && (!q.x || !q.dest || !q.rows)))
+            return refuse(h, why, why_len, "x, dest, offsets and rows must be non-null device pointers");
+        p.x = q.x;
+        p.out = q.rows;
+    } else if (op == GG_OP_COMBINE) {
+        if (some && (!q.rows || !q.dest || !q.x))
+            return refuse(h, why, why_len, "rows, dest and x must be non-null device pointers");
+        p.x = q.rows;
+        p.out = q.x;
+    } else {
+        if (!q.offsets || (some && (!q.dy || !q.dest || !q.drows || (q.dweights && !q.rows))))
+            return refuse(h, why, why_len, "dy, rows, dest, offsets and drows must be non-null device pointers");
+        p.x = q.rows;
+        p.dy = q.dy;
+        p.out = q.drows;
+        p.dweights = q.dweights;
+    }
+    if (!aligned16({q.x, q.rows, q.dy, q.drows}) || !aligned4({q.dest, q.offsets, q.weights, q.dweights}))
+        return refuse(h, why, why_len, "x, rows, dy and drows must be 16-byte aligned, the other operands 4-byte aligned");
+    int num_sms = 0;
+    if (const int rc = bind_device(h, stream, num_sms, why, why_len))
+        return rc;
+    p.dest = q.dest;
+    p.offsets = q.offsets;
+    p.weights = q.weights;
+    p.status = h->d_status;
+    p.tokens = q.tokens;
+    p.rows = q.tokens * q.top_k;
+    p.experts = q.experts;
+    p.top_k = q.top_k;
+    p.vecs = int(q.hidden / 8);
+    set_params(h, p);
+    const bool half = q.dtype == GG_FP16;
+    const void *fn = op == GG_OP_DISPATCH ? reinterpret_cast<const void *>(&gg::moe::dispatch_rows)
+                     : op == GG_OP_COMBINE
+                         ? (half ? reinterpret_cast<const void *>(&gg::moe::combine_rows<__half>)
+                                 : reinterpret_cast<const void *>(&gg::moe::combine_rows<__nv_bfloat16>))
+                         : (half ? reinterpret_cast<const void *>(&gg::moe::combine_grad_rows<__half>)
+                                 : reinterpret_cast<const void *>(&gg::moe::combine_grad_rows<__nv_bfloat16>));
+    const int64_t blocks = std::min<int64_t>(q.tokens, int64_t(num_sms) * 32);
+    char detail[160];
+    std::snprintf(detail, sizeof(detail), "gg_%s<%s> hidden=%lld top_k=%d blocks=%d",
+                  op == GG_OP_DISPATCH ? "dispatch" : op == GG_OP_COMBINE ? "combine" : "combine_grad", type_name(q.dtype),
+                  static_cast<long long>(q.hidden), q.top_k, int(blocks));
+    return finish(h, stream, {MoeLaunch{fn, unsigned(blocks), gg::moe::kPermuteThreads, 0}}, detail);
+}
+
+// ---- 4-bit products ----
+
+template <class T> const void *w4_fn(int group) {
+    return group == 32   ? reinterpret_cast<const void *>(&gg::moe::w4_rows<T, 32>)
+           : group == 64 ? reinterpret_cast<const void *>(&gg::moe::w4_rows<T, 64>)
+                         : reinterpret_cast<const void *>(&gg::moe::w4_rows<T, 128>);
+}
+
+int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *why, size_t why_len) {
+    if (q.dtype != GG_BF16 && q.dtype != GG_FP16)
+        return refuse(h, why, why_len, "dtype must be bf16 (0) or fp16 (1)");
+    if (q.experts < 1 || q.experts > gg::moe::kW4MaxExperts)
+        return refuse(h, why, why_len, "experts must be 1..1024");
+    if (q.n < 1 || q.n % 8 != 0 || q.n > (int64_t(1) << 30))
+        return refuse(h, why, why_len, "n must be a multiple of 8 (16-byte output row stride) in 8..2^30");
+    if (q.k < 1 || q.k % 32 != 0 || q.k > (int64_t(1) << 30))
+        return refuse(h, why, why_len, "k must be a multiple of 32 (16-byte stride of 4-bit rows) in 32..2^30");
+    if (q.group_size != 32 && q.group_size != 64 && q.group_size != 128)
+        return refuse(h, why, why_len, "group_size must be 32, 64 or 128");
+    if (q.rows < 0 || q.rows >= kMaxIndex)
+        return refuse(h, why, why_len, "rows must be 0..2^31 - 1");
+    if (q.src && (q.tokens < 0 || q.tokens >= kMaxIndex || q.top_k < 1 || q.tokens * q.top_k >= kMaxIndex))
+        return refuse(h, why, why_len, "with src, tokens must be >= 0, top_k >= 1 and tokens * top_k below 2^31");
+    if (!q.offsets || !q.qweight || !q.scales || (q.rows > 0 && (!q.x || !q.out)))
+        return refuse(h, why, why_len, "x, qweight, scales, offsets and out must be non-null device pointers");
+    if (!aligned16({q.x, q.qweight, q.scales, q.zeros, q.out}) || !aligned4({q.offsets, q.src}))
+        return refuse(h, why, why_len, "x, qweight, scales, zeros and out must be 16-byte aligned, offsets and src 4-byte aligned");
+    int num_sms = 0;
+    if (const int rc = bind_device(h, stream, num_sms, why, why_len))
+        return rc;
+    gg::moe::W4Params p{};
+    p.x = q.x;
+    p.qweight = static_cast<const uint8_t *>(q.qweight);
+    p.scales = q.scales;
+    p.zeros = static_cast<const uint8_t *>(q.zeros);
+    p.offsets = q.offsets;
+    p.src = q.src;
+    p.out = q.out;
+    p.status = h->d_status;
+    p.rows = q.rows;
+    p.slots = q.src ? q.tokens * q.top_k : 0;
+    p.n = int(q.n);
+    p.k = int(q.k);
+    p.groups = int((q.k + q.group_size - 1) / q.group_size);
+    p.experts = q.experts;
+    p.top_k = q.src ? q.top_k : 1;
+    p.tiles = int((q.n + gg::moe::kW4Rows - 1) / gg::moe::kW4Rows);
+    set_params(h, p);
+    const void *fn = q.dtype == GG_FP16 ? w4_fn<__half>(q.group_size) : w4_fn<__nv_bfloat16>(q.group_size);
+    int per_sm = 0;
+    GG_CUDA(h, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, gg::moe::kW4Threads, 0));
+    // an upper bound of the work items: every row in an expert (or a full chunk) of its own
+    const int64_t chunks = std::min<int64_t>(q.rows, q.experts + q.rows / gg::moe::kW4Tokens);
+    const int64_t blocks = q.rows > 0 ? std::min<int64_t>(std::max<int64_t>(1, chunks * p.tiles), int64_t(num_sms) * std::max(1, per_sm)) : 0;
+    char detail[160];
+    std::snprintf(detail, sizeof(detail), "gg_w4<%s> n=%lld k=%lld group=%d blocks=%d", type_name(q.dtype), static_cast<long long>(q.n),
+                  static_cast<long long>(q.k), q.group_size, int(blocks));
+    return finish(h, stream, {MoeLaunch{fn, unsigned(blocks), gg::moe::kW4Threads, 0}}, detail);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gg_prepare_route(gg_handle *h, const gg_route_problem *p, gg_stream_t stream, char *why, size_t why_len) {
+    return guarded(h, [&] {
+        if (const int rc = begin(h, p, why, why_len))
+            return rc;
+        return prepare_route(h, *p, stream, why, why_len);
+    });
+}
+
+int gg_prepare_route_grad(gg_handle *h, const gg_route_grad_problem *p, gg_stream_t stream, char *why, size_t why_len) {
+    return guarded(h, [&] {
+        if (const int rc = begin(h, p, why, why_len))
+            return rc;
+        return prepare_route_grad(h, *p, stream, why, why_len);
+    });
+}
+
+int gg_prepare_permute(gg_handle *h, const gg_permute_problem *p, int32_t op, gg_stream_t stream, char *why, size_t why_len) {
+    return guarded(h, [&] {
+        if (const int rc = begin(h, p, why, why_len))
+            return rc;
+        if (op != GG_OP_DISPATCH && op != GG_OP_COMBINE && op != GG_OP_COMBINE_GRAD)
+            return fail(h, GG_ERR_ARG, "op must be GG_OP_DISPATCH (3), GG_OP_COMBINE (4) or GG_OP_COMBINE_GRAD (5)");
+        return prepare_permute(h, *p, op, stream, why, why_len);
+    });
+}
+
+int gg_prepare_w4(gg_handle *h, const gg_w4_problem *p, gg_stream_t stream, char *why, size_t why_len) {
+    return guarded(h, [&] {
+        if (const int rc = begin(h, p, why, why_len))
+            return rc;
+        return prepare_w4(h, *p, stream, why, why_len);
+    });
+}
+
+}  // extern "C"

@@ -34,7 +34,7 @@ typedef struct CUstream_st *gg_stream_t; /* == cudaStream_t */
 typedef struct gg_handle gg_handle;
 
 /* Element types (tunemax::DType, common/backend.hpp:27). */
-enum gg_dtype { GG_BF16 = 0, GG_FP16 = 1 };
+enum gg_dtype { GG_BF16 = 0, GG_FP16 = 1, GG_F32 = 2 /* router logits only */ };
 
 /* Return codes. */
 enum gg_status {
@@ -109,9 +109,157 @@ typedef struct gg_grad_problem {
 int gg_prepare_grad(gg_handle *h, const gg_grad_problem *p, int32_t op, gg_stream_t stream, char *why,
                     size_t why_len);
 
+/* ---- The layer around the grouped GEMM ----
+ *
+ * Router, token movement and 4-bit products of the same mixture-of-experts layer. The reference
+ * benchmarks the grouped GEMM alone, on rows that are in expert order already; these calls produce
+ * that order, take the rows there and back, and serve few tokens from small weights. Each prepare
+ * call below is used as gg_prepare: it validates (GG_NOT_SUPPORTED with a reason in `why`), allocates
+ * what the handle needs and waits for `stream`; then gg_run() enqueues the operator on any stream
+ * without waiting and allocates nothing (it can be captured in a CUDA graph). A handle holds one
+ * prepared operator at a time and its launches must not overlap on the GPU. Operands are device
+ * pointers to contiguous arrays that the caller owns; the contents may change between runs.
+ *
+ * Indices that come from device memory (dest, src, ids, offsets) are checked by the kernels: one
+ * that is out of range is skipped and reported by gg_device_status (GG_ERR_DEVICE, status
+ * 0x2000 | site: 0x10 dest, 0x11 src, 0x12 offsets, 0x13 ids); nothing is read or written out of
+ * bounds. Sums and softmax statistics are held in fp32; results do not depend on the order in which
+ * the GPU runs blocks (the same inputs give the same bits). */
+
+/* Router. For each token t with logits l_t [experts]:
+ *
+ *   lse_t = log sum_e exp(l_te)        p_te = exp(l_te - lse_t)
+ *   ids_t: the top_k largest logits, falling, ties to the lower expert; -1 where fewer than top_k
+ *          logits are above -inf (an expert at -inf is closed to the token)
+ *   weights_tj = scale * p_t,ids_tj, or with `normalize` scale * exp(l_t,ids_tj) / sum_i exp(l_t,ids_ti);
+ *          0 where ids is -1
+ *
+ * A token whose mask byte is 0, or all of whose logits are -inf, is not live: ids -1, weights 0, lse -inf,
+ * and nothing of its logits (NaN included) goes anywhere. In a live row NaN counts as larger than +inf for
+ * the choice, and a row that holds NaN or +inf has NaN weights and lse (as the formulas give).
+ *
+ *   counts_e: slots (t, j) of expert e       offsets: their exclusive prefix sums, [experts + 1]
+ *   dest_tj: place of slot (t, j) in the order by expert, slots of one expert in (t, j) order; -1 for none
+ *   src: the slot t * top_k + j at each place, -1 from offsets[experts] on
+ *   live: number of live tokens
+ *   prob_e = (1 / live) sum_t p_te
+ *   losses[0] = experts * sum_e counts_e / (top_k live) * prob_e        (balance loss)
+ *   losses[1] = (1 / live) sum_t lse_t^2                                (z loss); both 0 if live is 0
+ *
+ * experts 1..1024, top_k 1..32 (at most experts), tokens * top_k < 2^31; logits 16-byte aligned. */
+typedef struct gg_route_problem {
+    int32_t logits_type;  /* GG_BF16, GG_FP16 or GG_F32 */
+    int32_t experts;
+    int32_t top_k;
+    int32_t normalize;    /* 0 or 1 */
+    float scale;          /* factor of the weights, 1 for none */
+    int64_t tokens;       /* >= 0 */
+    const void *logits;   /* [tokens, experts] */
+    const uint8_t *mask;  /* [tokens], 0 = padding token; or NULL */
+    int32_t *ids;         /* out [tokens, top_k] */
+    float *weights;       /* out [tokens, top_k] */
+    float *lse;           /* out [tokens], or NULL (gg_prepare_route_grad needs it) */
+    int32_t *counts;      /* out [experts] */
+    int32_t *offsets;     /* out [experts + 1] */
+    int32_t *live;        /* out [1] */
+    int32_t *dest;        /* out [tokens, top_k] */
+    int32_t *src;         /* out [tokens * top_k] */
+    float *prob;          /* out [experts], or NULL */
+    float *losses;        /* out [2], or NULL */
+} gg_route_problem;
+
+int gg_prepare_route(gg_handle *h, const gg_route_problem *p, gg_stream_t stream, char *why, size_t why_len);
+
+/* Gradient of the router's weights and losses with respect to the logits, from what gg_prepare_route's
+ * run wrote (ids, lse, counts, live) and the same logits, mask, normalize and scale. counts are constants
+ * of the balance loss, as usual. dweights or dlosses may be NULL (zero). Tokens that are not live and
+ * closed experts get zero; what dweights holds at slots without an expert is not read. */
+typedef struct gg_route_grad_problem {
+    int32_t logits_type;
+    int32_t experts;
+    int32_t top_k;
+    int32_t normalize;
+    float scale;
+    int64_t tokens;
+    const void *logits;     /* [tokens, experts] */
+    const uint8_t *mask;    /* [tokens] or NULL */
+    const int32_t *ids;     /* [tokens, top_k] */
+    const float *lse;       /* [tokens] */
+    const int32_t *counts;  /* [experts] */
+    const int32_t *live;    /* [1] */
+    const float *dweights;  /* [tokens, top_k] or NULL */
+    const float *dlosses;   /* [2]: of the balance and of the z loss; or NULL */
+    void *dlogits;          /* out [tokens, experts], type of the logits */
+} gg_route_grad_problem;
+
+int gg_prepare_route_grad(gg_handle *h, const gg_route_grad_problem *p, gg_stream_t stream, char *why, size_t why_len);
+
+/* Tokens into expert order and back, over the places `dest` that the router gives:
+ *
+ *   GG_OP_DISPATCH:     rows[dest_tj] = x_t; rows from offsets[experts] on are zero
+ *   GG_OP_COMBINE:      x_t = sum_j weights_tj * rows[dest_tj] (fp32 sum; weights NULL = 1, which is the
+ *                       gradient of dispatch)
+ *   GG_OP_COMBINE_GRAD: drows[dest_tj] = weights_tj * dy_t (rows from offsets[experts] on are zero) and
+ *                       dweights_tj = <dy_t, rows[dest_tj]> (0 without a place; dweights may be NULL)
+ *
+ * bf16 or fp16, hidden a multiple of 8, rows [tokens * top_k, hidden], 16-byte aligned; dest's entries
+ * distinct, as the router's are. */
+enum gg_permute_op { GG_OP_DISPATCH = 3, GG_OP_COMBINE = 4, GG_OP_COMBINE_GRAD = 5 };
+
+typedef struct gg_permute_problem {
+    int32_t dtype;
+    int32_t experts;         /* length of offsets - 1 */
+    int32_t top_k;
+    int64_t tokens;
+    int64_t hidden;
+    void *x;                 /* [tokens, hidden]: read by dispatch, written by combine */
+    void *rows;              /* [tokens * top_k, hidden]: written by dispatch, else read */
+    const void *dy;          /* [tokens, hidden] (combine_grad) */
+    void *drows;             /* out [tokens * top_k, hidden] (combine_grad) */
+    const int32_t *dest;     /* [tokens, top_k] */
+    const int32_t *offsets;  /* [experts + 1] (dispatch, combine_grad) */
+    const float *weights;    /* [tokens, top_k], or NULL = 1 */
+    float *dweights;         /* out [tokens, top_k] (combine_grad), or NULL */
+} gg_permute_problem;
+
+int gg_prepare_permute(gg_handle *h, const gg_permute_problem *p, int32_t op, gg_stream_t stream, char *why, size_t why_len);
+
+/* Products with 4-bit weights for few rows an expert (decoding):
+ *
+ *   out[r, n] = sum over groups g of scales[e, n, g] * sum_{k in g} (q[e, n, k] - zeros[e, n, g]) * x[row(r), k]
+ *
+ * for the rows r of expert e, offsets[e] <= r < offsets[e + 1]; row(r) = src[r] / top_k, or r without
+ * src (so the first product of a layer gathers its tokens itself). Rows of no expert are zero. offsets and src are
+ * the router's, in device memory: no count goes to the host. q is 4 bits, two to a byte (even k in the low
+ * half), zeros NULL = 8 everywhere (else its low four bits). The integers q - zero are exact in 16 bits,
+ * products are summed in fp32, the scale is applied to each group's fp32 sum, and the result rounded once.
+ *
+ * bf16 or fp16 x, scales and out; experts 1..1024, n a multiple of 8, k a multiple of 32 (the last group
+ * may be shorter), group_size 32, 64 or 128; x, qweight, scales, zeros and out 16-byte aligned. */
+typedef struct gg_w4_problem {
+    int32_t dtype;
+    int32_t experts;
+    int32_t group_size;
+    int32_t top_k;           /* with src */
+    int64_t n;
+    int64_t k;
+    int64_t rows;            /* rows of out */
+    int64_t tokens;          /* rows of x, with src */
+    const void *x;           /* [tokens, k] with src, else [rows, k] */
+    const void *qweight;     /* [experts, n, k / 2] bytes */
+    const void *scales;      /* [experts, n, ceil(k / group_size)] */
+    const void *zeros;       /* [experts, n, ceil(k / group_size)] bytes, or NULL */
+    const int32_t *offsets;  /* [experts + 1] */
+    const int32_t *src;      /* [rows] or NULL */
+    void *out;               /* [rows, n] */
+} gg_w4_problem;
+
+int gg_prepare_w4(gg_handle *h, const gg_w4_problem *p, gg_stream_t stream, char *why, size_t why_len);
+
 /* Backend::run() (common/backend.hpp:67; ck_kernel/ck_grouped_gemm.cpp:140, :114-121). Timed:
  * enqueues one grouped GEMM on `stream` and does not synchronise: one kernel launch, or two for
- * a split launch ("tail_launch" below). */
+ * a split launch ("tail_launch" below). After one of the layer operators' prepare calls it enqueues
+ * that operator instead. */
 int gg_run(gg_handle *h, gg_stream_t stream);
 
 /* Backend::release() (common/backend.hpp:69; ck_kernel/ck_grouped_gemm.cpp:142-146): frees
