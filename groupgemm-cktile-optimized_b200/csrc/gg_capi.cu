@@ -909,8 +909,8 @@ int gg_device_status(gg_handle *h, gg_stream_t stream, uint32_t *status) {
         if (h->d_counters)
             GG_CUDA(h, cudaMemset(h->d_counters, 0, h->counters_cap));
         return fail(h, GG_ERR_DEVICE, "%s: status 0x%x",
-                    h->moe.launches > 0                ? "index out of range"
-                    : (*status & gg::kStatusBounds) ? "debug bounds check failed" : "kernel bounded wait timed out", *status);
+                    !(*status & gg::kStatusBounds) ? "kernel bounded wait timed out"
+                    : h->moe.launches > 0         ? "index out of range" : "debug bounds check failed", *status);
     }
     return GG_OK;
 }

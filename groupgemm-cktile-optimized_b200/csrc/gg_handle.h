@@ -15,16 +15,20 @@
 namespace gg {
 
 // One kernel of a prepared layer operator (router, dispatch / combine, 4-bit product): gg_run
-// launches them in order, each with the operator's parameter block as its one argument.
+// launches them in order, each with the operator's parameter block as its argument (after the tensor
+// map where it has one).
 struct MoeLaunch {
     const void *fn = nullptr;
     unsigned grid = 0, block = 0;
     size_t smem = 0;
+    bool map = false;  // the kernel takes MoePlan::map first
+    unsigned grid_y = 1;
 };
 
 struct MoePlan {
     int launches = 0;  // 0: the handle holds no layer operator
     MoeLaunch launch[2];
+    CUtensorMap map{};
     alignas(16) unsigned char params[256];
 };
 

@@ -27,15 +27,15 @@ int run_moe(gg_handle *h, cudaStream_t stream) {
     cfg.attrs = attr;
     cfg.numAttrs = h->opt_pdl ? 1 : 0;
     cfg.stream = stream;
-    void *args[1] = {h->moe.params};
+    void *args[2] = {&h->moe.map, h->moe.params};
     for (int i = 0; i < h->moe.launches; ++i) {
         const MoeLaunch &l = h->moe.launch[i];
         if (!l.grid)
             continue;  // nothing to do
-        cfg.gridDim = dim3(l.grid, 1, 1);
+        cfg.gridDim = dim3(l.grid, l.grid_y, 1);
         cfg.blockDim = dim3(l.block, 1, 1);
         cfg.dynamicSmemBytes = l.smem;
-        GG_CUDA(h, cudaLaunchKernelExC(&cfg, l.fn, args));
+        GG_CUDA(h, cudaLaunchKernelExC(&cfg, l.fn, l.map ? args : args + 1));
     }
     return GG_OK;
 }
@@ -103,6 +103,41 @@ int reserve(gg_handle *h, size_t bytes) {
     h->ws_cap = 0;
     GG_CUDA(h, cudaMalloc(&h->d_ws, bytes));
     h->ws_cap = bytes;
+    return GG_OK;
+}
+
+int reserve_counters(gg_handle *h, size_t bytes, gg_stream_t stream) {
+    if (h->counters_cap < bytes) {
+        if (h->d_counters)
+            cudaFree(h->d_counters);
+        h->d_counters = nullptr;
+        h->counters_cap = 0;
+        GG_CUDA(h, cudaMalloc(&h->d_counters, bytes));
+        h->counters_cap = bytes;
+    }
+    GG_CUDA(h, cudaMemsetAsync(h->d_counters, 0, bytes, stream));
+    return GG_OK;
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The handle's tensor map over bytes [depth, rows, cols] in boxes of box_cols (64, with that swizzle) x box_rows.
+int encode_bytes_3d(gg_handle *h, const void *base, int64_t cols, int64_t rows, int64_t depth, uint32_t box_cols, uint32_t box_rows) {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    GG_CUDA(h, cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !fn)
+        return fail(h, GG_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+    const cuuint64_t dim[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(depth)};
+    const cuuint64_t stride[2] = {cuuint64_t(cols), cuuint64_t(cols) * cuuint64_t(rows)};
+    const cuuint32_t box[3] = {box_cols, box_rows, 1}, estride[3] = {1, 1, 1};
+    const CUresult r = reinterpret_cast<EncodeTiledFn>(fn)(
+        &h->moe.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dim, stride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(h, GG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
     return GG_OK;
 }
 
@@ -327,10 +362,17 @@ int prepare_permute(gg_handle *h, const gg_permute_problem &q, int32_t op, gg_st
 
 // ---- 4-bit products ----
 
-template <class T> const void *w4_fn(int group) {
-    return group == 32   ? reinterpret_cast<const void *>(&gg::moe::w4_rows<T, 32>)
-           : group == 64 ? reinterpret_cast<const void *>(&gg::moe::w4_rows<T, 64>)
-                         : reinterpret_cast<const void *>(&gg::moe::w4_rows<T, 128>);
+struct W4Variant {
+    const void *fn;
+    int tokens;  // of a chunk
+    size_t smem;
+};
+template <class T, int G> W4Variant w4_variant() {
+    using C = gg::moe::W4Cfg<G>;
+    return {reinterpret_cast<const void *>(&gg::moe::w4_rows<T, G>), C::kTokens, C::kSmemBytes};
+}
+template <class T> W4Variant w4_variant(int group) {
+    return group == 32 ? w4_variant<T, 32>() : group == 64 ? w4_variant<T, 64>() : w4_variant<T, 128>();
 }
 
 int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *why, size_t why_len) {
@@ -352,12 +394,24 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
         return refuse(h, why, why_len, "x, qweight, scales, offsets and out must be non-null device pointers");
     if (!aligned16({q.x, q.qweight, q.scales, q.zeros, q.out}) || !aligned4({q.offsets, q.src}))
         return refuse(h, why, why_len, "x, qweight, scales, zeros and out must be 16-byte aligned, offsets and src 4-byte aligned");
+    if (q.n * (q.k / 2) >= int64_t(1) << 39)
+        return refuse(h, why, why_len, "one expert's weights are too large for a TMA descriptor");
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
+    const W4Variant v = q.dtype == GG_FP16 ? w4_variant<__half>(q.group_size) : w4_variant<__nv_bfloat16>(q.group_size);
+    GG_CUDA(h, cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(v.smem)));
+    if (const int rc = encode_bytes_3d(h, q.qweight, q.k / 2, q.n, q.experts, gg::moe::kW4StepK / 2, gg::moe::kW4TileRows))
+        return rc;
+    const int blocks = q.rows > 0 ? num_sms : 0;
+    const int64_t steps = (q.k + gg::moe::kW4StepK - 1) / gg::moe::kW4StepK;
+    const size_t sums = size_t(2 * num_sms) * size_t(v.tokens) * gg::moe::kW4TileRows * 4;
+    if (const int rc = reserve(h, sums + size_t(q.rows + 8 * int64_t(q.experts)) * size_t(steps) * 256))
+        return rc;
+    if (const int rc = reserve_counters(h, size_t(num_sms) * 4, stream))
+        return rc;
     gg::moe::W4Params p{};
     p.x = q.x;
-    p.qweight = static_cast<const uint8_t *>(q.qweight);
     p.scales = q.scales;
     p.zeros = static_cast<const uint8_t *>(q.zeros);
     p.offsets = q.offsets;
@@ -371,18 +425,22 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     p.groups = int((q.k + q.group_size - 1) / q.group_size);
     p.experts = q.experts;
     p.top_k = q.src ? q.top_k : 1;
-    p.tiles = int((q.n + gg::moe::kW4Rows - 1) / gg::moe::kW4Rows);
+    p.tiles = int((q.n + gg::moe::kW4TileRows - 1) / gg::moe::kW4TileRows);
+    p.steps = int(steps);
+    p.chunk = v.tokens;
+    p.ws = h->d_ws;
+    p.xs = reinterpret_cast<uint8_t *>(h->d_ws) + sums;
+    p.counters = h->d_counters;
+    p.timeout_ns = uint64_t(h->opt_timeout_ms) * 1000000u;
     set_params(h, p);
-    const void *fn = q.dtype == GG_FP16 ? w4_fn<__half>(q.group_size) : w4_fn<__nv_bfloat16>(q.group_size);
-    int per_sm = 0;
-    GG_CUDA(h, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, gg::moe::kW4Threads, 0));
-    // an upper bound of the work items: every row in an expert (or a full chunk) of its own
-    const int64_t chunks = std::min<int64_t>(q.rows, q.experts + q.rows / gg::moe::kW4Tokens);
-    const int64_t blocks = q.rows > 0 ? std::min<int64_t>(std::max<int64_t>(1, chunks * p.tiles), int64_t(num_sms) * std::max(1, per_sm)) : 0;
     char detail[160];
     std::snprintf(detail, sizeof(detail), "gg_w4<%s> n=%lld k=%lld group=%d blocks=%d", type_name(q.dtype), static_cast<long long>(q.n),
-                  static_cast<long long>(q.k), q.group_size, int(blocks));
-    return finish(h, stream, {MoeLaunch{fn, unsigned(blocks), gg::moe::kW4Threads, 0}}, detail);
+                  static_cast<long long>(q.k), q.group_size, blocks);
+    MoeLaunch gather{q.dtype == GG_FP16 ? reinterpret_cast<const void *>(&gg::moe::w4_gather<__half>)
+                                        : reinterpret_cast<const void *>(&gg::moe::w4_gather<__nv_bfloat16>),
+                     unsigned(std::min<int64_t>(q.rows, 65536)), gg::moe::kW4GatherThreads, 0};
+    gather.grid_y = unsigned((steps * 16 + gg::moe::kW4GatherThreads - 1) / gg::moe::kW4GatherThreads);
+    return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), gg::moe::kW4Threads, v.smem, true}}, detail);
 }
 
 }  // namespace

@@ -1,5 +1,23 @@
 // Rows in expert order times their expert's 4-bit weights with group scales, for few rows an expert:
 //   out[r, n] = sum over groups g of scale[e, n, g] * sum_{k in g} (q[e, n, k] - zero[e, n, g]) x[row(r), k]
+//
+// What bounds it: the weights are read once, 1/2 byte each, and at HBM's rate that is 46 weights a
+// cycle and SM: the arithmetic that makes a 16-bit operand of each is what has to keep up. So each
+// weight is widened once, by the thread that owns its row, whatever the number of tokens, and
+// the products go to the tensor cores from Tensor Memory:
+//
+//   warp 0       TMA: 256 weight rows x 128 k (16 KB, 64-byte swizzle) a step into a shared-memory ring
+//   warp 3       a bulk copy of the tokens' 128 k a step (w4_gather lays them out so beforehand, see there)
+//   warps 4-19   four warpgroups, by half of the weight rows and by odd and even steps, a thread a row: 16 bytes at a
+//                time from the ring, widened to q - zero (exact) in registers, tcgen05.st into the group's A operand;
+//                before that tcgen05.ld of the products of its step before, and the fp32 sum with the group's scale (one
+//                scalar a thread)
+//   warps 1, 2   a half each: tcgen05.mma, D[weight row, token] = A (Tensor Memory) x B (tokens), a fresh accumulator
+//                a group
+//
+// Work split: the steps of all (expert, token chunk, 256-row tile) items in a row, dealt out to the CTAs in
+// equal contiguous ranges, so that one token through a few experts still keeps every SM reading. A tile that is
+// cut leaves fp32 partial sums in the workspace; the CTA that arrives last adds them in order of k.
 #pragma once
 
 #include "gg_moe.cuh"
@@ -7,36 +25,103 @@
 namespace gg {
 namespace moe {
 
-constexpr int kW4Warps = 8;
-constexpr int kW4Threads = kW4Warps * 32;
-constexpr int kW4Rows = 32;    // weight rows (output columns) of a work item
-constexpr int kW4Tokens = 32;  // rows of x of a work item
+constexpr int kW4Threads = 640;
+constexpr int kW4TileRows = 256;
+constexpr int kW4StepK = 128;
 constexpr int kW4MaxExperts = 1024;
+constexpr int kW4WeightBytes = kW4TileRows * kW4StepK / 2;
 
 struct W4Params {
     const void *x;           // [tokens or rows, k]
-    const uint8_t *qweight;  // [experts, n, k / 2], even k in the low four bits
     const void *scales;      // [experts, n, groups]
     const uint8_t *zeros;    // [experts, n, groups] or null = 8
     const int32_t *offsets;  // [experts + 1]
     const int32_t *src;      // [rows] slots, or null: row r reads x[r]
     void *out;               // [rows, n]
-    uint32_t *status;
-    int64_t rows, slots;  // slots: tokens * top_k
-    int n, k, groups, experts, top_k, tiles;
+    uint32_t *status;        // [0] status word, [2] timeouts of this launch
+    uint8_t *xs;             // [rows + 8 experts][steps] 256 bytes: the rows of x as the products read them
+    float *ws;               // [2 x grid][tokens of a chunk][256] partial sums
+    int32_t *counters;       // [grid] arrivals at a cut tile, 0 between launches
+    int64_t rows, slots;     // slots: tokens * top_k
+    uint64_t timeout_ns;
+    int n, k, groups, experts, top_k, tiles, steps;  // steps: of 128 k
+    int chunk;       // tokens of a chunk
 };
 
-// D (16 x 8, fp32) += A (16 x 16) B (16 x 8), 16-bit operands.
-template <class T>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// Tokens of a chunk: at most 32 (a thread holds a sum a token), and D needs a column a token and group of a step, 64 for
+// each warpgroup.
+template <int G> struct W4Cfg {
+    static constexpr int kSub = kW4StepK / G;  // groups a step
+    static constexpr int kTokens = kSub == 4 ? 16 : 32;
+    static constexpr int kStageBytes = kW4WeightBytes + kTokens * kW4StepK * 2;
+    static constexpr int kStages = 160 * 1024 / kStageBytes / 2 * 2;  // even: a stage is of odd steps or of even ones
+    static constexpr int kBars = 4 * kStages + 8;
+    static constexpr int kTableBytes = 2 * (kW4MaxExperts + 1) * 4;
+    static constexpr int kJoinBytes = kTokens * kW4TileRows * 4;
+    static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kJoinBytes + kBars * 8 + kTableBytes + 64;
+};
+
+// ---- instructions this kernel adds to gg_ptx.cuh's ----
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16],"
+                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32"
+                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+// One step's eight MMAs of 16 k for 128 weight rows: D (Tensor Memory) = A (Tensor Memory, two 16-bit values a column)
+// x B (shared memory, descriptors hi:lo and, for k from 64 on, hi:lo64), a D of its own for each group of G. Issued where pred != 0. In one block, with
+// addresses that are one add away from its operands: issued one by one from C++ the eight took 350 cycles, most of them in
+// address arithmetic.
+#define GG_W4_MMA(i, base, acc) \
+    "add.u32 d, %0, " #i "*16/%8*%7;\n\tadd.u32 a, %1, " #i "*8;\n\tadd.u32 l, %" #base ", (" #i "&3)*2;\n\tmov.b64 b, {l, %3};\n\t" \
+    "@q tcgen05.mma.cta_group::1.kind::f16 [d], [a], b, %4, " acc ";\n\t"
+template <int G, int kTokens>
+__device__ __forceinline__ void w4_mma_step(uint32_t d, uint32_t a, uint32_t lo, uint32_t lo64, uint32_t hi, uint32_t idesc, uint32_t pred) {
+#define GG_W4_STEP(a1, a2, a3, a4, a5, a6, a7)                                                                                          \
+    asm volatile("{\n\t.reg .pred q, t, f;\n\t.reg .b32 d, a, l;\n\t.reg .b64 b;\n\tsetp.ne.b32 q, %5, 0;\n\t"                            \
+                 "setp.eq.b32 t, 0, 0;\n\tsetp.ne.b32 f, 0, 0;\n\t" GG_W4_MMA(0, 2, "f") GG_W4_MMA(1, 2, a1) GG_W4_MMA(2, 2, a2) GG_W4_MMA(3, 2, a3) \
+                     GG_W4_MMA(4, 6, a4) GG_W4_MMA(5, 6, a5) GG_W4_MMA(6, 6, a6) GG_W4_MMA(7, 6, a7) "}" ::"r"(d),                                  \
+                 "r"(a), "r"(lo), "r"(hi), "r"(idesc), "r"(pred), "r"(lo64), "n"(kTokens), "n"(G)                         \
+                 : "memory")
+    if constexpr (G == 128)
+        GG_W4_STEP("t", "t", "t", "t", "t", "t", "t");
+    else if constexpr (G == 64)
+        GG_W4_STEP("t", "t", "t", "f", "t", "t", "t");
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        GG_W4_STEP("t", "f", "t", "f", "t", "f", "t");
+#undef GG_W4_STEP
+}
+#undef GG_W4_MMA
+// `bytes` (a multiple of 16) from global to shared memory, counted on an mbarrier; where pred != 0.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar, uint32_t pred) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+                 "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar), "r"(pred)
+                 : "memory");
+}
+__device__ __forceinline__ void named_sync(int bar, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 
 // Four bits as a 16-bit float without a conversion: placed in the low mantissa bits of a power of two
@@ -49,262 +134,525 @@ template <> struct W4Magic<__half> {
 template <> struct W4Magic<__nv_bfloat16> {
     static constexpr uint32_t kBias = 0x43004300u;
 };
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b, __half) {
+template <class T> __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t sub2<__half>(uint32_t a, uint32_t b) {
     const __half2 r = __hsub2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b, __nv_bfloat16) {
+template <> __device__ __forceinline__ uint32_t sub2<__nv_bfloat16>(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-template <class T> __device__ __forceinline__ uint32_t nibbles(uint32_t w, int s, uint32_t bias_zero) {
-    return sub2(((w >> (4 * s)) & 0x000f000fu) | W4Magic<T>::kBias, bias_zero, T());
+// The eight weights of a word as four pairs (k, k + 4): the pairs that masks and shifts of the whole word give. Each
+// eight values of x are put into that order in shared memory, so the products pair up.
+// (a & b) | c in one instruction: with b and c in registers the compiler does not make two of it.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
 }
-
-// 4 x 4 transpose of words within each quad of lanes: lane t's word c becomes lane c's word t.
-__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4]) {
-    const int t = threadIdx.x & 3;
-    {
-        const bool odd = t & 1;
-        const uint32_t s0 = odd ? w[0] : w[1], s1 = odd ? w[2] : w[3];
-        const uint32_t r0 = __shfl_xor_sync(0xffffffffu, s0, 1), r1 = __shfl_xor_sync(0xffffffffu, s1, 1);
-        if (odd) {
-            w[0] = r0;
-            w[2] = r1;
-        } else {
-            w[1] = r0;
-            w[3] = r1;
+struct W4Masks {
+    uint32_t low, high, bias;
+};
+template <class T> __device__ __forceinline__ W4Masks w4_masks() {
+    W4Masks m;
+    asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x00f000f0;\n\tmov.b32 %2, %3;"
+                 : "=r"(m.low), "=r"(m.high), "=r"(m.bias)
+                 : "n"(W4Magic<T>::kBias));
+    return m;
+}
+template <class T> __device__ __forceinline__ void widen(uint32_t w, uint32_t zero, const W4Masks &m, uint32_t *out) {
+    if constexpr (std::is_same<T, __half>::value) {
+        // fp16 has room for a nibble four bits up: 1024 + 16 q, and a 16th of it less 64 + zero is exact
+        const uint32_t low = zero + W4Magic<T>::kBias, high = (zero << 4) + 0x54005400u;  // 1024 + zero, 64 + zero
+        const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t v = w >> (8 * j), hi = and_or(v, m.high, m.bias);
+            out[2 * j] = sub2<T>(and_or(v, m.low, m.bias), low);
+            const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&hi), sixteenth, __hneg2(*reinterpret_cast<const __half2 *>(&high)));
+            out[2 * j + 1] = *reinterpret_cast<const uint32_t *>(&r);
         }
-    }
-    {
-        const bool high = t & 2;
-        const uint32_t s0 = high ? w[0] : w[2], s1 = high ? w[1] : w[3];
-        const uint32_t r0 = __shfl_xor_sync(0xffffffffu, s0, 2), r1 = __shfl_xor_sync(0xffffffffu, s1, 2);
-        if (high) {
-            w[0] = r0;
-            w[1] = r1;
-        } else {
-            w[2] = r0;
-            w[3] = r1;
-        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            out[j] = sub2<T>(and_or(w >> (4 * j), m.low, m.bias), zero + W4Magic<T>::kBias);
     }
 }
 
-__device__ __forceinline__ uint4 ld_stream(const void *p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+// Bounded wait of a converged warp, as wait_all, with a hint that lets the hardware hold the thread: twenty warps wait
+// here in turn, and their polling would take issue slots from the widening.
+__device__ __forceinline__ bool try_wait_hint(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity), "r"(10000)
+                 : "memory");
+    return ok != 0;
 }
-
-// Sum of one work item: 32 weight rows x up to 8 NT rows of x, over this warp's part of K.
-template <class T, int G, int NT>
-__device__ __forceinline__ void w4_item(const W4Params &p, int e, int n0, const int32_t *row_of, int c0, int c1, float (&total)[2][NT][4]) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const T *x = static_cast<const T *>(p.x);
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                total[m][j][i] = 0.0f;
-    const T *xrow[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int r = row_of[8 * j + g];
-        xrow[j] = r >= 0 ? x + int64_t(r) * p.k : nullptr;
-    }
-    for (int c = c0; c < c1; ++c) {
-        const int kc = c * 128;
-        uint32_t w[2][2][4];
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int n = n0 + 16 * m + 8 * h + g;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (n < p.n && kc + 32 * t < p.k)
-                    v = ld_stream(p.qweight + ((int64_t(e) * p.n + n) * p.k + kc) / 2 + 16 * t);
-                w[m][h][0] = v.x;
-                w[m][h][1] = v.y;
-                w[m][h][2] = v.z;
-                w[m][h][3] = v.w;
-                if (G < 128)
-                    quad_transpose(w[m][h]);
+__device__ __noinline__ inline bool w4_wait_slow(uint32_t bar, uint32_t parity, const Abort ab, uint32_t code) {
+    const uint64_t t0 = ptx::globaltimer();
+    for (uint32_t it = 1;; ++it) {
+        if (__all_sync(0xffffffffu, try_wait_hint(bar, parity)))
+            return true;
+        if ((it & 15u) == 0) {
+            bool stop = *ab.flag != 0u || *(volatile uint32_t *)ab.status != 0u;
+            if (!stop && ptx::globaltimer() - t0 > ab.timeout_ns) {
+                atomicCAS(ab.status, 0u, code);
+                stop = true;
             }
-        constexpr int kParts = 128 / G;  // groups of this stretch of 128
-#pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-            const int group = (kc + part * G) / G;
-            if (group >= p.groups)
-                break;
-            float scale[2][2];
-            uint32_t bias[2][2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int n = n0 + 16 * m + 8 * h + g;
-                    const int64_t at = (int64_t(e) * p.n + n) * p.groups + group;
-                    scale[m][h] = 0.0f;
-                    uint32_t z = 8;
-                    if (n < p.n) {
-                        scale[m][h] = to_f32(static_cast<const T *>(p.scales)[at]);
-                        if (p.zeros)
-                            z = p.zeros[at] & 15u;
-                    }
-                    bias[m][h] = W4Magic<T>::kBias + z * 0x00010001u;
-                }
-            float acc[2][NT][4] = {};
-#pragma unroll
-            for (int q = 0; q < 4 / kParts; ++q) {
-                const int word = part * (4 / kParts) + q;
-                const int kx = kc + (G < 128 ? 32 * word + 8 * t : 32 * t + 8 * word);
-                uint32_t b[NT][4];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (xrow[j] && kx < p.k)
-                        v = *reinterpret_cast<const uint4 *>(xrow[j] + kx);
-                    b[j][0] = __byte_perm(v.x, v.z, 0x5410);  // k, k + 4
-                    b[j][1] = __byte_perm(v.x, v.z, 0x7632);  // k + 1, k + 5
-                    b[j][2] = __byte_perm(v.y, v.w, 0x5410);
-                    b[j][3] = __byte_perm(v.y, v.w, 0x7632);
-                }
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int s = 0; s < 4; s += 2) {
-                        const uint32_t a0 = nibbles<T>(w[m][0][word], s, bias[m][0]), a1 = nibbles<T>(w[m][1][word], s, bias[m][1]);
-                        const uint32_t a2 = nibbles<T>(w[m][0][word], s + 1, bias[m][0]), a3 = nibbles<T>(w[m][1][word], s + 1, bias[m][1]);
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-                            mma16816<T>(acc[m][j], a0, a1, a2, a3, b[j][s], b[j][s + 1]);
-                    }
+            if (__any_sync(0xffffffffu, stop)) {
+                *ab.flag = 1u;
+                return false;
             }
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        total[m][j][i] = fmaf(scale[m][i >> 1], acc[m][j][i], total[m][j][i]);
         }
     }
 }
-
-template <class T, int G, int NT>
-__device__ __forceinline__ void w4_run(const W4Params &p, int e, int n0, const int32_t *row_of, int r0, int count, float *sums) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int chunks = (p.k + 127) / 128, per = (chunks + kW4Warps - 1) / kW4Warps;
-    float total[2][NT][4];
-    w4_item<T, G, NT>(p, e, n0, row_of, min(chunks, warp * per), min(chunks, (warp + 1) * per), total);
-    // the warps' sums, [warp][row of x][weight row]
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sums[(warp * 8 * NT + 8 * j + 2 * t + (i & 1)) * kW4Rows + 16 * m + 8 * (i >> 1) + g] = total[m][j][i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < count * kW4Rows; i += kW4Threads) {
-        const int r = i / kW4Rows, c = i % kW4Rows;
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kW4Warps; ++w)
-            s += sums[(w * 8 * NT + r) * kW4Rows + c];
-        if (n0 + c < p.n)
-            static_cast<T *>(p.out)[int64_t(r0 + r) * p.n + n0 + c] = from_f32<T>(s);
-    }
-    __syncthreads();
+__device__ __forceinline__ bool w4_wait(uint32_t bar, uint32_t parity, const Abort &ab, uint32_t code) {
+    return __all_sync(0xffffffffu, try_wait_hint(bar, parity)) || w4_wait_slow(bar, parity, ab, code);
+}
+// A look at a barrier ahead of the wait for it, so that its latency passes behind other work: `seen` goes to w4_wait_seen.
+__device__ __forceinline__ bool look(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool w4_wait_seen(bool seen, uint32_t bar, uint32_t parity, const Abort &ab, uint32_t code) {
+    return __all_sync(0xffffffffu, seen) || w4_wait_slow(bar, parity, ab, code);
 }
 
-template <class T, int G> __global__ void __launch_bounds__(kW4Threads) w4_rows(const W4Params p) {
-    __shared__ int start[kW4MaxExperts + 1];  // first row of each expert, checked
-    __shared__ int first[kW4MaxExperts + 1];  // row chunks of the experts before
-    __shared__ int32_t row_of[kW4Tokens];
-    __shared__ float sums[kW4Warps * kW4Tokens * kW4Rows];
-    ptx::griddep_wait();
-    ptx::griddep_launch_dependents();
-    const int E = p.experts, tid = threadIdx.x;
-    // offsets come from the device: each is held to the range the rows allow
-    for (int e = tid; e <= E; e += kW4Threads) {
-        const int64_t v = p.offsets[e];
-        const int64_t before = e ? p.offsets[e - 1] : 0;
+// The launch's work: items in expert order, an item's steps in order of k.
+struct W4Item {
+    int e, n0, r0, count;
+};
+__device__ __forceinline__ W4Item w4_item(const W4Params &p, const int *start, const int *first, int64_t item, int chunk_tokens) {
+    // the last expert whose first chunk's items start at or before the item
+    int lo = 0, hi = p.experts - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (int64_t(first[mid]) * p.tiles <= item)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const int chunks = first[lo + 1] - first[lo];
+    const int at = int(item - int64_t(first[lo]) * p.tiles);
+    const int tile = at / chunks, chunk = at - tile * chunks;
+    const int r0 = start[lo] + chunk * chunk_tokens;
+    return {lo, tile * kW4TileRows, r0, min(chunk_tokens, start[lo + 1] - r0)};
+}
+__device__ __forceinline__ int w4_cta_of(int64_t step, int64_t total, int ctas) { return int(((step + 1) * ctas - 1) / total); }
+
+// offsets come from the device: each is held to the range that the rows allow
+__device__ __forceinline__ void w4_starts(const W4Params &p, int *start) {
+    for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) {
+        const int64_t v = p.offsets[e], before = e ? p.offsets[e - 1] : 0;
         if (v < before || v > p.rows || before < 0)
             report(p.status, kSiteOffsets);
         start[e] = int(max(int64_t(0), min(v, p.rows)));
     }
+}
+
+// The rows of x in expert order, gathered through src, as the products read them: for each chunk of `chunk` tokens of an
+// expert and each step of 128 k a shared-memory image of B (K-major, two halves of 64 k, each a row of 128 bytes a token with the
+// 128-byte swizzle; token count rounded up to 8) so that one bulk copy loads it; eight values at a time in the order
+// in which masks and shifts take the weights out of a word. One 16-byte piece a thread. (Done by warps of the product
+// kernel instead, with cp.async and shared memory, this took them 1400 cycles a step at 16 tokens: twice what HBM allows.) Rows of
+// no expert are set to zero in out.
+constexpr int kW4GatherThreads = 128;
+template <class T> __global__ void __launch_bounds__(kW4GatherThreads) w4_gather(const __grid_constant__ W4Params p) {
+    __shared__ int start[kW4MaxExperts + 1];
+    ptx::griddep_wait();
+    // The product kernel may start now. It reads what earlier kernels wrote (offsets, scales, weights) without waiting for this one
+    // to end: every block of this one has passed its own wait by then. Before it reads xs it waits for this one.
+    ptx::griddep_launch_dependents();
+    w4_starts(p, start);
     __syncthreads();
-    {
-        const int per = (E + kW4Threads - 1) / kW4Threads;
-        int sum = 0;
-        for (int i = 0; i < per; ++i) {
-            const int e = tid * per + i;
-            if (e < E)
-                sum += (max(0, start[e + 1] - start[e]) + kW4Tokens - 1) / kW4Tokens;
+    const int piece = int(blockIdx.y) * kW4GatherThreads + int(threadIdx.x);  // of a row: 8 values
+    const int step = piece >> 4, half = (piece >> 3) & 1, c = piece & 7;
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        if (r < start[0] || r >= start[p.experts]) {
+            for (int col = piece; col < p.n; col += int(gridDim.y) * kW4GatherThreads)
+                static_cast<T *>(p.out)[r * p.n + col] = from_f32<T>(0.0f);
+            continue;
         }
-        int total, at = block_scan(sum, total);
-        for (int i = 0; i < per; ++i) {
-            const int e = tid * per + i;
-            if (e < E) {
-                first[e] = at;
-                at += (max(0, start[e + 1] - start[e]) + kW4Tokens - 1) / kW4Tokens;
-            }
-        }
-        if (tid == 0)
-            first[E] = total;
-        __syncthreads();
-    }
-    const int64_t items = int64_t(first[E]) * p.tiles;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        // the item's expert: the last one whose first chunk's items start at or before it
-        int lo = 0, hi = E - 1;
+        if (step >= p.steps)
+            continue;
+        int lo = 0, hi = p.experts - 1;  // the last expert that starts at or before the row
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (int64_t(first[mid]) * p.tiles <= item)
+            if (start[mid] <= r)
                 lo = mid;
             else
                 hi = mid - 1;
         }
-        const int e = lo;
-        const int chunks = first[e + 1] - first[e];
-        const int64_t at = item - int64_t(first[e]) * p.tiles;
-        const int tile = int(at / chunks), chunk = int(at % chunks);
-        const int r0 = start[e] + chunk * kW4Tokens, count = min(kW4Tokens, start[e + 1] - r0);
-        if (tid < kW4Tokens) {
-            int64_t r = -1;
-            if (tid < count) {
-                r = r0 + tid;
-                if (p.src) {
-                    const int s = p.src[r];
-                    if (s < 0 || s >= p.slots) {
-                        report(p.status, kSiteSrc);
-                        r = -1;
-                    } else {
-                        r = s / p.top_k;
-                    }
+        const int in_expert = int(r) - start[lo], i = in_expert % p.chunk;
+        const int count = (min(p.chunk, start[lo + 1] - (int(r) - i)) + 7) & ~7;
+        if (i >= count)
+            continue;  // falling offsets, reported
+        int64_t row = r;
+        if (p.src) {
+            const int s = p.src[r];
+            row = s < 0 || s >= p.slots ? -1 : s / p.top_k;
+            if (row < 0 && piece == 0)
+                report(p.status, kSiteSrc);
+        }
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row >= 0 && piece * 8 < p.k)
+            v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + row * p.k + piece * 8);
+        const int64_t base = int64_t(int(r) - i + 8 * lo) * p.steps * 256;
+        *reinterpret_cast<uint4 *>(p.xs + base + (int64_t(step * 2 + half) * count + i) * 128 + ((c ^ (i & 7)) << 4)) =
+            make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                       __byte_perm(v.y, v.w, 0x7632));
+    }
+}
+
+template <class T, int G>
+__global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ W4Params p) {
+    using C = W4Cfg<G>;
+    constexpr int kTokens = C::kTokens, kSub = C::kSub, kStages = C::kStages;
+    extern __shared__ __align__(1024) uint8_t w4_smem[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(w4_smem) + 1023) & ~uintptr_t(1023));
+    const uint32_t ring = ptx::smem_addr(smem);
+    // x tiles first (1024-byte aligned swizzle atoms), then the weights (16 KB each)
+    auto x_at = [&](int s) { return ring + uint32_t(s) * (kTokens * kW4StepK * 2); };
+    auto w_at = [&](int s) { return ring + uint32_t(kStages * kTokens * kW4StepK * 2 + s * kW4WeightBytes); };
+    float *join = reinterpret_cast<float *>(smem + kStages * C::kStageBytes);  // odd steps' sums at a piece's end
+    uint8_t *after = smem + kStages * C::kStageBytes + C::kJoinBytes;
+    const uint32_t bars = ptx::smem_addr(after);
+    auto wfull = [&](int s) { return bars + 8u * s; };
+    auto wempty = [&](int s) { return bars + 8u * (kStages + s); };
+    auto xfull = [&](int s) { return bars + 8u * (2 * kStages + s); };
+    auto xempty = [&](int s) { return bars + 8u * (3 * kStages + s); };
+    auto afull = [&](int h, int b) { return bars + 8u * (4 * kStages + 2 * h + b); };       // b: odd steps or even ones
+    auto done = [&](int h, int b) { return bars + 8u * (4 * kStages + 4 + 2 * h + b); };  // A read, D written
+    int *start = reinterpret_cast<int *>(after + C::kBars * 8);  // first row of each expert, checked
+    int *first = start + kW4MaxExperts + 1;                      // token chunks of the experts before
+    uint32_t *slots = reinterpret_cast<uint32_t *>(first + kW4MaxExperts + 1);
+    volatile uint32_t *abort_flag = slots + 1;
+    volatile int32_t *arrived = reinterpret_cast<volatile int32_t *>(slots + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            ptx::mbar_init(wfull(s), 1);
+            ptx::mbar_init(wempty(s), 8);
+            ptx::mbar_init(xfull(s), 1);
+            ptx::mbar_init(xempty(s), 2);
+        }
+        for (int i = 0; i < 4; ++i) {
+            ptx::mbar_init(afull(i >> 1, i & 1), 4);
+            ptx::mbar_init(done(i >> 1, i & 1), 1);
+        }
+        *abort_flag = 0u;
+        ptx::fence_mbar_init();
+        ptx::fence_proxy_async_smem();
+        ptx::prefetch_tmap(&tmap_w);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<1>(ptx::smem_addr(slots), 512);
+        ptx::tmem_relinquish<1>();
+    }
+    // No wait here: w4_gather lets this kernel start when all before it has completed.
+    ptx::fence_proxy_async_global();
+    ptx::griddep_launch_dependents();
+    const int E = p.experts;
+    w4_starts(p, start);
+    __syncthreads();
+    {
+        auto chunks_of = [&](int e) { return (max(0, start[e + 1] - start[e]) + kTokens - 1) / kTokens; };
+        const int per = (E + kW4Threads - 1) / kW4Threads;
+        int sum = 0;
+        for (int e = tid * per; e < min(E, (tid + 1) * per); ++e)
+            sum += chunks_of(e);
+        int total, at = block_scan(sum, total);
+        for (int e = tid * per; e < min(E, (tid + 1) * per); ++e) {
+            first[e] = at;
+            at += chunks_of(e);
+        }
+        if (tid == 0)
+            first[E] = total;
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = slots[0];
+    const int64_t total = int64_t(first[E]) * p.tiles * p.steps;  // steps of the launch
+    const int ctas = int(min(int64_t(gridDim.x), total));
+    const int cta = blockIdx.x;
+    const int64_t s_begin = cta < ctas ? total * cta / ctas : 0, s_end = cta < ctas ? total * (cta + 1) / ctas : 0;
+    const Abort ab{p.status + 2, abort_flag, p.timeout_ns};
+    auto a_col = [&](int h, int b) { return tmem + uint32_t(128 * h + 64 * b); };
+    auto d_col = [&](int h, int b) { return tmem + uint32_t(256 + 128 * h + 64 * b); };
+    // pieces of the range, item by item: f(item, first step, steps) in every role alike
+    auto pieces = [&](auto &&f) {
+        for (int64_t s = s_begin; s < s_end;) {
+            const int64_t item = s / p.steps;
+            const int k0 = int(s - item * p.steps), n = int(min(int64_t(p.steps - k0), s_end - s));
+            f(w4_item(p, start, first, item, kTokens), item, k0, n);
+            s += n;
+        }
+    };
+
+    if (warp == 0) {
+        const uint32_t leader = ptx::elect_one_sync();
+        int st = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        pieces([&](const W4Item &it, int64_t, int k0, int n) {
+            for (int j = 0; ok && j < n; ++j) {
+                ok = w4_wait(wempty(st), ph ^ 1u, ab, kStatusTimeout | kRoleProducer | uint32_t(st));
+                if (!ok)
+                    break;
+                ptx::mbar_arrive_expect_tx(wfull(st), kW4WeightBytes, leader);
+                ptx::tma_load_3d(w_at(st), &tmap_w, wfull(st), (k0 + j) * (kW4StepK / 2), it.n0, it.e, leader);
+                if (++st == kStages) {
+                    st = 0;
+                    ph ^= 1u;
                 }
             }
-            row_of[tid] = int(r);
-        }
-        __syncthreads();
-        if (count <= 8)
-            w4_run<T, G, 1>(p, e, tile * kW4Rows, row_of, r0, count, sums);
-        else if (count <= 16)
-            w4_run<T, G, 2>(p, e, tile * kW4Rows, row_of, r0, count, sums);
-        else
-            w4_run<T, G, 4>(p, e, tile * kW4Rows, row_of, r0, count, sums);
+        });
+    } else if (warp < 3) {
+        const int h = warp - 1;
+        const uint32_t leader = ptx::elect_one_sync();
+        int st = 0;
+        uint32_t ph = 0, par = 0;  // par: bit b, the phase of the half's A and D of odd or even steps
+        bool ok = true;
+        pieces([&](const W4Item &it, int64_t, int, int n) {
+            const uint32_t idesc = ptx::f16_idesc(Fmt<T>::kUmma, 128, (it.count + 15) & ~15);
+            const uint32_t atom = uint32_t(((it.count + 7) & ~7) * 128 / 16);  // between a step's halves of 64 k
+            const bool active = it.n0 + 128 * h < p.n;
+            for (int j = 0; ok && j < n; ++j) {
+                const int b = st & 1;
+                if (active) {
+                    const bool seen = look(xfull(st), ph);
+                    ok = w4_wait(afull(h, b), (par >> b) & 1u, ab, kStatusTimeout | kRoleMma | 0x40u | uint32_t(2 * h + b)) &&
+                         w4_wait_seen(seen, xfull(st), ph, ab, kStatusTimeout | kRoleMma | uint32_t(st));
+                    if (!ok)
+                        break;
+                    par ^= 1u << b;
+                    ptx::tc_fence_after();
+                    const uint64_t bd = ptx::sw128_kmajor_desc(x_at(st));
+                    w4_mma_step<G, kTokens>(d_col(h, b), a_col(h, b), uint32_t(bd), uint32_t(bd) + atom, uint32_t(bd >> 32), idesc, leader);
+                    ptx::umma_commit<1>(done(h, b), leader);
+                } else {
+                    ok = w4_wait(xfull(st), ph, ab, kStatusTimeout | kRoleMma | uint32_t(st));
+                    if (!ok)
+                        break;
+                }
+                ptx::umma_commit<1>(xempty(st), leader);
+                if (++st == kStages) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
+        });
+    } else if (warp == 3) {
+        const uint32_t leader = ptx::elect_one_sync();
+        int st = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        // what precedes the launch of w4_gather is done (see there), its own writes only now
+        ptx::griddep_wait();
+        ptx::fence_proxy_async_global();
+        pieces([&](const W4Item &it, int64_t, int k0, int n) {
+            const uint32_t bytes = uint32_t(((it.count + 7) & ~7) * 256);
+            const uint8_t *from = p.xs + (int64_t(it.r0 + 8 * it.e) * p.steps) * 256 + int64_t(k0) * bytes;
+            for (int j = 0; ok && j < n; ++j) {
+                ok = w4_wait(xempty(st), ph ^ 1u, ab, kStatusTimeout | kRoleProducer | 0x80u | uint32_t(st));
+                if (!ok)
+                    break;
+                ptx::mbar_arrive_expect_tx(xfull(st), bytes, leader);
+                bulk_load(x_at(st), from + int64_t(j) * bytes, bytes, xfull(st), leader);
+                if (++st == kStages) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
+        });
+    } else {
+        const int h = (warp - 4) >> 2 & 1, b = (warp - 4) >> 3;  // half; odd steps or even ones
+        const int row = (warp & 3) * 32 + lane;                  // row within the half
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const W4Masks masks = w4_masks<T>();
+        const uint32_t w_row = uint32_t((128 * h + row) * 64), w_swz = uint32_t(row >> 1) & 3u;
+        int st = 0;  // stage of the next step, of either kind
+        uint32_t ph = 0, par = 0;
+        bool ok = true;
+        pieces([&](const W4Item &it, int64_t item, int k0, int n) {
+            const int col = it.n0 + 128 * h + row;
+            const bool active = it.n0 + 128 * h < p.n;  // of the whole half
+            const int npad = (it.count + 15) & ~15;
+            const int64_t at = (int64_t(it.e) * p.n + min(col, p.n - 1)) * p.groups;
+            float sum[kTokens];
+#pragma unroll
+            for (int i = 0; i < kTokens; ++i)
+                sum[i] = 0.0f;
+            // The zeros of the next step, and the scales of the one whose products are being computed: loaded a step ahead.
+            uint32_t ze[kSub];
+            T sc[kSub] = {};
+            auto group = [&](int step, int s) { return kSub > 1 ? min(step * kSub + s, p.groups - 1) : step; };  // past the end x is zero
+            auto load_zeros = [&](int step) {
+#pragma unroll
+                for (int s = 0; s < kSub; ++s)
+                    ze[s] = p.zeros ? p.zeros[at + group(step, s)] : 8u;
+            };
+            // adds the products of this group's step before
+            auto take = [&]() {
+                ok = w4_wait(done(h, b), par, ab, kStatusTimeout | kRoleEpilogue | uint32_t(2 * h + b));
+                if (!ok)
+                    return;
+                par ^= 1u;
+                ptx::tc_fence_after();
+#pragma unroll
+                for (int s = 0; s < kSub; ++s) {
+                    const float scale = to_f32(sc[s]);
+#pragma unroll
+                    for (int q = 0; q < kTokens / 16; ++q)
+                        if (16 * q < npad) {
+                            uint32_t r[16];
+                            tmem_ld_x16(d_col(h, b) + lanes + uint32_t(s * kTokens + 16 * q), r);
+                            tmem_wait_ld16(r);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                sum[16 * q + i] = fmaf(scale, __uint_as_float(r[i]), sum[16 * q + i]);
+                        }
+                }
+            };
+            const int j0 = (st & 1) ^ b;  // the piece's first step of this kind
+            if (active && j0 < n)
+                load_zeros(k0 + j0);
+            if (j0 && n) {  // over a step of the other kind
+                if (++st == kStages) {
+                    st = 0;
+                    ph ^= 1u;
+                }
+            }
+            bool before = false;
+            for (int j = j0; ok && j < n; j += 2) {
+                uint32_t zero[kSub];
+                ok = w4_wait(wfull(st), ph, ab, kStatusTimeout | kRoleEpilogue | 0x80u | uint32_t(st));
+                if (!ok)
+                    break;
+                if (active) {
+                    if (before)
+                        take();  // and with it the A operand's and D's columns are free
+                    if (!ok)
+                        break;
+                    before = true;
+                    ptx::tc_fence_after();
+#pragma unroll
+                    for (int s = 0; s < kSub; ++s) {
+                        sc[s] = static_cast<const T *>(p.scales)[at + group(k0 + j, s)];
+                        zero[s] = (ze[s] & 15u) * 0x00010001u;
+                    }
+                    if (j + 2 < n && p.zeros)
+                        load_zeros(k0 + j + 2);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint4 v = lds128(w_at(st) + w_row + ((uint32_t(c) ^ w_swz) << 4));
+                        const uint32_t z = zero[c * 32 / G];
+                        uint32_t r[16];
+                        widen<T>(v.x, z, masks, r);
+                        widen<T>(v.y, z, masks, r + 4);
+                        widen<T>(v.z, z, masks, r + 8);
+                        widen<T>(v.w, z, masks, r + 12);
+                        tmem_st_x16(a_col(h, b) + lanes + uint32_t(16 * c), r);
+                    }
+                    tmem_wait_st();
+                    ptx::tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(wempty(st));
+                    if (active)
+                        ptx::mbar_arrive(afull(h, b));
+                }
+                // on to the next step of this kind
+                const int skip = min(2, n - j);
+                st += skip;
+                if (st >= kStages) {
+                    st -= kStages;
+                    ph ^= 1u;
+                }
+            }
+            if (ok && before)
+                take();
+            // odd steps' sums join the even ones'
+            named_sync(1, 512);
+            if (b == 1) {
+#pragma unroll
+                for (int i = 0; i < kTokens; ++i)
+                    if (i < it.count)
+                        join[i * kW4TileRows + 128 * h + row] = sum[i];
+            }
+            named_sync(1, 512);
+            if (b == 1)
+                return;
+#pragma unroll
+            for (int i = 0; i < kTokens; ++i)
+                if (i < it.count)
+                    sum[i] += join[i * kW4TileRows + 128 * h + row];
+            // ---- the piece's sums: to out, or where the tile is cut to the workspace ----
+            T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + col;
+            const bool there = ok && col < p.n;
+            if (n == p.steps) {
+                if (there) {
+#pragma unroll
+                    for (int i = 0; i < kTokens; ++i)
+                        if (i < it.count)
+                            out[int64_t(i) * p.n] = from_f32<T>(sum[i]);
+                }
+                return;
+            }
+            const int64_t a = item * p.steps;
+            const int c0 = w4_cta_of(a, total, ctas), c1 = w4_cta_of(a + p.steps - 1, total, ctas);
+            // slot 0 of a CTA: a piece that begins inside its tile; slot 1: one that begins its tile
+            auto slot = [&](int c) { return p.ws + int64_t(2 * c + (c == c0 ? 1 : 0)) * (kTokens * kW4TileRows) + 128 * h + row; };
+            if (there) {
+                float *mine = slot(cta);
+#pragma unroll
+                for (int i = 0; i < kTokens; ++i)
+                    if (i < it.count)
+                        __stcg(mine + i * kW4TileRows, sum[i]);
+            }
+            __threadfence();
+            named_sync(2, 256);
+            if (tid == 128)
+                *arrived = ok ? atomicAdd(p.counters + c0, 1) : -1;
+            named_sync(2, 256);
+            if (*arrived != c1 - c0)
+                return;
+            __threadfence();
+            if (tid == 128)
+                p.counters[c0] = 0;
+            if (there) {
+                for (int i = 0; i < it.count; ++i) {
+                    float s = 0.0f;
+                    for (int c = c0; c <= c1; ++c)
+                        s += __ldcg(slot(c) + i * kW4TileRows);
+                    out[int64_t(i) * p.n] = from_f32<T>(s);
+                }
+            }
+        });
     }
-    // rows of no expert are zero
-    const int64_t head = start[0], tail = start[E];
-    const int64_t none = head + (p.rows - tail);
-    for (int64_t i = blockIdx.x; i < none; i += gridDim.x) {
-        const int64_t r = i < head ? i : tail + (i - head);
-        for (int c = tid; c < p.n; c += kW4Threads)
-            static_cast<T *>(p.out)[r * p.n + c] = from_f32<T>(0.0f);
+
+    // ---- teardown ----
+    if (*abort_flag != 0u) {
+        // let copies and MMAs already issued drain before the memory they target goes away
+        const uint64_t t0 = ptx::globaltimer();
+        while (ptx::globaltimer() - t0 < 200000ull)
+            __nanosleep(1000);
+        atomicCAS(p.status, 0u, *reinterpret_cast<volatile uint32_t *>(p.status + 2));
     }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    if (warp == 1)
+        ptx::tmem_dealloc<1>(tmem, 512);
 }
 
 }  // namespace moe
