@@ -8,12 +8,17 @@
 //
 //   warp 0       TMA: 256 weight rows x 128 k (16 KB, 64-byte swizzle) a step into a shared-memory ring
 //   warp 3       a bulk copy of the tokens' 128 k a step (w4_gather lays them out so beforehand, see there)
-//   warps 4-19   four warpgroups, by half of the weight rows and by odd and even steps, a thread a row: 16 bytes at a
-//                time from the ring, widened to q - zero (exact) in registers, tcgen05.st into the group's A operand;
-//                before that tcgen05.ld of the products of its step before, and the fp32 sum with the group's scale (one
-//                scalar a thread)
+//   warps 4-11   a group of four for each half of the weight rows, a thread a row: 16 bytes at a time from the ring,
+//                widened to q - zero (exact) in registers, tcgen05.st into the half's next A operand
 //   warps 1, 2   a half each: tcgen05.mma, D[weight row, token] = A (Tensor Memory) x B (tokens), a fresh accumulator
 //                a group
+//   warps 12-19  a half each four: tcgen05.ld of a step's products and the fp32 sum with the group's scale (one scalar a
+//                thread); output
+//
+// Three A operands and two D a half keep the widening from waiting for the MMAs: beside four widening warps a scheduler the
+// MMA warp's eight take 530 cycles to issue, against 95 alone. (Also built: mma.sync m16n8k16 from registers, 54 / 139 / 693 us on
+// one token, 148 and 1024 rows: above 8 tokens it is bound by its own rate, 11 cycles a scheduler; and four
+// groups that widen odd and even steps with an A operand each and add up themselves, 45 / 104 / 361 us.)
 //
 // Work split: the steps of all (expert, token chunk, 256-row tile) items in a row, dealt out to the CTAs in
 // equal contiguous ranges, so that one token through a few experts still keeps every SM reading. A tile that is
@@ -48,17 +53,19 @@ struct W4Params {
     int chunk;       // tokens of a chunk
 };
 
-// Tokens of a chunk: at most 32 (a thread holds a sum a token), and D needs a column a token and group of a step, 64 for
-// each warpgroup.
+// Tokens of a chunk: at most 32 (a thread holds a sum a token). Tensor Memory's 512 columns hold for each half kA operands of
+// 64 columns and two D of a column a token and group of a step.
 template <int G> struct W4Cfg {
     static constexpr int kSub = kW4StepK / G;  // groups a step
     static constexpr int kTokens = kSub == 4 ? 16 : 32;
+    static constexpr int kA = kSub == 1 ? 3 : 2;
+    static constexpr int kD = kSub * kTokens;  // columns of a D
     static constexpr int kStageBytes = kW4WeightBytes + kTokens * kW4StepK * 2;
-    static constexpr int kStages = 160 * 1024 / kStageBytes / 2 * 2;  // even: a stage is of odd steps or of even ones
-    static constexpr int kBars = 4 * kStages + 8;
+    static constexpr int kStages = 6;  // a multiple of 2 and of kA: a stage always meets the same D and A
+    static constexpr int kBars = 4 * kStages + 4 * kA + 4;
     static constexpr int kTableBytes = 2 * (kW4MaxExperts + 1) * 4;
-    static constexpr int kJoinBytes = kTokens * kW4TileRows * 4;
-    static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kJoinBytes + kBars * 8 + kTableBytes + 64;
+    static_assert(2 * (64 * kA + 2 * kD) <= 512 && kStages % kA == 0 && kStages % 2 == 0, "Tensor Memory");
+    static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBars * 8 + kTableBytes + 64;
 };
 
 // ---- instructions this kernel adds to gg_ptx.cuh's ----
@@ -87,19 +94,19 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
                  : "memory");
 }
 // One step's eight MMAs of 16 k for 128 weight rows: D (Tensor Memory) = A (Tensor Memory, two 16-bit values a column)
-// x B (shared memory, descriptors hi:lo and, for k from 64 on, hi:lo64), a D of its own for each group of G. Issued where pred != 0. In one block, with
-// addresses that are one add away from its operands: issued one by one from C++ the eight took 350 cycles, most of them in
-// address arithmetic.
-#define GG_W4_MMA(i, base, acc) \
-    "add.u32 d, %0, " #i "*16/%8*%7;\n\tadd.u32 a, %1, " #i "*8;\n\tadd.u32 l, %" #base ", (" #i "&3)*2;\n\tmov.b64 b, {l, %3};\n\t" \
+// x B (shared memory, descriptor hi:lo), a D of its own for each group of G. Issued where pred != 0. In one block with
+// addresses one add away from its operands, in a loop that is not unrolled: with the stages unrolled and every address a constant the
+// warps of the other roles stalled three issue slots of four on the instruction cache.
+#define GG_W4_MMA(i, acc) \
+    "add.u32 d, %0, " #i "*16/%8*%7;\n\tadd.u32 a, %1, " #i "*8;\n\tadd.u32 l, %2, " #i "/4*%6+(" #i "&3)*2;\n\tmov.b64 b, {l, %3};\n\t" \
     "@q tcgen05.mma.cta_group::1.kind::f16 [d], [a], b, %4, " acc ";\n\t"
 template <int G, int kTokens>
-__device__ __forceinline__ void w4_mma_step(uint32_t d, uint32_t a, uint32_t lo, uint32_t lo64, uint32_t hi, uint32_t idesc, uint32_t pred) {
+__device__ __forceinline__ void w4_mma_step(uint32_t d, uint32_t a, uint32_t lo, uint32_t hi, uint32_t idesc, uint32_t pred) {
 #define GG_W4_STEP(a1, a2, a3, a4, a5, a6, a7)                                                                                          \
     asm volatile("{\n\t.reg .pred q, t, f;\n\t.reg .b32 d, a, l;\n\t.reg .b64 b;\n\tsetp.ne.b32 q, %5, 0;\n\t"                            \
-                 "setp.eq.b32 t, 0, 0;\n\tsetp.ne.b32 f, 0, 0;\n\t" GG_W4_MMA(0, 2, "f") GG_W4_MMA(1, 2, a1) GG_W4_MMA(2, 2, a2) GG_W4_MMA(3, 2, a3) \
-                     GG_W4_MMA(4, 6, a4) GG_W4_MMA(5, 6, a5) GG_W4_MMA(6, 6, a6) GG_W4_MMA(7, 6, a7) "}" ::"r"(d),                                  \
-                 "r"(a), "r"(lo), "r"(hi), "r"(idesc), "r"(pred), "r"(lo64), "n"(kTokens), "n"(G)                         \
+                 "setp.eq.b32 t, 0, 0;\n\tsetp.ne.b32 f, 0, 0;\n\t" GG_W4_MMA(0, "f") GG_W4_MMA(1, a1) GG_W4_MMA(2, a2) GG_W4_MMA(3, a3) \
+                     GG_W4_MMA(4, a4) GG_W4_MMA(5, a5) GG_W4_MMA(6, a6) GG_W4_MMA(7, a7) "}" ::"r"(d),                                  \
+                 "r"(a), "r"(lo), "r"(hi), "r"(idesc), "r"(pred), "n"(kTokens * 128 / 16), "n"(kTokens), "n"(G)                         \
                  : "memory")
     if constexpr (G == 128)
         GG_W4_STEP("t", "t", "t", "t", "t", "t", "t");
@@ -124,59 +131,46 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     return v;
 }
 
-// Four bits as a 16-bit float without a conversion: placed in the low mantissa bits of a power of two
-// (1024 in fp16, 128 in bf16) the value is that power + q, exactly; the power + zero is taken away again,
-// exactly too (all are integers below 256 resp. 2048).
-template <class T> struct W4Magic;
-template <> struct W4Magic<__half> {
-    static constexpr uint32_t kBias = 0x64006400u;
+// Four bits as a 16-bit float without a conversion or a power of two to put them on: where a format's exponent field is 0 or
+// 1 its value is linear in its bits, i * 2^-24 (fp16, i below 2048) and i * 2^-133 (bf16, i below 256). So a masked nibble in bits
+// 0-3 or 4-7 is q or 16 q times that unit, and one fma by a power of two brings both to (q - zero) * W4Unit::kValue, exactly (the
+// subnormal inputs are not flushed by it). bf16 cannot reach 1 in one multiplication, so its weights stay in units of 2^-9, which
+// the group's scale takes back in fp32. A word costs 5 instructions on the ALU pipe (one shift, four masks) and 4 on the
+// FMA pipe; with powers of two or'ed in, bf16 had needed 7 and 4: 150 ns for a warp's step of 32 rows x 128 k against 111.
+template <class T> struct W4Unit;
+template <> struct W4Unit<__half> {
+    static constexpr uint32_t kLow = 0x6c006c00u;     // 2^12: with kHigh 2^8, weights in units of 2^-12
+    static constexpr uint32_t kHigh = 0x5c005c00u;    // 2^8
+    static constexpr float kBack = 4096.0f;
 };
-template <> struct W4Magic<__nv_bfloat16> {
-    static constexpr uint32_t kBias = 0x43004300u;
+template <> struct W4Unit<__nv_bfloat16> {
+    static constexpr uint32_t kLow = 0x7d807d80u;     // 2^124
+    static constexpr uint32_t kHigh = 0x7b807b80u;    // 2^120
+    static constexpr float kBack = 512.0f;
 };
-template <class T> __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b);
-template <> __device__ __forceinline__ uint32_t sub2<__half>(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
-template <> __device__ __forceinline__ uint32_t sub2<__nv_bfloat16>(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
-// The eight weights of a word as four pairs (k, k + 4): the pairs that masks and shifts of the whole word give. Each
-// eight values of x are put into that order in shared memory, so the products pair up.
-// (a & b) | c in one instruction: with b and c in registers the compiler does not make two of it.
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+template <class T> __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c);
+template <> __device__ __forceinline__ uint32_t fma2<__half>(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
-struct W4Masks {
-    uint32_t low, high, bias;
-};
-template <class T> __device__ __forceinline__ W4Masks w4_masks() {
-    W4Masks m;
-    asm volatile("mov.b32 %0, 0x000f000f;\n\tmov.b32 %1, 0x00f000f0;\n\tmov.b32 %2, %3;"
-                 : "=r"(m.low), "=r"(m.high), "=r"(m.bias)
-                 : "n"(W4Magic<T>::kBias));
-    return m;
+template <> __device__ __forceinline__ uint32_t fma2<__nv_bfloat16>(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
 }
-template <class T> __device__ __forceinline__ void widen(uint32_t w, uint32_t zero, const W4Masks &m, uint32_t *out) {
-    if constexpr (std::is_same<T, __half>::value) {
-        // fp16 has room for a nibble four bits up: 1024 + 16 q, and a 16th of it less 64 + zero is exact
-        const uint32_t low = zero + W4Magic<T>::kBias, high = (zero << 4) + 0x54005400u;  // 1024 + zero, 64 + zero
-        const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
+// -zero in the weights' unit, twice.
+template <class T> __device__ __forceinline__ uint32_t w4_minus(uint32_t zero) {
+    return fma2<T>(zero * 0x00010001u, W4Unit<T>::kLow ^ 0x80008000u, 0u);
+}
+// The eight weights of a word as four pairs (k, k + 4): the pairs that masks and shifts of the whole word give. Each
+// eight values of x are put into that order, so the products pair up.
+template <class T> __device__ __forceinline__ void widen(uint32_t w, uint32_t minus, uint32_t *out) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t v = w >> (8 * j), hi = and_or(v, m.high, m.bias);
-            out[2 * j] = sub2<T>(and_or(v, m.low, m.bias), low);
-            const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&hi), sixteenth, __hneg2(*reinterpret_cast<const __half2 *>(&high)));
-            out[2 * j + 1] = *reinterpret_cast<const uint32_t *>(&r);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            out[j] = sub2<T>(and_or(w >> (4 * j), m.low, m.bias), zero + W4Magic<T>::kBias);
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t v = w >> (8 * j);
+        out[2 * j] = fma2<T>(v & 0x000f000fu, W4Unit<T>::kLow, minus);
+        out[2 * j + 1] = fma2<T>(v & 0x00f000f0u, W4Unit<T>::kHigh, minus);
     }
 }
 
@@ -258,7 +252,7 @@ __device__ __forceinline__ void w4_starts(const W4Params &p, int *start) {
 
 // The rows of x in expert order, gathered through src, as the products read them: for each chunk of `chunk` tokens of an
 // expert and each step of 128 k a shared-memory image of B (K-major, two halves of 64 k, each a row of 128 bytes a token with the
-// 128-byte swizzle; token count rounded up to 8) so that one bulk copy loads it; eight values at a time in the order
+// 128-byte swizzle; token count rounded up to 8) so that a bulk copy a half loads it; eight values at a time in the order
 // in which masks and shifts take the weights out of a word. One 16-byte piece a thread. (Done by warps of the product
 // kernel instead, with cp.async and shared memory, this took them 1400 cycles a step at 16 tokens: twice what HBM allows.) Rows of
 // no expert are set to zero in out.
@@ -313,22 +307,24 @@ template <class T> __global__ void __launch_bounds__(kW4GatherThreads) w4_gather
 template <class T, int G>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ W4Params p) {
     using C = W4Cfg<G>;
-    constexpr int kTokens = C::kTokens, kSub = C::kSub, kStages = C::kStages;
+    constexpr int kTokens = C::kTokens, kSub = C::kSub, kStages = C::kStages, kA = C::kA;
     extern __shared__ __align__(1024) uint8_t w4_smem[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(w4_smem) + 1023) & ~uintptr_t(1023));
     const uint32_t ring = ptx::smem_addr(smem);
     // x tiles first (1024-byte aligned swizzle atoms), then the weights (16 KB each)
     auto x_at = [&](int s) { return ring + uint32_t(s) * (kTokens * kW4StepK * 2); };
     auto w_at = [&](int s) { return ring + uint32_t(kStages * kTokens * kW4StepK * 2 + s * kW4WeightBytes); };
-    float *join = reinterpret_cast<float *>(smem + kStages * C::kStageBytes);  // odd steps' sums at a piece's end
-    uint8_t *after = smem + kStages * C::kStageBytes + C::kJoinBytes;
+    uint8_t *after = smem + kStages * C::kStageBytes;
     const uint32_t bars = ptx::smem_addr(after);
     auto wfull = [&](int s) { return bars + 8u * s; };
     auto wempty = [&](int s) { return bars + 8u * (kStages + s); };
     auto xfull = [&](int s) { return bars + 8u * (2 * kStages + s); };
     auto xempty = [&](int s) { return bars + 8u * (3 * kStages + s); };
-    auto afull = [&](int h, int b) { return bars + 8u * (4 * kStages + 2 * h + b); };       // b: odd steps or even ones
-    auto done = [&](int h, int b) { return bars + 8u * (4 * kStages + 4 + 2 * h + b); };  // A read, D written
+    auto afull = [&](int h, int a) { return bars + 8u * (4 * kStages + kA * h + a); };
+    auto done = [&](int h, int a) { return bars + 8u * (4 * kStages + kA * (2 + h) + a); };  // A read, D written
+    auto dempty = [&](int h, int d) { return bars + 8u * (4 * kStages + 4 * kA + 2 * h + d); };
+    auto a_col = [&](int h, int a) { return uint32_t(64 * (kA * h + a)); };
+    auto d_col = [&](int h, int d) { return uint32_t(128 * kA + C::kD * (2 * h + d)); };
     int *start = reinterpret_cast<int *>(after + C::kBars * 8);  // first row of each expert, checked
     int *first = start + kW4MaxExperts + 1;                      // token chunks of the experts before
     uint32_t *slots = reinterpret_cast<uint32_t *>(first + kW4MaxExperts + 1);
@@ -343,9 +339,13 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
             ptx::mbar_init(xfull(s), 1);
             ptx::mbar_init(xempty(s), 2);
         }
-        for (int i = 0; i < 4; ++i) {
-            ptx::mbar_init(afull(i >> 1, i & 1), 4);
-            ptx::mbar_init(done(i >> 1, i & 1), 1);
+        for (int h = 0; h < 2; ++h) {
+            for (int a = 0; a < kA; ++a) {
+                ptx::mbar_init(afull(h, a), 4);
+                ptx::mbar_init(done(h, a), 1);
+            }
+            for (int d = 0; d < 2; ++d)
+                ptx::mbar_init(dempty(h, d), 4);
         }
         *abort_flag = 0u;
         ptx::fence_mbar_init();
@@ -379,14 +379,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
-    const uint32_t tmem = slots[0];
+    const uint32_t tmem = slots[0];  // column 0: all of them are allocated
     const int64_t total = int64_t(first[E]) * p.tiles * p.steps;  // steps of the launch
     const int ctas = int(min(int64_t(gridDim.x), total));
     const int cta = blockIdx.x;
     const int64_t s_begin = cta < ctas ? total * cta / ctas : 0, s_end = cta < ctas ? total * (cta + 1) / ctas : 0;
     const Abort ab{p.status + 2, abort_flag, p.timeout_ns};
-    auto a_col = [&](int h, int b) { return tmem + uint32_t(128 * h + 64 * b); };
-    auto d_col = [&](int h, int b) { return tmem + uint32_t(256 + 128 * h + 64 * b); };
     // pieces of the range, item by item: f(item, first step, steps) in every role alike
     auto pieces = [&](auto &&f) {
         for (int64_t s = s_begin; s < s_end;) {
@@ -418,32 +416,35 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
     } else if (warp < 3) {
         const int h = warp - 1;
         const uint32_t leader = ptx::elect_one_sync();
-        int st = 0;
-        uint32_t ph = 0, par = 0;  // par: bit b, the phase of the half's A and D of odd or even steps
+        int st = 0, a = 0, d = 0;
+        uint32_t ph = 0, a_ph = 0, d_ph = 3;  // bits: the phases of each A's and D's next use
         bool ok = true;
         pieces([&](const W4Item &it, int64_t, int, int n) {
             const uint32_t idesc = ptx::f16_idesc(Fmt<T>::kUmma, 128, (it.count + 15) & ~15);
-            const uint32_t atom = uint32_t(((it.count + 7) & ~7) * 128 / 16);  // between a step's halves of 64 k
             const bool active = it.n0 + 128 * h < p.n;
+#pragma unroll 1
             for (int j = 0; ok && j < n; ++j) {
-                const int b = st & 1;
                 if (active) {
-                    const bool seen = look(xfull(st), ph);
-                    ok = w4_wait(afull(h, b), (par >> b) & 1u, ab, kStatusTimeout | kRoleMma | 0x40u | uint32_t(2 * h + b)) &&
-                         w4_wait_seen(seen, xfull(st), ph, ab, kStatusTimeout | kRoleMma | uint32_t(st));
+                    const bool s0 = look(xfull(st), ph), s1 = look(dempty(h, d), (d_ph >> d) & 1u);
+                    ok = w4_wait(afull(h, a), (a_ph >> a) & 1u, ab, kStatusTimeout | kRoleMma | 0x40u | uint32_t(a)) &&
+                         w4_wait_seen(s0, xfull(st), ph, ab, kStatusTimeout | kRoleMma | uint32_t(st)) &&
+                         w4_wait_seen(s1, dempty(h, d), (d_ph >> d) & 1u, ab, kStatusTimeout | kRoleMma | 0x60u | uint32_t(d));
                     if (!ok)
                         break;
-                    par ^= 1u << b;
+                    a_ph ^= 1u << a;
+                    d_ph ^= 1u << d;
                     ptx::tc_fence_after();
                     const uint64_t bd = ptx::sw128_kmajor_desc(x_at(st));
-                    w4_mma_step<G, kTokens>(d_col(h, b), a_col(h, b), uint32_t(bd), uint32_t(bd) + atom, uint32_t(bd >> 32), idesc, leader);
-                    ptx::umma_commit<1>(done(h, b), leader);
+                    w4_mma_step<G, kTokens>(d_col(h, d), a_col(h, a), uint32_t(bd), uint32_t(bd >> 32), idesc, leader);
+                    ptx::umma_commit<1>(done(h, a), leader);
                 } else {
                     ok = w4_wait(xfull(st), ph, ab, kStatusTimeout | kRoleMma | uint32_t(st));
                     if (!ok)
                         break;
                 }
                 ptx::umma_commit<1>(xempty(st), leader);
+                d ^= 1;
+                a = a + 1 == kA ? 0 : a + 1;
                 if (++st == kStages) {
                     st = 0;
                     ph ^= 1u;
@@ -466,136 +467,154 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
                 if (!ok)
                     break;
                 ptx::mbar_arrive_expect_tx(xfull(st), bytes, leader);
-                bulk_load(x_at(st), from + int64_t(j) * bytes, bytes, xfull(st), leader);
+                bulk_load(x_at(st), from, bytes / 2, xfull(st), leader);
+                bulk_load(x_at(st) + uint32_t(kTokens * 128), from + bytes / 2, bytes / 2, xfull(st), leader);
+                from += bytes;
                 if (++st == kStages) {
                     st = 0;
                     ph ^= 1u;
                 }
             }
         });
-    } else {
-        const int h = (warp - 4) >> 2 & 1, b = (warp - 4) >> 3;  // half; odd steps or even ones
-        const int row = (warp & 3) * 32 + lane;                  // row within the half
+    } else if (warp < 12) {
+        const int h = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;  // row within the half
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const W4Masks masks = w4_masks<T>();
-        const uint32_t w_row = uint32_t((128 * h + row) * 64), w_swz = uint32_t(row >> 1) & 3u;
-        int st = 0;  // stage of the next step, of either kind
-        uint32_t ph = 0, par = 0;
+        const uint32_t w_row = uint32_t((128 * h + row) * 64) + ((uint32_t(row >> 1) & 3u) << 4);
+        int st = 0, a = 0;                   // the next step's stage and A
+        uint32_t ph = 0, a_ph = (1u << kA) - 1u;  // a_ph: bit a, the phase of the A's last use
+        bool ok = true;
+        auto next = [&]() {
+            a = a + 1 == kA ? 0 : a + 1;
+            if (++st == kStages) {
+                st = 0;
+                ph ^= 1u;
+            }
+        };
+        pieces([&](const W4Item &it, int64_t, int k0, int n) {
+            if (it.n0 + 128 * h >= p.n) {  // no columns: on with the ring
+                for (int j = 0; ok && j < n; ++j) {
+                    ok = w4_wait(wfull(st), ph, ab, kStatusTimeout | kRoleEpilogue | 0x80u | uint32_t(st));
+                    if (ok && lane == 0)
+                        ptx::mbar_arrive(wempty(st));
+                    next();
+                }
+                return;
+            }
+            const uint8_t *zeros = p.zeros ? p.zeros + (int64_t(it.e) * p.n + min(it.n0 + 128 * h + row, p.n - 1)) * p.groups : nullptr;
+            uint32_t ze[kSub];  // of the next step
+            auto load_zeros = [&](int step) {
+#pragma unroll
+                for (int s = 0; s < kSub; ++s)
+                    ze[s] = zeros[kSub > 1 ? min(step * kSub + s, p.groups - 1) : step];  // past the end x is zero
+            };
+#pragma unroll
+            for (int s = 0; s < kSub; ++s)
+                ze[s] = 8u;
+            if (zeros)
+                load_zeros(k0);
+            for (int j = 0; j < n; ++j) {
+                const uint32_t a_par = (a_ph >> a) & 1u;
+                const bool seen = look(done(h, a), a_par);
+                ok = w4_wait(wfull(st), ph, ab, kStatusTimeout | kRoleEpilogue | 0x80u | uint32_t(st));
+                if (!ok)
+                    return;
+                const uint32_t from = w_at(st) + w_row, to = a_col(h, a) + lanes;
+                uint32_t minus[kSub];
+#pragma unroll
+                for (int s = 0; s < kSub; ++s)
+                    minus[s] = w4_minus<T>(ze[s] & 15u);
+                if (zeros && j + 1 < n)
+                    load_zeros(k0 + j + 1);
+                // the MMAs that read this A last are done
+                ok = w4_wait_seen(seen, done(h, a), a_par, ab, kStatusTimeout | kRoleEpilogue | 0x40u | uint32_t(a));
+                if (!ok)
+                    return;
+                ptx::tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint4 v = lds128(from ^ uint32_t(c << 4));
+                    const uint32_t z = minus[c * 32 / G];
+                    uint32_t r[16];
+                    widen<T>(v.x, z, r);
+                    widen<T>(v.y, z, r + 4);
+                    widen<T>(v.z, z, r + 8);
+                    widen<T>(v.w, z, r + 12);
+                    tmem_st_x16(to + uint32_t(16 * c), r);
+                }
+                tmem_wait_st();
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(wempty(st));
+                    ptx::mbar_arrive(afull(h, a));
+                }
+                a_ph ^= 1u << a;
+                next();
+            }
+        });
+    } else {
+        const int h = (warp - 12) >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        int a = 0, d = 0;
+        uint32_t a_ph = 0;
         bool ok = true;
         pieces([&](const W4Item &it, int64_t item, int k0, int n) {
             const int col = it.n0 + 128 * h + row;
-            const bool active = it.n0 + 128 * h < p.n;  // of the whole half
             const int npad = (it.count + 15) & ~15;
-            const int64_t at = (int64_t(it.e) * p.n + min(col, p.n - 1)) * p.groups;
+            const T *scales = static_cast<const T *>(p.scales) + (int64_t(it.e) * p.n + min(col, p.n - 1)) * p.groups;
             float sum[kTokens];
 #pragma unroll
             for (int i = 0; i < kTokens; ++i)
                 sum[i] = 0.0f;
-            // The zeros of the next step, and the scales of the one whose products are being computed: loaded a step ahead.
-            uint32_t ze[kSub];
-            T sc[kSub] = {};
-            auto group = [&](int step, int s) { return kSub > 1 ? min(step * kSub + s, p.groups - 1) : step; };  // past the end x is zero
-            auto load_zeros = [&](int step) {
+            // the scales are loaded two steps ahead: [0] for even steps of the piece, [1] for odd ones
+            T sc[2][kSub] = {};
+            auto load_scales = [&](int step, T(&v)[kSub]) {
 #pragma unroll
                 for (int s = 0; s < kSub; ++s)
-                    ze[s] = p.zeros ? p.zeros[at + group(step, s)] : 8u;
+                    v[s] = scales[kSub > 1 ? min(step * kSub + s, p.groups - 1) : step];
             };
-            // adds the products of this group's step before
-            auto take = [&]() {
-                ok = w4_wait(done(h, b), par, ab, kStatusTimeout | kRoleEpilogue | uint32_t(2 * h + b));
+            auto take = [&](int j, T(&v)[kSub]) {
+                ok = w4_wait(done(h, a), (a_ph >> a) & 1u, ab, kStatusTimeout | kRoleEpilogue | uint32_t(a));
                 if (!ok)
                     return;
-                par ^= 1u;
+                a_ph ^= 1u << a;
                 ptx::tc_fence_after();
 #pragma unroll
                 for (int s = 0; s < kSub; ++s) {
-                    const float scale = to_f32(sc[s]);
+                    const float scale = to_f32(v[s]) * W4Unit<T>::kBack;
 #pragma unroll
                     for (int q = 0; q < kTokens / 16; ++q)
                         if (16 * q < npad) {
                             uint32_t r[16];
-                            tmem_ld_x16(d_col(h, b) + lanes + uint32_t(s * kTokens + 16 * q), r);
+                            tmem_ld_x16(d_col(h, d) + lanes + uint32_t(s * kTokens + 16 * q), r);
                             tmem_wait_ld16(r);
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
                                 sum[16 * q + i] = fmaf(scale, __uint_as_float(r[i]), sum[16 * q + i]);
                         }
                 }
-            };
-            const int j0 = (st & 1) ^ b;  // the piece's first step of this kind
-            if (active && j0 < n)
-                load_zeros(k0 + j0);
-            if (j0 && n) {  // over a step of the other kind
-                if (++st == kStages) {
-                    st = 0;
-                    ph ^= 1u;
-                }
-            }
-            bool before = false;
-            for (int j = j0; ok && j < n; j += 2) {
-                uint32_t zero[kSub];
-                ok = w4_wait(wfull(st), ph, ab, kStatusTimeout | kRoleEpilogue | 0x80u | uint32_t(st));
-                if (!ok)
-                    break;
-                if (active) {
-                    if (before)
-                        take();  // and with it the A operand's and D's columns are free
-                    if (!ok)
-                        break;
-                    before = true;
-                    ptx::tc_fence_after();
-#pragma unroll
-                    for (int s = 0; s < kSub; ++s) {
-                        sc[s] = static_cast<const T *>(p.scales)[at + group(k0 + j, s)];
-                        zero[s] = (ze[s] & 15u) * 0x00010001u;
-                    }
-                    if (j + 2 < n && p.zeros)
-                        load_zeros(k0 + j + 2);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const uint4 v = lds128(w_at(st) + w_row + ((uint32_t(c) ^ w_swz) << 4));
-                        const uint32_t z = zero[c * 32 / G];
-                        uint32_t r[16];
-                        widen<T>(v.x, z, masks, r);
-                        widen<T>(v.y, z, masks, r + 4);
-                        widen<T>(v.z, z, masks, r + 8);
-                        widen<T>(v.w, z, masks, r + 12);
-                        tmem_st_x16(a_col(h, b) + lanes + uint32_t(16 * c), r);
-                    }
-                    tmem_wait_st();
-                    ptx::tc_fence_before();
-                }
+                ptx::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    ptx::mbar_arrive(wempty(st));
-                    if (active)
-                        ptx::mbar_arrive(afull(h, b));
+                if (lane == 0)
+                    ptx::mbar_arrive(dempty(h, d));
+                if (j + 2 < n)
+                    load_scales(k0 + j + 2, v);
+                d ^= 1;
+                a = a + 1 == kA ? 0 : a + 1;
+            };
+            if (it.n0 + 128 * h < p.n) {
+                load_scales(k0, sc[0]);
+                if (n > 1)
+                    load_scales(k0 + 1, sc[1]);
+                for (int j = 0; ok && j < n; j += 2) {
+                    take(j, sc[0]);
+                    if (ok && j + 1 < n)
+                        take(j + 1, sc[1]);
                 }
-                // on to the next step of this kind
-                const int skip = min(2, n - j);
-                st += skip;
-                if (st >= kStages) {
-                    st -= kStages;
-                    ph ^= 1u;
-                }
+            } else {
+                a = (a + n) % kA;
+                d = (d + n) & 1;
             }
-            if (ok && before)
-                take();
-            // odd steps' sums join the even ones'
-            named_sync(1, 512);
-            if (b == 1) {
-#pragma unroll
-                for (int i = 0; i < kTokens; ++i)
-                    if (i < it.count)
-                        join[i * kW4TileRows + 128 * h + row] = sum[i];
-            }
-            named_sync(1, 512);
-            if (b == 1)
-                return;
-#pragma unroll
-            for (int i = 0; i < kTokens; ++i)
-                if (i < it.count)
-                    sum[i] += join[i * kW4TileRows + 128 * h + row];
             // ---- the piece's sums: to out, or where the tile is cut to the workspace ----
             T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + col;
             const bool there = ok && col < p.n;
@@ -621,13 +640,13 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
             }
             __threadfence();
             named_sync(2, 256);
-            if (tid == 128)
+            if (tid == 384)
                 *arrived = ok ? atomicAdd(p.counters + c0, 1) : -1;
             named_sync(2, 256);
             if (*arrived != c1 - c0)
                 return;
             __threadfence();
-            if (tid == 128)
+            if (tid == 384)
                 p.counters[c0] = 0;
             if (there) {
                 for (int i = 0; i < it.count; ++i) {
