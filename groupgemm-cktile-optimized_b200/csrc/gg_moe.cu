@@ -362,17 +362,22 @@ int prepare_permute(gg_handle *h, const gg_permute_problem &q, int32_t op, gg_st
 
 // ---- 4-bit products ----
 
-struct W4Variant {
-    const void *fn;
+struct W4Form {
+    const void *fn, *gather;
     int tokens;  // of a chunk
+    int threads, ctas_per_sm;
     size_t smem;
 };
-template <class T, int G> W4Variant w4_variant() {
-    using C = gg::moe::W4Cfg<G>;
-    return {reinterpret_cast<const void *>(&gg::moe::w4_rows<T, G>), C::kTokens, C::kSmemBytes};
+template <class T, int G> W4Form w4_form(bool few, bool zeros) {
+    using namespace gg::moe;
+    if (few)
+        return {zeros ? reinterpret_cast<const void *>(&w4_few<T, G, true>) : reinterpret_cast<const void *>(&w4_few<T, G, false>),
+                reinterpret_cast<const void *>(&w4_gather<T, true>), kW4FewTokens, kW4FewThreads, 2, kW4FewSmem};
+    return {reinterpret_cast<const void *>(&w4_many<T, G>), reinterpret_cast<const void *>(&w4_gather<T, false>), W4Many<G>::kTokens,
+            kW4ManyThreads, 1, W4Many<G>::kSmemBytes};
 }
-template <class T> W4Variant w4_variant(int group) {
-    return group == 32 ? w4_variant<T, 32>() : group == 64 ? w4_variant<T, 64>() : w4_variant<T, 128>();
+template <class T> W4Form w4_form(int group, bool few, bool zeros) {
+    return group == 32 ? w4_form<T, 32>(few, zeros) : group == 64 ? w4_form<T, 64>(few, zeros) : w4_form<T, 128>(few, zeros);
 }
 
 int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *why, size_t why_len) {
@@ -399,21 +404,29 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
-    const W4Variant v = q.dtype == GG_FP16 ? w4_variant<__half>(q.group_size) : w4_variant<__nv_bfloat16>(q.group_size);
+    // Up to 6 rows an expert on average, chunks of 8 with mma.sync; above, chunks of 32 with tcgen05. Measured on 8 experts of 4096 x
+    // 7168, us more for each further 117 MB of weights, few / many: 1 row an expert 22 / 28, 8 rows 24 / 29, 16 rows 42 / 30 (the weights
+    // are then widened twice by the first); a mean of 6 already has experts with more than 8.
+    const bool few = q.rows <= 6 * int64_t(q.experts);
+    const W4Form v = q.dtype == GG_FP16 ? w4_form<__half>(q.group_size, few, q.zeros) : w4_form<__nv_bfloat16>(q.group_size, few, q.zeros);
     GG_CUDA(h, cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(v.smem)));
     if (const int rc = encode_bytes_3d(h, q.qweight, q.k / 2, q.n, q.experts, gg::moe::kW4StepK / 2, gg::moe::kW4TileRows))
         return rc;
-    const int blocks = q.rows > 0 ? num_sms : 0;
+    const int ctas = v.ctas_per_sm * num_sms;
+    const int blocks = q.rows > 0 ? ctas : 0;
     const int64_t steps = (q.k + gg::moe::kW4StepK - 1) / gg::moe::kW4StepK;
-    const size_t sums = size_t(2 * num_sms) * size_t(v.tokens) * gg::moe::kW4TileRows * 4;
-    if (const int rc = reserve(h, sums + size_t(q.rows + 8 * int64_t(q.experts)) * size_t(steps) * 256))
+    const size_t sums = size_t(2 * ctas) * size_t(v.tokens) * gg::moe::kW4TileRows * 4;
+    if (const int rc = reserve(h, sums + size_t(q.rows + 8 * int64_t(q.experts)) * size_t(steps) * gg::moe::kW4TokenBytes))
         return rc;
-    if (const int rc = reserve_counters(h, size_t(num_sms) * 4, stream))
+    if (const int rc = reserve_counters(h, size_t(ctas) * 4, stream))
         return rc;
     gg::moe::W4Params p{};
     p.x = q.x;
     p.scales = q.scales;
     p.zeros = static_cast<const uint8_t *>(q.zeros);
+    const int64_t metas = int64_t(q.experts) * q.n * ((q.k + q.group_size - 1) / q.group_size);
+    p.scales_end = static_cast<const uint8_t *>(q.scales) + 2 * metas;  // n is a multiple of 8
+    p.zeros_end = static_cast<const uint8_t *>(q.zeros) + metas;
     p.offsets = q.offsets;
     p.src = q.src;
     p.out = q.out;
@@ -434,13 +447,11 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     p.timeout_ns = uint64_t(h->opt_timeout_ms) * 1000000u;
     set_params(h, p);
     char detail[160];
-    std::snprintf(detail, sizeof(detail), "gg_w4<%s> n=%lld k=%lld group=%d blocks=%d", type_name(q.dtype), static_cast<long long>(q.n),
-                  static_cast<long long>(q.k), q.group_size, blocks);
-    MoeLaunch gather{q.dtype == GG_FP16 ? reinterpret_cast<const void *>(&gg::moe::w4_gather<__half>)
-                                        : reinterpret_cast<const void *>(&gg::moe::w4_gather<__nv_bfloat16>),
-                     unsigned(std::min<int64_t>(q.rows, 65536)), gg::moe::kW4GatherThreads, 0};
+    std::snprintf(detail, sizeof(detail), "gg_w4<%s,%s> n=%lld k=%lld group=%d blocks=%d", type_name(q.dtype), few ? "few" : "many",
+                  static_cast<long long>(q.n), static_cast<long long>(q.k), q.group_size, blocks);
+    MoeLaunch gather{v.gather, unsigned(std::min<int64_t>(q.rows, 65536)), gg::moe::kW4GatherThreads, 0};
     gather.grid_y = unsigned((steps * 16 + gg::moe::kW4GatherThreads - 1) / gg::moe::kW4GatherThreads);
-    return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), gg::moe::kW4Threads, v.smem, true}}, detail);
+    return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), unsigned(v.threads), v.smem, true}}, detail);
 }
 
 }  // namespace

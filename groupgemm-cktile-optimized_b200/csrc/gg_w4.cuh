@@ -1,28 +1,17 @@
 // Rows in expert order times their expert's 4-bit weights with group scales, for few rows an expert:
 //   out[r, n] = sum over groups g of scale[e, n, g] * sum_{k in g} (q[e, n, k] - zero[e, n, g]) x[row(r), k]
 //
-// What bounds it: the weights are read once, 1/2 byte each, and at HBM's rate that is 46 weights a
-// cycle and SM: the arithmetic that makes a 16-bit operand of each is what has to keep up. So each
-// weight is widened once, by the thread that owns its row, whatever the number of tokens, and
-// the products go to the tensor cores from Tensor Memory:
+// What bounds it: the weights are read once, half a byte each; at HBM's rate that leaves 712 cycles an SM for a step of 256 weight
+// rows x 128 k. What has to fit into them is the widening of each weight into a 16-bit operand, 9 instructions a word of 8, 5 of
+// them on the ALU pipe, which starts 64 lanes a cycle (106 ns for a warp's share of a step, 32 rows: 420 of the 712 cycles), and
+// the products. So each weight is widened once, whatever the number of tokens, and whatever else is on the way is kept small. Two
+// forms, by how many rows an expert has (w4_few and w4_many, each explained there), share:
 //
-//   warp 0       TMA: 256 weight rows x 128 k (16 KB, 64-byte swizzle) a step into a shared-memory ring
-//   warp 3       a bulk copy of the tokens' 128 k a step (w4_gather lays them out so beforehand, see there)
-//   warps 4-11   a group of four for each half of the weight rows, a thread a row: 16 bytes at a time from the ring,
-//                widened to q - zero (exact) in registers, tcgen05.st into the half's next A operand
-//   warps 1, 2   a half each: tcgen05.mma, D[weight row, token] = A (Tensor Memory) x B (tokens), a fresh accumulator
-//                a group
-//   warps 12-19  a half each four: tcgen05.ld of a step's products and the fp32 sum with the group's scale (one scalar a
-//                thread); output
-//
-// Three A operands and two D a half keep the widening from waiting for the MMAs: beside four widening warps a scheduler the
-// MMA warp's eight take 530 cycles to issue, against 95 alone. (Also built: mma.sync m16n8k16 from registers, 54 / 139 / 693 us on
-// one token, 148 and 1024 rows: above 8 tokens it is bound by its own rate, 11 cycles a scheduler; and four
-// groups that widen odd and even steps with an A operand each and add up themselves, 45 / 104 / 361 us.)
-//
-// Work split: the steps of all (expert, token chunk, 256-row tile) items in a row, dealt out to the CTAs in
-// equal contiguous ranges, so that one token through a few experts still keeps every SM reading. A tile that is
-// cut leaves fp32 partial sums in the workspace; the CTA that arrives last adds them in order of k.
+//   Work split: the steps of all (expert, token chunk, 256-row tile) items in a row, dealt out to the CTAs in equal contiguous
+//   ranges, so that one token through a few experts still keeps every SM reading. A tile that is cut leaves fp32 partial sums in
+//   the workspace; the CTA that arrives last adds them in order of k. A CTA looks after its cut tiles (two at most) when
+//   all its steps are done: fence, arrival and sum took 3 us where they stood between two pieces.
+//   w4_gather: the rows of x in expert order, laid out as the products read them, so that bulk copies load them.
 #pragma once
 
 #include "gg_moe.cuh"
@@ -30,93 +19,30 @@
 namespace gg {
 namespace moe {
 
-constexpr int kW4Threads = 640;
 constexpr int kW4TileRows = 256;
 constexpr int kW4StepK = 128;
 constexpr int kW4MaxExperts = 1024;
-constexpr int kW4WeightBytes = kW4TileRows * kW4StepK / 2;
+constexpr int kW4WeightBytes = kW4TileRows * kW4StepK / 2;  // of a step
+constexpr int kW4TokenBytes = kW4StepK * 2;                 // of a token and step
 
 struct W4Params {
     const void *x;           // [tokens or rows, k]
     const void *scales;      // [experts, n, groups]
     const uint8_t *zeros;    // [experts, n, groups] or null = 8
+    const void *scales_end, *zeros_end;
     const int32_t *offsets;  // [experts + 1]
     const int32_t *src;      // [rows] slots, or null: row r reads x[r]
     void *out;               // [rows, n]
     uint32_t *status;        // [0] status word, [2] timeouts of this launch
-    uint8_t *xs;             // [rows + 8 experts][steps] 256 bytes: the rows of x as the products read them
+    uint8_t *xs;             // [rows + 8 experts][steps] 256 bytes: the rows of x as the products read them (w4_gather)
     float *ws;               // [2 x grid][tokens of a chunk][256] partial sums
     int32_t *counters;       // [grid] arrivals at a cut tile, 0 between launches
     int64_t rows, slots;     // slots: tokens * top_k
     uint64_t timeout_ns;
     int n, k, groups, experts, top_k, tiles, steps;  // steps: of 128 k
-    int chunk;       // tokens of a chunk
+    int chunk;  // tokens of a chunk
 };
 
-// Tokens of a chunk: at most 32 (a thread holds a sum a token). Tensor Memory's 512 columns hold for each half kA operands of
-// 64 columns and two D of a column a token and group of a step.
-template <int G> struct W4Cfg {
-    static constexpr int kSub = kW4StepK / G;  // groups a step
-    static constexpr int kTokens = kSub == 4 ? 16 : 32;
-    static constexpr int kA = kSub == 1 ? 3 : 2;
-    static constexpr int kD = kSub * kTokens;  // columns of a D
-    static constexpr int kStageBytes = kW4WeightBytes + kTokens * kW4StepK * 2;
-    static constexpr int kStages = 6;  // a multiple of 2 and of kA: a stage always meets the same D and A
-    static constexpr int kBars = 4 * kStages + 4 * kA + 4;
-    static constexpr int kTableBytes = 2 * (kW4MaxExperts + 1) * 4;
-    static_assert(2 * (64 * kA + 2 * kD) <= 512 && kStages % kA == 0 && kStages % 2 == 0, "Tensor Memory");
-    static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBars * 8 + kTableBytes + 64;
-};
-
-// ---- instructions this kernel adds to gg_ptx.cuh's ----
-
-__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16],"
-                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
-                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32"
-                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
-// One step's eight MMAs of 16 k for 128 weight rows: D (Tensor Memory) = A (Tensor Memory, two 16-bit values a column)
-// x B (shared memory, descriptor hi:lo), a D of its own for each group of G. Issued where pred != 0. In one block with
-// addresses one add away from its operands, in a loop that is not unrolled: with the stages unrolled and every address a constant the
-// warps of the other roles stalled three issue slots of four on the instruction cache.
-#define GG_W4_MMA(i, acc) \
-    "add.u32 d, %0, " #i "*16/%8*%7;\n\tadd.u32 a, %1, " #i "*8;\n\tadd.u32 l, %2, " #i "/4*%6+(" #i "&3)*2;\n\tmov.b64 b, {l, %3};\n\t" \
-    "@q tcgen05.mma.cta_group::1.kind::f16 [d], [a], b, %4, " acc ";\n\t"
-template <int G, int kTokens>
-__device__ __forceinline__ void w4_mma_step(uint32_t d, uint32_t a, uint32_t lo, uint32_t hi, uint32_t idesc, uint32_t pred) {
-#define GG_W4_STEP(a1, a2, a3, a4, a5, a6, a7)                                                                                          \
-    asm volatile("{\n\t.reg .pred q, t, f;\n\t.reg .b32 d, a, l;\n\t.reg .b64 b;\n\tsetp.ne.b32 q, %5, 0;\n\t"                            \
-                 "setp.eq.b32 t, 0, 0;\n\tsetp.ne.b32 f, 0, 0;\n\t" GG_W4_MMA(0, "f") GG_W4_MMA(1, a1) GG_W4_MMA(2, a2) GG_W4_MMA(3, a3) \
-                     GG_W4_MMA(4, a4) GG_W4_MMA(5, a5) GG_W4_MMA(6, a6) GG_W4_MMA(7, a7) "}" ::"r"(d),                                  \
-                 "r"(a), "r"(lo), "r"(hi), "r"(idesc), "r"(pred), "n"(kTokens * 128 / 16), "n"(kTokens), "n"(G)                         \
-                 : "memory")
-    if constexpr (G == 128)
-        GG_W4_STEP("t", "t", "t", "t", "t", "t", "t");
-    else if constexpr (G == 64)
-        GG_W4_STEP("t", "t", "t", "f", "t", "t", "t");
-    else
-        GG_W4_STEP("t", "f", "t", "f", "t", "f", "t");
-#undef GG_W4_STEP
-}
-#undef GG_W4_MMA
 // `bytes` (a multiple of 16) from global to shared memory, counted on an mbarrier; where pred != 0.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar, uint32_t pred) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
@@ -218,55 +144,142 @@ __device__ __forceinline__ bool w4_wait_seen(bool seen, uint32_t bar, uint32_t p
     return __all_sync(0xffffffffu, seen) || w4_wait_slow(bar, parity, ab, code);
 }
 
-// The launch's work: items in expert order, an item's steps in order of k.
+// A launch's work as one CTA sees it: items in expert order, an item's steps in order of k, and this CTA's range of steps.
 struct W4Item {
     int e, n0, r0, count;
 };
-__device__ __forceinline__ W4Item w4_item(const W4Params &p, const int *start, const int *first, int64_t item, int chunk_tokens) {
-    // the last expert whose first chunk's items start at or before the item
-    int lo = 0, hi = p.experts - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (int64_t(first[mid]) * p.tiles <= item)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    const int chunks = first[lo + 1] - first[lo];
-    const int at = int(item - int64_t(first[lo]) * p.tiles);
-    const int tile = at / chunks, chunk = at - tile * chunks;
-    const int r0 = start[lo] + chunk * chunk_tokens;
-    return {lo, tile * kW4TileRows, r0, min(chunk_tokens, start[lo + 1] - r0)};
-}
-__device__ __forceinline__ int w4_cta_of(int64_t step, int64_t total, int ctas) { return int(((step + 1) * ctas - 1) / total); }
+struct W4Work {
+    const int *start, *first;  // shared: first row of each expert (checked), token chunks of the experts before
+    int64_t total, begin, end;  // steps: of the launch, this CTA's range
+    int ctas;
 
-// offsets come from the device: each is held to the range that the rows allow
-__device__ __forceinline__ void w4_starts(const W4Params &p, int *start) {
-    for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) {
-        const int64_t v = p.offsets[e], before = e ? p.offsets[e - 1] : 0;
-        if (v < before || v > p.rows || before < 0)
-            report(p.status, kSiteOffsets);
-        start[e] = int(max(int64_t(0), min(v, p.rows)));
+    // offsets come from the device: each is held to the range that the rows allow
+    static __device__ __forceinline__ void starts(const W4Params &p, int *start) {
+        for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) {
+            const int64_t v = p.offsets[e], before = e ? p.offsets[e - 1] : 0;
+            if (v < before || v > p.rows || before < 0)
+                report(p.status, kSiteOffsets);
+            start[e] = int(max(int64_t(0), min(v, p.rows)));
+        }
+    }
+    __device__ __forceinline__ W4Work(const W4Params &p, int *start_, int *first_) : start(start_), first(first_) {
+        const int E = p.experts, tid = threadIdx.x;
+        starts(p, start_);
+        __syncthreads();
+        auto chunks_of = [&](int e) { return (max(0, start[e + 1] - start[e]) + p.chunk - 1) / p.chunk; };
+        const int per = (E + int(blockDim.x) - 1) / int(blockDim.x);
+        int sum = 0, chunks;
+        for (int e = tid * per; e < min(E, (tid + 1) * per); ++e)
+            sum += chunks_of(e);
+        int at = block_scan(sum, chunks);
+        for (int e = tid * per; e < min(E, (tid + 1) * per); ++e) {
+            first_[e] = at;
+            at += chunks_of(e);
+        }
+        if (tid == 0)
+            first_[E] = chunks;
+        __syncthreads();
+        total = int64_t(chunks) * p.tiles * p.steps;
+        ctas = int(min(int64_t(gridDim.x), total));
+        const int cta = blockIdx.x;
+        begin = cta < ctas ? total * cta / ctas : 0;
+        end = cta < ctas ? total * (cta + 1) / ctas : 0;
+    }
+    __device__ __forceinline__ W4Item at(const W4Params &p, int64_t item) const {
+        int lo = 0, hi = p.experts - 1;  // the last expert whose first chunk's items start at or before the item
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (int64_t(first[mid]) * p.tiles <= item)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        const int chunks = first[lo + 1] - first[lo];
+        const int64_t in = item - int64_t(first[lo]) * p.tiles;
+        const int tile = int(in / chunks), chunk = int(in - int64_t(tile) * chunks);
+        const int r0 = start[lo] + chunk * p.chunk;
+        return {lo, tile * kW4TileRows, r0, min(p.chunk, start[lo + 1] - r0)};
+    }
+    // The range's pieces, item by item, alike in every warp: f(place of the item, its number, first step, steps).
+    template <class F> __device__ __forceinline__ void pieces(const W4Params &p, F &&f) const {
+        for (int64_t s = begin; s < end;) {
+            const int64_t item = s / p.steps;
+            const int k0 = int(s - item * p.steps), n = int(min(int64_t(p.steps - k0), end - s));
+            f(at(p, item), item, k0, n);
+            s += n;
+        }
+    }
+    __device__ __forceinline__ int cta_of(int64_t step) const { return int(((step + 1) * ctas - 1) / total); }
+    __device__ __forceinline__ int first_cta(const W4Params &p, int64_t item) const { return cta_of(item * p.steps); }
+    __device__ __forceinline__ int last_cta(const W4Params &p, int64_t item) const { return cta_of(item * p.steps + p.steps - 1); }
+    // Partial sums [token][256] of CTA c's piece of a cut item: slot 0 where the piece begins inside its tile, 1 where it begins it.
+    __device__ __forceinline__ float *slot(const W4Params &p, int c, int first_of_item) const {
+        return p.ws + int64_t(2 * c + (c == first_of_item ? 1 : 0)) * (p.chunk * kW4TileRows);
+    }
+};
+
+// When a CTA's steps are done: its cut tiles. kThreads = 256 threads, `t` of them, a weight row each, that wrote the partial sums.
+// `cut`: the cut items' numbers, -1 for none; `ok`: whether the sums are sound.
+template <class T>
+__device__ __forceinline__ void w4_join(const W4Params &p, const W4Work &work, const int64_t (&cut)[2], bool ok, int t, int bar,
+                                        volatile int *arrived) {
+    if (cut[0] < 0 && cut[1] < 0)
+        return;
+    __threadfence();
+    named_sync(bar, kW4TileRows);
+    if (t < 2 && cut[t] >= 0)
+        arrived[t] = ok ? atomicAdd(p.counters + work.first_cta(p, cut[t]), 1) : -1;
+    named_sync(bar, kW4TileRows);
+    __threadfence();
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+        if (cut[i] < 0)
+            continue;
+        const int c0 = work.first_cta(p, cut[i]), c1 = work.last_cta(p, cut[i]);
+        if (arrived[i] != c1 - c0)
+            continue;
+        if (t == 0)
+            p.counters[c0] = 0;
+        const W4Item it = work.at(p, cut[i]);
+        if (it.n0 + t >= p.n)
+            continue;
+        T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + it.n0 + t;
+        for (int i0 = 0; i0 < it.count; i0 += 8) {  // eight tokens' loads at a time
+            float v[8] = {};
+#pragma unroll 4
+            for (int c = c0; c <= c1; ++c) {
+                const float *from = work.slot(p, c, c0) + t;
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    v[u] += __ldcg(from + min(i0 + u, it.count - 1) * kW4TileRows);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (i0 + u < it.count)
+                    out[int64_t(i0 + u) * p.n] = from_f32<T>(v[u]);
+        }
     }
 }
 
-// The rows of x in expert order, gathered through src, as the products read them: for each chunk of `chunk` tokens of an
-// expert and each step of 128 k a shared-memory image of B (K-major, two halves of 64 k, each a row of 128 bytes a token with the
-// 128-byte swizzle; token count rounded up to 8) so that a bulk copy a half loads it; eight values at a time in the order
-// in which masks and shifts take the weights out of a word. One 16-byte piece a thread. (Done by warps of the product
-// kernel instead, with cp.async and shared memory, this took them 1400 cycles a step at 16 tokens: twice what HBM allows.) Rows of
-// no expert are set to zero in out.
+// The rows of x in expert order, gathered through src, as the products read them: for each chunk of an expert's tokens and each
+// step of 128 k, pieces of eight values in the order in which masks and shifts take the weights out of a word, placed
+//   kFragments: as mma.sync's B fragments of 8 tokens (a word of k after another, 16 bytes a lane),
+//   else:       as a shared-memory image of tcgen05's B (K-major, two halves of 64 k, each a row of 128 bytes a token with the
+//               128-byte swizzle).
+// Token count rounded up to 8: what the places of the missing tokens hold goes into columns that nothing reads. One piece
+// a thread. (Done by warps of the product kernel instead, with cp.async and shared memory, this took them 1400 cycles a step
+// at 16 tokens: twice what HBM allows.) Rows of no expert are set to zero in out.
 constexpr int kW4GatherThreads = 128;
-template <class T> __global__ void __launch_bounds__(kW4GatherThreads) w4_gather(const __grid_constant__ W4Params p) {
+template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherThreads) w4_gather(const __grid_constant__ W4Params p) {
     __shared__ int start[kW4MaxExperts + 1];
     ptx::griddep_wait();
     // The product kernel may start now. It reads what earlier kernels wrote (offsets, scales, weights) without waiting for this one
     // to end: every block of this one has passed its own wait by then. Before it reads xs it waits for this one.
     ptx::griddep_launch_dependents();
-    w4_starts(p, start);
+    W4Work::starts(p, start);
     __syncthreads();
-    const int piece = int(blockIdx.y) * kW4GatherThreads + int(threadIdx.x);  // of a row: 8 values
-    const int step = piece >> 4, half = (piece >> 3) & 1, c = piece & 7;
+    const int piece = int(blockIdx.y) * kW4GatherThreads + int(threadIdx.x);  // of a row
+    const int step = piece >> 4, c = piece & 15;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         if (r < start[0] || r >= start[p.experts]) {
             for (int col = piece; col < p.n; col += int(gridDim.y) * kW4GatherThreads)
@@ -297,18 +310,352 @@ template <class T> __global__ void __launch_bounds__(kW4GatherThreads) w4_gather
         uint4 v = make_uint4(0, 0, 0, 0);
         if (row >= 0 && piece * 8 < p.k)
             v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + row * p.k + piece * 8);
-        const int64_t base = int64_t(int(r) - i + 8 * lo) * p.steps * 256;
-        *reinterpret_cast<uint4 *>(p.xs + base + (int64_t(step * 2 + half) * count + i) * 128 + ((c ^ (i & 7)) << 4)) =
+        const int64_t base = int64_t(int(r) - i + 8 * lo) * p.steps + int64_t(step) * count;
+        const int at = kFragments ? (((i >> 3) * 4 + (c >> 2)) * 32 + (i & 7) * 4 + (c & 3)) * 16
+                                  : ((c >> 3) * count + i) * 128 + (((c & 7) ^ (i & 7)) << 4);
+        *reinterpret_cast<uint4 *>(p.xs + base * kW4TokenBytes + at) =
             make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
                        __byte_perm(v.y, v.w, 0x7632));
     }
 }
 
+// ---- few rows an expert: chunks of 8 tokens, mma.sync ----
+//
+// The words of weights that ldmatrix hands to a lane are those of its place in the A fragment, so they are widened in the
+// registers that mma.sync reads, and nothing but a wait and an arrival stands between a step's bytes and its products. 8 warps of 32
+// weight rows and two loading warps (a TMA box of weights, a bulk copy of tokens a step, a ring of 4 steps), two CTAs an SM.
+// 22 us for 117 MB of weights (5.3 TB/s, 82% of the measured copy rate) at 1 row an expert, 24 at 8. Above that mma.sync's own rate
+// binds (11 cycles an instruction and scheduler: 16 tokens in one pass 36 us).
+constexpr int kW4FewTokens = 8;
+constexpr int kW4FewThreads = kW4TileRows + 64;
+constexpr int kW4FewStages = 4;
+constexpr int kW4FewSmem = 1024 + kW4FewStages * (kW4WeightBytes + kW4FewTokens * kW4TokenBytes);
+
+// D (16 x 8, fp32) += A (16 x 16) B (16 x 8), 16-bit operands.
+template <class T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same with zero for D's old values.
+template <class T>
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// Four 8 x 16-byte matrices; lane l gets word l % 4 of row l / 4 of each.
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+// Eight values of kBytes each (a scale or a zero of a group each) of a row that starts at any multiple of kBytes, as a queue of
+// 32-bit words, and the next eight on the way.
+template <int kBytes> struct W4Queue {
+    static constexpr int kWords = 2 * kBytes;  // of eight values
+    const uint32_t *from;                      // the aligned word that holds the next visit's first value
+    const uint32_t *end;                       // past the array's last word
+    int at;                                    // that visit's first group
+    uint32_t shift;                            // bits from the word's start to the value
+    uint32_t raw[kWords + 1], word[kWords];
+
+    __device__ __forceinline__ W4Queue(const void *array, int64_t row, const void *array_end, int first) : at(first) {
+        const uintptr_t p = reinterpret_cast<uintptr_t>(array) + uintptr_t((row + first) * kBytes);
+        from = reinterpret_cast<const uint32_t *>(p & ~uintptr_t(3));
+        shift = uint32_t(p & 3) * 8;
+        end = static_cast<const uint32_t *>(array_end);
+        if (array)
+            load();
+    }
+    __device__ __forceinline__ void load() {
+#pragma unroll
+        for (int i = 0; i <= kWords; ++i)
+            raw[i] = from + i < end ? __ldg(from + i) : 0u;
+        from += kWords;
+    }
+    __device__ __forceinline__ void refill(int groups) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+            word[i] = __funnelshift_r(raw[i], raw[i + 1], shift);
+        at += 8;
+        if (at < groups)
+            load();
+    }
+    __device__ __forceinline__ uint32_t take() {
+        const uint32_t v = word[0] & ((1u << (8 * kBytes)) - 1u);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+            word[i] = __funnelshift_r(word[i], i + 1 < kWords ? word[i + 1] : 0u, 8 * kBytes);
+        return v;
+    }
+};
+
+template <class T, int G, bool kZeros>
+__global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ W4Params p) {
+    constexpr int kSub = kW4StepK / G;  // groups a step
+    constexpr int kXBytes = kW4FewTokens * kW4TokenBytes;
+    extern __shared__ __align__(1024) uint8_t w4_smem[];
+    __shared__ int start[kW4MaxExperts + 1], first[kW4MaxExperts + 1];
+    __shared__ uint64_t bar_words[2 * kW4FewStages];
+    __shared__ uint32_t abort_word;
+    __shared__ int arrived[2];
+    volatile uint32_t *abort_flag = &abort_word;
+    const uint32_t smem = (ptx::smem_addr(w4_smem) + 1023) & ~1023u, bars = ptx::smem_addr(bar_words);
+    auto w_at = [&](int s) { return smem + uint32_t(s * kW4WeightBytes); };
+    auto x_at = [&](int s) { return smem + uint32_t(kW4FewStages * kW4WeightBytes + s * kXBytes); };
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (kW4FewStages + s); };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x, g = lane >> 2, t = lane & 3;
+    if (tid == 0) {
+        for (int s = 0; s < kW4FewStages; ++s) {
+            ptx::mbar_init(full(s), 2);  // weights and tokens
+            ptx::mbar_init(empty(s), 8);
+        }
+        *abort_flag = 0u;
+        ptx::fence_mbar_init();
+        ptx::fence_proxy_async_smem();
+        ptx::prefetch_tmap(&tmap_w);
+    }
+    // No wait here: w4_gather lets this kernel start when all before it has completed.
+    ptx::fence_proxy_async_global();
+    ptx::griddep_launch_dependents();
+    const W4Work work(p, start, first);
+    const Abort ab{p.status + 2, abort_flag, p.timeout_ns};
+    int st = 0;
+    uint32_t ph = 0;
+    auto next = [&]() {
+        if (++st == kW4FewStages) {
+            st = 0;
+            ph ^= 1u;
+        }
+    };
+    bool ok = true;
+    if (warp >= 8) {
+        const bool tokens = warp == 9;
+        const uint32_t leader = ptx::elect_one_sync();
+        if (tokens) {  // what precedes the launch of w4_gather is done (see there), its own writes only now
+            ptx::griddep_wait();
+            ptx::fence_proxy_async_global();
+        }
+        work.pieces(p, [&](const W4Item &it, int64_t, int k0, int n) {
+            const uint8_t *from = p.xs + (int64_t(it.r0 + 8 * it.e) * p.steps + int64_t(k0) * kW4FewTokens) * kW4TokenBytes;
+            for (int j = 0; ok && j < n; ++j) {
+                ok = w4_wait(empty(st), ph ^ 1u, ab, kStatusTimeout | kRoleProducer | uint32_t(st));
+                if (!ok)
+                    break;
+                if (tokens) {
+                    ptx::mbar_arrive_expect_tx(full(st), kXBytes, leader);
+                    bulk_load(x_at(st), from, kXBytes, full(st), leader);
+                    from += kXBytes;
+                } else {
+                    ptx::mbar_arrive_expect_tx(full(st), kW4WeightBytes, leader);
+                    ptx::tma_load_3d(w_at(st), &tmap_w, full(st), (k0 + j) * (kW4StepK / 2), it.n0, it.e, leader);
+                }
+                next();
+            }
+        });
+    } else {
+        // of ldmatrix: row lane % 8 of the warp's, piece lane / 8 swizzled
+        const uint32_t w_lane = uint32_t((warp * 32 + (lane & 7)) * 64) + (uint32_t((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
+        int64_t cut[2] = {-1, -1};
+        work.pieces(p, [&](const W4Item &it, int64_t item, int k0, int n) {
+            float sum[2][4] = {};
+            // Scales and zeros of weight row `lane`, to be handed to the lanes whose fragments hold the row. A row's lie next to
+            // each other, the rows far apart, so each visit to a row's line takes eight groups: into `raw`, one visit ahead, and from
+            // there, moved to the row's odd alignment, into queues that give up their low end.
+            const int64_t meta = (int64_t(it.e) * p.n + min(it.n0 + warp * 32 + lane, p.n - 1)) * p.groups;
+            W4Queue<2> scales(p.scales, meta, p.scales_end, k0 * kSub);
+            W4Queue<1> zeros(p.zeros, meta, p.zeros_end, k0 * kSub);
+            int queued = 0;  // groups in the queues
+            for (int j = 0; j < n; ++j) {
+                ok = w4_wait(full(st), ph, ab, kStatusTimeout | kRoleMma | uint32_t(st));
+                if (!ok)
+                    break;
+                if (queued == 0) {
+                    scales.refill(p.groups);
+                    if constexpr (kZeros)
+                        zeros.refill(p.groups);
+                    queued = 8;
+                }
+                queued -= kSub;
+                uint32_t w[4][4];  // rows g + 8 i; word c holds k = 32 c + 8 t ...
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    ldmatrix_x4(w_at(st) + w_lane + uint32_t(i * 512), w[i]);
+                const uint32_t x_from = x_at(st) + uint32_t(lane * 16);
+#pragma unroll
+                for (int s = 0; s < kSub; ++s) {
+                    float acc[2][4];
+                    uint32_t minus[4];
+                    if constexpr (kZeros) {
+                        const uint32_t mine = w4_minus<T>(zeros.take() & 15u);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            minus[i] = __shfl_sync(0xffffffffu, mine, g + 8 * i);
+                    } else {
+                        minus[0] = minus[1] = minus[2] = minus[3] = w4_minus<T>(8u);
+                    }
+#pragma unroll
+                    for (int c = s * 4 / kSub; c < (s + 1) * 4 / kSub; ++c) {
+                        uint32_t a[4][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            widen<T>(w[i][c], minus[i], a[i]);
+                        const uint4 b = lds128(x_from + uint32_t(c * 512));
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            if (c == s * 4 / kSub)
+                                mma16816_first<T>(acc[m], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y);
+                            else
+                                mma16816<T>(acc[m], a[2 * m][0], a[2 * m + 1][0], a[2 * m][1], a[2 * m + 1][1], b.x, b.y);
+                            mma16816<T>(acc[m], a[2 * m][2], a[2 * m + 1][2], a[2 * m][3], a[2 * m + 1][3], b.z, b.w);
+                        }
+                    }
+                    if (s == kSub - 1) {
+                        // All of the stage is in registers. TMA writes it next: the lanes' reads are ordered before that by the
+                        // proxy fence (without it, reads still on the way met the next step's bytes).
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0)
+                            ptx::mbar_arrive(empty(st));
+                    }
+                    const uint16_t bits = uint16_t(scales.take());
+                    const float scale = to_f32(*reinterpret_cast<const T *>(&bits)) * W4Unit<T>::kBack;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float f = __shfl_sync(0xffffffffu, scale, g + 8 * i);
+                        float *to = sum[i >> 1] + 2 * (i & 1);
+                        to[0] = fmaf(f, acc[i >> 1][2 * (i & 1)], to[0]);
+                        to[1] = fmaf(f, acc[i >> 1][2 * (i & 1) + 1], to[1]);
+                    }
+                }
+                next();
+            }
+            const bool whole = n == p.steps;
+            if (!whole)
+                cut[k0 == 0] = item;
+            float *mine = whole ? nullptr : work.slot(p, blockIdx.x, work.first_cta(p, item));
+            T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + it.n0;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = warp * 32 + 16 * m + 8 * (i >> 1) + g, tok = 2 * t + (i & 1);
+                    if (!ok || tok >= it.count || it.n0 + row >= p.n)
+                        continue;
+                    if (whole)
+                        out[int64_t(tok) * p.n + row] = from_f32<T>(sum[m][i]);
+                    else
+                        __stcg(mine + tok * kW4TileRows + row, sum[m][i]);
+                }
+        });
+        w4_join<T>(p, work, cut, ok, tid, 1, arrived);
+    }
+    if (*abort_flag != 0u) {
+        // let copies already asked for drain before the memory they target goes away
+        const uint64_t t0 = ptx::globaltimer();
+        while (ptx::globaltimer() - t0 < 200000ull)
+            __nanosleep(1000);
+        atomicCAS(p.status, 0u, *reinterpret_cast<volatile uint32_t *>(p.status + 2));
+    }
+}
+
+// ---- more rows an expert: chunks of up to 32 tokens, tcgen05 ----
+//
+//   warp 0       TMA: a step's weights into a ring of 6 steps
+//   warp 3       bulk copies of a step's tokens
+//   warps 4-11   a group of four for each half of the weight rows, a thread a row: 16 bytes at a time from the ring,
+//                widened in registers, tcgen05.st into the half's next A operand
+//   warps 1, 2   a half each: tcgen05.mma, D[weight row, token] = A (Tensor Memory) x B (tokens), a fresh accumulator
+//                a group
+//   warps 12-19  a half each four: tcgen05.ld of a step's products and the fp32 sum with the group's scale (one scalar a
+//                thread); output
+//
+// Three A operands and two D a half keep the widening from waiting for the MMAs: beside widening warps the MMA warp's eight
+// take 300 cycles to issue and 530 beside four a scheduler, against 95 alone. 28 us for 117 MB of weights at 1 row an expert, 30 at 16, 33 at 32:
+// bound by instruction issue (3200 a step and SM, of which the widening is 1200), not by the number of tokens.
+constexpr int kW4ManyThreads = 640;
+
+// Tokens of a chunk: at most 32 (a thread holds a sum a token). Tensor Memory's 512 columns hold for each half kA operands of
+// 64 columns and two D of a column a token and group of a step.
+template <int G> struct W4Many {
+    static constexpr int kSub = kW4StepK / G;  // groups a step
+    static constexpr int kTokens = kSub == 4 ? 16 : 32;
+    static constexpr int kA = kSub == 1 ? 3 : 2;
+    static constexpr int kD = kSub * kTokens;  // columns of a D
+    static constexpr int kStageBytes = kW4WeightBytes + kTokens * kW4StepK * 2;
+    static constexpr int kStages = 6;  // a multiple of 2 and of kA: a stage always meets the same D and A
+    static constexpr int kBars = 4 * kStages + 4 * kA + 4;
+    static_assert(2 * (64 * kA + 2 * kD) <= 512 && kStages % kA == 0 && kStages % 2 == 0, "Tensor Memory");
+    static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kBars * 8 + 64;
+};
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16],"
+                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32"
+                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+// One step's eight MMAs of 16 k for 128 weight rows: D (Tensor Memory) = A (Tensor Memory, two 16-bit values a column)
+// x B (shared memory, descriptor hi:lo), a D of its own for each group of G. Issued where pred != 0. In one block with
+// addresses one add away from its operands, in a loop that is not unrolled: with the stages unrolled and every address a constant the
+// warps of the other roles stalled three issue slots of four on the instruction cache.
+#define GG_W4_MMA(i, acc) \
+    "add.u32 d, %0, " #i "*16/%8*%7;\n\tadd.u32 a, %1, " #i "*8;\n\tadd.u32 l, %2, " #i "/4*%6+(" #i "&3)*2;\n\tmov.b64 b, {l, %3};\n\t" \
+    "@q tcgen05.mma.cta_group::1.kind::f16 [d], [a], b, %4, " acc ";\n\t"
+template <int G, int kTokens>
+__device__ __forceinline__ void w4_mma_step(uint32_t d, uint32_t a, uint32_t lo, uint32_t hi, uint32_t idesc, uint32_t pred) {
+#define GG_W4_STEP(a1, a2, a3, a4, a5, a6, a7)                                                                                          \
+    asm volatile("{\n\t.reg .pred q, t, f;\n\t.reg .b32 d, a, l;\n\t.reg .b64 b;\n\tsetp.ne.b32 q, %5, 0;\n\t"                            \
+                 "setp.eq.b32 t, 0, 0;\n\tsetp.ne.b32 f, 0, 0;\n\t" GG_W4_MMA(0, "f") GG_W4_MMA(1, a1) GG_W4_MMA(2, a2) GG_W4_MMA(3, a3) \
+                     GG_W4_MMA(4, a4) GG_W4_MMA(5, a5) GG_W4_MMA(6, a6) GG_W4_MMA(7, a7) "}" ::"r"(d),                                  \
+                 "r"(a), "r"(lo), "r"(hi), "r"(idesc), "r"(pred), "n"(kTokens * 128 / 16), "n"(kTokens), "n"(G)                         \
+                 : "memory")
+    if constexpr (G == 128)
+        GG_W4_STEP("t", "t", "t", "t", "t", "t", "t");
+    else if constexpr (G == 64)
+        GG_W4_STEP("t", "t", "t", "f", "t", "t", "t");
+    else
+        GG_W4_STEP("t", "f", "t", "f", "t", "f", "t");
+#undef GG_W4_STEP
+}
+#undef GG_W4_MMA
 template <class T, int G>
-__global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ W4Params p) {
-    using C = W4Cfg<G>;
+__global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ W4Params p) {
+    using C = W4Many<G>;
     constexpr int kTokens = C::kTokens, kSub = C::kSub, kStages = C::kStages, kA = C::kA;
     extern __shared__ __align__(1024) uint8_t w4_smem[];
+    __shared__ int start[kW4MaxExperts + 1], first[kW4MaxExperts + 1];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(w4_smem) + 1023) & ~uintptr_t(1023));
     const uint32_t ring = ptx::smem_addr(smem);
     // x tiles first (1024-byte aligned swizzle atoms), then the weights (16 KB each)
@@ -325,12 +672,9 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
     auto dempty = [&](int h, int d) { return bars + 8u * (4 * kStages + 4 * kA + 2 * h + d); };
     auto a_col = [&](int h, int a) { return uint32_t(64 * (kA * h + a)); };
     auto d_col = [&](int h, int d) { return uint32_t(128 * kA + C::kD * (2 * h + d)); };
-    int *start = reinterpret_cast<int *>(after + C::kBars * 8);  // first row of each expert, checked
-    int *first = start + kW4MaxExperts + 1;                      // token chunks of the experts before
-    uint32_t *slots = reinterpret_cast<uint32_t *>(first + kW4MaxExperts + 1);
+    uint32_t *slots = reinterpret_cast<uint32_t *>(after + C::kBars * 8);
     volatile uint32_t *abort_flag = slots + 1;
-    volatile int32_t *arrived = reinterpret_cast<volatile int32_t *>(slots + 2);
-
+    volatile int *arrived = reinterpret_cast<volatile int *>(slots + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -359,48 +703,18 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
     // No wait here: w4_gather lets this kernel start when all before it has completed.
     ptx::fence_proxy_async_global();
     ptx::griddep_launch_dependents();
-    const int E = p.experts;
-    w4_starts(p, start);
-    __syncthreads();
-    {
-        auto chunks_of = [&](int e) { return (max(0, start[e + 1] - start[e]) + kTokens - 1) / kTokens; };
-        const int per = (E + kW4Threads - 1) / kW4Threads;
-        int sum = 0;
-        for (int e = tid * per; e < min(E, (tid + 1) * per); ++e)
-            sum += chunks_of(e);
-        int total, at = block_scan(sum, total);
-        for (int e = tid * per; e < min(E, (tid + 1) * per); ++e) {
-            first[e] = at;
-            at += chunks_of(e);
-        }
-        if (tid == 0)
-            first[E] = total;
-    }
+    const W4Work work(p, start, first);
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = slots[0];  // column 0: all of them are allocated
-    const int64_t total = int64_t(first[E]) * p.tiles * p.steps;  // steps of the launch
-    const int ctas = int(min(int64_t(gridDim.x), total));
-    const int cta = blockIdx.x;
-    const int64_t s_begin = cta < ctas ? total * cta / ctas : 0, s_end = cta < ctas ? total * (cta + 1) / ctas : 0;
     const Abort ab{p.status + 2, abort_flag, p.timeout_ns};
-    // pieces of the range, item by item: f(item, first step, steps) in every role alike
-    auto pieces = [&](auto &&f) {
-        for (int64_t s = s_begin; s < s_end;) {
-            const int64_t item = s / p.steps;
-            const int k0 = int(s - item * p.steps), n = int(min(int64_t(p.steps - k0), s_end - s));
-            f(w4_item(p, start, first, item, kTokens), item, k0, n);
-            s += n;
-        }
-    };
-
     if (warp == 0) {
         const uint32_t leader = ptx::elect_one_sync();
         int st = 0;
         uint32_t ph = 0;
         bool ok = true;
-        pieces([&](const W4Item &it, int64_t, int k0, int n) {
+        work.pieces(p, [&](const W4Item &it, int64_t, int k0, int n) {
             for (int j = 0; ok && j < n; ++j) {
                 ok = w4_wait(wempty(st), ph ^ 1u, ab, kStatusTimeout | kRoleProducer | uint32_t(st));
                 if (!ok)
@@ -419,7 +733,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
         int st = 0, a = 0, d = 0;
         uint32_t ph = 0, a_ph = 0, d_ph = 3;  // bits: the phases of each A's and D's next use
         bool ok = true;
-        pieces([&](const W4Item &it, int64_t, int, int n) {
+        work.pieces(p, [&](const W4Item &it, int64_t, int, int n) {
             const uint32_t idesc = ptx::f16_idesc(Fmt<T>::kUmma, 128, (it.count + 15) & ~15);
             const bool active = it.n0 + 128 * h < p.n;
 #pragma unroll 1
@@ -459,9 +773,9 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
         // what precedes the launch of w4_gather is done (see there), its own writes only now
         ptx::griddep_wait();
         ptx::fence_proxy_async_global();
-        pieces([&](const W4Item &it, int64_t, int k0, int n) {
+        work.pieces(p, [&](const W4Item &it, int64_t, int k0, int n) {
             const uint32_t bytes = uint32_t(((it.count + 7) & ~7) * 256);
-            const uint8_t *from = p.xs + (int64_t(it.r0 + 8 * it.e) * p.steps) * 256 + int64_t(k0) * bytes;
+            const uint8_t *from = p.xs + (int64_t(it.r0 + 8 * it.e) * p.steps) * kW4TokenBytes + int64_t(k0) * bytes;
             for (int j = 0; ok && j < n; ++j) {
                 ok = w4_wait(xempty(st), ph ^ 1u, ab, kStatusTimeout | kRoleProducer | 0x80u | uint32_t(st));
                 if (!ok)
@@ -490,7 +804,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
                 ph ^= 1u;
             }
         };
-        pieces([&](const W4Item &it, int64_t, int k0, int n) {
+        work.pieces(p, [&](const W4Item &it, int64_t, int k0, int n) {
             if (it.n0 + 128 * h >= p.n) {  // no columns: on with the ring
                 for (int j = 0; ok && j < n; ++j) {
                     ok = w4_wait(wfull(st), ph, ab, kStatusTimeout | kRoleEpilogue | 0x80u | uint32_t(st));
@@ -557,8 +871,9 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         int a = 0, d = 0;
         uint32_t a_ph = 0;
+        int64_t cut[2] = {-1, -1};
         bool ok = true;
-        pieces([&](const W4Item &it, int64_t item, int k0, int n) {
+        work.pieces(p, [&](const W4Item &it, int64_t item, int k0, int n) {
             const int col = it.n0 + 128 * h + row;
             const int npad = (it.count + 15) & ~15;
             const T *scales = static_cast<const T *>(p.scales) + (int64_t(it.e) * p.n + min(col, p.n - 1)) * p.groups;
@@ -615,48 +930,26 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_rows(const __grid_constant__
                 a = (a + n) % kA;
                 d = (d + n) & 1;
             }
-            // ---- the piece's sums: to out, or where the tile is cut to the workspace ----
-            T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + col;
-            const bool there = ok && col < p.n;
-            if (n == p.steps) {
-                if (there) {
-#pragma unroll
-                    for (int i = 0; i < kTokens; ++i)
-                        if (i < it.count)
-                            out[int64_t(i) * p.n] = from_f32<T>(sum[i]);
-                }
+            const bool whole = n == p.steps;
+            if (!whole)
+                cut[k0 == 0] = item;
+            if (!ok || col >= p.n)
                 return;
-            }
-            const int64_t a = item * p.steps;
-            const int c0 = w4_cta_of(a, total, ctas), c1 = w4_cta_of(a + p.steps - 1, total, ctas);
-            // slot 0 of a CTA: a piece that begins inside its tile; slot 1: one that begins its tile
-            auto slot = [&](int c) { return p.ws + int64_t(2 * c + (c == c0 ? 1 : 0)) * (kTokens * kW4TileRows) + 128 * h + row; };
-            if (there) {
-                float *mine = slot(cta);
+            if (whole) {
+                T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + col;
+#pragma unroll
+                for (int i = 0; i < kTokens; ++i)
+                    if (i < it.count)
+                        out[int64_t(i) * p.n] = from_f32<T>(sum[i]);
+            } else {
+                float *mine = work.slot(p, blockIdx.x, work.first_cta(p, item)) + 128 * h + row;
 #pragma unroll
                 for (int i = 0; i < kTokens; ++i)
                     if (i < it.count)
                         __stcg(mine + i * kW4TileRows, sum[i]);
             }
-            __threadfence();
-            named_sync(2, 256);
-            if (tid == 384)
-                *arrived = ok ? atomicAdd(p.counters + c0, 1) : -1;
-            named_sync(2, 256);
-            if (*arrived != c1 - c0)
-                return;
-            __threadfence();
-            if (tid == 384)
-                p.counters[c0] = 0;
-            if (there) {
-                for (int i = 0; i < it.count; ++i) {
-                    float s = 0.0f;
-                    for (int c = c0; c <= c1; ++c)
-                        s += __ldcg(slot(c) + i * kW4TileRows);
-                    out[int64_t(i) * p.n] = from_f32<T>(s);
-                }
-            }
         });
+        w4_join<T>(p, work, cut, ok, tid - 384, 2, arrived);
     }
 
     // ---- teardown ----
