@@ -237,8 +237,10 @@ int prepare_route(gg_handle *h, const gg_route_problem &q, gg_stream_t stream, c
     p.top_k = q.top_k;
     p.normalize = q.normalize != 0;
     p.scale = q.scale;
-    const int64_t wanted = std::max<int64_t>(1, (q.tokens + gg::moe::kRouteWarps - 1) / gg::moe::kRouteWarps);
-    p.blocks = int(std::min<int64_t>(wanted, num_sms));
+    // One block where a warp gets two tokens at most (it finishes alone, in one launch); else a block for every 8 tokens, up to one an SM.
+    const int v = (q.experts + 31) / 32, warps = gg::moe::route_warps(v <= 8 ? 8 : v <= 16 ? 16 : 32);
+    const bool alone = q.tokens <= 2 * warps && q.experts <= 32 * warps;
+    p.blocks = alone ? 1 : int(std::max<int64_t>(1, std::min<int64_t>((q.tokens + 7) / 8, num_sms)));
     p.per_block = std::max<int64_t>(1, (q.tokens + p.blocks - 1) / p.blocks);
     const size_t entries = size_t(p.blocks) * size_t(q.experts + 1);
     if (const int rc = reserve(h, 2 * entries * 4))
@@ -246,9 +248,11 @@ int prepare_route(gg_handle *h, const gg_route_problem &q, gg_stream_t stream, c
     p.block_sums = h->d_ws;
     p.block_counts = reinterpret_cast<int32_t *>(h->d_ws + entries);
     set_params(h, p);
-    MoeLaunch topk{route_fn(q.logits_type, q.experts, false), unsigned(p.blocks), gg::moe::kRouteThreads,
-                   size_t(gg::moe::kRouteWarps) * size_t(q.experts) * 4};
-    MoeLaunch place{reinterpret_cast<const void *>(&gg::moe::route_place), unsigned(p.blocks), gg::moe::kRouteThreads, 0};
+    const size_t smem = size_t(warps) * (size_t(q.experts) + 128) * 4;
+    const void *fn = route_fn(q.logits_type, q.experts, false);
+    GG_CUDA(h, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    MoeLaunch topk{fn, unsigned(p.blocks), unsigned(warps) * 32, smem};
+    MoeLaunch place{reinterpret_cast<const void *>(&gg::moe::route_place), alone ? 0u : unsigned(p.blocks) + 1, gg::moe::kPlaceThreads, 0};
     char detail[160];
     std::snprintf(detail, sizeof(detail), "gg_route<%s> experts=%d top_k=%d blocks=%d", type_name(q.logits_type), q.experts, q.top_k, p.blocks);
     return finish(h, stream, {topk, place}, detail);
@@ -282,11 +286,13 @@ int prepare_route_grad(gg_handle *h, const gg_route_grad_problem &q, gg_stream_t
     p.scale = q.scale;
     set_params(h, p);
     const void *fn = route_fn(q.logits_type, q.experts, true);
-    const size_t smem = size_t(1 + gg::moe::kRouteWarps) * size_t(q.experts) * 4;
-    const int64_t blocks = std::min<int64_t>((q.tokens + gg::moe::kRouteWarps - 1) / gg::moe::kRouteWarps, int64_t(num_sms) * 8);
+    const size_t smem = size_t(gg::moe::kGradWarps) * size_t(q.experts) * 4;
+    int per_sm = 0;
+    GG_CUDA(h, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, gg::moe::kGradThreads, smem));
+    const int64_t blocks = std::min<int64_t>((q.tokens + gg::moe::kGradWarps - 1) / gg::moe::kGradWarps, int64_t(num_sms) * std::max(1, per_sm));
     char detail[160];
     std::snprintf(detail, sizeof(detail), "gg_route_grad<%s> experts=%d top_k=%d blocks=%d", type_name(q.logits_type), q.experts, q.top_k, int(blocks));
-    return finish(h, stream, {MoeLaunch{fn, unsigned(blocks), gg::moe::kRouteThreads, smem}}, detail);
+    return finish(h, stream, {MoeLaunch{fn, unsigned(blocks), gg::moe::kGradThreads, smem}}, detail);
 }
 
 // ---- dispatch / combine ----

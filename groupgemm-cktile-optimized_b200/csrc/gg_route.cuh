@@ -10,10 +10,14 @@
 namespace gg {
 namespace moe {
 
-constexpr int kRouteWarps = 8;
-constexpr int kRouteThreads = kRouteWarps * 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 32;
+// Warps of a block of route_topk, by logits a lane (V = experts / 32 rounded up to a power of two): as many as the registers
+// allow, since a warp waits for its token's row and for its reductions most of the time.
+__host__ __device__ constexpr int route_warps(int v) { return v <= 8 ? 32 : v == 16 ? 16 : 8; }
+constexpr int kGradWarps = 8;
+constexpr int kGradThreads = kGradWarps * 32;
+constexpr int kPlaceThreads = 1024;
 
 struct RouteParams {
     const void *logits;   // [tokens, experts]
@@ -50,12 +54,11 @@ struct RouteGradParams {
     float scale;
 };
 
-// Logits as unsigned keys in the same order: -0 and +0 alike, every NaN alike and above +inf.
+// Logits as unsigned keys in the same order. The addition makes -0 and +0 alike, and every NaN the one NaN that arithmetic gives
+// (0x7fffffff), whose key is above +inf's.
 __device__ __forceinline__ uint32_t key_of(float v) {
-    if (v != v)
-        return 0xffffffffu;
-    const uint32_t u = __float_as_uint(v + 0.0f);
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    const uint32_t u = __float_as_uint(__fadd_rn(v, 0.0f));
+    return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
@@ -71,22 +74,140 @@ template <class T, int V> __device__ __forceinline__ void load_row(float (&v)[V]
     }
 }
 
+// The k largest of a warp's keys (lane + 32 i: expert), ties to the lower expert: lane j < k gets the j-th one's expert and key,
+// the others -1. `mine`: the lane's largest key. `list`: 128 words of the warp's.
+//
+// With L the k-th largest of the lanes' own largest keys, the k largest keys are all at least L, and few others are: those
+// candidates, compacted in order of expert, are ranked against one another, a lane each. 160 instructions for 256
+// experts and k = 8, against 440 for k rounds of a maximum over all keys, which remain for more than 32 candidates (ties).
+template <int V> __device__ __forceinline__ void top_keys(uint32_t (&key)[V], uint32_t mine, int k, uint32_t *list, int &id, uint32_t &id_key) {
+    const int lane = threadIdx.x & 31;
+    uint32_t least = 0, m = mine;
+    for (int found = 0;;) {
+        least = __reduce_max_sync(0xffffffffu, m);
+        if (least <= kKeyMinusInf) {
+            least = kKeyMinusInf + 1;  // fewer lanes than k hold an open expert: every open one is a candidate
+            break;
+        }
+        found += __popc(__ballot_sync(0xffffffffu, m == least));
+        if (found >= k)
+            break;
+        if (m == least)
+            m = 0;
+    }
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const bool in = key[i] >= least;
+        const uint32_t all = __ballot_sync(0xffffffffu, in);
+        const int at = total + __popc(all & ((1u << lane) - 1u));
+        if (in && at < 32) {
+            list[at] = key[i];
+            list[32 + at] = uint32_t(lane + 32 * i);
+        }
+        total += __popc(all);
+    }
+    id = -1;
+    id_key = kKeyMinusInf;
+    if (total <= 32) {
+        __syncwarp();
+        const uint32_t mykey = lane < total ? list[lane] : 0u, myid = list[32 + lane];
+        int rank = 0;
+        for (int q = 0; q < total; ++q) {
+            const uint32_t other = __shfl_sync(0xffffffffu, mykey, q);
+            rank += other > mykey || (other == mykey && q < lane);
+        }
+        if (lane < total && rank < k) {
+            list[64 + rank] = mykey;
+            list[96 + rank] = myid;
+        }
+        __syncwarp();
+        if (lane < min(total, k)) {
+            id_key = list[64 + lane];
+            id = int(list[96 + lane]);
+        }
+        return;
+    }
+    for (int j = 0; j < k; ++j) {
+        uint32_t bk = 0;
+        int bi = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (key[i] > bk) {
+                bk = key[i];
+                bi = lane + 32 * i;
+            }
+        const uint32_t best = __reduce_max_sync(0xffffffffu, bk);
+        if (best <= kKeyMinusInf)
+            break;
+        const int e = int(__reduce_min_sync(0xffffffffu, bk == best ? unsigned(bi) : 0x7fffffffu));
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (lane + 32 * i == e)
+                key[i] = 0;
+        if (lane == j) {
+            id = e;
+            id_key = best;
+        }
+    }
+}
+
+// The totals' outputs and the losses, by one block: tot and sum are the thread's expert's (thread e).
+__device__ __forceinline__ void route_totals(const RouteParams &p, int tot, int at, int total, float sum, int live, float z) {
+    const int e = threadIdx.x, E = p.experts;
+    const float inv = 1.0f / float(max(live, 1));
+    float balance = 0.0f;
+    if (e < E) {
+        p.offsets[e] = at;
+        p.counts[e] = tot;
+        if (p.prob)
+            p.prob[e] = sum * inv;
+        balance = float(tot) * (sum * inv);
+    }
+    if (e == 0) {
+        p.offsets[E] = total;
+        *p.live = live;
+    }
+    if (!p.losses)
+        return;
+    __shared__ float red[32];
+    balance = warp_sum(balance);
+    if ((e & 31) == 0)
+        red[e >> 5] = balance;
+    __syncthreads();
+    if (e == 0) {
+        float s = 0.0f;
+        for (int w = 0; w < int(blockDim.x) >> 5; ++w)
+            s += red[w];
+        p.losses[0] = s * float(E) / float(p.top_k) * inv;
+        p.losses[1] = z * inv;
+    }
+}
+
 // One warp a token, V logits a lane. A block takes a contiguous run of tokens and each of its
 // warps a contiguous part of it, so that a warp's own counter of each expert gives the rank of a slot
 // among the warp's slots in order; the ranks are raised by the warps before in the block here and by the
-// blocks before in route_place.
-template <class T, int V> __global__ void __launch_bounds__(kRouteThreads) route_topk(const RouteParams p) {
-    extern __shared__ int32_t route_smem[];  // [warps][experts]
-    __shared__ float z_of[kRouteWarps];
-    __shared__ int live_of[kRouteWarps];
+// blocks before in route_place, or here where one block takes all tokens. Bound by instruction issue (330 a token with 256 experts).
+template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32) route_topk(const RouteParams p) {
+    constexpr int W = route_warps(V), kThreads = W * 32;
+    extern __shared__ int32_t route_smem[];  // [warps][experts] counters, then [warps][128] for top_keys
+    __shared__ float z_of[W];
+    __shared__ int live_of[W];
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     const int E = p.experts, k = p.top_k;
-    const int64_t first = blockIdx.x * p.per_block, end = min(p.tokens, first + p.per_block);
-    const int64_t per_warp = (p.per_block + kRouteWarps - 1) / kRouteWarps;
-    const int64_t w0 = min(end, first + warp * per_warp), w1 = min(end, w0 + per_warp);
+    const int64_t begin = blockIdx.x * p.per_block, end = min(p.tokens, begin + p.per_block);
+    const int64_t per_warp = (p.per_block + W - 1) / W;
+    const int64_t w0 = min(end, begin + warp * per_warp), w1 = min(end, w0 + per_warp);
     int32_t *hist = route_smem + warp * E;
+    uint32_t *list = reinterpret_cast<uint32_t *>(route_smem + W * E + warp * 128);
+    float v[V];
+    auto load = [&](int64_t t) {
+        load_row<T, V>(v, static_cast<const T *>(p.logits) + t * E, E, !p.mask || p.mask[t] != 0);
+    };
+    if (w0 < w1)
+        load(w0);
     for (int e = lane; e < E; e += 32)
         hist[e] = 0;
     __syncwarp();
@@ -97,16 +218,13 @@ template <class T, int V> __global__ void __launch_bounds__(kRouteThreads) route
     float z = 0.0f;
     int live = 0;
     for (int64_t t = w0; t < w1; ++t) {
-        const bool there = !p.mask || p.mask[t] != 0;
-        float v[V];
-        load_row<T, V>(v, static_cast<const T *>(p.logits) + t * E, E, there);
-        uint32_t key[V], best = 0;
+        uint32_t key[V], mine = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             key[i] = key_of(v[i]);
-            best = max(best, key[i]);
+            mine = max(mine, key[i]);
         }
-        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
         int32_t id = -1;
         float weight = 0.0f, lse = -INFINITY;
         if (top > kKeyMinusInf) {
@@ -114,7 +232,7 @@ template <class T, int V> __global__ void __launch_bounds__(kRouteThreads) route
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[i] = expf(v[i] - mx);
+                v[i] = __expf(v[i] - mx);
                 sum += v[i];
             }
             sum = warp_sum(sum);
@@ -122,35 +240,18 @@ template <class T, int V> __global__ void __launch_bounds__(kRouteThreads) route
             const float inv = 1.0f / sum;
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                acc[i] += v[i] * inv;
-            z += lse * lse;
+                acc[i] = fmaf(v[i], inv, acc[i]);
+            z = fmaf(lse, lse, z);
             ++live;
-            uint32_t mine = kKeyMinusInf;
-            for (int j = 0; j < k; ++j) {
-                uint32_t bk = 0;
-                int bi = 0;
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (key[i] > bk) {
-                        bk = key[i];
-                        bi = lane + 32 * i;
-                    }
-                const uint32_t m = __reduce_max_sync(0xffffffffu, bk);
-                if (m <= kKeyMinusInf)
-                    break;
-                const int e = int(__reduce_min_sync(0xffffffffu, bk == m ? unsigned(bi) : 0x7fffffffu));
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (lane + 32 * i == e)
-                        key[i] = 0;
-                if (lane == j) {
-                    id = e;
-                    mine = m;
-                }
-            }
-            const float ex = id >= 0 ? expf(value_of(mine) - mx) : 0.0f;
+            if (t + 1 < w1)
+                load(t + 1);  // arrives behind the selection
+            uint32_t id_key;
+            top_keys<V>(key, mine, k, list, id, id_key);
+            const float ex = id >= 0 ? __expf(value_of(id_key) - mx) : 0.0f;
             weight = p.normalize ? ex / warp_sum(ex) : ex * inv;
             weight = id >= 0 ? weight * p.scale : 0.0f;
+        } else if (t + 1 < w1) {
+            load(t + 1);
         }
         if (lane < k) {
             int rank = -1;
@@ -169,88 +270,156 @@ template <class T, int V> __global__ void __launch_bounds__(kRouteThreads) route
         live_of[warp] = live;
     }
     __syncthreads();
+    const bool alone = gridDim.x == 1;
     int32_t *counts = p.block_counts + int64_t(blockIdx.x) * (E + 1);
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) {
+    float *sums = p.block_sums + int64_t(blockIdx.x) * (E + 1);
+    int own[(kMaxExperts + kThreads - 1) / kThreads] = {};  // this thread's experts' slots (one expert where a block is alone)
+#pragma unroll
+    for (int i = 0; i < (kMaxExperts + kThreads - 1) / kThreads; ++i) {
+        const int e = tid + i * kThreads;
+        if (e >= E)
+            break;
         int run = 0;
-        for (int w = 0; w < kRouteWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
             const int c = route_smem[w * E + e];
             route_smem[w * E + e] = run;
             run += c;
         }
-        counts[e] = run;
+        own[i] = run;
+        if (!alone)
+            counts[e] = run;
     }
-    if (threadIdx.x == 0) {
-        int n = 0;
-        float s = 0.0f;
-        for (int w = 0; w < kRouteWarps; ++w) {
-            n += live_of[w];
-            s += z_of[w];
-        }
+    int n = 0;
+    float zs = 0.0f;
+    for (int w = 0; w < W; ++w) {
+        n += live_of[w];
+        zs += z_of[w];
+    }
+    if (!alone && tid == 0) {
         counts[E] = n;
-        p.block_sums[int64_t(blockIdx.x) * (E + 1) + E] = s;
+        sums[E] = zs;
+    }
+    int at = 0, total = 0;
+    if (alone) {  // route_place's part too: the experts' first places into the warps' counters
+        at = block_scan(own[0], total);
+        if (tid < E)
+            for (int w = 0; w < W; ++w)
+                route_smem[w * E + tid] += at;
     }
     __syncthreads();
     for (int64_t s = w0 * k + lane; s < w1 * k; s += 32) {
         const int id = p.ids[s];
-        if (id >= 0)
-            p.dest[s] += hist[id];
+        if (id >= 0) {
+            const int d = p.dest[s] + hist[id];
+            p.dest[s] = d;
+            if (alone)
+                p.src[d] = int(s);
+        }
+    }
+    if (alone)
+        for (int64_t r = total + tid; r < p.tokens * k; r += kThreads)
+            p.src[r] = -1;
+    if (!p.prob && !p.losses) {
+        if (alone)
+            route_totals(p, own[0], at, total, 0.0f, n, zs);
+        return;
     }
     __syncthreads();
-    float *sums = reinterpret_cast<float *>(route_smem);
+    float *part = reinterpret_cast<float *>(route_smem);
 #pragma unroll
     for (int i = 0; i < V; ++i)
         if (lane + 32 * i < E)
-            sums[warp * E + lane + 32 * i] = acc[i];
+            part[warp * E + lane + 32 * i] = acc[i];
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) {
+    float mine = 0.0f;
+    for (int e = tid; e < E; e += kThreads) {
         float s = 0.0f;
-        for (int w = 0; w < kRouteWarps; ++w)
-            s += sums[w * E + e];
-        p.block_sums[int64_t(blockIdx.x) * (E + 1) + e] = s;
+        for (int w = 0; w < W; ++w)
+            s += part[w * E + e];
+        if (!alone)
+            sums[e] = s;
+        mine = s;
     }
+    if (alone)
+        route_totals(p, own[0], at, total, mine, n, zs);
 }
 
 // Every block sums the blocks' counts (all of them for the experts' offsets, those before it for its own
-// slots), places its slots and writes its part of src's unused end; block 0 writes the totals.
-__global__ void __launch_bounds__(kRouteThreads) route_place(const RouteParams p) {
+// slots), places its slots and writes its part of src's unused end; one block more writes the totals and losses. Its 1024
+// threads share the blocks' rows of an expert, so that 148 rows of 256 experts take 37 loads a thread.
+__global__ void __launch_bounds__(kPlaceThreads) route_place(const RouteParams p) {
+    __shared__ int part[2][kPlaceThreads];
     __shared__ int base[kMaxExperts];
-    __shared__ float red[kRouteWarps];
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    const int E = p.experts, k = p.top_k, tid = threadIdx.x;
-    constexpr int kPer = kMaxExperts / kRouteThreads;
-    int tot[kPer], pre[kPer], sum = 0;
-    const int per = (E + kRouteThreads - 1) / kRouteThreads;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        tot[i] = pre[i] = 0;
-        const int e = tid * per + i;
-        if (i < per && e < E)
-            for (int b = 0; b < p.blocks; ++b) {
-                const int c = p.block_counts[int64_t(b) * (E + 1) + e];
-                tot[i] += c;
-                if (b < int(blockIdx.x))
-                    pre[i] += c;
-            }
-        sum += tot[i];
-    }
-    int total;
-    int at = block_scan(sum, total);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = tid * per + i;
-        if (i < per && e < E) {
-            base[e] = at + pre[i];
-            if (blockIdx.x == 0) {
-                p.offsets[e] = at;
-                p.counts[e] = tot[i];
-            }
+    const int E = p.experts, k = p.top_k, tid = threadIdx.x, b = blockIdx.x;
+    const bool last = b == p.blocks;
+    int span = 32;  // a power of two of at least E threads takes one row
+    while (span < E)
+        span *= 2;
+    const int rows = kPlaceThreads / span, e = tid % span, row = tid / span;
+    int tot = 0, pre = 0;
+    float sum = 0.0f;
+    if (e < E) {
+#pragma unroll 8
+        for (int r = row; r < p.blocks; r += rows) {
+            const int c = p.block_counts[int64_t(r) * (E + 1) + e];
+            tot += c;
+            pre += r < b ? c : 0;
         }
-        at += tot[i];
+        if (last && (p.prob || p.losses)) {
+#pragma unroll 8
+            for (int r = row; r < p.blocks; r += rows)
+                sum += p.block_sums[int64_t(r) * (E + 1) + e];
+        }
     }
+    auto across = [&](auto v, auto *words) {  // of the threads of one expert, in order; complete in the first
+        words[tid] = v;
+        __syncthreads();
+        if (tid < span)
+            for (int r = 1; r < rows; ++r)
+                v += words[r * span + tid];
+        __syncthreads();
+        return v;
+    };
+    tot = across(tot, part[0]);
+    pre = across(pre, part[1]);
+    if (last)
+        sum = across(sum, reinterpret_cast<float *>(part[0]));
+    if (tid >= E)
+        tot = 0;
+    int total;
+    const int at = block_scan(tot, total);
+    if (last) {
+        int live = 0;
+        float z = 0.0f;
+        for (int r = tid; r < p.blocks; r += kPlaceThreads) {  // blocks: at most one a thread
+            live += p.block_counts[int64_t(r) * (E + 1) + E];
+            z += p.block_sums[int64_t(r) * (E + 1) + E];
+        }
+        part[0][tid] = live;
+        part[1][tid] = __float_as_int(z);
+        __syncthreads();
+        live = 0;
+        z = 0.0f;
+        if (tid < 32) {
+            for (int r = tid; r < kPlaceThreads; r += 32) {
+                live += part[0][r];
+                z += __int_as_float(part[1][r]);
+            }
+            live = __reduce_add_sync(0xffffffffu, live);
+            z = warp_sum(z);
+            part[0][0] = live;
+        }
+        __syncthreads();
+        route_totals(p, tot, at, total, sum, part[0][0], z);
+        return;
+    }
+    if (tid < E)
+        base[tid] = at + pre;
     __syncthreads();
-    const int64_t first = min(p.tokens, blockIdx.x * p.per_block) * k, end = min(p.tokens, (blockIdx.x + 1) * p.per_block) * k;
-    for (int64_t s = first + tid; s < end; s += kRouteThreads) {
+    const int64_t first = min(p.tokens, b * p.per_block) * k, end = min(p.tokens, (b + 1) * p.per_block) * k;
+    for (int64_t s = first + tid; s < end; s += kPlaceThreads) {
         const int id = p.ids[s];
         if (id >= 0) {
             const int d = p.dest[s] + base[id];
@@ -258,126 +427,109 @@ __global__ void __launch_bounds__(kRouteThreads) route_place(const RouteParams p
             p.src[d] = int(s);
         }
     }
-    for (int64_t r = total + int64_t(blockIdx.x) * kRouteThreads + tid; r < p.tokens * k; r += int64_t(p.blocks) * kRouteThreads)
+    for (int64_t r = total + int64_t(b) * kPlaceThreads + tid; r < p.tokens * k; r += int64_t(p.blocks) * kPlaceThreads)
         p.src[r] = -1;
-    if (blockIdx.x != 0)
-        return;
-    int live = 0;
-    float z = 0.0f;
-    for (int b = 0; b < p.blocks; ++b) {
-        live += p.block_counts[int64_t(b) * (E + 1) + E];
-        z += p.block_sums[int64_t(b) * (E + 1) + E];
-    }
-    if (tid == 0) {
-        p.offsets[E] = total;
-        *p.live = live;
-    }
-    if (!p.prob && !p.losses)
-        return;
-    const float inv = 1.0f / float(max(live, 1));
-    float balance = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = tid * per + i;
-        if (i < per && e < E) {
-            float s = 0.0f;
-            for (int b = 0; b < p.blocks; ++b)
-                s += p.block_sums[int64_t(b) * (E + 1) + e];
-            s *= inv;
-            if (p.prob)
-                p.prob[e] = s;
-            balance += float(tot[i]) * s;
-        }
-    }
-    balance = warp_sum(balance);
-    if ((tid & 31) == 0)
-        red[tid >> 5] = balance;
-    __syncthreads();
-    if (tid == 0 && p.losses) {
-        float s = 0.0f;
-        for (int w = 0; w < kRouteWarps; ++w)
-            s += red[w];
-        p.losses[0] = s * float(E) / float(k) * inv;
-        p.losses[1] = z * inv;
-    }
 }
 
 // One warp a token:  d l_e = p_e (g_e - sum p g - sum_j [plain weights] p_j s dw_j + 2 dz lse / live) + add_e
 // with p = exp(l - lse), g_e = dbal E c_e / (k live^2), and add the slots' own part:
-// p_j s dw_j for plain weights, q_j s (dw_j - sum q dw) for normalised ones (q: softmax over the chosen).
-template <class T, int V> __global__ void __launch_bounds__(kRouteThreads) route_grad(const RouteGradParams p) {
-    extern __shared__ float grad_smem[];  // balance term [experts], then per warp the slots' part [experts]
+// p_j s dw_j for plain weights, q_j s (dw_j - sum q dw) for normalised ones (q: softmax over the chosen). The balance term's g is
+// the same for all tokens and stays in registers, the slots' part meets the row in shared memory. A row is loaded while the one
+// before is computed. Bound by DRAM in the end (logits in, gradient out).
+template <class T, int V> __global__ void __launch_bounds__(kGradThreads) route_grad(const RouteGradParams p) {
+    extern __shared__ float grad_smem[];  // per warp the slots' part [experts], zero between tokens
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int E = p.experts, k = p.top_k;
-    float *bal = grad_smem, *add = grad_smem + E * (1 + warp);
+    float *add = grad_smem + E * warp;
     const float n = float(max(*p.live, 1));
     const float db = p.dlosses ? p.dlosses[0] * float(E) / (float(k) * n * n) : 0.0f;
     const float dz = p.dlosses ? 2.0f * p.dlosses[1] / n : 0.0f;
-    for (int e = threadIdx.x; e < E; e += kRouteThreads)
-        bal[e] = db * float(p.counts[e]);
-    for (int e = lane; e < E; e += 32)
-        add[e] = 0.0f;
-    __syncthreads();
-    for (int64_t t = int64_t(blockIdx.x) * kRouteWarps + warp; t < p.tokens; t += int64_t(gridDim.x) * kRouteWarps) {
-        T *out = static_cast<T *>(p.dlogits) + t * E;
+    float bal[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = lane + 32 * i;
+        bal[i] = e < E ? db * float(p.counts[e]) : 0.0f;
+        if (e < E)
+            add[e] = 0.0f;
+    }
+    __syncwarp();
+    struct Row {
+        float v[V], lse, dw;
+        int id;
+    } next;
+    // what a token's gradient needs: its row, lse, and in lane j slot j's expert and scaled gradient
+    auto load = [&](int64_t t) {
         const float lse = p.lse[t];
-        const bool there = (!p.mask || p.mask[t] != 0) && lse != -INFINITY;
-        if (!there) {
-            for (int e = lane; e < E; e += 32)
-                out[e] = from_f32<T>(0.0f);
+        next.lse = p.mask && p.mask[t] == 0 ? -INFINITY : lse;
+        load_row<T, V>(next.v, static_cast<const T *>(p.logits) + t * E, E, true);
+        next.id = -1;
+        next.dw = 0.0f;
+        if (p.dweights && lane < k) {
+            next.id = p.ids[t * k + lane];
+            next.dw = p.dweights[t * k + lane] * p.scale;
+        }
+    };
+    const int64_t stride = int64_t(gridDim.x) * kGradWarps;
+    int64_t t = int64_t(blockIdx.x) * kGradWarps + warp;
+    if (t < p.tokens)
+        load(t);
+    for (; t < p.tokens; t += stride) {
+        Row r = next;
+        if (t + stride < p.tokens)
+            load(t + stride);
+        T *out = static_cast<T *>(p.dlogits) + t * E;
+        if (r.lse == -INFINITY) {  // not live
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (lane + 32 * i < E)
+                    out[lane + 32 * i] = from_f32<T>(0.0f);
             continue;
         }
-        const T *row = static_cast<const T *>(p.logits) + t * E;
-        float v[V], dot = 0.0f;
-        load_row<T, V>(v, row, E, true);
+        float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            v[i] = expf(v[i] - lse);
-            if (lane + 32 * i < E)
-                dot += v[i] * bal[lane + 32 * i];
-        }
-        int id = -1;
-        if (p.dweights && lane < k) {
-            id = p.ids[t * k + lane];
-            if (id < -1 || id >= E) {
-                report(p.status, kSiteExpert);
-                id = -1;
-            }
+            r.v[i] = __expf(r.v[i] - r.lse);
+            dot = fmaf(r.v[i], bal[i], dot);
         }
         if (p.dweights) {
-            const float l = id >= 0 ? to_f32(row[id]) : -INFINITY;
-            const float dw = id >= 0 ? p.dweights[t * k + lane] * p.scale : 0.0f;
+            if (r.id < -1 || r.id >= E) {
+                report(p.status, kSiteExpert);
+                r.id = -1;
+            }
+            const bool slot = r.id >= 0;
+            const float l = slot ? to_f32(static_cast<const T *>(p.logits)[t * E + r.id]) : -INFINITY;
+            const float dw = slot ? r.dw : 0.0f;
             float mine;
             if (p.normalize) {
                 float mx = l;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1)
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const float ex = id >= 0 ? expf(l - mx) : 0.0f;
+                const float ex = slot ? __expf(l - mx) : 0.0f;
                 const float sum = warp_sum(ex);
-                const float q = id >= 0 ? ex / sum : 0.0f;
+                const float q = slot ? ex / sum : 0.0f;
                 mine = q * (dw - warp_sum(q * dw));
             } else {
-                mine = id >= 0 ? expf(l - lse) * dw : 0.0f;
+                mine = slot ? __expf(l - r.lse) * dw : 0.0f;
                 dot += mine;
             }
-            if (id >= 0)
-                atomicAdd(&add[id], mine);  // one addend a place: a token's experts are distinct
+            if (slot)
+                atomicAdd(&add[r.id], mine);  // one addend a place: a token's experts are distinct
         }
         dot = warp_sum(dot);
         __syncwarp();
-        const float c = dz * lse - dot;
+        const float c = dz * r.lse - dot;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int e = lane + 32 * i;
             if (e < E)
-                out[e] = from_f32<T>(v[i] * (bal[e] + c) + add[e]);
+                out[e] = from_f32<T>(fmaf(r.v[i], bal[i] + c, add[e]));
         }
         __syncwarp();
-        if (id >= 0)
-            add[id] = 0.0f;
+        if (r.id >= 0)
+            add[r.id] = 0.0f;
         __syncwarp();
     }
 }
