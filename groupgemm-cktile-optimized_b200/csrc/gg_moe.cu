@@ -456,7 +456,9 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     std::snprintf(detail, sizeof(detail), "gg_w4<%s,%s> n=%lld k=%lld group=%d blocks=%d", type_name(q.dtype), few ? "few" : "many",
                   static_cast<long long>(q.n), static_cast<long long>(q.k), q.group_size, blocks);
     MoeLaunch gather{v.gather, unsigned(std::min<int64_t>(q.rows, 65536)), gg::moe::kW4GatherThreads, 0};
-    gather.grid_y = unsigned((steps * 16 + gg::moe::kW4GatherThreads - 1) / gg::moe::kW4GatherThreads);
+// a block a row, and of few rows one for each 128 pieces
+    gather.grid_y = unsigned(std::max<int64_t>(1, std::min<int64_t>((steps * 16 + gg::moe::kW4GatherThreads - 1) / gg::moe::kW4GatherThreads,
+                                                                    4 * num_sms / std::max<int64_t>(1, q.rows))));
     return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), unsigned(v.threads), v.smem, true}}, detail);
 }
 

@@ -113,10 +113,12 @@ template <int V> __device__ __forceinline__ void top_keys(uint32_t (&key)[V], ui
         __syncwarp();
         const uint32_t mykey = lane < total ? list[lane] : 0u, myid = list[32 + lane];
         int rank = 0;
-        for (int q = 0; q < total; ++q) {
-            const uint32_t other = __shfl_sync(0xffffffffu, mykey, q);
-            rank += other > mykey || (other == mykey && q < lane);
-        }
+        for (int q0 = 0; q0 < total; q0 += 4)  // past the end the keys are 0
+#pragma unroll
+            for (int q = q0; q < q0 + 4; ++q) {
+                const uint32_t other = __shfl_sync(0xffffffffu, mykey, q);
+                rank += other > mykey || (other == mykey && q < lane);
+            }
         if (lane < total && rank < k) {
             list[64 + rank] = mykey;
             list[96 + rank] = myid;
@@ -175,10 +177,10 @@ __device__ __forceinline__ void route_totals(const RouteParams &p, int tot, int 
     if ((e & 31) == 0)
         red[e >> 5] = balance;
     __syncthreads();
+    if (e >= 32)
+        return;
+    const float s = warp_sum(e < int(blockDim.x) >> 5 ? red[e] : 0.0f);
     if (e == 0) {
-        float s = 0.0f;
-        for (int w = 0; w < int(blockDim.x) >> 5; ++w)
-            s += red[w];
         p.losses[0] = s * float(E) / float(p.top_k) * inv;
         p.losses[1] = z * inv;
     }
@@ -200,6 +202,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
     const int64_t begin = blockIdx.x * p.per_block, end = min(p.tokens, begin + p.per_block);
     const int64_t per_warp = (p.per_block + W - 1) / W;
     const int64_t w0 = min(end, begin + warp * per_warp), w1 = min(end, w0 + per_warp);
+    const int busy = int((end - begin + per_warp - 1) / per_warp);  // warps that have tokens
     int32_t *hist = route_smem + warp * E;
     uint32_t *list = reinterpret_cast<uint32_t *>(route_smem + W * E + warp * 128);
     float v[V];
@@ -280,7 +283,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
         if (e >= E)
             break;
         int run = 0;
-        for (int w = 0; w < W; ++w) {
+        for (int w = 0; w < busy; ++w) {
             const int c = route_smem[w * E + e];
             route_smem[w * E + e] = run;
             run += c;
@@ -291,7 +294,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
     }
     int n = 0;
     float zs = 0.0f;
-    for (int w = 0; w < W; ++w) {
+    for (int w = 0; w < busy; ++w) {
         n += live_of[w];
         zs += z_of[w];
     }
@@ -303,7 +306,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
     if (alone) {  // route_place's part too: the experts' first places into the warps' counters
         at = block_scan(own[0], total);
         if (tid < E)
-            for (int w = 0; w < W; ++w)
+            for (int w = 0; w < busy; ++w)
                 route_smem[w * E + tid] += at;
     }
     __syncthreads();
@@ -334,7 +337,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
     float mine = 0.0f;
     for (int e = tid; e < E; e += kThreads) {
         float s = 0.0f;
-        for (int w = 0; w < W; ++w)
+        for (int w = 0; w < busy; ++w)
             s += part[w * E + e];
         if (!alone)
             sums[e] = s;
@@ -358,20 +361,37 @@ __global__ void __launch_bounds__(kPlaceThreads) route_place(const RouteParams p
     while (span < E)
         span *= 2;
     const int rows = kPlaceThreads / span, e = tid % span, row = tid / span;
+    // the thread's first slot, on its way while the counts are summed
+    const int64_t first = min(p.tokens, b * p.per_block) * k, end = min(p.tokens, (b + 1) * p.per_block) * k;
+    int id0 = -1, rank0 = 0;
+    if (!last && first + tid < end) {
+        id0 = p.ids[first + tid];
+        rank0 = p.dest[first + tid];
+    }
     int tot = 0, pre = 0;
     float sum = 0.0f;
     if (e < E) {
-#pragma unroll 8
-        for (int r = row; r < p.blocks; r += rows) {
-            const int c = p.block_counts[int64_t(r) * (E + 1) + e];
-            tot += c;
-            pre += r < b ? c : 0;
+        for (int r0 = row; r0 < p.blocks; r0 += 8 * rows) {  // eight rows' loads at a time (16 and more at once were slower)
+            int c[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                c[i] = r0 + i * rows < p.blocks ? __ldcg(p.block_counts + (r0 + i * rows) * (E + 1) + e) : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                tot += c[i];
+                pre += r0 + i * rows < b ? c[i] : 0;
+            }
         }
-        if (last && (p.prob || p.losses)) {
-#pragma unroll 8
-            for (int r = row; r < p.blocks; r += rows)
-                sum += p.block_sums[int64_t(r) * (E + 1) + e];
-        }
+        if (last && (p.prob || p.losses))
+            for (int r0 = row; r0 < p.blocks; r0 += 8 * rows) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    f[i] = r0 + i * rows < p.blocks ? __ldcg(p.block_sums + (r0 + i * rows) * (E + 1) + e) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    sum += f[i];
+            }
     }
     auto across = [&](auto v, auto *words) {  // of the threads of one expert, in order; complete in the first
         words[tid] = v;
@@ -418,11 +438,11 @@ __global__ void __launch_bounds__(kPlaceThreads) route_place(const RouteParams p
     if (tid < E)
         base[tid] = at + pre;
     __syncthreads();
-    const int64_t first = min(p.tokens, b * p.per_block) * k, end = min(p.tokens, (b + 1) * p.per_block) * k;
     for (int64_t s = first + tid; s < end; s += kPlaceThreads) {
-        const int id = p.ids[s];
+        const bool head = s == first + tid;
+        const int id = head ? id0 : p.ids[s];
         if (id >= 0) {
-            const int d = p.dest[s] + base[id];
+            const int d = (head ? rank0 : p.dest[s]) + base[id];
             p.dest[s] = d;
             p.src[d] = int(s);
         }

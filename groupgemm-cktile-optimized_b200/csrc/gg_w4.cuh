@@ -266,8 +266,7 @@ __device__ __forceinline__ void w4_join(const W4Params &p, const W4Work &work, c
 //   kFragments: as mma.sync's B fragments of 8 tokens (a word of k after another, 16 bytes a lane),
 //   else:       as a shared-memory image of tcgen05's B (K-major, two halves of 64 k, each a row of 128 bytes a token with the
 //               128-byte swizzle).
-// Token count rounded up to 8: what the places of the missing tokens hold goes into columns that nothing reads. One piece
-// a thread. (Done by warps of the product kernel instead, with cp.async and shared memory, this took them 1400 cycles a step
+// Token count rounded up to 8: what the places of the missing tokens hold goes into columns that nothing reads. (Done by warps of the product kernel instead, with cp.async and shared memory, this took them 1400 cycles a step
 // at 16 tokens: twice what HBM allows.) Rows of no expert are set to zero in out.
 constexpr int kW4GatherThreads = 128;
 template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherThreads) w4_gather(const __grid_constant__ W4Params p) {
@@ -278,16 +277,21 @@ template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherT
     ptx::griddep_launch_dependents();
     W4Work::starts(p, start);
     __syncthreads();
-    const int piece = int(blockIdx.y) * kW4GatherThreads + int(threadIdx.x);  // of a row
-    const int step = piece >> 4, c = piece & 15;
+    const int pieces = p.steps * (kW4StepK / 8), first_piece = int(blockIdx.y) * kW4GatherThreads + int(threadIdx.x);
+    const int more = int(gridDim.y) * kW4GatherThreads;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         if (r < start[0] || r >= start[p.experts]) {
-            for (int col = piece; col < p.n; col += int(gridDim.y) * kW4GatherThreads)
+            for (int col = first_piece; col < p.n; col += more)
                 static_cast<T *>(p.out)[r * p.n + col] = from_f32<T>(0.0f);
             continue;
         }
-        if (step >= p.steps)
-            continue;
+        int64_t row = r;
+        if (p.src) {
+            const int s = p.src[r];
+            row = s < 0 || s >= p.slots ? -1 : s / p.top_k;
+            if (row < 0 && first_piece == 0)
+                report(p.status, kSiteSrc);
+        }
         int lo = 0, hi = p.experts - 1;  // the last expert that starts at or before the row
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -300,22 +304,20 @@ template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherT
         const int count = (min(p.chunk, start[lo + 1] - (int(r) - i)) + 7) & ~7;
         if (i >= count)
             continue;  // falling offsets, reported
-        int64_t row = r;
-        if (p.src) {
-            const int s = p.src[r];
-            row = s < 0 || s >= p.slots ? -1 : s / p.top_k;
-            if (row < 0 && piece == 0)
-                report(p.status, kSiteSrc);
+        const T *from = static_cast<const T *>(p.x) + row * p.k;
+        uint8_t *to = p.xs + int64_t(int(r) - i + 8 * lo) * p.steps * kW4TokenBytes;
+#pragma unroll 4
+        for (int piece = first_piece; piece < pieces; piece += more) {
+            const int step = piece >> 4, c = piece & 15;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row >= 0 && piece * 8 < p.k)
+                v = __ldg(reinterpret_cast<const uint4 *>(from + piece * 8));
+            const int at = kFragments ? (((i >> 3) * 4 + (c >> 2)) * 32 + (i & 7) * 4 + (c & 3)) * 16
+                                      : ((c >> 3) * count + i) * 128 + (((c & 7) ^ (i & 7)) << 4);
+            *reinterpret_cast<uint4 *>(to + int64_t(step) * count * kW4TokenBytes + at) =
+                make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                           __byte_perm(v.y, v.w, 0x7632));
         }
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row >= 0 && piece * 8 < p.k)
-            v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + row * p.k + piece * 8);
-        const int64_t base = int64_t(int(r) - i + 8 * lo) * p.steps + int64_t(step) * count;
-        const int at = kFragments ? (((i >> 3) * 4 + (c >> 2)) * 32 + (i & 7) * 4 + (c & 3)) * 16
-                                  : ((c >> 3) * count + i) * 128 + (((c & 7) ^ (i & 7)) << 4);
-        *reinterpret_cast<uint4 *>(p.xs + base * kW4TokenBytes + at) =
-            make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                       __byte_perm(v.y, v.w, 0x7632));
     }
 }
 
