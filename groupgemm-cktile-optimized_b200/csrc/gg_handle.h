@@ -27,7 +27,7 @@ struct MoeLaunch {
 
 struct MoePlan {
     int launches = 0;  // 0: the handle holds no layer operator
-    MoeLaunch launch[2];
+    MoeLaunch launch[3];
     CUtensorMap map{};
     alignas(16) unsigned char params[256];
 };

@@ -369,7 +369,7 @@ int prepare_permute(gg_handle *h, const gg_permute_problem &q, int32_t op, gg_st
 // ---- 4-bit products ----
 
 struct W4Form {
-    const void *fn, *gather;
+    const void *fn, *gather, *add;
     int tokens;  // of a chunk
     int threads, ctas_per_sm;
     size_t smem;
@@ -378,8 +378,8 @@ template <class T, int G> W4Form w4_form(bool few, bool zeros) {
     using namespace gg::moe;
     if (few)
         return {zeros ? reinterpret_cast<const void *>(&w4_few<T, G, true>) : reinterpret_cast<const void *>(&w4_few<T, G, false>),
-                reinterpret_cast<const void *>(&w4_gather<T, true>), kW4FewTokens, kW4FewThreads, 2, kW4FewSmem};
-    return {reinterpret_cast<const void *>(&w4_many<T, G>), reinterpret_cast<const void *>(&w4_gather<T, false>), W4Many<G>::kTokens,
+                reinterpret_cast<const void *>(&w4_gather<T, true>), reinterpret_cast<const void *>(&w4_add<T>), kW4FewTokens, kW4FewThreads, 2, kW4FewSmem};
+    return {reinterpret_cast<const void *>(&w4_many<T, G>), reinterpret_cast<const void *>(&w4_gather<T, false>), nullptr, W4Many<G>::kTokens,
             kW4ManyThreads, 1, W4Many<G>::kSmemBytes};
 }
 template <class T> W4Form w4_form(int group, bool few, bool zeros) {
@@ -421,7 +421,18 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     const int ctas = v.ctas_per_sm * num_sms;
     const int blocks = q.rows > 0 ? ctas : 0;
     const int64_t steps = (q.k + gg::moe::kW4StepK - 1) / gg::moe::kW4StepK;
-    const size_t sums = size_t(2 * ctas) * size_t(v.tokens) * gg::moe::kW4TileRows * 4;
+    // partial sums: of the two cut tiles of a CTA, or (few) of the units of split items; counters: an arrival count a CTA, or the next unit
+    const int64_t tiles = (q.n + gg::moe::kW4TileRows - 1) / gg::moe::kW4TileRows;
+    const int64_t items = std::min<int64_t>(q.rows, q.experts + q.rows / v.tokens) * tiles;
+    int64_t span = steps;
+    if (few && items < gg::moe::kW4FewUnits * int64_t(ctas)) {
+        const int64_t most = (gg::moe::kW4FewUnits * int64_t(ctas) + items - 1) / std::max<int64_t>(1, items);  // splits
+        span = std::max(std::min<int64_t>(8, steps), (steps + most - 1) / most);
+    }
+    const int64_t splits = (steps + span - 1) / span;
+    const size_t sums = size_t(!few ? 2 * ctas : splits > 1 ? items * splits : 0) * size_t(v.tokens) * gg::moe::kW4TileRows * 4;
+    if (items > (int64_t(1) << 27))
+        return refuse(h, why, why_len, "too many weight rows and experts for one launch");
     if (const int rc = reserve(h, sums + size_t(q.rows + 8 * int64_t(q.experts)) * size_t(steps) * gg::moe::kW4TokenBytes))
         return rc;
     if (const int rc = reserve_counters(h, size_t(ctas) * 4, stream))
@@ -447,6 +458,9 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     p.tiles = int((q.n + gg::moe::kW4TileRows - 1) / gg::moe::kW4TileRows);
     p.steps = int(steps);
     p.chunk = v.tokens;
+    p.max_items = items;
+    p.splits = int(splits);
+    p.span = int(span);
     p.ws = h->d_ws;
     p.xs = reinterpret_cast<uint8_t *>(h->d_ws) + sums;
     p.counters = h->d_counters;
@@ -459,7 +473,9 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
 // a block a row, and of few rows one for each 128 pieces
     gather.grid_y = unsigned(std::max<int64_t>(1, std::min<int64_t>((steps * 16 + gg::moe::kW4GatherThreads - 1) / gg::moe::kW4GatherThreads,
                                                                     4 * num_sms / std::max<int64_t>(1, q.rows))));
-    return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), unsigned(v.threads), v.smem, true}}, detail);
+    const MoeLaunch add{few && splits > 1 ? v.add : nullptr, few && splits > 1 ? unsigned(std::min<int64_t>(items, 4 * num_sms)) : 0u,
+                        gg::moe::kW4TileRows, 0};
+    return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), unsigned(v.threads), v.smem, true}, add}, detail);
 }
 
 }  // namespace

@@ -38,9 +38,11 @@ struct W4Params {
     float *ws;               // [2 x grid][tokens of a chunk][256] partial sums
     int32_t *counters;       // [grid] arrivals at a cut tile, 0 between launches
     int64_t rows, slots;     // slots: tokens * top_k
+    int64_t max_items;       // that rising offsets can give
     uint64_t timeout_ns;
     int n, k, groups, experts, top_k, tiles, steps;  // steps: of 128 k
-    int chunk;  // tokens of a chunk
+    int chunk;         // tokens of a chunk
+    int splits, span;  // w4_few: units of an item, steps of a unit
 };
 
 // `bytes` (a multiple of 16) from global to shared memory, counted on an mbarrier; where pred != 0.
@@ -185,18 +187,18 @@ struct W4Work {
         begin = cta < ctas ? total * cta / ctas : 0;
         end = cta < ctas ? total * (cta + 1) / ctas : 0;
     }
-    __device__ __forceinline__ W4Item at(const W4Params &p, int64_t item) const {
-        int lo = 0, hi = p.experts - 1;  // the last expert whose first chunk's items start at or before the item
+    __device__ __forceinline__ W4Item at(const W4Params &p, int item) const {
+        const int run = item / p.tiles;  // token chunk of the launch, were a chunk's tiles in a row
+        int lo = 0, hi = p.experts - 1;  // the last expert whose first chunk is at or before it
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (int64_t(first[mid]) * p.tiles <= item)
+            if (first[mid] <= run)
                 lo = mid;
             else
                 hi = mid - 1;
         }
-        const int chunks = first[lo + 1] - first[lo];
-        const int64_t in = item - int64_t(first[lo]) * p.tiles;
-        const int tile = int(in / chunks), chunk = int(in - int64_t(tile) * chunks);
+        const int chunks = first[lo + 1] - first[lo], in = item - first[lo] * p.tiles;
+        const int tile = in / chunks, chunk = in - tile * chunks;
         const int r0 = start[lo] + chunk * p.chunk;
         return {lo, tile * kW4TileRows, r0, min(p.chunk, start[lo + 1] - r0)};
     }
@@ -205,7 +207,7 @@ struct W4Work {
         for (int64_t s = begin; s < end;) {
             const int64_t item = s / p.steps;
             const int k0 = int(s - item * p.steps), n = int(min(int64_t(p.steps - k0), end - s));
-            f(at(p, item), item, k0, n);
+            f(at(p, int(item)), item, k0, n);
             s += n;
         }
     }
@@ -240,7 +242,7 @@ __device__ __forceinline__ void w4_join(const W4Params &p, const W4Work &work, c
             continue;
         if (t == 0)
             p.counters[c0] = 0;
-        const W4Item it = work.at(p, cut[i]);
+        const W4Item it = work.at(p, int(cut[i]));
         if (it.n0 + t >= p.n)
             continue;
         T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + it.n0 + t;
@@ -329,7 +331,9 @@ template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherT
 // 22 us for 117 MB of weights (5.3 TB/s, 82% of the measured copy rate) at 1 row an expert, 24 at 8. Above that mma.sync's own rate
 // binds (11 cycles an instruction and scheduler: 16 tokens in one pass 36 us).
 constexpr int kW4FewTokens = 8;
-constexpr int kW4FewThreads = kW4TileRows + 64;
+constexpr int kW4FewThreads = kW4TileRows + 32;
+constexpr int kW4FewUnits = 4;  // units of work a CTA, where items have to be split for that
+constexpr int kW4FewRing = 8;   // units that the loading warp may be ahead: stages and two
 constexpr int kW4FewStages = 4;
 constexpr int kW4FewSmem = 1024 + kW4FewStages * (kW4WeightBytes + kW4FewTokens * kW4TokenBytes);
 
@@ -374,13 +378,14 @@ template <int kBytes> struct W4Queue {
     uint32_t shift;                            // bits from the word's start to the value
     uint32_t raw[kWords + 1], word[kWords];
 
-    __device__ __forceinline__ W4Queue(const void *array, int64_t row, const void *array_end, int first) : at(first) {
+    // From now on the row's values from `first` on: the visit is on its way, to be taken by the next refill.
+    __device__ __forceinline__ void begin(const void *array, int64_t row, const void *array_end, int first) {
+        at = first;
         const uintptr_t p = reinterpret_cast<uintptr_t>(array) + uintptr_t((row + first) * kBytes);
         from = reinterpret_cast<const uint32_t *>(p & ~uintptr_t(3));
         shift = uint32_t(p & 3) * 8;
         end = static_cast<const uint32_t *>(array_end);
-        if (array)
-            load();
+        load();
     }
     __device__ __forceinline__ void load() {
 #pragma unroll
@@ -388,12 +393,13 @@ template <int kBytes> struct W4Queue {
             raw[i] = from + i < end ? __ldg(from + i) : 0u;
         from += kWords;
     }
-    __device__ __forceinline__ void refill(int groups) {
+    // Eight values into the queue, and the next visit on its way where there is one before group `last`.
+    __device__ __forceinline__ void refill(int last) {
 #pragma unroll
         for (int i = 0; i < kWords; ++i)
             word[i] = __funnelshift_r(raw[i], raw[i + 1], shift);
         at += 8;
-        if (at < groups)
+        if (at < last)
             load();
     }
     __device__ __forceinline__ uint32_t take() {
@@ -405,15 +411,60 @@ template <int kBytes> struct W4Queue {
     }
 };
 
+// Items of the launch; none where falling and rising offsets (reported) make more of them than the workspace holds.
+__device__ __forceinline__ int w4_items(const W4Params &p, const int *first) {
+    const int64_t items = int64_t(first[p.experts]) * p.tiles;
+    return items > p.max_items ? 0 : int(items);
+}
+// A unit's sums [token][256], where items are split.
+__device__ __forceinline__ float *w4_sums(const W4Params &p, int item, int split) {
+    return p.ws + (int64_t(item) * p.splits + split) * (kW4FewTokens * kW4TileRows);
+}
+
+// Adds the sums of split items, in order of k. A kernel of its own: joined inside w4_few, by the last unit of an item to arrive, each
+// arrival's fence waited some microseconds behind the streaming weights, and one unit more a CTA cost as much.
+template <class T> __global__ void __launch_bounds__(kW4TileRows) w4_add(const __grid_constant__ W4Params p) {
+    __shared__ int start[kW4MaxExperts + 1], first[kW4MaxExperts + 1];
+    ptx::griddep_launch_dependents();
+    const W4Work work(p, start, first);  // the offsets are older than w4_few
+    const int items = w4_items(p, first), t = threadIdx.x;
+    bool waited = false;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const W4Item it = work.at(p, item);
+        if (!waited)
+            ptx::griddep_wait();
+        waited = true;
+        float v[kW4FewTokens] = {};
+#pragma unroll 4
+        for (int split = 0; split < p.splits; ++split)
+#pragma unroll
+            for (int u = 0; u < kW4FewTokens; ++u)
+                if (u < it.count)
+                    v[u] += __ldcg(w4_sums(p, item, split) + u * kW4TileRows + t);
+        if (it.n0 + t >= p.n)
+            continue;
+#pragma unroll
+        for (int u = 0; u < kW4FewTokens; ++u)
+            if (u < it.count)
+                static_cast<T *>(p.out)[int64_t(it.r0 + u) * p.n + it.n0 + t] = from_f32<T>(v[u]);
+    }
+    if (!waited)
+        ptx::griddep_wait();  // this kernel ends after w4_few
+}
+
 template <class T, int G, bool kZeros>
 __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ W4Params p) {
     constexpr int kSub = kW4StepK / G;  // groups a step
     constexpr int kXBytes = kW4FewTokens * kW4TokenBytes;
     extern __shared__ __align__(1024) uint8_t w4_smem[];
     __shared__ int start[kW4MaxExperts + 1], first[kW4MaxExperts + 1];
-    __shared__ uint64_t bar_words[2 * kW4FewStages];
+    __shared__ uint64_t bar_words[2 * kW4FewStages + 1];
+    struct Unit {
+        W4Item it;
+        int item, split, k0, n;  // n: steps; 0: no more units
+    };
+    __shared__ Unit ring[kW4FewRing];  // the CTA's units, each there before the last eight groups of the one before it are
     __shared__ uint32_t abort_word;
-    __shared__ int arrived[2];
     volatile uint32_t *abort_flag = &abort_word;
     const uint32_t smem = (ptx::smem_addr(w4_smem) + 1023) & ~1023u, bars = ptx::smem_addr(bar_words);
     auto w_at = [&](int s) { return smem + uint32_t(s * kW4WeightBytes); };
@@ -423,9 +474,10 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x, g = lane >> 2, t = lane & 3;
     if (tid == 0) {
         for (int s = 0; s < kW4FewStages; ++s) {
-            ptx::mbar_init(full(s), 2);  // weights and tokens
+            ptx::mbar_init(full(s), 1);
             ptx::mbar_init(empty(s), 8);
         }
+        ptx::mbar_init(bars + 8u * (2 * kW4FewStages), 1);
         *abort_flag = 0u;
         ptx::fence_mbar_init();
         ptx::fence_proxy_async_smem();
@@ -435,6 +487,7 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
     ptx::fence_proxy_async_global();
     ptx::griddep_launch_dependents();
     const W4Work work(p, start, first);
+    const int items = w4_items(p, first), units = items * p.splits, ctas = min(int(gridDim.x), units);
     const Abort ab{p.status + 2, abort_flag, p.timeout_ns};
     int st = 0;
     uint32_t ph = 0;
@@ -445,52 +498,111 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
         }
     };
     bool ok = true;
-    if (warp >= 8) {
-        const bool tokens = warp == 9;
+    if (warp == 8) {
         const uint32_t leader = ptx::elect_one_sync();
-        if (tokens) {  // what precedes the launch of w4_gather is done (see there), its own writes only now
-            ptx::griddep_wait();
-            ptx::fence_proxy_async_global();
-        }
-        work.pieces(p, [&](const W4Item &it, int64_t, int k0, int n) {
-            const uint8_t *from = p.xs + (int64_t(it.r0 + 8 * it.e) * p.steps + int64_t(k0) * kW4FewTokens) * kW4TokenBytes;
-            for (int j = 0; ok && j < n; ++j) {
+        auto publish = [&](int seq, int u) {
+            Unit r{};
+            if (u < units) {
+                r.item = u / p.splits;
+                r.split = u - r.item * p.splits;
+                r.k0 = r.split * p.span;
+                r.n = min(p.span, p.steps - r.k0);
+                r.it = work.at(p, r.item);
+            }
+            if (leader)
+                ring[seq % kW4FewRing] = r;
+            return r;
+        };
+        bool gathered = false;
+        auto ask = [&]() {  // for the CTA's next unit; the last of the launch's askers puts the counter back
+            int v = 0;
+            if (lane == 0) {
+                v = atomicAdd(p.counters, 1);
+                if (v == units - 1)
+                    *p.counters = 0;
+            }
+            return v;
+        };
+        Unit r = publish(0, int(blockIdx.x));
+        int asked = r.n > 0 ? ask() : 0;
+        ptx::mbar_arrive_expect_tx(bars + 8u * (2 * kW4FewStages), 0, leader);  // the first unit is there
+        for (int seq = 1; ok && r.n > 0; ++seq) {
+            Unit after{};
+            const uint8_t *from = p.xs + (int64_t(r.it.r0 + 8 * r.it.e) * p.steps + int64_t(r.k0) * kW4FewTokens) * kW4TokenBytes;
+            auto weights = [&](int j) {
+                if (j == max(0, r.n - 8 / kSub)) {  // before the consumers' last visit to this unit's scales
+                    after = publish(seq, ctas + __shfl_sync(0xffffffffu, asked, 0));
+                    if (after.n > 0)
+                        asked = ask();
+                }
+                ptx::mbar_arrive_expect_tx(full(st), kW4WeightBytes + kXBytes, leader);
+                ptx::tma_load_3d(w_at(st), &tmap_w, full(st), (r.k0 + j) * (kW4StepK / 2), r.it.n0, r.it.e, leader);
+            };
+            auto tokens = [&](int j, int s) { bulk_load(x_at(s), from + j * kXBytes, kXBytes, full(s), leader); };
+            int j = 0;
+            if (!gathered) {
+                // What precedes the launch of w4_gather is done (see there), its own writes only after this wait: the first steps' weights
+                // are asked for before it.
+                const int ahead = min(kW4FewStages, r.n);
+                for (; j < ahead; ++j) {
+                    weights(j);
+                    next();
+                }
+                ptx::griddep_wait();
+                ptx::fence_proxy_async_global();
+                for (int i = 0; i < ahead; ++i)
+                    tokens(i, i);
+                gathered = true;
+            }
+            for (; ok && j < r.n; ++j) {
                 ok = w4_wait(empty(st), ph ^ 1u, ab, kStatusTimeout | kRoleProducer | uint32_t(st));
                 if (!ok)
                     break;
-                if (tokens) {
-                    ptx::mbar_arrive_expect_tx(full(st), kXBytes, leader);
-                    bulk_load(x_at(st), from, kXBytes, full(st), leader);
-                    from += kXBytes;
-                } else {
-                    ptx::mbar_arrive_expect_tx(full(st), kW4WeightBytes, leader);
-                    ptx::tma_load_3d(w_at(st), &tmap_w, full(st), (k0 + j) * (kW4StepK / 2), it.n0, it.e, leader);
-                }
+                weights(j);
+                tokens(j, st);
                 next();
             }
-        });
+            r = after;
+        }
+        if (!gathered)
+            ptx::griddep_wait();  // this kernel ends after w4_gather
     } else {
         // of ldmatrix: row lane % 8 of the warp's, piece lane / 8 swizzled
         const uint32_t w_lane = uint32_t((warp * 32 + (lane & 7)) * 64) + (uint32_t((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
-        int64_t cut[2] = {-1, -1};
-        work.pieces(p, [&](const W4Item &it, int64_t item, int k0, int n) {
+        // Scales and zeros of weight row `lane`, to be handed to the lanes whose fragments hold the row. A row's lie next to
+        // each other, the rows far apart, so each visit to a row's line takes eight groups: into `raw`, one visit ahead, and from
+        // there, moved to the row's odd alignment, into queues that give up their low end.
+        W4Queue<2> scales;
+        W4Queue<1> zeros;
+        auto begin = [&](const Unit &r) {
+            const int64_t meta = (int64_t(r.it.e) * p.n + min(r.it.n0 + warp * 32 + lane, p.n - 1)) * p.groups;
+            scales.begin(p.scales, meta, p.scales_end, r.k0 * kSub);
+            if constexpr (kZeros)
+                zeros.begin(p.zeros, meta, p.zeros_end, r.k0 * kSub);
+        };
+        ok = w4_wait(bars + 8u * (2 * kW4FewStages), 0, ab, kStatusTimeout | kRoleMma | 0x80u);
+        Unit r{};
+        if (ok)
+            r = ring[0];
+        if (r.n > 0)
+            begin(r);
+        for (int seq = 1; ok && r.n > 0; ++seq) {
             float sum[2][4] = {};
-            // Scales and zeros of weight row `lane`, to be handed to the lanes whose fragments hold the row. A row's lie next to
-            // each other, the rows far apart, so each visit to a row's line takes eight groups: into `raw`, one visit ahead, and from
-            // there, moved to the row's odd alignment, into queues that give up their low end.
-            const int64_t meta = (int64_t(it.e) * p.n + min(it.n0 + warp * 32 + lane, p.n - 1)) * p.groups;
-            W4Queue<2> scales(p.scales, meta, p.scales_end, k0 * kSub);
-            W4Queue<1> zeros(p.zeros, meta, p.zeros_end, k0 * kSub);
             int queued = 0;  // groups in the queues
-            for (int j = 0; j < n; ++j) {
+            for (int j = 0; j < r.n; ++j) {
                 ok = w4_wait(full(st), ph, ab, kStatusTimeout | kRoleMma | uint32_t(st));
                 if (!ok)
                     break;
                 if (queued == 0) {
-                    scales.refill(p.groups);
+                    scales.refill((r.k0 + r.n) * kSub);
                     if constexpr (kZeros)
-                        zeros.refill(p.groups);
+                        zeros.refill((r.k0 + r.n) * kSub);
                     queued = 8;
+                    if (j + 8 / kSub >= r.n) {  // this unit's last visit: the next one's scales are on their way from here
+                        const Unit after = ring[seq % kW4FewRing];
+                        if (after.n > 0)
+                            begin(after);
+                    }
                 }
                 queued -= kSub;
                 uint32_t w[4][4];  // rows g + 8 i; word c holds k = 32 c + 8 t ...
@@ -546,25 +658,25 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
                 }
                 next();
             }
-            const bool whole = n == p.steps;
-            if (!whole)
-                cut[k0 == 0] = item;
-            float *mine = whole ? nullptr : work.slot(p, blockIdx.x, work.first_cta(p, item));
-            T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + it.n0;
+            if (!ok)
+                break;
+            const W4Item &it = r.it;
+            T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + it.n0 + warp * 32;
+            float *mine = w4_sums(p, r.item, r.split) + warp * 32;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int row = warp * 32 + 16 * m + 8 * (i >> 1) + g, tok = 2 * t + (i & 1);
-                    if (!ok || tok >= it.count || it.n0 + row >= p.n)
+                    const int row = 16 * m + 8 * (i >> 1) + g, tok = 2 * t + (i & 1);
+                    if (tok >= it.count || it.n0 + warp * 32 + row >= p.n)
                         continue;
-                    if (whole)
+                    if (p.splits == 1)
                         out[int64_t(tok) * p.n + row] = from_f32<T>(sum[m][i]);
                     else
                         __stcg(mine + tok * kW4TileRows + row, sum[m][i]);
                 }
-        });
-        w4_join<T>(p, work, cut, ok, tid, 1, arrived);
+            r = ring[seq % kW4FewRing];
+        }
     }
     if (*abort_flag != 0u) {
         // let copies already asked for drain before the memory they target goes away
