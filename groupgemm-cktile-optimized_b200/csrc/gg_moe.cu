@@ -379,7 +379,7 @@ template <class T, int G> W4Form w4_form(bool few, bool zeros) {
     if (few)
         return {zeros ? reinterpret_cast<const void *>(&w4_few<T, G, true>) : reinterpret_cast<const void *>(&w4_few<T, G, false>),
                 reinterpret_cast<const void *>(&w4_gather<T, true>), reinterpret_cast<const void *>(&w4_add<T>), kW4FewTokens, kW4FewThreads, 2, kW4FewSmem};
-    return {reinterpret_cast<const void *>(&w4_many<T, G>), reinterpret_cast<const void *>(&w4_gather<T, false>), nullptr, W4Many<G>::kTokens,
+    return {reinterpret_cast<const void *>(&w4_many<T, G>), reinterpret_cast<const void *>(&w4_gather<T, false>), reinterpret_cast<const void *>(&w4_join<T>), W4Many<G>::kTokens,
             kW4ManyThreads, 1, W4Many<G>::kSmemBytes};
 }
 template <class T> W4Form w4_form(int group, bool few, bool zeros) {
@@ -421,7 +421,7 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     const int ctas = v.ctas_per_sm * num_sms;
     const int blocks = q.rows > 0 ? ctas : 0;
     const int64_t steps = (q.k + gg::moe::kW4StepK - 1) / gg::moe::kW4StepK;
-    // partial sums: of the two cut tiles of a CTA, or (few) of the units of split items; counters: an arrival count a CTA, or the next unit
+    // partial sums: of the two cut tiles of a CTA, or (few) of the units of split items; a counter: the next unit (few)
     const int64_t tiles = (q.n + gg::moe::kW4TileRows - 1) / gg::moe::kW4TileRows;
     const int64_t items = std::min<int64_t>(q.rows, q.experts + q.rows / v.tokens) * tiles;
     int64_t span = steps;
@@ -435,7 +435,7 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
         return refuse(h, why, why_len, "too many weight rows and experts for one launch");
     if (const int rc = reserve(h, sums + size_t(q.rows + 8 * int64_t(q.experts)) * size_t(steps) * gg::moe::kW4TokenBytes))
         return rc;
-    if (const int rc = reserve_counters(h, size_t(ctas) * 4, stream))
+    if (const int rc = reserve_counters(h, 4, stream))
         return rc;
     gg::moe::W4Params p{};
     p.x = q.x;
@@ -459,6 +459,7 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     p.steps = int(steps);
     p.chunk = v.tokens;
     p.max_items = items;
+    p.ctas = ctas;
     p.splits = int(splits);
     p.span = int(span);
     p.ws = h->d_ws;
@@ -473,8 +474,9 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
 // a block a row, and of few rows one for each 128 pieces
     gather.grid_y = unsigned(std::max<int64_t>(1, std::min<int64_t>((steps * 16 + gg::moe::kW4GatherThreads - 1) / gg::moe::kW4GatherThreads,
                                                                     4 * num_sms / std::max<int64_t>(1, q.rows))));
-    const MoeLaunch add{few && splits > 1 ? v.add : nullptr, few && splits > 1 ? unsigned(std::min<int64_t>(items, 4 * num_sms)) : 0u,
-                        gg::moe::kW4TileRows, 0};
+    MoeLaunch add{v.add, few ? (splits > 1 ? unsigned(std::min<int64_t>(items, 4 * num_sms)) : 0u) : unsigned(blocks), gg::moe::kW4TileRows, 0};
+    if (!few)
+        add.grid_y = unsigned(v.tokens) / 8;
     return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), unsigned(v.threads), v.smem, true}, add}, detail);
 }
 

@@ -7,10 +7,8 @@
 // the products. So each weight is widened once, whatever the number of tokens, and whatever else is on the way is kept small. Two
 // forms, by how many rows an expert has (w4_few and w4_many, each explained there), share:
 //
-//   Work split: the steps of all (expert, token chunk, 256-row tile) items in a row, dealt out to the CTAs in equal contiguous
-//   ranges, so that one token through a few experts still keeps every SM reading. A tile that is cut leaves fp32 partial sums in
-//   the workspace; the CTA that arrives last adds them in order of k. A CTA looks after its cut tiles (two at most) when
-//   all its steps are done: fence, arrival and sum took 3 us where they stood between two pieces.
+//   Work split: items (expert, token chunk, 256-row tile), cut along k where there are few, so that one token through a few experts
+//   still keeps every SM reading. What is cut leaves fp32 partial sums in the workspace, which a last kernel adds in order of k.
 //   w4_gather: the rows of x in expert order, laid out as the products read them, so that bulk copies load them.
 #pragma once
 
@@ -36,12 +34,13 @@ struct W4Params {
     uint32_t *status;        // [0] status word, [2] timeouts of this launch
     uint8_t *xs;             // [rows + 8 experts][steps] 256 bytes: the rows of x as the products read them (w4_gather)
     float *ws;               // [2 x grid][tokens of a chunk][256] partial sums
-    int32_t *counters;       // [grid] arrivals at a cut tile, 0 between launches
+    int32_t *counters;       // w4_few: the next unit of work, 0 between launches
     int64_t rows, slots;     // slots: tokens * top_k
     int64_t max_items;       // that rising offsets can give
     uint64_t timeout_ns;
     int n, k, groups, experts, top_k, tiles, steps;  // steps: of 128 k
     int chunk;         // tokens of a chunk
+    int ctas;          // of the product kernel
     int splits, span;  // w4_few: units of an item, steps of a unit
 };
 
@@ -182,7 +181,7 @@ struct W4Work {
             first_[E] = chunks;
         __syncthreads();
         total = int64_t(chunks) * p.tiles * p.steps;
-        ctas = int(min(int64_t(gridDim.x), total));
+        ctas = int(min(int64_t(p.ctas), total));
         const int cta = blockIdx.x;
         begin = cta < ctas ? total * cta / ctas : 0;
         end = cta < ctas ? total * (cta + 1) / ctas : 0;
@@ -219,49 +218,6 @@ struct W4Work {
         return p.ws + int64_t(2 * c + (c == first_of_item ? 1 : 0)) * (p.chunk * kW4TileRows);
     }
 };
-
-// When a CTA's steps are done: its cut tiles. kThreads = 256 threads, `t` of them, a weight row each, that wrote the partial sums.
-// `cut`: the cut items' numbers, -1 for none; `ok`: whether the sums are sound.
-template <class T>
-__device__ __forceinline__ void w4_join(const W4Params &p, const W4Work &work, const int64_t (&cut)[2], bool ok, int t, int bar,
-                                        volatile int *arrived) {
-    if (cut[0] < 0 && cut[1] < 0)
-        return;
-    __threadfence();
-    named_sync(bar, kW4TileRows);
-    if (t < 2 && cut[t] >= 0)
-        arrived[t] = ok ? atomicAdd(p.counters + work.first_cta(p, cut[t]), 1) : -1;
-    named_sync(bar, kW4TileRows);
-    __threadfence();
-#pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-        if (cut[i] < 0)
-            continue;
-        const int c0 = work.first_cta(p, cut[i]), c1 = work.last_cta(p, cut[i]);
-        if (arrived[i] != c1 - c0)
-            continue;
-        if (t == 0)
-            p.counters[c0] = 0;
-        const W4Item it = work.at(p, int(cut[i]));
-        if (it.n0 + t >= p.n)
-            continue;
-        T *out = static_cast<T *>(p.out) + int64_t(it.r0) * p.n + it.n0 + t;
-        for (int i0 = 0; i0 < it.count; i0 += 8) {  // eight tokens' loads at a time
-            float v[8] = {};
-#pragma unroll 4
-            for (int c = c0; c <= c1; ++c) {
-                const float *from = work.slot(p, c, c0) + t;
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    v[u] += __ldcg(from + min(i0 + u, it.count - 1) * kW4TileRows);
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (i0 + u < it.count)
-                    out[int64_t(i0 + u) * p.n] = from_f32<T>(v[u]);
-        }
-    }
-}
 
 // The rows of x in expert order, gathered through src, as the products read them: for each chunk of an expert's tokens and each
 // step of 128 k, pieces of eight values in the order in which masks and shifts take the weights out of a word, placed
@@ -788,7 +744,6 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
     auto d_col = [&](int h, int d) { return uint32_t(128 * kA + C::kD * (2 * h + d)); };
     uint32_t *slots = reinterpret_cast<uint32_t *>(after + C::kBars * 8);
     volatile uint32_t *abort_flag = slots + 1;
-    volatile int *arrived = reinterpret_cast<volatile int *>(slots + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -928,18 +883,10 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
                 }
                 return;
             }
-            const uint8_t *zeros = p.zeros ? p.zeros + (int64_t(it.e) * p.n + min(it.n0 + 128 * h + row, p.n - 1)) * p.groups : nullptr;
-            uint32_t ze[kSub];  // of the next step
-            auto load_zeros = [&](int step) {
-#pragma unroll
-                for (int s = 0; s < kSub; ++s)
-                    ze[s] = zeros[kSub > 1 ? min(step * kSub + s, p.groups - 1) : step];  // past the end x is zero
-            };
-#pragma unroll
-            for (int s = 0; s < kSub; ++s)
-                ze[s] = 8u;
-            if (zeros)
-                load_zeros(k0);
+            W4Queue<1> zeros;
+            int queued = 0;  // groups in it
+            if (p.zeros)
+                zeros.begin(p.zeros, (int64_t(it.e) * p.n + min(it.n0 + 128 * h + row, p.n - 1)) * p.groups, p.zeros_end, k0 * kSub);
             for (int j = 0; j < n; ++j) {
                 const uint32_t a_par = (a_ph >> a) & 1u;
                 const bool seen = look(done(h, a), a_par);
@@ -950,9 +897,17 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
                 uint32_t minus[kSub];
 #pragma unroll
                 for (int s = 0; s < kSub; ++s)
-                    minus[s] = w4_minus<T>(ze[s] & 15u);
-                if (zeros && j + 1 < n)
-                    load_zeros(k0 + j + 1);
+                    minus[s] = w4_minus<T>(8u);
+                if (p.zeros) {
+                    if (queued == 0) {
+                        zeros.refill((k0 + n) * kSub);
+                        queued = 8;
+                    }
+                    queued -= kSub;
+#pragma unroll
+                    for (int s = 0; s < kSub; ++s)
+                        minus[s] = w4_minus<T>(zeros.take() & 15u);
+                }
                 // the MMAs that read this A last are done
                 ok = w4_wait_seen(seen, done(h, a), a_par, ab, kStatusTimeout | kRoleEpilogue | 0x40u | uint32_t(a));
                 if (!ok)
@@ -985,24 +940,17 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         int a = 0, d = 0;
         uint32_t a_ph = 0;
-        int64_t cut[2] = {-1, -1};
         bool ok = true;
         work.pieces(p, [&](const W4Item &it, int64_t item, int k0, int n) {
             const int col = it.n0 + 128 * h + row;
             const int npad = (it.count + 15) & ~15;
-            const T *scales = static_cast<const T *>(p.scales) + (int64_t(it.e) * p.n + min(col, p.n - 1)) * p.groups;
             float sum[kTokens];
 #pragma unroll
             for (int i = 0; i < kTokens; ++i)
                 sum[i] = 0.0f;
-            // the scales are loaded two steps ahead: [0] for even steps of the piece, [1] for odd ones
-            T sc[2][kSub] = {};
-            auto load_scales = [&](int step, T(&v)[kSub]) {
-#pragma unroll
-                for (int s = 0; s < kSub; ++s)
-                    v[s] = scales[kSub > 1 ? min(step * kSub + s, p.groups - 1) : step];
-            };
-            auto take = [&](int j, T(&v)[kSub]) {
+            W4Queue<2> scales;
+            int queued = 0;  // groups in it
+            auto take = [&]() {
                 ok = w4_wait(done(h, a), (a_ph >> a) & 1u, ab, kStatusTimeout | kRoleEpilogue | uint32_t(a));
                 if (!ok)
                     return;
@@ -1010,7 +958,8 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
                 ptx::tc_fence_after();
 #pragma unroll
                 for (int s = 0; s < kSub; ++s) {
-                    const float scale = to_f32(v[s]) * W4Unit<T>::kBack;
+                    const uint16_t bits = uint16_t(scales.take());
+                    const float scale = to_f32(*reinterpret_cast<const T *>(&bits)) * W4Unit<T>::kBack;
 #pragma unroll
                     for (int q = 0; q < kTokens / 16; ++q)
                         if (16 * q < npad) {
@@ -1026,27 +975,24 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
                 __syncwarp();
                 if (lane == 0)
                     ptx::mbar_arrive(dempty(h, d));
-                if (j + 2 < n)
-                    load_scales(k0 + j + 2, v);
                 d ^= 1;
                 a = a + 1 == kA ? 0 : a + 1;
             };
             if (it.n0 + 128 * h < p.n) {
-                load_scales(k0, sc[0]);
-                if (n > 1)
-                    load_scales(k0 + 1, sc[1]);
-                for (int j = 0; ok && j < n; j += 2) {
-                    take(j, sc[0]);
-                    if (ok && j + 1 < n)
-                        take(j + 1, sc[1]);
+                scales.begin(p.scales, (int64_t(it.e) * p.n + min(col, p.n - 1)) * p.groups, p.scales_end, k0 * kSub);
+                for (int j = 0; ok && j < n; ++j) {
+                    if (queued == 0) {
+                        scales.refill((k0 + n) * kSub);
+                        queued = 8;
+                    }
+                    queued -= kSub;
+                    take();
                 }
             } else {
                 a = (a + n) % kA;
                 d = (d + n) & 1;
             }
             const bool whole = n == p.steps;
-            if (!whole)
-                cut[k0 == 0] = item;
             if (!ok || col >= p.n)
                 return;
             if (whole) {
@@ -1063,7 +1009,6 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
                         __stcg(mine + i * kW4TileRows, sum[i]);
             }
         });
-        w4_join<T>(p, work, cut, ok, tid - 384, 2, arrived);
     }
 
     // ---- teardown ----
@@ -1079,6 +1024,38 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
     ptx::tc_fence_after();
     if (warp == 1)
         ptx::tmem_dealloc<1>(tmem, 512);
+}
+
+// Adds the partial sums of the tiles that w4_many's ranges cut, in order of k: block c those of the tile in which CTA c's range begins
+// after the CTA before has begun it, eight tokens a row of blocks. (Inside w4_many, by the last to arrive, fence, arrival and sum
+// took 5 us and more with the tokens.)
+template <class T> __global__ void __launch_bounds__(kW4TileRows) w4_join(const __grid_constant__ W4Params p) {
+    __shared__ int start[kW4MaxExperts + 1], first[kW4MaxExperts + 1];
+    ptx::griddep_launch_dependents();
+    const W4Work work(p, start, first);  // the offsets are older than w4_many
+    const int64_t item = work.begin / p.steps;
+    const int c = blockIdx.x, u0 = int(blockIdx.y) * 8, t = threadIdx.x;
+    const bool cut = work.begin < work.end && work.begin % p.steps != 0 && work.first_cta(p, item) == c - 1;
+    ptx::griddep_wait();
+    if (!cut)
+        return;
+    const W4Item it = work.at(p, int(item));
+    if (it.n0 + t >= p.n)
+        return;
+    float v[8] = {};
+    const int last = work.last_cta(p, item);
+#pragma unroll 2
+    for (int i = c - 1; i <= last; ++i) {
+        const float *from = work.slot(p, i, c - 1) + t;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (u0 + u < it.count)
+                v[u] += __ldcg(from + (u0 + u) * kW4TileRows);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+        if (u0 + u < it.count)
+            static_cast<T *>(p.out)[int64_t(it.r0 + u0 + u) * p.n + it.n0 + t] = from_f32<T>(v[u]);
 }
 
 }  // namespace moe
