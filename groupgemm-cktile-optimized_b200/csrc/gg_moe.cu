@@ -358,12 +358,23 @@ int prepare_permute(gg_handle *h, const gg_permute_problem &q, int32_t op, gg_st
                                  : reinterpret_cast<const void *>(&gg::moe::combine_rows<__nv_bfloat16>))
                          : (half ? reinterpret_cast<const void *>(&gg::moe::combine_grad_rows<__half>)
                                  : reinterpret_cast<const void *>(&gg::moe::combine_grad_rows<__nv_bfloat16>));
-    const int64_t blocks = std::min<int64_t>(q.tokens, int64_t(num_sms) * 32);
+    // Threads a token, us with at most 128 / 256 / 512 / 1024 of them: dispatch 16384 x 8 x 7168 356 / 354 / 344 / 336; combine 16384 x 8 x
+    // 4096 194 / 198 / 210 / 218, its gradient 7999 x 2 x 2880 40 / 41 / 48 / 48, but combine of 64 tokens 8.9 / 5.9 / 3.9 / 3.1. So dispatch takes
+    // 1024, the others 128, or as many more as fill the SMs. Then as few vectors a thread as that allows, and no idle warp.
+    int most = gg::moe::kPermuteThreads;
+    if (op != GG_OP_DISPATCH) {
+        most = 128;
+        while (most < gg::moe::kPermuteThreads && q.tokens * most < int64_t(num_sms) * 2048)
+            most *= 2;
+    }
+    const int each = (p.vecs + most - 1) / most;
+    const unsigned threads = unsigned(((p.vecs + each - 1) / each + 31) / 32 * 32);
+    const int64_t blocks = q.tokens;
     char detail[160];
     std::snprintf(detail, sizeof(detail), "gg_%s<%s> hidden=%lld top_k=%d blocks=%d",
                   op == GG_OP_DISPATCH ? "dispatch" : op == GG_OP_COMBINE ? "combine" : "combine_grad", type_name(q.dtype),
                   static_cast<long long>(q.hidden), q.top_k, int(blocks));
-    return finish(h, stream, {MoeLaunch{fn, unsigned(blocks), gg::moe::kPermuteThreads, 0}}, detail);
+    return finish(h, stream, {MoeLaunch{fn, unsigned(blocks), threads, 0}}, detail);
 }
 
 // ---- 4-bit products ----

@@ -7,7 +7,7 @@
 namespace gg {
 namespace moe {
 
-constexpr int kPermuteThreads = 256;
+constexpr int kPermuteThreads = 1024;  // at most
 
 struct PermuteParams {
     const void *x;           // dispatch: x; combine: rows; combine_grad: rows
@@ -23,6 +23,10 @@ struct PermuteParams {
     int vecs;  // 16-byte vectors a row
 };
 
+// A block a token, each thread 16 bytes of its row at a time, and a block of its own for every token: all three are bound by DRAM,
+// and it is the many rows in flight that fill it (a warp a token, with four of its rows in flight, took 290 us for combine's
+// 16384 x 8 rows of 4096 against 194). The host picks the threads. A thread's loads of dest are one broadcast.
+//
 // dest's entry of a slot, -1 where it has none (or one that is out of range).
 __device__ __forceinline__ int64_t slot_row(const PermuteParams &p, int64_t slot) {
     const int d = p.dest[slot];
@@ -42,7 +46,7 @@ __device__ __forceinline__ void zero_tail(const PermuteParams &p) {
         return;
     }
     for (int64_t r = total + blockIdx.x; r < p.rows; r += gridDim.x)
-        for (int i = threadIdx.x; i < p.vecs; i += kPermuteThreads)
+        for (int i = threadIdx.x; i < p.vecs; i += blockDim.x)
             static_cast<uint4 *>(p.out)[r * p.vecs + i] = make_uint4(0, 0, 0, 0);
 }
 
@@ -50,7 +54,7 @@ __global__ void __launch_bounds__(kPermuteThreads) dispatch_rows(const PermutePa
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x)
-        for (int i = threadIdx.x; i < p.vecs; i += kPermuteThreads) {
+        for (int i = threadIdx.x; i < p.vecs; i += blockDim.x) {
             const uint4 v = static_cast<const uint4 *>(p.x)[t * p.vecs + i];
             for (int j = 0; j < p.top_k; ++j) {
                 const int64_t d = slot_row(p, t * p.top_k + j);
@@ -65,7 +69,7 @@ template <class T> __global__ void __launch_bounds__(kPermuteThreads) combine_ro
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x)
-        for (int i = threadIdx.x; i < p.vecs; i += kPermuteThreads) {
+        for (int i = threadIdx.x; i < p.vecs; i += blockDim.x) {
             float acc[8] = {};
             for (int j = 0; j < p.top_k; ++j) {
                 const int64_t d = slot_row(p, t * p.top_k + j);
@@ -95,7 +99,7 @@ template <class T> __global__ void __launch_bounds__(kPermuteThreads) combine_gr
             const int64_t d = slot_row(p, t * p.top_k + j);
             const float w = p.weights ? p.weights[t * p.top_k + j] : 1.0f;
             float dot = 0.0f;
-            for (int i = threadIdx.x; d >= 0 && i < p.vecs; i += kPermuteThreads) {
+            for (int i = threadIdx.x; d >= 0 && i < p.vecs; i += blockDim.x) {
                 const uint4 g = static_cast<const uint4 *>(p.dy)[t * p.vecs + i];
                 const uint4 v = p.dweights ? static_cast<const uint4 *>(p.x)[d * p.vecs + i] : make_uint4(0, 0, 0, 0);
                 const uint32_t a[4] = {g.x, g.y, g.z, g.w}, b[4] = {v.x, v.y, v.z, v.w};
@@ -116,7 +120,7 @@ template <class T> __global__ void __launch_bounds__(kPermuteThreads) combine_gr
             __syncthreads();
             if (threadIdx.x == 0) {
                 float s = 0.0f;
-                for (int w2 = 0; w2 < kPermuteThreads / 32; ++w2)
+                for (int w2 = 0; w2 < int(blockDim.x) / 32; ++w2)
                     s += red[w2];
                 p.dweights[t * p.top_k + j] = d >= 0 ? s : 0.0f;
             }
