@@ -324,39 +324,58 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
                  : "r"(addr)
                  : "memory");
 }
-// Eight values of kBytes each (a scale or a zero of a group each) of a row that starts at any multiple of kBytes, as a queue of
-// 32-bit words, and the next eight on the way.
+// Eight values of kBytes each (a scale or a zero of a group each) of a row as a queue of 32-bit words, and the next eight on
+// the way. Where rows are a multiple of eight groups long a visit is one load at a multiple of eight; else a row starts at
+// any multiple of kBytes and a visit is its words one by one. The lanes' rows lie in lines of their own, so each load costs a
+// warp 32 visits to L1, and five a visit instead of one showed: 37 tokens x 4 of 32 experts of 7168 x 2048 in groups of 64 with
+// zeros took 73.4 us against 69.6, 8 experts of 4096 x 7168 in groups of 128 0.5 to 1 us of 36 to 51.
 template <int kBytes> struct W4Queue {
     static constexpr int kWords = 2 * kBytes;  // of eight values
     const uint32_t *from;                      // the aligned word that holds the next visit's first value
     const uint32_t *end;                       // past the array's last word
     int at;                                    // that visit's first group
+    int drop;                                  // its values before the first one asked for
     uint32_t shift;                            // bits from the word's start to the value
     uint32_t raw[kWords + 1], word[kWords];
 
-    // From now on the row's values from `first` on: the visit is on its way, to be taken by the next refill.
-    __device__ __forceinline__ void begin(const void *array, int64_t row, const void *array_end, int first) {
-        at = first;
-        const uintptr_t p = reinterpret_cast<uintptr_t>(array) + uintptr_t((row + first) * kBytes);
+    // From now on the values from `first` on of a row of `groups`: the visit is on its way, to be taken by the next refill.
+    __device__ __forceinline__ void begin(const void *array, int64_t row, int groups, const void *array_end, int first) {
+        drop = groups % 8 == 0 ? first & 7 : 0;
+        at = first - drop;
+        const uintptr_t p = reinterpret_cast<uintptr_t>(array) + uintptr_t((row * groups + at) * kBytes);
         from = reinterpret_cast<const uint32_t *>(p & ~uintptr_t(3));
         shift = uint32_t(p & 3) * 8;
         end = static_cast<const uint32_t *>(array_end);
-        load();
+        load(groups);
     }
-    __device__ __forceinline__ void load() {
+    __device__ __forceinline__ void load(int groups) {
+        if (groups % 8 == 0) {
+            if constexpr (kBytes == 2) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(from));
+                raw[0] = v.x, raw[1] = v.y, raw[2] = v.z, raw[3] = v.w;
+            } else {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(from));
+                raw[0] = v.x, raw[1] = v.y;
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i <= kWords; ++i)
-            raw[i] = from + i < end ? __ldg(from + i) : 0u;
+            for (int i = 0; i <= kWords; ++i)
+                raw[i] = from + i < end ? __ldg(from + i) : 0u;
+        }
         from += kWords;
     }
-    // Eight values into the queue, and the next visit on its way where there is one before group `last`.
-    __device__ __forceinline__ void refill(int last) {
+    // Up to eight values into the queue (returned: how many), and the next visit on its way where there is one before group `last`.
+    __device__ __forceinline__ int refill(int groups, int last) {
 #pragma unroll
         for (int i = 0; i < kWords; ++i)
             word[i] = __funnelshift_r(raw[i], raw[i + 1], shift);
         at += 8;
         if (at < last)
-            load();
+            load(groups);
+        const int values = 8 - drop;
+        for (; drop > 0; --drop)
+            take();
+        return values;
     }
     __device__ __forceinline__ uint32_t take() {
         const uint32_t v = word[0] & ((1u << (8 * kBytes)) - 1u);
@@ -525,16 +544,14 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
     } else {
         // of ldmatrix: row lane % 8 of the warp's, piece lane / 8 swizzled
         const uint32_t w_lane = uint32_t((warp * 32 + (lane & 7)) * 64) + (uint32_t((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
-        // Scales and zeros of weight row `lane`, to be handed to the lanes whose fragments hold the row. A row's lie next to
-        // each other, the rows far apart, so each visit to a row's line takes eight groups: into `raw`, one visit ahead, and from
-        // there, moved to the row's odd alignment, into queues that give up their low end.
+        // Scales and zeros of weight row `lane`, to be handed to the lanes whose fragments hold the row.
         W4Queue<2> scales;
         W4Queue<1> zeros;
         auto begin = [&](const Unit &r) {
-            const int64_t meta = (int64_t(r.it.e) * p.n + min(r.it.n0 + warp * 32 + lane, p.n - 1)) * p.groups;
-            scales.begin(p.scales, meta, p.scales_end, r.k0 * kSub);
+            const int64_t row = int64_t(r.it.e) * p.n + min(r.it.n0 + warp * 32 + lane, p.n - 1);
+            scales.begin(p.scales, row, p.groups, p.scales_end, r.k0 * kSub);
             if constexpr (kZeros)
-                zeros.begin(p.zeros, meta, p.zeros_end, r.k0 * kSub);
+                zeros.begin(p.zeros, row, p.groups, p.zeros_end, r.k0 * kSub);
         };
         ok = w4_wait(bars + 8u * (2 * kW4FewStages), 0, ab, kStatusTimeout | kRoleMma | 0x80u);
         Unit r{};
@@ -550,11 +567,10 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
                 if (!ok)
                     break;
                 if (queued == 0) {
-                    scales.refill((r.k0 + r.n) * kSub);
+                    queued = scales.refill(p.groups, (r.k0 + r.n) * kSub);
                     if constexpr (kZeros)
-                        zeros.refill((r.k0 + r.n) * kSub);
-                    queued = 8;
-                    if (j + 8 / kSub >= r.n) {  // this unit's last visit: the next one's scales are on their way from here
+                        zeros.refill(p.groups, (r.k0 + r.n) * kSub);
+                    if (scales.at >= (r.k0 + r.n) * kSub) {  // this unit's last visit: the next one's scales are on their way from here
                         const Unit after = ring[seq % kW4FewRing];
                         if (after.n > 0)
                             begin(after);
@@ -886,7 +902,7 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
             W4Queue<1> zeros;
             int queued = 0;  // groups in it
             if (p.zeros)
-                zeros.begin(p.zeros, (int64_t(it.e) * p.n + min(it.n0 + 128 * h + row, p.n - 1)) * p.groups, p.zeros_end, k0 * kSub);
+                zeros.begin(p.zeros, int64_t(it.e) * p.n + min(it.n0 + 128 * h + row, p.n - 1), p.groups, p.zeros_end, k0 * kSub);
             for (int j = 0; j < n; ++j) {
                 const uint32_t a_par = (a_ph >> a) & 1u;
                 const bool seen = look(done(h, a), a_par);
@@ -899,10 +915,8 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
                 for (int s = 0; s < kSub; ++s)
                     minus[s] = w4_minus<T>(8u);
                 if (p.zeros) {
-                    if (queued == 0) {
-                        zeros.refill((k0 + n) * kSub);
-                        queued = 8;
-                    }
+                    if (queued == 0)
+                        queued = zeros.refill(p.groups, (k0 + n) * kSub);
                     queued -= kSub;
 #pragma unroll
                     for (int s = 0; s < kSub; ++s)
@@ -979,12 +993,10 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
                 a = a + 1 == kA ? 0 : a + 1;
             };
             if (it.n0 + 128 * h < p.n) {
-                scales.begin(p.scales, (int64_t(it.e) * p.n + min(col, p.n - 1)) * p.groups, p.scales_end, k0 * kSub);
+                scales.begin(p.scales, int64_t(it.e) * p.n + min(col, p.n - 1), p.groups, p.scales_end, k0 * kSub);
                 for (int j = 0; ok && j < n; ++j) {
-                    if (queued == 0) {
-                        scales.refill((k0 + n) * kSub);
-                        queued = 8;
-                    }
+                    if (queued == 0)
+                        queued = scales.refill(p.groups, (k0 + n) * kSub);
                     queued -= kSub;
                     take();
                 }

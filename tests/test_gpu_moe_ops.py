@@ -666,6 +666,18 @@ def test_w4(gg, counts, n, k, group, zeros, kind, top_k, extra):
     assert torch.equal(first.view(torch.int16), out.t.view(torch.int16))
 
 
+@pytest.mark.parametrize("counts,n,k,group,zeros,kind", [
+    ([1, 2, 0, 5, 1, 1, 1, 1], 8192, 7168, 128, False, "bf16"),  # units of 12 steps
+    ([3] * 8, 4608, 4096, 64, True, "fp16"),
+    ([17, 9, 30, 8], 1032, 4096, 128, True, "bf16"),  # work cut at any step
+    ([33, 9, 30, 20], 776, 2048, 32, True, "fp16"),
+    ([33, 9, 30, 20], 776, 2016, 32, True, "bf16"),
+])
+def test_w4_rows_of_groups_in_eights(gg, counts, n, k, group, zeros, kind):
+    """Rows of scales in multiples of eight, and one that is not, with work that begins inside an eight."""
+    test_w4(gg, counts, n, k, group, zeros, kind, 0, 0)
+
+
 def test_w4_special_values(gg):
     """Infinities and NaN stay in their own row of x, and in their own weight row."""
     torch = _torch()
