@@ -422,8 +422,8 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
     // Up to 6 rows an expert on average, chunks of 8 with mma.sync; above, chunks of 32 with tcgen05. Measured on 8 experts of 4096 x
-    // 7168, us more for each further 117 MB of weights, few / many: 1 row an expert 22 / 28, 8 rows 24 / 29, 16 rows 42 / 30 (the weights
-    // are then widened twice by the first); a mean of 6 already has experts with more than 8.
+    // 7168, us, few / many: 1 row an expert 36 / 47, 8 rows 39 / 50, 16 rows 53 / 51 (the weights are then widened twice by the
+    // first), 24 rows 80 / 54, 32 rows 91 / 55; a mean of 6 already has experts with more than 8.
     const bool few = q.rows <= 6 * int64_t(q.experts);
     const W4Form v = q.dtype == GG_FP16 ? w4_form<__half>(q.group_size, few, q.zeros) : w4_form<__nv_bfloat16>(q.group_size, few, q.zeros);
     GG_CUDA(h, cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(v.smem)));

@@ -65,6 +65,13 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 constexpr uint32_t kKeyMinusInf = 0x007fffffu;  // key_of(-inf): not to be chosen
 
+// e^x for x <= 0, below 2^-126 as 0: three instructions where results below that cost four more.
+__device__ __forceinline__ float exp_of(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
+
 template <class T, int V> __device__ __forceinline__ void load_row(float (&v)[V], const T *row, int experts, bool there) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -82,36 +89,31 @@ template <class T, int V> __device__ __forceinline__ void load_row(float (&v)[V]
 // experts and k = 8, against 440 for k rounds of a maximum over all keys, which remain for more than 32 candidates (ties).
 template <int V> __device__ __forceinline__ void top_keys(uint32_t (&key)[V], uint32_t mine, int k, uint32_t *list, int &id, uint32_t &id_key) {
     const int lane = threadIdx.x & 31;
-    uint32_t least = 0, m = mine;
+    uint32_t least, m = mine;
     for (int found = 0;;) {
         least = __reduce_max_sync(0xffffffffu, m);
-        if (least <= kKeyMinusInf) {
-            least = kKeyMinusInf + 1;  // fewer lanes than k hold an open expert: every open one is a candidate
-            break;
-        }
-        found += __popc(__ballot_sync(0xffffffffu, m == least));
+        found += __popc(__ballot_sync(0xffffffffu, m == least));  // all lanes, once none is left
         if (found >= k)
             break;
-        if (m == least)
-            m = 0;
+        m = m == least ? 0u : m;
     }
+    least = max(least, kKeyMinusInf + 1);  // fewer lanes than k hold an open expert: every open one is a candidate
     int total = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const bool in = key[i] >= least;
         const uint32_t all = __ballot_sync(0xffffffffu, in);
         const int at = total + __popc(all & ((1u << lane) - 1u));
-        if (in && at < 32) {
-            list[at] = key[i];
-            list[32 + at] = uint32_t(lane + 32 * i);
-        }
+        if (in && at < 32)
+            reinterpret_cast<uint2 *>(list)[at] = make_uint2(key[i], uint32_t(lane + 32 * i));
         total += __popc(all);
     }
     id = -1;
     id_key = kKeyMinusInf;
     if (total <= 32) {
         __syncwarp();
-        const uint32_t mykey = lane < total ? list[lane] : 0u, myid = list[32 + lane];
+        const uint2 own = reinterpret_cast<const uint2 *>(list)[lane];
+        const uint32_t mykey = lane < total ? own.x : 0u;
         int rank = 0;
         for (int q0 = 0; q0 < total; q0 += 4)  // past the end the keys are 0
 #pragma unroll
@@ -119,14 +121,13 @@ template <int V> __device__ __forceinline__ void top_keys(uint32_t (&key)[V], ui
                 const uint32_t other = __shfl_sync(0xffffffffu, mykey, q);
                 rank += other > mykey || (other == mykey && q < lane);
             }
-        if (lane < total && rank < k) {
-            list[64 + rank] = mykey;
-            list[96 + rank] = myid;
-        }
+        if (lane < total && rank < k)
+            reinterpret_cast<uint2 *>(list)[32 + rank] = own;
         __syncwarp();
         if (lane < min(total, k)) {
-            id_key = list[64 + lane];
-            id = int(list[96 + lane]);
+            const uint2 chosen = reinterpret_cast<const uint2 *>(list)[32 + lane];
+            id_key = chosen.x;
+            id = int(chosen.y);
         }
         return;
     }
@@ -235,7 +236,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[i] = __expf(v[i] - mx);
+                v[i] = exp_of(v[i] - mx);
                 sum += v[i];
             }
             sum = warp_sum(sum);
@@ -250,7 +251,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
                 load(t + 1);  // arrives behind the selection
             uint32_t id_key;
             top_keys<V>(key, mine, k, list, id, id_key);
-            const float ex = id >= 0 ? __expf(value_of(id_key) - mx) : 0.0f;
+            const float ex = id >= 0 ? exp_of(value_of(id_key) - mx) : 0.0f;
             weight = p.normalize ? ex / warp_sum(ex) : ex * inv;
             weight = id >= 0 ? weight * p.scale : 0.0f;
         } else if (t + 1 < w1) {
@@ -510,7 +511,7 @@ template <class T, int V> __global__ void __launch_bounds__(kGradThreads) route_
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            r.v[i] = __expf(r.v[i] - r.lse);
+            r.v[i] = exp_of(r.v[i] - r.lse);
             dot = fmaf(r.v[i], bal[i], dot);
         }
         if (p.dweights) {
@@ -527,12 +528,12 @@ template <class T, int V> __global__ void __launch_bounds__(kGradThreads) route_
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1)
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const float ex = slot ? __expf(l - mx) : 0.0f;
+                const float ex = slot ? exp_of(l - mx) : 0.0f;
                 const float sum = warp_sum(ex);
                 const float q = slot ? ex / sum : 0.0f;
                 mine = q * (dw - warp_sum(q * dw));
             } else {
-                mine = slot ? __expf(l - r.lse) * dw : 0.0f;
+                mine = slot ? exp_of(l - r.lse) * dw : 0.0f;
                 dot += mine;
             }
             if (slot)

@@ -283,9 +283,12 @@ template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherT
 //
 // The words of weights that ldmatrix hands to a lane are those of its place in the A fragment, so they are widened in the
 // registers that mma.sync reads, and nothing but a wait and an arrival stands between a step's bytes and its products. 8 warps of 32
-// weight rows and two loading warps (a TMA box of weights, a bulk copy of tokens a step, a ring of 4 steps), two CTAs an SM.
-// 22 us for 117 MB of weights (5.3 TB/s, 82% of the measured copy rate) at 1 row an expert, 24 at 8. Above that mma.sync's own rate
-// binds (11 cycles an instruction and scheduler: 16 tokens in one pass 36 us).
+// weight rows and a loading warp (a TMA box of weights, a bulk copy of tokens a step, a ring of 4 steps), two CTAs an SM. Units
+// of work are taken from a counter, so that CTAs that share an SM with a slower one do not wait for it at the end.
+// Measured: 8 experts of 4096 x 7168 (117 MB of weights) in groups of 128, 1 row each, 35.3 us, and 24.5 us for each further 117 MB
+// (4.8 TB/s, 73% of the measured copy rate): the rest is the start of three launches, the first loads and the sum of split items.
+// 8 rows each 39.4. Above that an expert's weights are widened again for each 8 tokens; in one pass mma.sync's own rate binds (11
+// cycles an instruction and scheduler: 16 tokens 36 us for each further 117 MB).
 constexpr int kW4FewTokens = 8;
 constexpr int kW4FewThreads = kW4TileRows + 32;
 constexpr int kW4FewUnits = 4;  // units of work a CTA, where items have to be split for that
@@ -670,9 +673,11 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
 //   warps 12-19  a half each four: tcgen05.ld of a step's products and the fp32 sum with the group's scale (one scalar a
 //                thread); output
 //
-// Three A operands and two D a half keep the widening from waiting for the MMAs: beside widening warps the MMA warp's eight
-// take 300 cycles to issue and 530 beside four a scheduler, against 95 alone. 28 us for 117 MB of weights at 1 row an expert, 30 at 16, 33 at 32:
-// bound by instruction issue (3200 a step and SM, of which the widening is 1200), not by the number of tokens.
+// Three A operands and two D a half keep the widening from waiting for the MMAs. Measured: 8 experts of 4096 x 7168 (117 MB of
+// weights) in groups of 128, 8 rows each, 50.5 us, 16 51.3, 32 55.0, and 30.5, 30.7 and 33.3 us for each further 117 MB. No one part binds it:
+// without the widening 26, without that and tcgen05.st 24, without the products 27, without the sums 28, with all weights from L2 30;
+// the parts share the schedulers' issue slots (3200 instructions a step and SM, 1200 of them widening). Four warps that
+// issue the products in place of two gained 1 us at 8 rows and none at 32; eight more widening warps lost 3.
 constexpr int kW4ManyThreads = 640;
 
 // Tokens of a chunk: at most 32 (a thread holds a sum a token). Tensor Memory's 512 columns hold for each half kA operands of
