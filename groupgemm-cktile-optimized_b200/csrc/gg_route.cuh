@@ -240,8 +240,8 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
                 sum += v[i];
             }
             sum = warp_sum(sum);
-            lse = mx + logf(sum);
-            const float inv = 1.0f / sum;
+            lse = mx + __logf(sum);
+            const float inv = __fdividef(1.0f, sum);
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 acc[i] = fmaf(v[i], inv, acc[i]);
@@ -252,7 +252,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
             uint32_t id_key;
             top_keys<V>(key, mine, k, list, id, id_key);
             const float ex = id >= 0 ? exp_of(value_of(id_key) - mx) : 0.0f;
-            weight = p.normalize ? ex / warp_sum(ex) : ex * inv;
+            weight = p.normalize ? __fdividef(ex, warp_sum(ex)) : ex * inv;
             weight = id >= 0 ? weight * p.scale : 0.0f;
         } else if (t + 1 < w1) {
             load(t + 1);
