@@ -91,13 +91,19 @@ def build(force: bool = False, verbose: bool = False) -> list[str]:
 
 
 _OP = {"0": "forward", "1": "dgrad", "2": "wgrad"}
+_TYPE = {"f": "fp32", "6__half": "fp16", "13__nv_bfloat16": "bf16"}
 
 
 def _kernel_name(mangled: str) -> str:
-    """Readable name of a grouped_gemm_sm100<T, kCG, kBN, kAtoms, kOp> instantiation."""
+    """Readable name of a grouped_gemm_sm100<T, kCG, kBN, kAtoms, kOp> instantiation, or of a layer operator's kernel."""
     m = re.search(r"grouped_gemm_sm100I(6__half|13__nv_bfloat16)Li(\d+)ELi(\d+)ELi(\d+)ELi(\d+)E", mangled)
     if not m:
-        return re.sub(r"^_ZN.*?\d+([a-z_]+)E.*$", r"\1", mangled)
+        m = re.match(r"_ZN2gg3moe(\d+)(.*)$", mangled)  # a kernel of the layer operators
+        if not m:
+            return re.sub(r"^_ZN.*?\d+([a-z_]+)E.*$", r"\1", mangled)
+        name, rest = m.group(2)[: int(m.group(1))], m.group(2)[int(m.group(1)):]
+        args = re.match(r"I(f|6__half|13__nv_bfloat16)((?:L[ib]\d+E)*)E", rest)
+        return name + ("<" + ", ".join([_TYPE[args.group(1)]] + re.findall(r"L[ib](\d+)E", args.group(2))) + ">" if args else "")
     dt = "fp16" if m.group(1) == "6__half" else "bf16"
     return f"grouped_gemm_sm100<{dt}, cta_group={m.group(2)}, BN={m.group(3)}, atoms={m.group(4)}, {_OP[m.group(5)]}>"
 

@@ -100,24 +100,32 @@ public:
         const gg_problem q{p.dtype == DType::BF16 ? GG_BF16 : GG_FP16, p.group_num, p.n, p.k, p.group_m.data(),
                            p.x, p.w, p.out};
         char why[256];
-        const int rc = gg_prepare(h_, &q, stream, why, sizeof(why));
-        if (rc == GG_OK)
-            return "";
-        if (rc == GG_NOT_SUPPORTED)
-            return why;
-        throw CudaError(gg_last_error(h_));
+        return answer(gg_prepare(h_, &q, stream, why, sizeof(why)), why);
     }
 
     // Backward grouped GEMM of the same layer (GG_OP_DGRAD or GG_OP_WGRAD, gg_prepare_grad);
     // run()/release()/detail() then apply to it. Returns "" or the N/A reason.
     std::string prepare_grad(const gg_grad_problem &q, int32_t op, cudaStream_t stream) {
         char why[256];
-        const int rc = gg_prepare_grad(h_, &q, op, stream, why, sizeof(why));
-        if (rc == GG_OK)
-            return "";
-        if (rc == GG_NOT_SUPPORTED)
-            return why;
-        throw CudaError(gg_last_error(h_));
+        return answer(gg_prepare_grad(h_, &q, op, stream, why, sizeof(why)), why);
+    }
+
+    // The operators around the products (gg_prepare_route, _route_grad, _permute, _w4), likewise.
+    std::string prepare_route(const gg_route_problem &q, cudaStream_t stream) {
+        char why[256];
+        return answer(gg_prepare_route(h_, &q, stream, why, sizeof(why)), why);
+    }
+    std::string prepare_route_grad(const gg_route_grad_problem &q, cudaStream_t stream) {
+        char why[256];
+        return answer(gg_prepare_route_grad(h_, &q, stream, why, sizeof(why)), why);
+    }
+    std::string prepare_permute(const gg_permute_problem &q, int32_t op, cudaStream_t stream) {
+        char why[256];
+        return answer(gg_prepare_permute(h_, &q, op, stream, why, sizeof(why)), why);
+    }
+    std::string prepare_w4(const gg_w4_problem &q, cudaStream_t stream) {
+        char why[256];
+        return answer(gg_prepare_w4(h_, &q, stream, why, sizeof(why)), why);
     }
 
     void run(cudaStream_t stream) override {
@@ -143,6 +151,15 @@ public:
     }
 
 private:
+    // A prepare call's result: "" or the N/A reason; throws on an error.
+    std::string answer(int rc, const char *why) const {
+        if (rc == GG_OK)
+            return "";
+        if (rc == GG_NOT_SUPPORTED)
+            return why;
+        throw CudaError(gg_last_error(h_));
+    }
+
     gg_handle *h_;
 };
 
