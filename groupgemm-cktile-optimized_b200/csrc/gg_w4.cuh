@@ -111,7 +111,7 @@ __device__ __forceinline__ bool try_wait_hint(uint32_t bar, uint32_t parity) {
                  : "memory");
     return ok != 0;
 }
-__device__ __noinline__ inline bool w4_wait_slow(uint32_t bar, uint32_t parity, const Abort ab, uint32_t code) {
+__device__ __forceinline__ bool w4_wait_slow(uint32_t bar, uint32_t parity, const Abort ab, uint32_t code) {
     const uint64_t t0 = ptx::globaltimer();
     for (uint32_t it = 1;; ++it) {
         if (__all_sync(0xffffffffu, try_wait_hint(bar, parity)))

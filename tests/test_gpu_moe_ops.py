@@ -678,6 +678,13 @@ def test_w4_rows_of_groups_in_eights(gg, counts, n, k, group, zeros, kind):
     test_w4(gg, counts, n, k, group, zeros, kind, 0, 0)
 
 
+@pytest.mark.parametrize("group,zeros,kind", [(32, True, "bf16"), (64, False, "fp16"), (128, True, "bf16"), (128, False, "fp16")])
+def test_w4_chunks_of_every_length(gg, group, zeros, kind):
+    """Chunks of tokens that need one accumulator and chunks that need both, after one another and in either order; the last tile of
+    256 weight rows is there in part of its first half only."""
+    test_w4(gg, [40, 3, 70, 0, 33, 64, 16, 17, 130, 32, 1, 65, 48], 600, 1152, group, zeros, kind, 0, 2)
+
+
 def test_w4_special_values(gg):
     """Infinities and NaN stay in their own row of x, and in their own weight row."""
     torch = _torch()
