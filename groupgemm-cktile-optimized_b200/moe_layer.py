@@ -216,7 +216,11 @@ def main() -> None:
     leaves = [v.double().requires_grad_() for v in (x, w)] + [logits.double().requires_grad_()]
     py, pl = plain_layer(leaves[0], leaves[1], leaves[2], top_k, mask)
     (torch.sum(py * dy.double()) + torch.sum(pl * dlosses.double())).backward()
-    far = lambda a, b: ((a.double() - b.double()).norm() / b.double().norm()).item()  # noqa: E731
+    def far(a, b):
+        d = ((a.double() - b.double()).norm() / b.double().norm()).item()
+        assert d < 2e-2, d  # five roundings to bf16
+        return d
+
     print("training: y %.2g losses %.2g dx %.2g dw %.2g dlogits %.2g (relative to 64 bits)" % (
         far(y, py), far(losses, pl), far(dx, leaves[0].grad), far(dw, leaves[1].grad), far(dlogits, leaves[2].grad)))
 
