@@ -22,7 +22,7 @@ struct MoeLaunch {
     unsigned grid = 0, block = 0;
     size_t smem = 0;
     bool map = false;  // the kernel takes MoePlan::map first
-    unsigned grid_y = 1;
+    unsigned grid_y = 1, cluster = 1;  // cluster: blocks of one along x
 };
 
 struct MoePlan {

@@ -18,6 +18,7 @@ __host__ __device__ constexpr int route_warps(int v) { return v <= 8 ? 32 : v ==
 constexpr int kGradWarps = 8;
 constexpr int kGradThreads = kGradWarps * 32;
 constexpr int kPlaceThreads = 1024;
+constexpr int kPlaceCluster = 4;
 
 struct RouteParams {
     const void *logits;   // [tokens, experts]
@@ -79,6 +80,12 @@ template <class T, int V> __device__ __forceinline__ void load_row(float (&v)[V]
         const int e = lane + 32 * i;
         v[i] = there && e < experts ? to_f32(row[e]) : -INFINITY;
     }
+}
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+    return v;
 }
 
 // The k largest of a warp's keys (lane + 32 i: expert), ties to the lower expert: lane j < k gets the j-th one's expert and key,
@@ -350,16 +357,21 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
         route_totals(p, own[0], at, total, mine, n, zs);
 }
 
-// Every block sums the blocks' counts (all of them for the experts' offsets, those before it for its own
-// slots), places its slots and writes its part of src's unused end; one block more writes the totals and losses. Its 1024
-// threads share the blocks' rows of an expert, so that 148 rows of 256 experts take 37 loads a thread.
-__global__ void __launch_bounds__(kPlaceThreads) route_place(const RouteParams p) {
+// Every block needs the blocks' counts (all of them for the experts' offsets, those before it for its own
+// slots); it places its slots and writes its part of src's unused end; one block more writes the totals and losses. Its 1024
+// threads share the blocks' rows of an expert: 37 loads a thread for 148 rows of 256 experts. Where that is much, a cluster of C
+// blocks shares the sums: each adds every C-th row and reads the others' sums from their shared memory, and adds the few rows of
+// its own cluster before it.
+template <int C> __global__ void __launch_bounds__(kPlaceThreads) route_place(const RouteParams p) {
     __shared__ int part[2][kPlaceThreads];
     __shared__ int base[kMaxExperts];
+    __shared__ int share[C > 1 ? 3 : 1][C > 1 ? kPlaceThreads : 1];  // this block's part of tot, pre and sum
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int E = p.experts, k = p.top_k, tid = threadIdx.x, b = blockIdx.x;
-    const bool last = b == p.blocks;
+    const int turn = b % C, c0 = b - turn;  // c0: the cluster's first block
+    const bool last = b == p.blocks, sums = p.blocks - c0 < C && (p.prob || p.losses);
+    const int mine = (p.blocks - turn + C - 1) / C;  // rows of this block's part: turn, turn + C, ...
     int span = 32;  // a power of two of at least E threads takes one row
     while (span < E)
         span *= 2;
@@ -367,35 +379,39 @@ __global__ void __launch_bounds__(kPlaceThreads) route_place(const RouteParams p
     // the thread's first slot, on its way while the counts are summed
     const int64_t first = min(p.tokens, b * p.per_block) * k, end = min(p.tokens, (b + 1) * p.per_block) * k;
     int id0 = -1, rank0 = 0;
-    if (!last && first + tid < end) {
+    if (first + tid < end) {
         id0 = p.ids[first + tid];
         rank0 = p.dest[first + tid];
     }
     int tot = 0, pre = 0;
     float sum = 0.0f;
     if (e < E) {
-        for (int r0 = row; r0 < p.blocks; r0 += 8 * rows) {  // eight rows' loads at a time (16 and more at once were slower)
+        for (int r0 = row; r0 < mine; r0 += 8 * rows) {  // eight rows' loads at a time (16 and more at once were slower)
             int c[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                c[i] = r0 + i * rows < p.blocks ? __ldcg(p.block_counts + (r0 + i * rows) * (E + 1) + e) : 0;
+                c[i] = r0 + i * rows < mine ? __ldcg(p.block_counts + (turn + C * (r0 + i * rows)) * (E + 1) + e) : 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 tot += c[i];
-                pre += r0 + i * rows < b ? c[i] : 0;
+                pre += turn + C * (r0 + i * rows) < c0 ? c[i] : 0;
             }
         }
-        if (last && (p.prob || p.losses))
-            for (int r0 = row; r0 < p.blocks; r0 += 8 * rows) {
+        if (sums)
+            for (int r0 = row; r0 < mine; r0 += 8 * rows) {
                 float f[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    f[i] = r0 + i * rows < p.blocks ? __ldcg(p.block_sums + (r0 + i * rows) * (E + 1) + e) : 0.0f;
+                    f[i] = r0 + i * rows < mine ? __ldcg(p.block_sums + (turn + C * (r0 + i * rows)) * (E + 1) + e) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     sum += f[i];
             }
     }
+    int near = 0;
+    if (tid < E)
+        for (int i = c0; i < min(b, p.blocks); ++i)
+            near += __ldcg(p.block_counts + i * (E + 1) + tid);
     auto across = [&](auto v, auto *words) {  // of the threads of one expert, in order; complete in the first
         words[tid] = v;
         __syncthreads();
@@ -407,8 +423,28 @@ __global__ void __launch_bounds__(kPlaceThreads) route_place(const RouteParams p
     };
     tot = across(tot, part[0]);
     pre = across(pre, part[1]);
-    if (last)
+    if (sums)
         sum = across(sum, reinterpret_cast<float *>(part[0]));
+    if constexpr (C > 1) {
+        share[0][tid] = tot;
+        share[1][tid] = pre;
+        share[2][tid] = __float_as_int(sum);
+        ptx::cluster_sync();
+        tot = pre = 0;
+        sum = 0.0f;
+        if (tid < E)
+#pragma unroll
+            for (int q = 0; q < C; ++q) {
+                tot += int(ld_cluster_u32(ptx::mapa(ptx::smem_addr(&share[0][tid]), q)));
+                pre += int(ld_cluster_u32(ptx::mapa(ptx::smem_addr(&share[1][tid]), q)));
+                if (sums)
+                    sum += __uint_as_float(ld_cluster_u32(ptx::mapa(ptx::smem_addr(&share[2][tid]), q)));
+            }
+        ptx::cluster_sync();  // no block ends while another still reads from it
+    }
+    if (b > p.blocks)
+        return;
+    pre += near;
     if (tid >= E)
         tot = 0;
     int total;

@@ -184,6 +184,10 @@ ROUTES = [
     (2500, 128, 4, "bf16", True, 0.05, 0.05, True),
     (20011, 256, 8, "f32", True, 0.02, 0.0, False),
     (20011, 8, 2, "fp16", True, 0.02, 0.1, True),
+    (1031, 512, 7, "f32", False, 0.1, 0.1, False),
+    (2000, 1000, 8, "bf16", True, 0.0, 0.3, False),
+    (8192, 256, 8, "f32", True, 0.0, 0.0, False),
+    (9000, 130, 4, "fp16", False, 0.9, 0.2, True),
 ]
 
 
