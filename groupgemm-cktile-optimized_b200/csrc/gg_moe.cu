@@ -257,15 +257,16 @@ int prepare_route(gg_handle *h, const gg_route_problem &q, gg_stream_t stream, c
     p.top_k = q.top_k;
     p.normalize = q.normalize != 0;
     p.scale = q.scale;
-    // One block where a warp gets two tokens at most (it finishes alone, in one launch). Else 8 tokens a block, up to 64 as long as that
-    // leaves 64 blocks or more, and a block an SM at most: route_place's work grows with the blocks. Us of 256 experts and k = 8 with 8 / 16 / 32
-    // / 64 tokens a block: 256 tokens 10.6 / 11.0 / 12.7, 512 12.3 / 11.3 / 12.9, 1000 16.7 / 13.1 / 13.0 / 15.5, 2000 19.0 / 17.5 / 14.9 / 15.6,
-    // 4096 20.6 / - / 19.5 / 17.4.
+    // One block where a warp gets two tokens at most and a thread one expert (it finishes alone, in one launch). Else 8 tokens a block,
+    // up to 64 as long as that leaves 64 blocks or more, and a block an SM at most: route_place's work grows with the blocks. Us of 256
+    // experts and k = 8 with 8 / 16 / 32 / 64 tokens a block: 256 tokens 10.6 / 11.0 / 12.7, 512 12.3 / 11.3 / 12.9, 1000 16.7 / 13.1 / 13.0 /
+    // 15.5, 2000 19.0 / 17.5 / 14.9 / 15.6, 4096 20.6 / - / 19.5 / 17.4.
     const int v = (q.experts + 31) / 32, warps = gg::moe::route_warps(v <= 8 ? 8 : v <= 16 ? 16 : 32);
     const bool alone = q.tokens <= 2 * warps && q.experts <= 32 * warps;
     int64_t each = 8;
     while (each < 64 && (q.tokens + each - 1) / each >= 64)
         each *= 2;
+    p.alone = alone;
     p.blocks = alone ? 1 : int(std::max<int64_t>(1, std::min<int64_t>((q.tokens + each - 1) / each, num_sms)));
     // Clusters that share route_place's sums cost their barriers, up to 1.5 us: taken where a thread would load more than 16 rows, with
     // as many blocks as fit at once in clusters (33 of 4; with one more the last runs alone). Us without / with: 16384 tokens of 256 experts

@@ -37,6 +37,7 @@ struct RouteParams {
     float *block_sums;      // [blocks, experts + 1]: probability sums, then the sum of lse^2
     int64_t tokens, per_block;
     int experts, top_k, blocks, normalize;
+    int alone;  // one block finishes without route_place: it has a thread an expert
     float scale;
 };
 
@@ -283,7 +284,7 @@ template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32)
         live_of[warp] = live;
     }
     __syncthreads();
-    const bool alone = gridDim.x == 1;
+    const bool alone = p.alone != 0;
     int32_t *counts = p.block_counts + int64_t(blockIdx.x) * (E + 1);
     float *sums = p.block_sums + int64_t(blockIdx.x) * (E + 1);
     int own[(kMaxExperts + kThreads - 1) / kThreads] = {};  // this thread's experts' slots (one expert where a block is alone)
