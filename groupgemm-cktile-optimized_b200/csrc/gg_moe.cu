@@ -212,6 +212,9 @@ const char *route_bad(int32_t type, int64_t tokens, int32_t experts, int32_t top
     return nullptr;
 }
 
+// Dynamic shared memory of route_topk: the warps' counters of `experts` experts and lists of top_keys.
+size_t route_smem(int warps, int experts) { return size_t(warps) * (size_t(experts) + 128) * 4; }
+
 // How many clusters of route_place the GPU holds at once.
 int place_clusters(gg_handle *h, int &fit) {
     cudaLaunchAttribute attr[1];
@@ -261,7 +264,10 @@ int prepare_route(gg_handle *h, const gg_route_problem &q, gg_stream_t stream, c
     // up to 64 as long as that leaves 64 blocks or more, and a block an SM at most: route_place's work grows with the blocks. Us of 256
     // experts and k = 8 with 8 / 16 / 32 / 64 tokens a block: 256 tokens 10.6 / 11.0 / 12.7, 512 12.3 / 11.3 / 12.9, 1000 16.7 / 13.1 / 13.0 /
     // 15.5, 2000 19.0 / 17.5 / 14.9 / 15.6, 4096 20.6 / - / 19.5 / 17.4.
-    const int v = (q.experts + 31) / 32, warps = gg::moe::route_warps(v <= 8 ? 8 : v <= 16 ? 16 : 32);
+    int v = 1;  // logits a lane: route_fn's V
+    while (32 * v < q.experts)
+        v *= 2;
+    const int warps = gg::moe::route_warps(v);
     const bool alone = q.tokens <= 2 * warps && q.experts <= 32 * warps;
     int64_t each = 8;
     while (each < 64 && (q.tokens + each - 1) / each >= 64)
@@ -292,10 +298,10 @@ int prepare_route(gg_handle *h, const gg_route_problem &q, gg_stream_t stream, c
     p.block_sums = h->d_ws;
     p.block_counts = reinterpret_cast<int32_t *>(h->d_ws + entries);
     set_params(h, p);
-    const size_t smem = size_t(warps) * (size_t(q.experts) + 128) * 4;
     const void *fn = route_fn(q.logits_type, q.experts, false);
-    GG_CUDA(h, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    MoeLaunch topk{fn, unsigned(p.blocks), unsigned(warps) * 32, smem};
+    // The limit belongs to the function, which other handles launch with up to 32 v experts: set for those, never for this problem's.
+    GG_CUDA(h, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(route_smem(warps, 32 * v))));
+    MoeLaunch topk{fn, unsigned(p.blocks), unsigned(warps) * 32, route_smem(warps, q.experts)};
     MoeLaunch place{cluster > 1 ? reinterpret_cast<const void *>(&gg::moe::route_place<gg::moe::kPlaceCluster>)
                                 : reinterpret_cast<const void *>(&gg::moe::route_place<1>),
                     alone ? 0u : (unsigned(p.blocks) / cluster + 1) * cluster, gg::moe::kPlaceThreads, 0};

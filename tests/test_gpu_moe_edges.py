@@ -24,3 +24,17 @@ def test_route_few_tokens_of_many_experts(gg, t, e, k, kind, normalize):
         again = r.run()
         for n in got:
             assert got[n].tobytes() == again[n].tobytes(), n
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("large,small", [(256, 129), (256, 160), (128, 65), (512, 300), (1024, 600)])
+def test_routers_of_one_kernel_beside_one_another(gg, kind, large, small):
+    """Two handles prepared before either runs, the second with fewer experts of the same kernel."""
+    torch = _torch()
+    made = []
+    for e in (large, small):
+        logits, mask = make_logits(torch, kind, 300, e, e, pad=0.1)
+        made.append((Route(gg, torch, kind, logits, mask, 4, True), logits, mask))
+    for _ in range(2):
+        for r, logits, mask in made:
+            check_route(r.run(), logits, mask, 4, True)
