@@ -45,7 +45,27 @@ def _ready(why: str) -> None:
 
 
 def _ptr(t) -> int:
-    return 0 if t is None else t.data_ptr()
+    """Address of a tensor as the kernels read it: row by row without gaps, on the current device."""
+    if t is None:
+        return 0
+    if not t.is_contiguous():
+        raise ValueError(f"a tensor of shape {tuple(t.shape)} and strides {t.stride()} is not contiguous")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"a tensor of shape {tuple(t.shape)} is on {t.device}, not on the current CUDA device")
+    return t.data_ptr()
+
+
+def _check(name: str, t, shape: tuple, *dtypes: torch.dtype):
+    """t, if it has this shape and one of these types: the kernels see an address only."""
+    if not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.dtype not in dtypes:
+        what = f"{t.dtype} {list(t.shape)}" if isinstance(t, torch.Tensor) else repr(t)
+        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)} {list(shape)}, not {what}")
+    return t
+
+
+HALF = (torch.bfloat16, torch.float16)
+LOGITS = (torch.float32,) + HALF
+MASK = (torch.uint8, torch.bool)  # a byte a token
 
 
 def _dtype(gg, dtype: torch.dtype) -> int:
@@ -59,7 +79,7 @@ def quantize_w4(w: torch.Tensor, group: int, symmetric: bool = True):
     e, n, k = w.shape
     groups = -(-k // group)
     x = torch.nn.functional.pad(w.float(), (0, groups * group - k)).view(e, n, groups, group)
-    dtype = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+    dtype = w.dtype if w.dtype in HALF else torch.bfloat16
     if symmetric:
         scales = (x.abs().amax(3) / 7).to(dtype)
     else:
@@ -74,11 +94,15 @@ def quantize_w4(w: torch.Tensor, group: int, symmetric: bool = True):
 
 
 class Router:
-    """The router's handle and outputs for `tokens` tokens (gg_prepare_route) of a logits buffer."""
+    """The router's handle and outputs (gg_prepare_route) for a buffer of logits [tokens, experts] and one of mask bytes [tokens], which
+    run() reads anew each time and which have to be contiguous for that."""
 
     def __init__(self, logits: torch.Tensor, top_k: int, mask: torch.Tensor | None = None, normalize: bool = True, losses: bool = True):
         gg = load_package()
         t, e = logits.shape
+        _check("logits", logits, (t, e), *LOGITS)
+        if mask is not None:
+            _check("mask", mask, (t,), *MASK)
         new = lambda *shape, dtype=torch.int32: torch.empty(*shape, dtype=dtype, device=logits.device)  # noqa: E731
         f32 = torch.float32
         self.logits, self.mask, self.top_k, self.normalize = logits, mask, top_k, normalize
@@ -99,6 +123,10 @@ class Router:
         """d logits of the last run, for gradients of the weights [tokens, top_k] and of the two losses [2]."""
         gg = load_package()
         t, e = self.logits.shape
+        if dweights is not None:
+            dweights = _check("dweights", dweights, (t, self.top_k), torch.float32).contiguous()
+        if dlosses is not None:
+            dlosses = _check("dlosses", dlosses, (2,), torch.float32).contiguous()
         dlogits = torch.empty_like(self.logits)
         b = gg.make_b200_backend()
         _ready(b.prepare_route_grad(
@@ -110,10 +138,14 @@ class Router:
 
 
 class TrainingLayer:
-    """One layer's forward and backward pass over 16-bit experts `w` [experts, n, k]."""
+    """One layer's forward and backward pass over 16-bit experts `w` [experts, n, k], which have to be contiguous. The tensors of a step
+    may have any strides (an expanded gradient, a transposed view): what is not contiguous is copied first."""
 
     def __init__(self, w: torch.Tensor, top_k: int, normalize: bool = True):
         self.gg = load_package()
+        e, n, k = w.shape
+        if not _check("w", w, (e, n, k), *HALF).is_contiguous():
+            raise ValueError("w must be contiguous")
         self.w, self.top_k, self.normalize = w, top_k, normalize
         self.backend = self.gg.make_b200_backend()
 
@@ -122,12 +154,16 @@ class TrainingLayer:
         self.backend.run(_stream())
 
     def forward(self, x: torch.Tensor, logits: torch.Tensor, mask: torch.Tensor | None = None):
-        """x [tokens, k], logits [tokens, experts] -> (y [tokens, n], losses [2]: balance and z)."""
-        gg, b, s = self.gg, self.backend, _stream()
+        """x [tokens, k] in w's type, logits [tokens, experts] -> (y [tokens, n], losses [2]: balance and z)."""
         (e, n, k), t = self.w.shape, x.shape[0]
-        dt = _dtype(gg, x.dtype)
+        x = _check("x", x, (t, k), self.w.dtype).contiguous()
+        logits = _check("logits", logits, (t, e), *LOGITS).contiguous()
+        if mask is not None:
+            mask = _check("mask", mask, (t,), *MASK).contiguous()
         self.router = r = Router(logits, self.top_k, mask, self.normalize)
         r.run()
+        gg, b, s = self.gg, self.backend, _stream()
+        dt = _dtype(gg, x.dtype)
         self.x_rows = torch.empty(t * self.top_k, k, dtype=x.dtype, device=x.device)
         self.rows = torch.empty(t * self.top_k, n, dtype=x.dtype, device=x.device)
         y = torch.empty(t, n, dtype=x.dtype, device=x.device)
@@ -138,9 +174,12 @@ class TrainingLayer:
         return y, r.losses
 
     def backward(self, dy: torch.Tensor, dlosses: torch.Tensor | None = None):
-        """(dx, dw, dlogits) of the last forward, for dy [tokens, n] and the losses' gradients [2]."""
+        """(dx, dw, dlogits) of the last forward, for dy [tokens, n] in w's type and the losses' gradients [2] in fp32."""
+        (e, n, k), (t, _) = self.w.shape, self.router.logits.shape
+        dy = _check("dy", dy, (t, n), self.w.dtype).contiguous()
+        if dlosses is not None:
+            dlosses = _check("dlosses", dlosses, (2,), torch.float32).contiguous()
         gg, b, s, r = self.gg, self.backend, _stream(), self.router
-        (e, n, k), t = self.w.shape, dy.shape[0]
         dt = _dtype(gg, dy.dtype)
         drows = torch.empty_like(self.rows)
         dweights = torch.empty_like(r.weights)
@@ -161,6 +200,10 @@ class ServingLayer:
         gg = load_package()
         e, n, half = qweight.shape
         k, dev, dtype = 2 * half, qweight.device, scales.dtype
+        _check("qweight", qweight, (e, n, half), torch.uint8)
+        _check("scales", scales, (e, n, -(-k // group)), *HALF)
+        if zeros is not None:
+            _check("zeros", zeros, (e, n, -(-k // group)), torch.uint8)
         self.keep = (qweight, scales, zeros)
         self.x = torch.zeros(tokens, k, dtype=dtype, device=dev)
         self.mask = torch.zeros(tokens, dtype=torch.uint8, device=dev)  # places without a token

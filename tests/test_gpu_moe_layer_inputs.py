@@ -1,0 +1,79 @@
+"""A training step of the layer (moe_layer.py) on tensors as autograd and slicing hand them on: the same bits as on dense copies."""
+import importlib.util
+import os
+
+import pytest
+
+from conftest import PKG_DIR
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def layer(gg):
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    spec = importlib.util.spec_from_file_location("moe_layer_inputs", os.path.join(PKG_DIR, "moe_layer.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def a_step(layer, w, top_k, x, logits, mask, dy, dlosses):
+    step = layer.TrainingLayer(w, top_k)
+    return step.forward(x, logits, mask) + step.backward(dy, dlosses)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_strides(layer, kind):
+    import torch
+
+    t, e, n, k, top_k = 150, 8, 136, 72, 3
+    dt = torch.bfloat16 if kind == "bf16" else torch.float16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    w = (rand(e, n, k) / k ** 0.5).to(dt)
+    views = dict(
+        x=[rand(k, t).to(dt).t(), rand(t, k + 8).to(dt)[:, :k], rand(2 * t, k).to(dt)[::2]],
+        logits=[rand(e, t).t(), rand(t, 2 * e)[:, ::2].bfloat16(), rand(1, e).expand(t, e)],
+        mask=[(rand(t, 2) > -1).to(torch.uint8)[:, 0], rand(t) > -1, None],
+        dy=[rand(()).to(dt).expand(t, n), rand(1, n).to(dt).expand(t, n), rand(n, t).to(dt).t()],  # the first: the gradient of y.sum()
+        dlosses=[rand(()).expand(2), rand(4)[::2], None])
+    for i in range(3):
+        at = [views[name][i] for name in ("x", "logits", "mask", "dy", "dlosses")]
+        dense = [v if v is None else v.clone(memory_format=torch.contiguous_format) for v in at]
+        for a, b in zip(a_step(layer, w, top_k, *at), a_step(layer, w, top_k, *dense)):
+            assert a.is_contiguous() and torch.equal(a, b)
+
+
+def test_refused_on_the_device(layer):
+    import torch
+
+    w = torch.zeros(4, 16, 32, dtype=torch.bfloat16, device="cuda")
+    step = layer.TrainingLayer(w, 2)
+    x, logits = torch.zeros(6, 32, dtype=torch.bfloat16, device="cuda"), torch.zeros(6, 4, device="cuda")
+    for bad in (dict(x=x.half()), dict(x=x.cpu()), dict(logits=logits.cpu()), dict(mask=torch.ones(6, dtype=torch.int64, device="cuda")),
+                dict(mask=torch.ones(6, dtype=torch.uint8))):
+        with pytest.raises(ValueError):
+            step.forward(**dict(dict(x=x, logits=logits), **bad))
+    step.forward(x, logits)
+    with pytest.raises(ValueError):
+        step.backward(torch.zeros(6, 16, device="cuda"))
+    with pytest.raises(ValueError):
+        step.backward(torch.zeros(6, 16, dtype=torch.bfloat16))
+    dx, dw, dlogits = step.backward(torch.zeros(6, 16, dtype=torch.bfloat16, device="cuda"))
+    assert (dx == 0).all() and (dw == 0).all() and (dlogits == 0).all()
+
+
+def test_no_live_token(layer):
+    """Nothing to route: outputs and gradients are zero, the experts' too."""
+    import torch
+
+    w = torch.randn(4, 16, 32, device="cuda").bfloat16()
+    step = layer.TrainingLayer(w, 2)
+    x, logits = torch.randn(6, 32, device="cuda").bfloat16(), torch.randn(6, 4, device="cuda")
+    y, losses = step.forward(x, logits, torch.zeros(6, dtype=torch.bool, device="cuda"))
+    for v in (y, losses) + step.backward(torch.randn(6, 16, device="cuda").bfloat16(), torch.ones(2, device="cuda")):
+        assert (v == 0).all()
