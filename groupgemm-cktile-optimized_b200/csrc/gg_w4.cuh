@@ -368,10 +368,19 @@ template <int kBytes> struct W4Queue {
         from += kWords;
     }
     // Up to eight values into the queue (returned: how many), and the next visit on its way where there is one before group `last`.
+    // Past the row's last group the values are 0: the sums of a step's groups there are 0, and the next row's scale may be infinite or NaN.
     __device__ __forceinline__ int refill(int groups, int last) {
 #pragma unroll
         for (int i = 0; i < kWords; ++i)
             word[i] = __funnelshift_r(raw[i], raw[i + 1], shift);
+        const int left = groups - at;
+        if (left < 8) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const int bits = 8 * (left * kBytes - 4 * i);  // of this word, inside the row
+                word[i] = bits >= 32 ? word[i] : bits > 0 ? word[i] & ((1u << bits) - 1u) : 0u;
+            }
+        }
         at += 8;
         if (at < last)
             load(groups);

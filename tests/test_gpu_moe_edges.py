@@ -1,9 +1,11 @@
 """The layer operators (router, dispatch / combine, 4-bit products) where sizes, handles and values meet the limits of a kernel's
 variant. Plain implementations, tolerances and helpers are those of test_gpu_moe_ops.py.
 """
+import math
+
 import pytest
 
-from test_gpu_moe_ops import Route, _torch, check_route, make_logits
+from test_gpu_moe_ops import Route, _torch, check_route, make_logits, run_w4, w4_case
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +40,27 @@ def test_routers_of_one_kernel_beside_one_another(gg, kind, large, small):
     for _ in range(2):
         for r, logits, mask in made:
             check_route(r.run(), logits, mask, 4, True)
+
+
+# ---- 4-bit products -----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("counts", [[2, 3], [40, 33]])  # one form and the other
+@pytest.mark.parametrize("k,group", [(96, 64), (160, 32), (2880, 64), (1056, 32), (480, 64), (992, 32)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_w4_scales_stay_in_their_row(gg, counts, k, group, bad, kind):
+    """A scale that is not finite makes its own weight row so, and no other: k ends inside a step, so the step has groups past the row."""
+    torch = _torch()
+    n = 24
+    for zeros in (False, True):
+        c = w4_case(torch, counts, n, k, group, zeros, kind, 0, 0)
+        clean, _ = run_w4(gg, torch, c, counts, n, k, group, kind, 0)
+        c["scales"][0, 5, 0] = bad
+        c["scales"][1, 0, 0] = bad
+        got, _ = run_w4(gg, torch, c, counts, n, k, group, kind, 0)
+        m = counts[0]
+        assert not torch.isfinite(got.t[:m, 5]).any() and not torch.isfinite(got.t[m:, 0]).any()
+        keep = [i for i in range(n) if i != 5]
+        assert torch.equal(got.t[:m][:, keep], clean.t[:m][:, keep])
+        assert torch.equal(got.t[m:, 1:], clean.t[m:, 1:])
