@@ -487,7 +487,7 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     const int64_t steps = (q.k + gg::moe::kW4StepK - 1) / gg::moe::kW4StepK;
     // partial sums: of the two cut tiles of a CTA, or (few) of the units of split items; a counter: the next unit (few)
     const int64_t tiles = (q.n + gg::moe::kW4TileRows - 1) / gg::moe::kW4TileRows;
-    const int64_t items = std::min<int64_t>(q.rows, q.experts + q.rows / v.tokens) * tiles;
+    const int64_t items = std::min<int64_t>(q.rows, q.experts + q.rows / v.tokens) * tiles;  // at most
     int64_t span = steps;
     if (few && items < gg::moe::kW4FewUnits * int64_t(ctas)) {
         const int64_t most = (gg::moe::kW4FewUnits * int64_t(ctas) + items - 1) / std::max<int64_t>(1, items);  // splits
@@ -522,7 +522,6 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     p.tiles = int((q.n + gg::moe::kW4TileRows - 1) / gg::moe::kW4TileRows);
     p.steps = int(steps);
     p.chunk = v.tokens;
-    p.max_items = items;
     p.ctas = ctas;
     p.splits = int(splits);
     p.span = int(span);

@@ -36,7 +36,6 @@ struct W4Params {
     float *ws;               // [2 x grid][tokens of a chunk][256] partial sums
     int32_t *counters;       // w4_few: the next unit of work, 0 between launches
     int64_t rows, slots;     // slots: tokens * top_k
-    int64_t max_items;       // that rising offsets can give
     uint64_t timeout_ns;
     int n, k, groups, experts, top_k, tiles, steps;  // steps: of 128 k
     int chunk;         // tokens of a chunk
@@ -154,20 +153,27 @@ struct W4Work {
     int64_t total, begin, end;  // steps: of the launch, this CTA's range
     int ctas;
 
-    // offsets come from the device: each is held to the range that the rows allow
+    // offsets come from the device: each is held to the range that the rows allow. Where they fall, no expert gets rows: what is sized by
+    // the rows (items, workspace, 32-bit indices) holds for rising offsets. By all threads of the block, which are together after it.
     static __device__ __forceinline__ void starts(const W4Params &p, int *start) {
+        bool falls = false;
         for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) {
             const int64_t v = p.offsets[e], before = e ? p.offsets[e - 1] : 0;
-            if (v < before || v > p.rows || before < 0)
+            falls |= v < before;
+            if (v < before || v > p.rows)
                 report(p.status, kSiteOffsets);
             start[e] = int(max(int64_t(0), min(v, p.rows)));
+        }
+        if (__syncthreads_or(falls)) {
+            for (int e = threadIdx.x; e <= p.experts; e += blockDim.x)
+                start[e] = 0;
+            __syncthreads();
         }
     }
     __device__ __forceinline__ W4Work(const W4Params &p, int *start_, int *first_) : start(start_), first(first_) {
         const int E = p.experts, tid = threadIdx.x;
         starts(p, start_);
-        __syncthreads();
-        auto chunks_of = [&](int e) { return (max(0, start[e + 1] - start[e]) + p.chunk - 1) / p.chunk; };
+        auto chunks_of = [&](int e) { return (start[e + 1] - start[e] + p.chunk - 1) / p.chunk; };
         const int per = (E + int(blockDim.x) - 1) / int(blockDim.x);
         int sum = 0, chunks;
         for (int e = tid * per; e < min(E, (tid + 1) * per); ++e)
@@ -234,7 +240,6 @@ template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherT
     // to end: every block of this one has passed its own wait by then. Before it reads xs it waits for this one.
     ptx::griddep_launch_dependents();
     W4Work::starts(p, start);
-    __syncthreads();
     const int pieces = p.steps * (kW4StepK / 8), first_piece = int(blockIdx.y) * kW4GatherThreads + int(threadIdx.x);
     const int more = int(gridDim.y) * kW4GatherThreads;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -260,8 +265,6 @@ template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherT
         }
         const int in_expert = int(r) - start[lo], i = in_expert % p.chunk;
         const int count = (min(p.chunk, start[lo + 1] - (int(r) - i)) + 7) & ~7;
-        if (i >= count)
-            continue;  // falling offsets, reported
         const T *from = static_cast<const T *>(p.x) + row * p.k;
         uint8_t *to = p.xs + int64_t(int(r) - i + 8 * lo) * p.steps * kW4TokenBytes;
 #pragma unroll 4
@@ -398,11 +401,8 @@ template <int kBytes> struct W4Queue {
     }
 };
 
-// Items of the launch; none where falling and rising offsets (reported) make more of them than the workspace holds.
-__device__ __forceinline__ int w4_items(const W4Params &p, const int *first) {
-    const int64_t items = int64_t(first[p.experts]) * p.tiles;
-    return items > p.max_items ? 0 : int(items);
-}
+// Items of the launch.
+__device__ __forceinline__ int w4_items(const W4Params &p, const int *first) { return first[p.experts] * p.tiles; }
 // A unit's sums [token][256], where items are split.
 __device__ __forceinline__ float *w4_sums(const W4Params &p, int item, int split) {
     return p.ws + (int64_t(item) * p.splits + split) * (kW4FewTokens * kW4TileRows);

@@ -229,8 +229,8 @@ int gg_prepare_permute(gg_handle *h, const gg_permute_problem *p, int32_t op, gg
  *   out[r, n] = sum over groups g of scales[e, n, g] * sum_{k in g} (q[e, n, k] - zeros[e, n, g]) * x[row(r), k]
  *
  * for the rows r of expert e, offsets[e] <= r < offsets[e + 1]; row(r) = src[r] / top_k, or r without
- * src (so the first product of a layer gathers its tokens itself). Rows of no expert are zero. offsets and src are
- * the router's, in device memory: no count goes to the host. q is 4 bits, two to a byte (even k in the low
+ * src (so the first product of a layer gathers its tokens itself). Rows of no expert are zero, and all rows where offsets
+ * fall (which is reported). offsets and src are the router's, in device memory: no count goes to the host. q is 4 bits, two to a byte (even k in the low
  * half), zeros NULL = 8 everywhere (else its low four bits). The integers q - zero are exact in 16 bits,
  * products are summed in fp32, the scale is applied to each group's fp32 sum, and the result rounded once.
  *

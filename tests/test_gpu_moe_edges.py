@@ -64,3 +64,21 @@ def test_w4_scales_stay_in_their_row(gg, counts, k, group, bad, kind):
         keep = [i for i in range(n) if i != 5]
         assert torch.equal(got.t[:m][:, keep], clean.t[:m][:, keep])
         assert torch.equal(got.t[m:, 1:], clean.t[m:, 1:])
+
+
+@pytest.mark.parametrize("counts", [[2, 3, 0, 1], [40, 33, 0, 20]])
+@pytest.mark.parametrize("top_k", [0, 2])
+def test_w4_falling_offsets(gg, counts, top_k):
+    """Offsets that fall are reported and leave no expert any rows; those that only reach past the rows are cut there."""
+    torch = _torch()
+    n, k, group, rows = 600, 256, 128, sum(counts)
+    c = w4_case(torch, counts, n, k, group, False, "bf16", top_k, 0)
+    good, _ = run_w4(gg, torch, c, counts, n, k, group, "bf16", top_k)
+    for bad in ([0, rows, 0, rows, 0], [0, rows, 0, rows, rows], [-5, 0, 1, 2, rows], [0, 2, 1, 5, rows], [0, 1, 2, 2, -(1 << 31)], [0, 1 << 30, 0, 1 << 30, rows]):
+        offsets = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        got, _ = run_w4(gg, torch, dict(c, offsets=offsets), counts, n, k, group, "bf16", top_k, status=0x2012)
+        assert (got.t == 0).all()
+    offsets = c["offsets"].clone()
+    offsets[-1] = (1 << 31) - 1
+    got, _ = run_w4(gg, torch, dict(c, offsets=offsets), counts, n, k, group, "bf16", top_k, status=0x2012)
+    assert torch.equal(got.t, good.t)
