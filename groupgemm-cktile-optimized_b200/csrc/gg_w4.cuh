@@ -60,14 +60,14 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 // Four bits as a 16-bit float without a conversion or a power of two to put them on: where a format's exponent field is 0 or
 // 1 its value is linear in its bits, i * 2^-24 (fp16, i below 2048) and i * 2^-133 (bf16, i below 256). So a masked nibble in bits
 // 0-3 or 4-7 is q or 16 q times that unit, and one fma by a power of two brings both to (q - zero) * W4Unit::kValue, exactly (the
-// subnormal inputs are not flushed by it). bf16 cannot reach 1 in one multiplication, so its weights stay in units of 2^-9, which
-// the group's scale takes back in fp32. A word costs 5 instructions on the ALU pipe (one shift, four masks) and 4 on the
+// subnormal inputs are not flushed by it). bf16 cannot reach 1 in one multiplication, so its weights stay in units of 2^-9 (fp16's of
+// 2^-12), which the fp32 sum over all groups takes back: in the scales they would carry those above 2^119 out of fp32's range. A word costs 5 instructions on the ALU pipe (one shift, four masks) and 4 on the
 // FMA pipe; with powers of two or'ed in, bf16 had needed 7 and 4: 150 ns for a warp's step of 32 rows x 128 k against 111.
 template <class T> struct W4Unit;
 template <> struct W4Unit<__half> {
     static constexpr uint32_t kLow = 0x6c006c00u;     // 2^12: with kHigh 2^8, weights in units of 2^-12
     static constexpr uint32_t kHigh = 0x5c005c00u;    // 2^8
-    static constexpr float kBack = 4096.0f;
+    static constexpr float kBack = 4096.0f;  // of a sum to its value
 };
 template <> struct W4Unit<__nv_bfloat16> {
     static constexpr uint32_t kLow = 0x7d807d80u;     // 2^124
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
                             ptx::mbar_arrive(empty(st));
                     }
                     const uint16_t bits = uint16_t(scales.take());
-                    const float scale = to_f32(*reinterpret_cast<const T *>(&bits)) * W4Unit<T>::kBack;
+                    const float scale = to_f32(*reinterpret_cast<const T *>(&bits));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float f = __shfl_sync(0xffffffffu, scale, g + 8 * i);
@@ -654,10 +654,11 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
                     const int row = 16 * m + 8 * (i >> 1) + g, tok = 2 * t + (i & 1);
                     if (tok >= it.count || it.n0 + warp * 32 + row >= p.n)
                         continue;
+                    const float v = sum[m][i] * W4Unit<T>::kBack;
                     if (p.splits == 1)
-                        out[int64_t(tok) * p.n + row] = from_f32<T>(sum[m][i]);
+                        out[int64_t(tok) * p.n + row] = from_f32<T>(v);
                     else
-                        __stcg(mine + tok * kW4TileRows + row, sum[m][i]);
+                        __stcg(mine + tok * kW4TileRows + row, v);
                 }
             r = ring[seq % kW4FewRing];
         }
@@ -988,7 +989,7 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
 #pragma unroll
                 for (int s = 0; s < kSub; ++s) {
                     const uint16_t bits = uint16_t(scales.take());
-                    const float scale = to_f32(*reinterpret_cast<const T *>(&bits)) * W4Unit<T>::kBack;
+                    const float scale = to_f32(*reinterpret_cast<const T *>(&bits));
 #pragma unroll
                     for (int q = 0; q < kTokens / 16; ++q)
                         if (16 * q < npad) {
@@ -1027,13 +1028,13 @@ __global__ void __launch_bounds__(kW4ManyThreads, 1) w4_many(const __grid_consta
 #pragma unroll
                 for (int i = 0; i < kTokens; ++i)
                     if (i < it.count)
-                        out[int64_t(i) * p.n] = from_f32<T>(sum[i]);
+                        out[int64_t(i) * p.n] = from_f32<T>(sum[i] * W4Unit<T>::kBack);
             } else {
                 float *mine = work.slot(p, blockIdx.x, work.first_cta(p, item)) + 128 * h + row;
 #pragma unroll
                 for (int i = 0; i < kTokens; ++i)
                     if (i < it.count)
-                        __stcg(mine + i * kW4TileRows, sum[i]);
+                        __stcg(mine + i * kW4TileRows, sum[i] * W4Unit<T>::kBack);
             }
         });
     }

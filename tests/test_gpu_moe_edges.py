@@ -5,7 +5,7 @@ import math
 
 import pytest
 
-from test_gpu_moe_ops import Route, _torch, check_route, make_logits, run_w4, w4_case
+from test_gpu_moe_ops import HALF_ULP, TINY, U, Route, _torch, check_route, close, make_logits, run_w4, w4_case, w4_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,24 @@ def test_w4_falling_offsets(gg, counts, top_k):
     offsets[-1] = (1 << 31) - 1
     got, _ = run_w4(gg, torch, dict(c, offsets=offsets), counts, n, k, group, "bf16", top_k, status=0x2012)
     assert torch.equal(got.t, good.t)
+
+
+@pytest.mark.parametrize("counts", [[2, 3], [40, 33]])
+@pytest.mark.parametrize("k,group", [(256, 128), (160, 32), (4096, 64)])
+@pytest.mark.parametrize("power", [127, -100])
+def test_w4_scales_of_any_size(gg, counts, k, group, power):
+    """Scales up to the type's largest times a small x, and scales near its smallest times a large x."""
+    torch = _torch()
+    n = 24
+    c = w4_case(torch, counts, n, k, group, True, "bf16", 0, 0)
+    c["scales"] = c["scales"] * 2.0 ** power
+    c["x"] = c["x"] * 2.0 ** (-100 if power > 0 else 90)
+    assert torch.isfinite(c["scales"]).all()
+    out, _ = run_w4(gg, torch, c, counts, n, k, group, "bf16", 0)
+    at = 0
+    for e, m in enumerate(counts):
+        ref, mag = w4_ref(torch, c["q"][e], c["scales"][e], c["zeros"][e], group, c["x"][at:at + m])
+        tol = (k / 8 + 64) * 2 * U * mag
+        tol = tol + HALF_ULP["bf16"] * (ref.abs() + tol) + TINY["bf16"]
+        close(out.t[at:at + m].double().cpu().numpy(), ref.cpu().numpy(), tol.cpu().numpy())
+        at += m
