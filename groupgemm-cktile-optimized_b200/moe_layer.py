@@ -95,9 +95,10 @@ def quantize_w4(w: torch.Tensor, group: int, symmetric: bool = True):
 
 class Router:
     """The router's handle and outputs (gg_prepare_route) for a buffer of logits [tokens, experts] and one of mask bytes [tokens], which
-    run() reads anew each time and which have to be contiguous for that."""
+    run() reads anew each time and which have to be contiguous for that. `backends`: the handles of the run and of the gradient."""
 
-    def __init__(self, logits: torch.Tensor, top_k: int, mask: torch.Tensor | None = None, normalize: bool = True, losses: bool = True):
+    def __init__(self, logits: torch.Tensor, top_k: int, mask: torch.Tensor | None = None, normalize: bool = True, losses: bool = True,
+                 backends=None):
         gg = load_package()
         t, e = logits.shape
         _check("logits", logits, (t, e), *LOGITS)
@@ -110,7 +111,7 @@ class Router:
         self.counts, self.offsets, self.live = new(e), new(e + 1), new(1)
         self.weights, self.lse = new(t, top_k, dtype=f32), new(t, dtype=f32)
         self.prob, self.losses = (new(e, dtype=f32), new(2, dtype=f32)) if losses else (None, None)
-        self.backend = gg.make_b200_backend()
+        self.backend, self.grad_backend = backends or (gg.make_b200_backend(), gg.make_b200_backend())
         _ready(self.backend.prepare_route(
             _dtype(gg, logits.dtype), t, e, top_k, _ptr(logits), _ptr(self.ids), _ptr(self.weights), _ptr(self.counts), _ptr(self.offsets),
             _ptr(self.live), _ptr(self.dest), _ptr(self.src), lse_ptr=_ptr(self.lse), prob_ptr=_ptr(self.prob), losses_ptr=_ptr(self.losses),
@@ -128,7 +129,7 @@ class Router:
         if dlosses is not None:
             dlosses = _check("dlosses", dlosses, (2,), torch.float32).contiguous()
         dlogits = torch.empty_like(self.logits)
-        b = gg.make_b200_backend()
+        b = self.grad_backend
         _ready(b.prepare_route_grad(
             _dtype(gg, self.logits.dtype), t, e, self.top_k, _ptr(self.logits), _ptr(dlogits), _ptr(self.ids), _ptr(self.lse),
             _ptr(self.counts), _ptr(self.live), dweights_ptr=_ptr(dweights), dlosses_ptr=_ptr(dlosses), mask_ptr=_ptr(self.mask),
@@ -139,7 +140,13 @@ class Router:
 
 class TrainingLayer:
     """One layer's forward and backward pass over 16-bit experts `w` [experts, n, k], which have to be contiguous. The tensors of a step
-    may have any strides (an expanded gradient, a transposed view): what is not contiguous is copied first."""
+    may have any strides (an expanded gradient, a transposed view): what is not contiguous is copied first.
+
+    Each operator has a handle of its own, so that what its kernels report (an index out of range, a wait that gave up) stays there for
+    check(), until the same operator is prepared again: the forward's until the next forward, the backward's until the next backward. check()
+    waits for the GPU and takes about 130 us, a third of a small step, so it is the caller's to call."""
+
+    OPERATORS = ("route", "dispatch", "products", "combine", "combine_grad", "dgrad", "wgrad", "dispatch_grad", "route_grad")
 
     def __init__(self, w: torch.Tensor, top_k: int, normalize: bool = True):
         self.gg = load_package()
@@ -147,11 +154,19 @@ class TrainingLayer:
         if not _check("w", w, (e, n, k), *HALF).is_contiguous():
             raise ValueError("w must be contiguous")
         self.w, self.top_k, self.normalize = w, top_k, normalize
-        self.backend = self.gg.make_b200_backend()
+        self.backends = {name: self.gg.make_b200_backend() for name in self.OPERATORS}
 
-    def _run(self, why: str) -> None:
-        _ready(why)
-        self.backend.run(_stream())
+    def check(self) -> None:
+        """Waits for the current stream and raises if a kernel of the last forward or backward reported an error."""
+        s = _stream()
+        bad = [f"{name}: {b.last_error()}" for name, b in self.backends.items() if b.device_status(s)]
+        if bad:
+            raise RuntimeError("; ".join(bad))
+
+    def _run(self, name: str, prepare: str, *args, **kw) -> None:
+        b, s = self.backends[name], _stream()
+        _ready(getattr(b, prepare)(*args, stream=s, **kw))
+        b.run(s)
 
     def forward(self, x: torch.Tensor, logits: torch.Tensor, mask: torch.Tensor | None = None):
         """x [tokens, k] in w's type, logits [tokens, experts] -> (y [tokens, n], losses [2]: balance and z)."""
@@ -160,17 +175,16 @@ class TrainingLayer:
         logits = _check("logits", logits, (t, e), *LOGITS).contiguous()
         if mask is not None:
             mask = _check("mask", mask, (t,), *MASK).contiguous()
-        self.router = r = Router(logits, self.top_k, mask, self.normalize)
+        self.router = r = Router(logits, self.top_k, mask, self.normalize, backends=(self.backends["route"], self.backends["route_grad"]))
         r.run()
-        gg, b, s = self.gg, self.backend, _stream()
-        dt = _dtype(gg, x.dtype)
+        dt = _dtype(self.gg, x.dtype)
         self.x_rows = torch.empty(t * self.top_k, k, dtype=x.dtype, device=x.device)
         self.rows = torch.empty(t * self.top_k, n, dtype=x.dtype, device=x.device)
         y = torch.empty(t, n, dtype=x.dtype, device=x.device)
-        self._run(b.prepare_dispatch(dt, t, self.top_k, e, k, _ptr(x), _ptr(r.dest), _ptr(r.offsets), _ptr(self.x_rows), stream=s))
+        self._run("dispatch", "prepare_dispatch", dt, t, self.top_k, e, k, _ptr(x), _ptr(r.dest), _ptr(r.offsets), _ptr(self.x_rows))
         self.group_m = r.counts.tolist()
-        self._run(b.prepare(dt, self.group_m, n, k, _ptr(self.x_rows), _ptr(self.w), _ptr(self.rows), stream=s))
-        self._run(b.prepare_combine(dt, t, self.top_k, e, n, _ptr(self.rows), _ptr(r.dest), _ptr(y), weights_ptr=_ptr(r.weights), stream=s))
+        self._run("products", "prepare", dt, self.group_m, n, k, _ptr(self.x_rows), _ptr(self.w), _ptr(self.rows))
+        self._run("combine", "prepare_combine", dt, t, self.top_k, e, n, _ptr(self.rows), _ptr(r.dest), _ptr(y), weights_ptr=_ptr(r.weights))
         return y, r.losses
 
     def backward(self, dy: torch.Tensor, dlosses: torch.Tensor | None = None):
@@ -179,16 +193,15 @@ class TrainingLayer:
         dy = _check("dy", dy, (t, n), self.w.dtype).contiguous()
         if dlosses is not None:
             dlosses = _check("dlosses", dlosses, (2,), torch.float32).contiguous()
-        gg, b, s, r = self.gg, self.backend, _stream(), self.router
-        dt = _dtype(gg, dy.dtype)
+        r, dt = self.router, _dtype(self.gg, dy.dtype)
         drows = torch.empty_like(self.rows)
         dweights = torch.empty_like(r.weights)
         dx_rows, dx, dw = torch.empty_like(self.x_rows), torch.empty(t, k, dtype=dy.dtype, device=dy.device), torch.empty_like(self.w)
-        self._run(b.prepare_combine_grad(dt, t, self.top_k, e, n, _ptr(dy), _ptr(self.rows), _ptr(r.dest), _ptr(r.offsets), _ptr(drows),
-                                         weights_ptr=_ptr(r.weights), dweights_ptr=_ptr(dweights), stream=s))
-        self._run(b.prepare_grad(gg.OP_DGRAD, dt, self.group_m, n, k, dy_ptr=_ptr(drows), w_ptr=_ptr(self.w), dx_ptr=_ptr(dx_rows), stream=s))
-        self._run(b.prepare_grad(gg.OP_WGRAD, dt, self.group_m, n, k, dy_ptr=_ptr(drows), x_ptr=_ptr(self.x_rows), dw_ptr=_ptr(dw), stream=s))
-        self._run(b.prepare_combine(dt, t, self.top_k, e, k, _ptr(dx_rows), _ptr(r.dest), _ptr(dx), stream=s))
+        self._run("combine_grad", "prepare_combine_grad", dt, t, self.top_k, e, n, _ptr(dy), _ptr(self.rows), _ptr(r.dest), _ptr(r.offsets),
+                  _ptr(drows), weights_ptr=_ptr(r.weights), dweights_ptr=_ptr(dweights))
+        self._run("dgrad", "prepare_grad", self.gg.OP_DGRAD, dt, self.group_m, n, k, dy_ptr=_ptr(drows), w_ptr=_ptr(self.w), dx_ptr=_ptr(dx_rows))
+        self._run("wgrad", "prepare_grad", self.gg.OP_WGRAD, dt, self.group_m, n, k, dy_ptr=_ptr(drows), x_ptr=_ptr(self.x_rows), dw_ptr=_ptr(dw))
+        self._run("dispatch_grad", "prepare_combine", dt, t, self.top_k, e, k, _ptr(dx_rows), _ptr(r.dest), _ptr(dx))
         return dx, dw, r.grad(dweights, dlosses)
 
 
@@ -256,6 +269,7 @@ def main() -> None:
     layer = TrainingLayer(w, top_k)
     y, losses = layer.forward(x, logits, mask)
     dx, dw, dlogits = layer.backward(dy, dlosses)
+    layer.check()
     leaves = [v.double().requires_grad_() for v in (x, w)] + [logits.double().requires_grad_()]
     py, pl = plain_layer(leaves[0], leaves[1], leaves[2], top_k, mask)
     (torch.sum(py * dy.double()) + torch.sum(pl * dlosses.double())).backward()

@@ -77,3 +77,46 @@ def test_no_live_token(layer):
     y, losses = step.forward(x, logits, torch.zeros(6, dtype=torch.bool, device="cuda"))
     for v in (y, losses) + step.backward(torch.randn(6, 16, device="cuda").bfloat16(), torch.ones(2, device="cuda")):
         assert (v == 0).all()
+
+
+def test_what_kernels_report_is_kept_for_check(layer):
+    """An index that a kernel finds out of range is reported though other operators ran after it."""
+    import torch
+
+    t, e, n, k = 50, 8, 64, 64
+    step = layer.TrainingLayer(torch.randn(e, n, k, device="cuda").bfloat16(), 2)
+    x, logits, dy = torch.randn(t, k, device="cuda").bfloat16(), torch.randn(t, e, device="cuda"), torch.randn(t, n, device="cuda").bfloat16()
+    step.forward(x, logits)
+    step.backward(dy)
+    step.check()
+    step.forward(x, logits)
+    step.router.offsets[e] = 1 << 30  # read by combine's gradient alone
+    step.backward(dy)
+    step.forward(x, logits)  # the forward's own handles are prepared again
+    with pytest.raises(RuntimeError, match="^combine_grad: index out of range: status 0x2012$"):
+        step.check()
+    step.check()  # read and cleared
+    step.router.ids[7, 1] = e  # read by the router's gradient alone
+    step.backward(dy)
+    with pytest.raises(RuntimeError, match="^route_grad: index out of range: status 0x2013$"):
+        step.check()
+    step.forward(x, logits)
+    step.backward(dy)
+    step.check()
+
+
+def test_one_layer_steps_of_many_sizes(layer):
+    """The handles are kept from step to step: other numbers of tokens, and no tokens, between two equal steps."""
+    import torch
+
+    e, n, k = 8, 136, 72
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    w = (rand(e, n, k) / k ** 0.5).bfloat16()
+    kept = layer.TrainingLayer(w, 3)
+    for t in (40, 700, 0, 1, 40, 3000, 40):
+        x, logits, dy, dlosses = rand(t, k).bfloat16(), rand(t, e), rand(t, n).bfloat16(), rand(2)
+        got = kept.forward(x, logits) + kept.backward(dy, dlosses)
+        kept.check()
+        for a, b in zip(got, a_step(layer, w, 3, x, logits, None, dy, dlosses)):
+            assert torch.equal(a, b)
