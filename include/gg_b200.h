@@ -137,6 +137,8 @@ int gg_prepare_grad(gg_handle *h, const gg_grad_problem *p, int32_t op, gg_strea
  * A token whose mask byte is 0, or all of whose logits are -inf, is not live: ids -1, weights 0, lse -inf,
  * and nothing of its logits (NaN included) goes anywhere. In a live row NaN counts as larger than +inf for
  * the choice, and a row that holds NaN or +inf has NaN weights and lse (as the formulas give).
+ * With u = 2^-24 and d a logit's distance from the row's largest, a probability's relative error is up to (2 d + 64) u, and
+ * one below 2^-126 of the largest counts as 0; lse's error is that of one rounding and of the sum, (|lse| + 64) u at most.
  *
  *   counts_e: slots (t, j) of expert e       offsets: their exclusive prefix sums, [experts + 1]
  *   dest_tj: place of slot (t, j) in the order by expert, slots of one expert in (t, j) order; -1 for none

@@ -3,6 +3,7 @@ variant. Plain implementations, tolerances and helpers are those of test_gpu_moe
 """
 import math
 
+import numpy as np
 import pytest
 
 from test_gpu_moe_ops import HALF_ULP, TINY, U, Route, _torch, check_route, close, make_logits, run_w4, w4_case, w4_ref
@@ -40,6 +41,20 @@ def test_routers_of_one_kernel_beside_one_another(gg, kind, large, small):
     for _ in range(2):
         for r, logits, mask in made:
             check_route(r.run(), logits, mask, 4, True)
+
+
+def test_route_lse_near_zero(gg):
+    """Rows of two open experts with logits 0 and x: lse = log(1 + e^x), whose sum rounds once (u) where its exponential is within (|x| + 4) u
+    and the logarithm within one unit in its last place (2 u). An approximate logarithm misses this by up to 2 u more."""
+    torch = _torch()
+    t, e = 4000, 8
+    x = torch.linspace(-10, -0.01, t, device="cuda")
+    logits = torch.full((t, e), -math.inf, device="cuda")
+    logits[:, 3], logits[:, 5] = 0.0, x
+    got = Route(gg, torch, "f32", logits, None, 2, True).run()["lse"]
+    x = x.double().cpu().numpy()
+    want = np.log1p(np.exp(x))
+    close(got, want, U * (1 + (4 - x) * np.exp(x) / (1 + np.exp(x)) + 2 * want))
 
 
 # ---- 4-bit products -----------------------------------------------------------------------------------
