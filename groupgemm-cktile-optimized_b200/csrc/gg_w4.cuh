@@ -33,7 +33,7 @@ struct W4Params {
     void *out;               // [rows, n]
     uint32_t *status;        // [0] status word, [2] timeouts of this launch
     uint8_t *xs;             // [rows + 8 experts][steps] 256 bytes: the rows of x as the products read them (w4_gather)
-    float *ws;               // [2 x grid][tokens of a chunk][256] partial sums
+    float *ws;               // partial sums: [items][splits][8][256] (w4_few), [2 x ctas][tokens of a chunk][256] (w4_many)
     int32_t *counters;       // w4_few: the next unit of work, 0 between launches
     int64_t rows, slots;     // slots: tokens * top_k
     uint64_t timeout_ns;
@@ -50,7 +50,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  "l"(src), "r"(bytes), "r"(bar), "r"(pred)
                  : "memory");
 }
-__device__ __forceinline__ void named_sync(int bar, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory"); }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
