@@ -398,7 +398,6 @@ int prepare_permute(gg_handle *h, const gg_permute_problem &q, int32_t op, gg_st
     p.offsets = q.offsets;
     p.weights = q.weights;
     p.status = h->d_status;
-    p.tokens = q.tokens;
     p.rows = q.tokens * q.top_k;
     p.experts = q.experts;
     p.top_k = q.top_k;
