@@ -6,7 +6,8 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_moe_ops import HALF_ULP, TINY, U, Route, _torch, check_route, close, make_logits, run_w4, w4_case, w4_ref
+from test_gpu_moe_ops import (HALF_ULP, TINY, U, Guarded, Route, _torch, _type, check_route, close, grad_ref, make_logits, run_w4, w4_case,
+                              w4_ref)
 
 pytestmark = pytest.mark.gpu
 
@@ -55,6 +56,78 @@ def test_route_lse_near_zero(gg):
     x = x.double().cpu().numpy()
     want = np.log1p(np.exp(x))
     close(got, want, U * (1 + (4 - x) * np.exp(x) / (1 + np.exp(x)) + 2 * want))
+
+
+@pytest.mark.parametrize("t,e,k,kind,normalize", [
+    (14000, 256, 8, "f32", True),
+    (14000, 256, 8, "bf16", False),
+    (30011, 33, 3, "fp16", True),
+    (30011, 32, 4, "f32", False),
+    (9001, 1000, 32, "bf16", True),
+])
+def test_route_grad_of_more_rows_than_warps(gg, t, e, k, kind, normalize):
+    """Each warp takes several rows: the next row on its way, the slots' own part cleared between rows, dead rows among live ones."""
+    torch = _torch()
+    logits, mask = make_logits(torch, kind, t, e, t + e, pad=0.2, closed=0.1)
+    logits[mask == 0] = math.nan
+    r = Route(gg, torch, kind, logits, mask, k, normalize)
+    o = r.run()
+    rng = np.random.RandomState(t)
+    dw = rng.randn(t, k).astype(np.float32)
+    dw[o["ids"] < 0] = np.nan
+    dl = np.array([0.3, 0.02], np.float32)
+    dwt, dlt = torch.from_numpy(dw).cuda(), torch.from_numpy(dl).cuda()
+    out = Guarded(torch, (t, e), logits.dtype)
+    b, s = gg.make_b200_backend(), torch.cuda.current_stream().cuda_stream
+    assert b.prepare_route_grad(_type(gg, kind), t, e, k, logits.data_ptr(), out.ptr(), r.out["ids"].ptr(), r.out["lse"].ptr(),
+                                r.out["counts"].ptr(), r.out["live"].ptr(), dweights_ptr=dwt.data_ptr(), dlosses_ptr=dlt.data_ptr(),
+                                mask_ptr=mask.data_ptr(), normalize=normalize) == ""
+    blocks = int(b.detail().split("blocks=")[1])
+    assert t > 2 * 8 * blocks, "a warp has to get more than two rows"
+    b.run(s)
+    assert b.device_status(s) == 0
+    out.check(torch)
+    got = out.t.float().cpu().numpy().astype(np.float64)
+    l = logits.float().cpu().numpy().astype(np.float64)
+    m = mask.cpu().numpy()
+    l[m == 0] = 0.0
+    dw64 = np.where(o["ids"] >= 0, dw, 0.0).astype(np.float64)
+    ref = grad_ref(l, m, o["ids"], o["counts"], int(o["live"][0]), dw64, dl.astype(np.float64), k, normalize, 1.0)
+    n = max(int(o["live"][0]), 1)
+    size = np.abs(dw64).sum(1) + dl[0] * e * o["counts"].max(initial=0) / (k * n * n) + 2 * dl[1] * np.abs(
+        np.where(np.isfinite(o["lse"]), o["lse"], 0)) / n
+    close(got, ref, 512 * U * size[:, None] + HALF_ULP[kind] * np.abs(ref) + TINY[kind])
+    assert (got[m == 0] == 0).all()
+    first = out.t.clone()
+    b.run(s)
+    assert torch.equal(first.view(torch.uint8), out.t.view(torch.uint8))
+
+
+def test_handles_on_two_streams(gg):
+    """Routers and products of different sizes on two streams at a time, over and over: each handle's own results, bit for bit."""
+    torch = _torch()
+    streams, jobs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i, (t, e, k, counts) in enumerate([(3000, 256, 8, [3] * 20), (2000, 200, 4, [40, 9, 33])]):
+        logits, mask = make_logits(torch, "f32", t, e, i, pad=0.1)
+        r = Route(gg, torch, "f32", logits, mask, k, True)
+        want = r.run()
+        c = w4_case(torch, counts, 1032, 2048, 64, True, "bf16", 0, 0, seed=i)
+        out, b = run_w4(gg, torch, c, counts, 1032, 2048, 64, "bf16", 0)
+        jobs.append((r, want, c, out, b, out.t.clone()))
+        for v in r.out.values():
+            v.t.zero_()
+        out.t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, (r, _, _, _, b, _) in zip(streams, jobs):
+            r.b.run(s.cuda_stream)
+            b.run(s.cuda_stream)
+    for s, (r, want, _, out, b, product) in zip(streams, jobs):
+        assert r.b.device_status(s.cuda_stream) == 0 and b.device_status(s.cuda_stream) == 0
+        torch.cuda.synchronize()
+        for n, v in r.out.items():
+            assert v.t.cpu().numpy().tobytes() == want[n].tobytes(), n
+        assert torch.equal(out.t.view(torch.int16), product.view(torch.int16))
 
 
 # ---- 4-bit products -----------------------------------------------------------------------------------
@@ -118,3 +191,23 @@ def test_w4_scales_of_any_size(gg, counts, k, group, power):
         tol = tol + HALF_ULP["bf16"] * (ref.abs() + tol) + TINY["bf16"]
         close(out.t[at:at + m].double().cpu().numpy(), ref.cpu().numpy(), tol.cpu().numpy())
         at += m
+
+
+@pytest.mark.parametrize("counts", [[70000], [1, 40000, 0, 29997], [5] * 1024])
+@pytest.mark.parametrize("top_k", [0, 3])
+def test_w4_many_rows(gg, counts, top_k):
+    """More rows than the gather has blocks (65536), and an expert of many chunks."""
+    torch = _torch()
+    n, k, group, extra = 8, 32, 32, 5
+    c = w4_case(torch, counts, n, k, group, True, "bf16", top_k, extra)
+    out, _ = run_w4(gg, torch, c, counts, n, k, group, "bf16", top_k)
+    at = 0
+    for e, m in enumerate(counts):
+        r = torch.arange(at, at + m, device="cuda")
+        x = c["x"][c["src"][r].long() // top_k] if top_k else c["x"][r]
+        ref, mag = w4_ref(torch, c["q"][e], c["scales"][e], c["zeros"][e], group, x)
+        tol = (k / 8 + 64) * 2 * U * mag
+        tol = tol + HALF_ULP["bf16"] * (ref.abs() + tol) + TINY["bf16"]
+        assert ((out.t[r].double() - ref).abs() <= tol).all(), e
+        at += m
+    assert (out.t[at:] == 0).all()
