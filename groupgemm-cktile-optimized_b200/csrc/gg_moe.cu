@@ -473,10 +473,12 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
-    // Up to 6 rows an expert on average, chunks of 8 with mma.sync; above, chunks of 32 with tcgen05. Measured on 8 experts of 4096 x
-    // 7168, us, few / many: 1 row an expert 36 / 47, 8 rows 39 / 50, 16 rows 53 / 51 (the weights are then widened twice by the
-    // first), 24 rows 80 / 54, 32 rows 91 / 55; a mean of 6 already has experts with more than 8.
-    const bool few = q.rows <= 6 * int64_t(q.experts);
+    // Up to a chunk of 8 rows an expert on average, chunks of 8 with mma.sync; above, chunks of up to 32 with tcgen05. Us, few / many. Equal
+    // rows an expert (the first form widens the weights a second time from 9 on): 8 experts of 4096 x 7168 in groups of 128, 7 rows 39 / 50, 8
+    // 39 / 51, 9 57 / 50; 32 of 7168 x 2048 in groups of 64 with zeros 65 / 96, 65 / 96, 109 / 96; 64 of 4096 x 2048 in groups of 128 59 / 99, 60 /
+    // 100, 100 / 99. Uneven rows (up to 3 to 5 times the mean), means of 6, 8, 10, 12, 16: 39 / 50, 48 / 47, 48 / 51, 52 / 51, 65 / 52; 75 / 104,
+    // 80 / 108, 95 / 104, 109 / 108, 126 / 118; 69 / 96, 81 / 101, 92 / 102, 99 / 105, 126 / 110.
+    const bool few = q.rows <= gg::moe::kW4FewTokens * int64_t(q.experts);
     const W4Form v = q.dtype == GG_FP16 ? w4_form<__half>(q.group_size, few, q.zeros) : w4_form<__nv_bfloat16>(q.group_size, few, q.zeros);
     GG_CUDA(h, cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(v.smem)));
     if (const int rc = encode_bytes_3d(h, q.qweight, q.k / 2, q.n, q.experts, gg::moe::kW4StepK / 2, gg::moe::kW4TileRows))
@@ -487,6 +489,10 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     // partial sums: of the two cut tiles of a CTA, or (few) of the units of split items; a counter: the next unit (few)
     const int64_t tiles = (q.n + gg::moe::kW4TileRows - 1) / gg::moe::kW4TileRows;
     const int64_t items = std::min<int64_t>(q.rows, q.experts + q.rows / v.tokens) * tiles;  // at most
+    // Units a CTA and steps a unit, us with 4 of 8 or more / 3 of 8 / 3 of 10 / 3 of 16 / 2 of 16, one token through 8 experts: 4096 x 7168 in
+    // groups of 128 36.6 / 36.8 / 37.8 / 38.3 / 38.4, 4096 x 14336 61.8 / 59.7 / 59.4 / 59.5 / 59.1, 4096 x 4096 24.7 / 24.8 / 27.5 / 23.5 / 23.5, 2048 x
+    // 2880 15.0 / 15.0 / 16.9 / 20.5 / 20.5; 7168 x 2048 in groups of 64 with zeros 27.6 / 27.6 / 30.5 / 24.3 / 24.3; 1024 x 2048 in groups of 32 14.3
+    // / 14.3 / 15.9 / 18.8 / 18.8. So no choice is best throughout.
     int64_t span = steps;
     if (few && items < gg::moe::kW4FewUnits * int64_t(ctas)) {
         const int64_t most = (gg::moe::kW4FewUnits * int64_t(ctas) + items - 1) / std::max<int64_t>(1, items);  // splits

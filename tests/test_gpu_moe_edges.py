@@ -211,3 +211,37 @@ def test_w4_many_rows(gg, counts, top_k):
         assert ((out.t[r].double() - ref).abs() <= tol).all(), e
         at += m
     assert (out.t[at:] == 0).all()
+
+
+@pytest.mark.parametrize("counts", [[3, 12], [40, 33]])
+def test_w4_bad_source_rows(gg, counts):
+    """A source that is not a slot: reported, and no row but its own differs, in either form."""
+    torch = _torch()
+    n, k, group = 48, 256, 128
+    c = w4_case(torch, counts, n, k, group, False, "bf16", 2, 0)
+    good, _ = run_w4(gg, torch, c, counts, n, k, group, "bf16", 2)
+    for bad in (-1, c["tokens"] * 2, (1 << 31) - 1, -(1 << 31)):
+        src = c["src"].clone()
+        src[4] = bad
+        got, _ = run_w4(gg, torch, dict(c, src=src), counts, n, k, group, "bf16", 2, status=0x2011)
+        keep = [r for r in range(sum(counts)) if r != 4]
+        assert torch.equal(got.t[keep], good.t[keep]) and (got.t[4] == 0).all()
+
+
+def test_w4_forms_meet(gg):
+    """Numbers of rows on both sides of the change from one form to the other: each has the results of the definition."""
+    torch = _torch()
+    n, k, group = 264, 1152, 128
+    seen = set()
+    for counts in ([8] * 4, [8, 8, 8, 9], [0, 31, 1, 0], [0, 32, 1, 0], [33, 0, 0, 0]):
+        c = w4_case(torch, counts, n, k, group, True, "fp16", 0, 0)
+        out, b = run_w4(gg, torch, c, counts, n, k, group, "fp16", 0)
+        seen.add(b.detail().split("<")[1].split(">")[0])
+        at = 0
+        for e, m in enumerate(counts):
+            ref, mag = w4_ref(torch, c["q"][e], c["scales"][e], c["zeros"][e], group, c["x"][at:at + m])
+            tol = (k / 8 + 64) * 2 * U * mag
+            tol = tol + HALF_ULP["fp16"] * (ref.abs() + tol) + TINY["fp16"]
+            close(out.t[at:at + m].double().cpu().numpy(), ref.cpu().numpy(), tol.cpu().numpy())
+            at += m
+    assert seen == {"fp16,few", "fp16,many"}
