@@ -152,9 +152,10 @@ struct W4Work {
     int64_t total, begin, end;  // steps: of the launch, this CTA's range
     int ctas;
 
-    // offsets come from the device: each is held to the range that the rows allow. Where they fall, no expert gets rows: what is sized by
-    // the rows (items, workspace, 32-bit indices) holds for rising offsets. By all threads of the block, which are together after it.
-    static __device__ __forceinline__ void starts(const W4Params &p, int *start) {
+    // offsets come from the device: each is held to the range that the rows allow. Returns whether they fall anywhere; then no expert gets
+    // rows: what is sized by the rows (items, workspace, 32-bit indices) holds for rising offsets. By all threads of the block, which are
+    // together after it. (Setting start to 0 here in place of a flag cost one token's products 0.6 us of 36.)
+    static __device__ __forceinline__ bool starts(const W4Params &p, int *start) {
         bool falls = false;
         for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) {
             const int64_t v = p.offsets[e], before = e ? p.offsets[e - 1] : 0;
@@ -163,15 +164,11 @@ struct W4Work {
                 report(p.status, kSiteOffsets);
             start[e] = int(max(int64_t(0), min(v, p.rows)));
         }
-        if (__syncthreads_or(falls)) {
-            for (int e = threadIdx.x; e <= p.experts; e += blockDim.x)
-                start[e] = 0;
-            __syncthreads();
-        }
+        return __syncthreads_or(falls) != 0;
     }
     __device__ __forceinline__ W4Work(const W4Params &p, int *start_, int *first_) : start(start_), first(first_) {
         const int E = p.experts, tid = threadIdx.x;
-        starts(p, start_);
+        const bool falls = starts(p, start_);
         auto chunks_of = [&](int e) { return (start[e + 1] - start[e] + p.chunk - 1) / p.chunk; };
         const int per = (E + int(blockDim.x) - 1) / int(blockDim.x);
         int sum = 0, chunks;
@@ -183,9 +180,9 @@ struct W4Work {
             at += chunks_of(e);
         }
         if (tid == 0)
-            first_[E] = chunks;
+            first_[E] = falls ? 0 : chunks;
         __syncthreads();
-        total = int64_t(chunks) * p.tiles * p.steps;
+        total = int64_t(falls ? 0 : chunks) * p.tiles * p.steps;
         ctas = int(min(int64_t(p.ctas), total));
         const int cta = blockIdx.x;
         begin = cta < ctas ? total * cta / ctas : 0;
@@ -238,11 +235,11 @@ template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherT
     // The product kernel may start now. It reads what earlier kernels wrote (offsets, scales, weights) without waiting for this one
     // to end: every block of this one has passed its own wait by then. Before it reads xs it waits for this one.
     ptx::griddep_launch_dependents();
-    W4Work::starts(p, start);
+    const bool falls = W4Work::starts(p, start);
     const int pieces = p.steps * (kW4StepK / 8), first_piece = int(blockIdx.y) * kW4GatherThreads + int(threadIdx.x);
     const int more = int(gridDim.y) * kW4GatherThreads;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        if (r < start[0] || r >= start[p.experts]) {
+        if (falls || r < start[0] || r >= start[p.experts]) {
             for (int col = first_piece; col < p.n; col += more)
                 static_cast<T *>(p.out)[r * p.n + col] = from_f32<T>(0.0f);
             continue;
