@@ -410,9 +410,10 @@ int prepare_permute(gg_handle *h, const gg_permute_problem &q, int32_t op, gg_st
                                  : reinterpret_cast<const void *>(&gg::moe::combine_rows<__nv_bfloat16>))
                          : (half ? reinterpret_cast<const void *>(&gg::moe::combine_grad_rows<__half>)
                                  : reinterpret_cast<const void *>(&gg::moe::combine_grad_rows<__nv_bfloat16>));
-    // Threads a token, us with at most 128 / 256 / 512 / 1024 of them: dispatch 16384 x 8 x 7168 356 / 354 / 344 / 336; combine 16384 x 8 x
-    // 4096 194 / 198 / 210 / 218, its gradient 7999 x 2 x 2880 40 / 41 / 48 / 48, but combine of 64 tokens 8.9 / 5.9 / 3.9 / 3.1. So dispatch takes
-    // 1024, the others 128, or as many more as fill the SMs. Then as few vectors a thread as that allows, and no idle warp.
+    // Threads a token, us with at most 128 / 256 / 512 / 1024 of them (launches of a graph): dispatch 16384 x 8 x 7168 356 / 354 / 339 / 330;
+    // combine 16384 x 8 x 4096 193 / 196 / 208 / 208, its gradient 7999 x 2 x 2880 39 / 41 / 47 / 47, but combine of 64 tokens x 4 x 7168 17.8 /
+    // 11.1 / 6.7 / 4.5. So dispatch takes 1024, the others 128, or as many more as fill the SMs. Then as few vectors a thread as that allows,
+    // and no idle warp.
     int most = gg::moe::kPermuteThreads;
     if (op != GG_OP_DISPATCH) {
         most = 128;

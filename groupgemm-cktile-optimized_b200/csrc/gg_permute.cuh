@@ -25,7 +25,7 @@ struct PermuteParams {
 
 // A block a token, each thread 16 bytes of its row at a time, and a block of its own for every token: all three are bound by DRAM,
 // and it is the many rows in flight that fill it (a warp a token, with four of its rows in flight, took 290 us for combine's
-// 16384 x 8 rows of 4096 against 194). The host picks the threads. A thread's loads of dest are one broadcast.
+// 16384 x 8 rows of 4096 against 198). The host picks the threads. A thread's loads of dest are one broadcast.
 //
 // dest's entry of a slot, -1 where it has none (or one that is out of range).
 __device__ __forceinline__ int64_t slot_row(const PermuteParams &p, int64_t slot) {

@@ -199,7 +199,7 @@ __device__ __forceinline__ void route_totals(const RouteParams &p, int tot, int 
 // One warp a token, V logits a lane. A block takes a contiguous run of tokens and each of its
 // warps a contiguous part of it, so that a warp's own counter of each expert gives the rank of a slot
 // among the warp's slots in order; the ranks are raised by the warps before in the block here and by the
-// blocks before in route_place, or here where one block takes all tokens. Bound by instruction issue: 690 a token with 256 experts
+// blocks before in route_place, or here where one block takes all tokens. Bound by instruction issue: 710 a token with 256 experts
 // and k = 8, 70% of the slots taken. 16384 tokens take 24.1 us with route_place (12% of that for the logits' bytes at the copy rate),
 // 1000 tokens of 33 experts 11.2, one token 6.4, which is what the call costs the host.
 template <class T, int V> __global__ void __launch_bounds__(route_warps(V) * 32) route_topk(const RouteParams p) {

@@ -682,9 +682,9 @@ __global__ void __launch_bounds__(kW4FewThreads, 2) w4_few(const __grid_constant
 // Three A operands and two D a half keep the widening from waiting for the MMAs. Measured: 8 experts of 4096 x 7168 (117 MB of
 // weights) in groups of 128, 8 rows each, 50.4 us, 16 51.1, 32 53.9, and 29.8, 29.8 and 32.9 us for each further 117 MB. No one part binds it (31 at the time):
 // without the widening 26, without that and tcgen05.st 24, without the products 27, without the sums 28, with all weights from L2 30;
-// the parts share the schedulers' issue slots (3200 instructions a step and SM, 1200 of them widening). Four warps that
+// the parts share the schedulers' issue slots (3000 instructions a step and SM, 1200 of them widening). Four warps that
 // issue the products in place of two gained 1 us at 8 rows and none at 32; eight more widening warps lost 3. Long runs of the
-// largest sizes meet the power cap: 128 tokens x 8 of 64 experts take 300 us in a burst and 335 in a second of calls.
+// largest sizes meet the power cap: 128 tokens x 8 of 64 experts take 300 us in 100 calls and 326 in 3000.
 constexpr int kW4ManyThreads = 640;
 
 // Tokens of a chunk: at most 32 (a thread holds a sum a token). Tensor Memory's 512 columns hold for each half kA operands of
