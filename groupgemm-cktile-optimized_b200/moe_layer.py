@@ -19,6 +19,7 @@ from __future__ import annotations
 import importlib.util
 import os
 import sys
+import weakref
 
 import torch
 
@@ -112,12 +113,19 @@ class Router:
         self.weights, self.lse = new(t, top_k, dtype=f32), new(t, dtype=f32)
         self.prob, self.losses = (new(e, dtype=f32), new(2, dtype=f32)) if losses else (None, None)
         self.backend, self.grad_backend = backends or (gg.make_b200_backend(), gg.make_b200_backend())
+        self._prepare()
+
+    def _prepare(self) -> None:
+        logits = self.logits
         _ready(self.backend.prepare_route(
-            _dtype(gg, logits.dtype), t, e, top_k, _ptr(logits), _ptr(self.ids), _ptr(self.weights), _ptr(self.counts), _ptr(self.offsets),
-            _ptr(self.live), _ptr(self.dest), _ptr(self.src), lse_ptr=_ptr(self.lse), prob_ptr=_ptr(self.prob), losses_ptr=_ptr(self.losses),
-            mask_ptr=_ptr(mask), normalize=normalize, stream=_stream()))
+            _dtype(load_package(), logits.dtype), *logits.shape, self.top_k, _ptr(logits), _ptr(self.ids), _ptr(self.weights), _ptr(self.counts),
+            _ptr(self.offsets), _ptr(self.live), _ptr(self.dest), _ptr(self.src), lse_ptr=_ptr(self.lse), prob_ptr=_ptr(self.prob),
+            losses_ptr=_ptr(self.losses), mask_ptr=_ptr(self.mask), normalize=self.normalize, stream=_stream()))
+        self.backend.router = weakref.ref(self)
 
     def run(self) -> None:
+        if self.backend.router() is not self:  # a handle that a later router was given too
+            self._prepare()
         self.backend.run(_stream())
 
     def grad(self, dweights: torch.Tensor | None, dlosses: torch.Tensor | None) -> torch.Tensor:

@@ -120,3 +120,23 @@ def test_one_layer_steps_of_many_sizes(layer):
         kept.check()
         for a, b in zip(got, a_step(layer, w, 3, x, logits, None, dy, dlosses)):
             assert torch.equal(a, b)
+
+
+def test_router_of_an_earlier_step(layer):
+    """The router of a step, kept by its user, stays that step's: it can be run again and differentiated after later steps."""
+    import torch
+
+    e, n, k = 8, 64, 64
+    step = layer.TrainingLayer(torch.randn(e, n, k, device="cuda").bfloat16(), 2)
+    a = torch.randn(50, e, device="cuda")
+    step.forward(torch.randn(50, k, device="cuda").bfloat16(), a)
+    first, dw = step.router, torch.randn(50, 2, device="cuda")
+    ids, d = first.ids.clone(), first.grad(dw, None)
+    step.forward(torch.randn(70, k, device="cuda").bfloat16(), torch.randn(70, e, device="cuda"))
+    later = step.router.ids.clone()
+    first.ids.zero_()
+    first.run()
+    assert torch.equal(first.ids, ids) and torch.equal(step.router.ids, later) and torch.equal(first.grad(dw, None), d)
+    step.router.ids.zero_()
+    step.router.run()
+    assert torch.equal(step.router.ids, later) and torch.equal(first.ids, ids)
