@@ -66,7 +66,8 @@ def _check(name: str, t, shape: tuple, *dtypes: torch.dtype):
 
 HALF = (torch.bfloat16, torch.float16)
 LOGITS = (torch.float32,) + HALF
-MASK = (torch.uint8, torch.bool)  # a byte a token
+BYTES = (torch.uint8, torch.int8)
+MASK = BYTES + (torch.bool,)  # a byte a token
 
 
 def _dtype(gg, dtype: torch.dtype) -> int:
@@ -221,10 +222,10 @@ class ServingLayer:
         gg = load_package()
         e, n, half = qweight.shape
         k, dev, dtype = 2 * half, qweight.device, scales.dtype
-        _check("qweight", qweight, (e, n, half), torch.uint8)
+        _check("qweight", qweight, (e, n, half), *BYTES)
         _check("scales", scales, (e, n, -(-k // group)), *HALF)
         if zeros is not None:
-            _check("zeros", zeros, (e, n, -(-k // group)), torch.uint8)
+            _check("zeros", zeros, (e, n, -(-k // group)), *BYTES)
         self.keep = (qweight, scales, zeros)
         self.x = torch.zeros(tokens, k, dtype=dtype, device=dev)
         self.mask = torch.zeros(tokens, dtype=torch.uint8, device=dev)  # places without a token

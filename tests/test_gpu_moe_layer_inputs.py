@@ -140,3 +140,25 @@ def test_router_of_an_earlier_step(layer):
     step.router.ids.zero_()
     step.router.run()
     assert torch.equal(step.router.ids, later) and torch.equal(first.ids, ids)
+
+
+def test_bytes_of_any_type(layer):
+    """Masks and packed weights are bytes: int8 and bool are read as uint8 is."""
+    import torch
+
+    t, e, n, k, top_k = 40, 4, 64, 64, 2
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    w, x, logits = rand(e, n, k).bfloat16(), rand(t, k).bfloat16(), rand(t, e)
+    mask = (rand(t) > 0).to(torch.uint8)
+    want = layer.TrainingLayer(w, top_k).forward(x, logits, mask)
+    for as_type in (torch.int8, torch.bool):
+        for a, b in zip(layer.TrainingLayer(w, top_k).forward(x, logits, mask.to(as_type)), want):
+            assert torch.equal(a, b)
+    q, scales, zeros = layer.quantize_w4(w, 32, symmetric=False)
+    out = []
+    for as_type in (torch.uint8, torch.int8):
+        s = layer.ServingLayer(q.view(as_type), scales, zeros.view(as_type), 32, t, top_k)
+        s.x.copy_(x), s.logits.copy_(logits), s.mask.copy_(mask)
+        out.append(s.run().clone())
+    assert torch.equal(*out) and (out[0][mask == 0] == 0).all()
