@@ -22,7 +22,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libgg_b200.so")
 DEBUG_LIB_PATH = os.path.join(HERE, "lib", "libgg_b200_debug.so")
 
 BF16, FP16 = 0, 1
-F32 = 2  # router logits only
+F32 = 2  # router logits, norm, rounding to 8 bits
 DTYPES = {"bf16": BF16, "fp16": FP16}
 
 GG_OK, GG_NOT_SUPPORTED, GG_ERR_ARG, GG_ERR_CUDA, GG_ERR_DEVICE = 0, 1, -1, -2, -3
@@ -89,6 +89,25 @@ class GGW4Problem(ctypes.Structure):
                 ("tokens", _i64)] + [(n, _vp) for n in ("x", "qweight", "scales", "zeros", "offsets", "src", "out")]
 
 
+class GGNormProblem(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("param_type", _i32), ("eps", _f32), ("tokens", _i64), ("hidden", _i64)] + [
+        (n, _vp) for n in ("x", "residual", "gamma", "beta", "sum", "y", "mean", "rstd", "q", "q_scales")]
+
+
+class GGNormGradProblem(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("param_type", _i32), ("tokens", _i64), ("hidden", _i64)] + [
+        (n, _vp) for n in ("x", "mean", "rstd", "gamma", "dy", "dsum", "dx", "dgamma", "dbeta")]
+
+
+class GGQuantProblem(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("rows", _i64), ("k", _i64)] + [(n, _vp) for n in ("x", "q", "scales")]
+
+
+class GGI8Problem(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("experts", _i32), ("top_k", _i32), ("n", _i64), ("k", _i64), ("rows", _i64), ("tokens", _i64)] + [
+        (n, _vp) for n in ("x", "x_scales", "weight", "scales", "offsets", "src", "out")]
+
+
 # Every symbol include/gg_b200.h declares, with its ctypes signature.
 SIGNATURES = {
     "gg_abi_version": (ctypes.c_int, []),
@@ -106,6 +125,10 @@ SIGNATURES = {
                                           ctypes.c_char_p, ctypes.c_size_t]),
     "gg_prepare_w4": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGW4Problem), ctypes.c_void_p, ctypes.c_char_p,
                                      ctypes.c_size_t]),
+    "gg_prepare_norm": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGNormProblem), ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
+    "gg_prepare_norm_grad": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGNormGradProblem), ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
+    "gg_prepare_quant": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGQuantProblem), ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
+    "gg_prepare_i8": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(GGI8Problem), ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
     "gg_run": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "gg_release": (None, [ctypes.c_void_p]),
     "gg_detail": (ctypes.c_char_p, [ctypes.c_void_p]),
@@ -284,6 +307,43 @@ class B200Backend:
                            src_ptr or None, out_ptr or None)
         why = ctypes.create_string_buffer(256)
         return self._prepared(self._lib.gg_prepare_w4(self._h, ctypes.byref(prob), ctypes.c_void_p(stream or None), why, 256), why)
+
+    def prepare_norm(self, dtype: int, tokens: int, hidden: int, x_ptr: int, y_ptr: int = 0, gamma_ptr: int = 0, beta_ptr: int = 0,
+                     param_type: int | None = None, residual_ptr: int = 0, sum_ptr: int = 0, mean_ptr: int = 0, rstd_ptr: int = 0,
+                     q_ptr: int = 0, q_scales_ptr: int = 0, eps: float = 1e-5, stream: int = 0) -> str:
+        """Prepare the layer norm (gg_prepare_norm) of x [tokens, hidden], plus residual where there is one: y, and where their pointers are
+        given sum, mean, rstd and y's 8-bit rows q with q_scales. param_type: of gamma and beta (dtype if None)."""
+        prob = GGNormProblem(int(dtype), int(dtype if param_type is None else param_type), float(eps), int(tokens), int(hidden), x_ptr or None,
+                             residual_ptr or None, gamma_ptr or None, beta_ptr or None, sum_ptr or None, y_ptr or None, mean_ptr or None,
+                             rstd_ptr or None, q_ptr or None, q_scales_ptr or None)
+        why = ctypes.create_string_buffer(256)
+        return self._prepared(self._lib.gg_prepare_norm(self._h, ctypes.byref(prob), ctypes.c_void_p(stream or None), why, 256), why)
+
+    def prepare_norm_grad(self, dtype: int, tokens: int, hidden: int, x_ptr: int, mean_ptr: int, rstd_ptr: int, dy_ptr: int, dx_ptr: int,
+                          gamma_ptr: int = 0, param_type: int | None = None, dsum_ptr: int = 0, dgamma_ptr: int = 0, dbeta_ptr: int = 0,
+                          stream: int = 0) -> str:
+        """Prepare the layer norm's backward pass (gg_prepare_norm_grad): dy [tokens, hidden] -> dx and, where their pointers are given,
+        dgamma and dbeta [hidden] in fp32. x is what was normalised (sum where there was a residual)."""
+        prob = GGNormGradProblem(int(dtype), int(dtype if param_type is None else param_type), int(tokens), int(hidden), x_ptr or None,
+                                 mean_ptr or None, rstd_ptr or None, gamma_ptr or None, dy_ptr or None, dsum_ptr or None, dx_ptr or None,
+                                 dgamma_ptr or None, dbeta_ptr or None)
+        why = ctypes.create_string_buffer(256)
+        return self._prepared(self._lib.gg_prepare_norm_grad(self._h, ctypes.byref(prob), ctypes.c_void_p(stream or None), why, 256), why)
+
+    def prepare_quant(self, dtype: int, rows: int, k: int, x_ptr: int, q_ptr: int, scales_ptr: int, stream: int = 0) -> str:
+        """Prepare the rounding of rows [rows, k] to 8-bit integers with a scale each (gg_prepare_quant)."""
+        prob = GGQuantProblem(int(dtype), int(rows), int(k), x_ptr or None, q_ptr or None, scales_ptr or None)
+        why = ctypes.create_string_buffer(256)
+        return self._prepared(self._lib.gg_prepare_quant(self._h, ctypes.byref(prob), ctypes.c_void_p(stream or None), why, 256), why)
+
+    def prepare_i8(self, dtype: int, experts: int, n: int, k: int, rows: int, x_ptr: int, weight_ptr: int, scales_ptr: int, offsets_ptr: int,
+                   out_ptr: int, x_scales_ptr: int = 0, src_ptr: int = 0, tokens: int = 0, top_k: int = 1, stream: int = 0) -> str:
+        """Prepare the products with 8-bit weights (gg_prepare_i8): out [rows, n] of x [tokens, k] through src, or of x [rows, k] without it,
+        by the router's offsets in device memory. x is in 8 bits with x_scales_ptr, else in dtype and rounded by the run."""
+        prob = GGI8Problem(int(dtype), int(experts), int(top_k), int(n), int(k), int(rows), int(tokens), x_ptr or None, x_scales_ptr or None,
+                           weight_ptr or None, scales_ptr or None, offsets_ptr or None, src_ptr or None, out_ptr or None)
+        why = ctypes.create_string_buffer(256)
+        return self._prepared(self._lib.gg_prepare_i8(self._h, ctypes.byref(prob), ctypes.c_void_p(stream or None), why, 256), why)
 
     def run(self, stream: int = 0) -> None:
         rc = self._lib.gg_run(self._h, ctypes.c_void_p(stream or None))

@@ -35,17 +35,18 @@ COMMON = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-I" + INCLUDE, "-I" + CSRC]
 GEMM_HEADERS = ["gg_kernel.cuh", "gg_ptx.cuh"]
 SOURCES = {
     "gg_capi.cu": GEMM_HEADERS + ["gg_handle.h", "gg_sched.h"],
-    "gg_moe.cu": GEMM_HEADERS + ["gg_handle.h", "gg_moe.cuh", "gg_route.cuh", "gg_permute.cuh", "gg_w4.cuh"],
+    "gg_moe.cu": GEMM_HEADERS + ["gg_handle.h", "gg_moe_host.h", "gg_moe.cuh", "gg_route.cuh", "gg_permute.cuh", "gg_w4.cuh"],
+    "gg_norm_i8.cu": GEMM_HEADERS + ["gg_handle.h", "gg_moe_host.h", "gg_moe.cuh", "gg_norm.cuh", "gg_i8.cuh"],
     "gg_bench_main.cu": [os.path.join("..", "..", "include", "gg_backend.hpp")],
     "gg_cublas_backends.cpp": [os.path.join("..", "..", "include", "gg_backend.hpp")],
 }
 
 TARGETS = {
-    "libgg_b200.so": {"srcs": ["gg_capi.cu", "gg_moe.cu"], "flags": ["-shared"]},
+    "libgg_b200.so": {"srcs": ["gg_capi.cu", "gg_moe.cu", "gg_norm_i8.cu"], "flags": ["-shared"]},
     # the same library with the kernel's bounds checks compiled in (-DGG_DEBUG): a failed check
     # records its site in the device status word and skips the access
-    "libgg_b200_debug.so": {"srcs": ["gg_capi.cu", "gg_moe.cu"], "flags": ["-shared"], "debug": True},
-    "gg_bench": {"srcs": ["gg_bench_main.cu", "gg_cublas_backends.cpp", "gg_capi.cu", "gg_moe.cu"], "flags": ["-lcublas"]},
+    "libgg_b200_debug.so": {"srcs": ["gg_capi.cu", "gg_moe.cu", "gg_norm_i8.cu"], "flags": ["-shared"], "debug": True},
+    "gg_bench": {"srcs": ["gg_bench_main.cu", "gg_cublas_backends.cpp", "gg_capi.cu", "gg_moe.cu", "gg_norm_i8.cu"], "flags": ["-lcublas"]},
 }
 
 
@@ -117,7 +118,8 @@ def resource_usage() -> list[dict]:
         cmd = [NVCC] + COMMON + ["-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v", "-o",
                                                                      os.path.join(d, "libgg_b200.so"),
                                                                      os.path.join(CSRC, "gg_capi.cu"),
-                                                                     os.path.join(CSRC, "gg_moe.cu")]
+                                                                     os.path.join(CSRC, "gg_moe.cu"),
+                                                                     os.path.join(CSRC, "gg_norm_i8.cu")]
         run = subprocess.run(cmd, check=True, capture_output=True, text=True)
     rows, cur = [], None
     for line in (run.stdout + run.stderr).splitlines():

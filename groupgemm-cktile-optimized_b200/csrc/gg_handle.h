@@ -14,21 +14,21 @@
 
 namespace gg {
 
-// One kernel of a prepared layer operator (router, dispatch / combine, 4-bit product): gg_run
-// launches them in order, each with the operator's parameter block as its argument (after the tensor
-// map where it has one).
+// One kernel of a prepared layer operator (router, dispatch / combine, norm, 4- and 8-bit products):
+// gg_run launches them in order, each with the operator's parameter block as its argument (after the
+// tensor maps where it has some). A kernel may take a part of the block that stands first in it.
 struct MoeLaunch {
     const void *fn = nullptr;
     unsigned grid = 0, block = 0;
     size_t smem = 0;
-    bool map = false;  // the kernel takes MoePlan::map first
+    int maps = 0;  // the kernel takes MoePlan::map[0 .. maps) first
     unsigned grid_y = 1, cluster = 1;  // cluster: blocks of one along x
 };
 
 struct MoePlan {
     int launches = 0;  // 0: the handle holds no layer operator
     MoeLaunch launch[3];
-    CUtensorMap map{};
+    CUtensorMap map[2]{};
     alignas(16) unsigned char params[256];
 };
 

@@ -12,6 +12,7 @@
 
 #include "gg_b200.h"
 #include "gg_handle.h"
+#include "gg_moe_host.h"
 #include "gg_permute.cuh"
 #include "gg_route.cuh"
 #include "gg_w4.cuh"
@@ -28,7 +29,6 @@ int run_moe(gg_handle *h, cudaStream_t stream) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.stream = stream;
-    void *args[2] = {&h->moe.map, h->moe.params};
     for (int i = 0; i < h->moe.launches; ++i) {
         const MoeLaunch &l = h->moe.launch[i];
         if (!l.grid)
@@ -39,7 +39,11 @@ int run_moe(gg_handle *h, cudaStream_t stream) {
         attr[0].val.clusterDim.x = l.cluster;
         cfg.attrs = l.cluster > 1 ? attr : attr + 1;
         cfg.numAttrs = (l.cluster > 1 ? 1 : 0) + (h->opt_pdl ? 1 : 0);
-        GG_CUDA(h, cudaLaunchKernelExC(&cfg, l.fn, l.map ? args : args + 1));
+        void *args[3];
+        for (int m = 0; m < l.maps; ++m)
+            args[m] = &h->moe.map[m];
+        args[l.maps] = h->moe.params;
+        GG_CUDA(h, cudaLaunchKernelExC(&cfg, l.fn, args));
     }
     return GG_OK;
 }
@@ -48,131 +52,10 @@ int run_moe(gg_handle *h, cudaStream_t stream) {
 
 namespace {
 
+using namespace gg::host;
 using gg::fail;
 using gg::MoeLaunch;
 using gg::refuse;
-
-constexpr int64_t kMaxIndex = int64_t(1) << 31;  // rows and slots are int32 in device memory
-
-bool aligned16(std::initializer_list<const void *> ptrs) {
-    uintptr_t all = 0;
-    for (const void *p : ptrs)
-        all |= reinterpret_cast<uintptr_t>(p);
-    return (all & 15u) == 0;
-}
-
-bool aligned4(std::initializer_list<const void *> ptrs) {
-    uintptr_t all = 0;
-    for (const void *p : ptrs)
-        all |= reinterpret_cast<uintptr_t>(p);
-    return (all & 3u) == 0;
-}
-
-// What every prepare call of this file begins with.
-int begin(gg_handle *h, const void *p, char *why, size_t why_len) {
-    if (!h)
-        return GG_ERR_ARG;
-    h->ready = false;
-    h->moe.launches = 0;
-    h->last_error.clear();
-    if (why && why_len)
-        why[0] = '\0';
-    if (!p)
-        return fail(h, GG_ERR_ARG, "null problem");
-    return GG_OK;
-}
-
-// The device's checks and the handle's status word, once the arguments are accepted.
-int bind_device(gg_handle *h, gg_stream_t stream, int &num_sms, char *why, size_t why_len) {
-    int dev = 0, major = 0, minor = 0;
-    GG_CUDA(h, cudaGetDevice(&dev));
-    GG_CUDA(h, cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev));
-    GG_CUDA(h, cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
-    GG_CUDA(h, cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev));
-    if (major != 10 || minor != 0)
-        return refuse(h, why, why_len, "needs an sm_100 GPU (B200/GB200)");
-    h->device = dev;
-    if (!h->d_status)
-        GG_CUDA(h, cudaMalloc(&h->d_status, 16));
-    GG_CUDA(h, cudaMemsetAsync(h->d_status, 0, 16, stream));
-    return GG_OK;
-}
-
-int reserve(gg_handle *h, size_t bytes) {
-    if (h->ws_cap >= bytes)
-        return GG_OK;
-    if (h->d_ws)
-        cudaFree(h->d_ws);
-    h->d_ws = nullptr;
-    h->ws_cap = 0;
-    GG_CUDA(h, cudaMalloc(&h->d_ws, bytes));
-    h->ws_cap = bytes;
-    return GG_OK;
-}
-
-int reserve_counters(gg_handle *h, size_t bytes, gg_stream_t stream) {
-    if (h->counters_cap < bytes) {
-        if (h->d_counters)
-            cudaFree(h->d_counters);
-        h->d_counters = nullptr;
-        h->counters_cap = 0;
-        GG_CUDA(h, cudaMalloc(&h->d_counters, bytes));
-        h->counters_cap = bytes;
-    }
-    GG_CUDA(h, cudaMemsetAsync(h->d_counters, 0, bytes, stream));
-    return GG_OK;
-}
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The handle's tensor map over bytes [depth, rows, cols] in boxes of box_cols (64, with that swizzle) x box_rows.
-int encode_bytes_3d(gg_handle *h, const void *base, int64_t cols, int64_t rows, int64_t depth, uint32_t box_cols, uint32_t box_rows) {
-    void *fn = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    GG_CUDA(h, cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found));
-    if (found != cudaDriverEntryPointSuccess || !fn)
-        return fail(h, GG_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
-    const cuuint64_t dim[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(depth)};
-    const cuuint64_t stride[2] = {cuuint64_t(cols), cuuint64_t(cols) * cuuint64_t(rows)};
-    const cuuint32_t box[3] = {box_cols, box_rows, 1}, estride[3] = {1, 1, 1};
-    const CUresult r = reinterpret_cast<EncodeTiledFn>(fn)(
-        &h->moe.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dim, stride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        return fail(h, GG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
-    return GG_OK;
-}
-
-template <class P> void set_params(gg_handle *h, const P &p) {
-    static_assert(sizeof(P) <= sizeof(h->moe.params), "parameter block too large");
-    std::memcpy(h->moe.params, &p, sizeof(P));
-}
-
-int finish(gg_handle *h, gg_stream_t stream, std::initializer_list<MoeLaunch> launches, const char *detail) {
-    int n = 0;
-    for (const MoeLaunch &l : launches)
-        h->moe.launch[n++] = l;
-    GG_CUDA(h, cudaStreamSynchronize(stream));  // as gg_prepare: the handle's own buffers are in place
-    h->detail = detail;
-    h->moe.launches = n;
-    h->ready = true;
-    return GG_OK;
-}
-
-// An entry of the C ABI lets no C++ exception out.
-template <class F> int guarded(gg_handle *h, F &&f) noexcept {
-    try {
-        return f();
-    } catch (...) {
-        if (h)
-            h->ready = false;
-        return GG_ERR_ARG;
-    }
-}
-
-const char *type_name(int t) { return t == GG_F32 ? "fp32" : t == GG_FP16 ? "fp16" : "bf16"; }
 
 // ---- router ----
 
@@ -482,7 +365,8 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     const bool few = q.rows <= gg::moe::kW4FewTokens * int64_t(q.experts);
     const W4Form v = q.dtype == GG_FP16 ? w4_form<__half>(q.group_size, few, q.zeros) : w4_form<__nv_bfloat16>(q.group_size, few, q.zeros);
     GG_CUDA(h, cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(v.smem)));
-    if (const int rc = encode_bytes_3d(h, q.qweight, q.k / 2, q.n, q.experts, gg::moe::kW4StepK / 2, gg::moe::kW4TileRows))
+    if (const int rc = encode_bytes_3d(h, h->moe.map[0], q.qweight, q.k / 2, q.n, q.experts, gg::moe::kW4StepK / 2, gg::moe::kW4TileRows,
+                                       CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
     const int ctas = v.ctas_per_sm * num_sms;
     const int blocks = q.rows > 0 ? ctas : 0;
@@ -546,7 +430,7 @@ int prepare_w4(gg_handle *h, const gg_w4_problem &q, gg_stream_t stream, char *w
     MoeLaunch add{v.add, few ? (splits > 1 ? unsigned(std::min<int64_t>(items, 4 * num_sms)) : 0u) : unsigned(blocks), gg::moe::kW4TileRows, 0};
     if (!few)
         add.grid_y = unsigned(v.tokens) / 8;
-    return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), unsigned(v.threads), v.smem, true}, add}, detail);
+    return finish(h, stream, {gather, MoeLaunch{v.fn, unsigned(blocks), unsigned(v.threads), v.smem, 1}, add}, detail);
 }
 
 }  // namespace

@@ -34,7 +34,7 @@ typedef struct CUstream_st *gg_stream_t; /* == cudaStream_t */
 typedef struct gg_handle gg_handle;
 
 /* Element types (tunemax::DType, common/backend.hpp:27). */
-enum gg_dtype { GG_BF16 = 0, GG_FP16 = 1, GG_F32 = 2 /* router logits only */ };
+enum gg_dtype { GG_BF16 = 0, GG_FP16 = 1, GG_F32 = 2 /* router logits, norm, rounding to 8 bits */ };
 
 /* Return codes. */
 enum gg_status {
@@ -257,6 +257,107 @@ typedef struct gg_w4_problem {
 } gg_w4_problem;
 
 int gg_prepare_w4(gg_handle *h, const gg_w4_problem *p, gg_stream_t stream, char *why, size_t why_len);
+
+/* Layer norm of each token, in front of the layer, with the residual that it is added to:
+ *
+ *   s = x + residual, rounded to dtype (or x)      mean_t = mean of s_t      rstd_t = 1 / sqrt(mean of (s_t - mean_t)^2 + eps)
+ *   y = (s - mean) * rstd * gamma + beta           sum = s
+ *   q, q_scales: y rounded to 8-bit integers as gg_prepare_quant does, in the same pass (for gg_prepare_i8)
+ *
+ * dtype bf16, fp16 or fp32 (x, residual, sum, y); param_type that or GG_F32 (gamma, beta). Statistics are fp32, of the squares
+ * around the mean. sum may be the same array as x or residual, y the same as x where sum is not asked for. hidden a multiple of 8 up to
+ * 16384; x, residual, gamma, beta, sum, y and q 16-byte aligned. */
+typedef struct gg_norm_problem {
+    int32_t dtype;
+    int32_t param_type;      /* of gamma and beta */
+    float eps;               /* >= 0 */
+    int64_t tokens;
+    int64_t hidden;
+    const void *x;           /* [tokens, hidden] */
+    const void *residual;    /* [tokens, hidden] or NULL */
+    const void *gamma;       /* [hidden], or NULL = 1 */
+    const void *beta;        /* [hidden], or NULL = 0 */
+    void *sum;               /* out [tokens, hidden], or NULL; with residual */
+    void *y;                 /* out [tokens, hidden]; NULL where q is enough */
+    float *mean;             /* out [tokens], or NULL */
+    float *rstd;             /* out [tokens], or NULL */
+    int8_t *q;               /* out [tokens, hidden], or NULL */
+    float *q_scales;         /* out [tokens], with q */
+} gg_norm_problem;
+
+int gg_prepare_norm(gg_handle *h, const gg_norm_problem *p, gg_stream_t stream, char *why, size_t why_len);
+
+/* Gradients of the layer norm, from what its run wrote: with c = (x - mean) * rstd and d = dy * gamma,
+ *
+ *   dx = rstd * (d - mean of d - c * mean of d c) + dsum       dgamma = sum over t of dy c       dbeta = sum over t of dy
+ *
+ * x is the norm's input: sum where there was a residual, whose gradient is dx, too. dsum is the gradient that reaches the
+ * sum by its other way (past the layer), or NULL. dgamma and dbeta are fp32, either may be NULL; the same inputs give the same bits. dx may be
+ * the same array as dy or dsum. Limits as gg_prepare_norm's. */
+typedef struct gg_norm_grad_problem {
+    int32_t dtype;
+    int32_t param_type;      /* of gamma */
+    int64_t tokens;
+    int64_t hidden;
+    const void *x;           /* [tokens, hidden] */
+    const float *mean;       /* [tokens] */
+    const float *rstd;       /* [tokens] */
+    const void *gamma;       /* [hidden], or NULL = 1 */
+    const void *dy;          /* [tokens, hidden] */
+    const void *dsum;        /* [tokens, hidden] or NULL */
+    void *dx;                /* out [tokens, hidden] */
+    float *dgamma;           /* out [hidden], or NULL */
+    float *dbeta;            /* out [hidden], or NULL */
+} gg_norm_grad_problem;
+
+int gg_prepare_norm_grad(gg_handle *h, const gg_norm_grad_problem *p, gg_stream_t stream, char *why, size_t why_len);
+
+/* Rows rounded to 8-bit integers with a scale each:
+ *
+ *   scales_r = max_k |x_rk| / 127 (fp32)      q_rk = the whole number nearest to 127 x_rk / max_k |x_rk|, halves to the even one
+ *
+ * of the exact quotient. A row of zeros has scale 0; one that holds NaN or an infinity has scale NaN and q 0, so that what is made of it
+ * is NaN. The weights of gg_prepare_i8 are made so from [experts * n, k]. k a multiple of 8; x and q 16-byte aligned. */
+typedef struct gg_quant_problem {
+    int32_t dtype;           /* bf16, fp16 or fp32 */
+    int64_t rows;
+    int64_t k;
+    const void *x;           /* [rows, k] */
+    int8_t *q;               /* out [rows, k] */
+    float *scales;           /* out [rows] */
+} gg_quant_problem;
+
+int gg_prepare_quant(gg_handle *h, const gg_quant_problem *p, gg_stream_t stream, char *why, size_t why_len);
+
+/* Products with 8-bit weights, for any number of rows an expert (decoding and prompts):
+ *
+ *   out[r, n] = x_scales[row(r)] * scales[e, n] * sum_k x[row(r), k] weight[e, n, k]
+ *
+ * for the rows r of expert e, offsets[e] <= r < offsets[e + 1]; row(r), offsets, src and the rows of no expert as in gg_prepare_w4. x is
+ * [.., k] in 8 bits with x_scales, or, where x_scales is NULL, in dtype: then the run rounds its rows first as gg_prepare_quant does (into
+ * the handle's memory). The sum is exact in 32 bits; its value is rounded to fp32 and multiplied by the scales there, and the result rounded
+ * once to dtype. A row whose src is no slot is zero (or NaN, with a scale that is not finite) and reported. A scale that is not finite makes
+ * NaN or infinities of its row or column alone.
+ *
+ * dtype bf16 or fp16; experts 1..1024, n a multiple of 8, k a multiple of 16 up to 131056; x, weight and out 16-byte aligned. */
+typedef struct gg_i8_problem {
+    int32_t dtype;           /* of out, and of x without x_scales */
+    int32_t experts;
+    int32_t top_k;           /* with src */
+    int64_t n;
+    int64_t k;
+    int64_t rows;            /* rows of out */
+    int64_t tokens;          /* rows of x, with src */
+    const void *x;           /* [tokens, k] with src, else [rows, k] */
+    const float *x_scales;   /* [tokens or rows], or NULL: x is in dtype */
+    const int8_t *weight;    /* [experts, n, k] */
+    const float *scales;     /* [experts, n] */
+    const int32_t *offsets;  /* [experts + 1] */
+    const int32_t *src;      /* [rows] or NULL */
+    void *out;               /* [rows, n] */
+} gg_i8_problem;
+
+int gg_prepare_i8(gg_handle *h, const gg_i8_problem *p, gg_stream_t stream, char *why, size_t why_len);
 
 /* Backend::run() (common/backend.hpp:67; ck_kernel/ck_grouped_gemm.cpp:140, :114-121). Timed:
  * enqueues one grouped GEMM on `stream` and does not synchronise: one kernel launch, or two for

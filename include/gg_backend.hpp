@@ -110,7 +110,7 @@ public:
         return answer(gg_prepare_grad(h_, &q, op, stream, why, sizeof(why)), why);
     }
 
-    // The operators around the products (gg_prepare_route, _route_grad, _permute, _w4), likewise.
+    // The operators around the products (gg_prepare_route, _route_grad, _permute, _w4, _norm, _norm_grad, _quant, _i8), likewise.
     std::string prepare_route(const gg_route_problem &q, cudaStream_t stream) {
         char why[256];
         return answer(gg_prepare_route(h_, &q, stream, why, sizeof(why)), why);
@@ -126,6 +126,22 @@ public:
     std::string prepare_w4(const gg_w4_problem &q, cudaStream_t stream) {
         char why[256];
         return answer(gg_prepare_w4(h_, &q, stream, why, sizeof(why)), why);
+    }
+    std::string prepare_norm(const gg_norm_problem &q, cudaStream_t stream) {
+        char why[256];
+        return answer(gg_prepare_norm(h_, &q, stream, why, sizeof(why)), why);
+    }
+    std::string prepare_norm_grad(const gg_norm_grad_problem &q, cudaStream_t stream) {
+        char why[256];
+        return answer(gg_prepare_norm_grad(h_, &q, stream, why, sizeof(why)), why);
+    }
+    std::string prepare_quant(const gg_quant_problem &q, cudaStream_t stream) {
+        char why[256];
+        return answer(gg_prepare_quant(h_, &q, stream, why, sizeof(why)), why);
+    }
+    std::string prepare_i8(const gg_i8_problem &q, cudaStream_t stream) {
+        char why[256];
+        return answer(gg_prepare_i8(h_, &q, stream, why, sizeof(why)), why);
     }
 
     void run(cudaStream_t stream) override {
