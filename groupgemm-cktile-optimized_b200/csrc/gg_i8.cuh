@@ -5,12 +5,14 @@
 //
 // tcgen05.mma kind::i8 on CTA pairs, the weights as A (256 rows a pair) and a chunk of tokens as B, as wide as the chunk has tokens
 // (32 to 256 in steps of 32): few rows an expert cost the bytes of its weights and next to no products, many rows run at the full
-// tile, and nothing is padded to a tile of tokens. Tokens are fetched through src by TMA gathers of four rows, so no copy in expert order is made.
+// tile, and nothing is padded to a tile of tokens.
 //
-//   Work split: items (expert, token chunk, 256 weight rows). Each pair takes whole items in turn; the items that would leave pairs
-//   idle at the end (or all, where there are few) are cut along k into equal ranges of steps, one a pair, taken first. What is cut
+//   i8_rows: the rows of x in expert order, rounded to 8 bits where they come in 16. (TMA gathers of four rows in the product kernel
+//   would spare it, but take 44 cycles each: a stage of 128 rows a CTA 1400 cycles, of which the products need 512.)
+//   i8_products. Work split: items (expert, token chunk, 256 weight rows). Each pair takes whole items in turn; the items that would leave
+//   pairs idle at the end (or all, where there are few) are cut along k into equal ranges of steps, one a pair, taken first. What is cut
 //   leaves its sums in the workspace, and the last warp to arrive adds them up (no order to keep).
-//   Warps: 0 loads (weights and tokens, a ring of stages), 1 issues the products (of the pair's first CTA), 2-5 take the sums out of
+//   Warps: 0 loads (weights and tokens, a ring of stages), 1 issues the products (of the pair's first CTA), 2-9 take the sums out of
 //   Tensor Memory, two accumulators in turn.
 #pragma once
 
@@ -28,37 +30,38 @@ constexpr int kI8MaxK = 131056;     // k * 128 * 128 stays below 2^31
 constexpr int kI8WeightBytes = 128 * kI8StepK;  // of a CTA and stage
 constexpr int kI8MaxStages = 12;
 constexpr int kI8Ring = 192 * 1024;
-constexpr int kI8Threads = 192;
+constexpr int kI8EpilogueWarps = 8;
+constexpr int kI8Threads = (2 + kI8EpilogueWarps) * 32;
 constexpr int kI8Smem = kI8Ring + 1024;
+#ifndef I8BOX
+#define I8BOX 32
+#define I8MIN 8
+#endif
+constexpr int kI8Box = I8BOX;         // rows of a token load at most
+constexpr int kI8MinSteps = I8MIN;     // of a cut piece
 constexpr int kI8Band = 8;          // tiles whose weights are visited together (see item)
-constexpr int kI8MinSteps = 4;      // of a cut piece
 
 struct I8Params {
-    QuantParams quant;        // first: the parameters of quant_rows, where the rows come in 16 bits
-    const float *x_scales;    // [tokens or rows]
+    const void *x;            // [tokens or rows, k], as the caller has them (i8_rows)
+    const float *x_scales;    // [tokens or rows], or null: x is in 16 bits (i8_rows)
+    int8_t *xq;               // [rows, k] in expert order
+    float *xq_scales;         // [rows]
     const float *scales;      // [experts, n]
     const int32_t *offsets;   // [experts + 1]
     const int32_t *src;       // [rows] slots, or null: row r is x[r]
     void *out;                // [rows, n]
     uint32_t *status;         // [0] status word, [2] timeouts of this launch
-    int32_t *ws;              // [2 x pairs][2 CTAs][4 warps][chunk / 32][8][32] int4
-    int32_t *counters;        // [pairs][2][4], 0 between launches
+    int32_t *ws;              // [2 x pairs][2 CTAs][4 quarters][chunk / 32][8][32] int4
+    int32_t *counters;        // [pairs][2 CTAs][8 warps], 0 between launches
     int64_t rows, slots;      // slots: tokens * top_k
     uint64_t timeout_ns;
     int n, k, experts, top_k, tiles, steps;
     int chunk;                // most tokens of a chunk, a multiple of 32
+    int box;                  // rows of a token load
     int stages, stage_bytes;
-    int after_quant;          // 1: quant_rows precedes, and everything before it is done when this kernel starts
+    int min_steps;            // of a cut piece
+    int after_rows;           // 1: i8_rows precedes, and everything before it is done when this kernel starts
 };
-
-// Four rows of a 2-D map into one 512-byte piece; the completion barrier may be the pair leader's.
-__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const void *tmap, uint32_t bar, int32_t c, int4 rows, uint32_t pred) {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %8, 0;\n\t"
-                 "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2"
-                 " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n\t}" ::"r"(dst),
-                 "l"(tmap), "r"(bar), "r"(c), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(pred)
-                 : "memory");
-}
 
 // Instruction descriptor of kind::i8: D s32 (2 at bit 4), A and B signed (1 at bits 7 and 10), both K-major, N >> 3, M >> 4.
 __host__ __device__ constexpr uint32_t i8_idesc(int m, int n) {
@@ -78,11 +81,12 @@ struct I8Plan {
     int cut, ranges, pairs, steps;
     int64_t begin, end;  // this pair's range
     int c;
-    __host__ __device__ __forceinline__ I8Plan(int64_t items_, int steps_, int pairs_, int c_) : items(items_), pairs(pairs_), steps(steps_), c(c_) {
+    __host__ __device__ __forceinline__ I8Plan(int64_t items_, int steps_, int min_steps, int pairs_, int c_)
+        : items(items_), pairs(pairs_), steps(steps_), c(c_) {
         const int64_t over = items % pairs;
         cut = over == 0 ? 0 : int(items < pairs ? items : pairs + over);
-        const int64_t total = int64_t(cut) * steps, most = total / kI8MinSteps;
-        ranges = int(most < 1 ? 1 : most < pairs ? most : pairs);
+        const int64_t total = int64_t(cut) * steps, pieces = total / min_steps > cut ? total / min_steps : cut;
+        ranges = int(pieces < 1 ? 1 : pieces < pairs ? pieces : pairs);
         begin = c < ranges ? total * c / ranges : 0;
         end = c < ranges ? total * (c + 1) / ranges : 0;
     }
@@ -171,16 +175,43 @@ struct I8Work {
     }
 };
 
-// The row of x behind place r of the expert order, or -1 (and a report) where src holds no slot.
-__device__ __forceinline__ int i8_row(const I8Params &p, int r, bool tell) {
-    if (!p.src)
-        return r;
-    const int s = __ldg(p.src + r);
-    if (s >= 0 && s < p.slots)
-        return s / p.top_k;
-    if (tell)
-        report(p.status, kSiteSrc);
-    return -1;
+// The rows in expert order: place r gets x[row(r)], rounded to 8 bits where x has 16, and its scale. A block a row (and every gridDim.x-th
+// after it). A src that is no slot gives scale 0, so that its row becomes zero.
+template <class T> __global__ void __launch_bounds__(512) i8_rows(const __grid_constant__ I8Params p) {
+    __shared__ uint32_t part[2][16];
+    ptx::griddep_wait();
+    // The product kernel may start now: what precedes this one is done (its blocks have waited), and before it reads xq it waits for this one.
+    ptx::griddep_launch_dependents();
+    const int64_t low = max(0, p.offsets[0]), high = min(p.rows, int64_t(p.offsets[p.experts]));
+    if (threadIdx.x == 0 && (p.offsets[0] < 0 || p.offsets[p.experts] > p.rows))
+        report(p.status, kSiteOffsets);  // before the src that such offsets reach
+    int turn = 0;
+    for (int64_t r = low + blockIdx.x; r < high; r += gridDim.x) {
+        int64_t row = r;
+        if (p.src) {
+            const int s = p.src[r];
+            row = s < 0 || s >= p.slots ? -1 : s / p.top_k;
+        }
+        if (row < 0) {
+            if (threadIdx.x == 0) {
+                report(p.status, kSiteSrc);
+                p.xq_scales[r] = 0.0f;
+            }
+            continue;
+        }
+        if (p.x_scales) {
+            const uint4 *from = reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(p.x) + row * p.k);
+            uint4 *to = reinterpret_cast<uint4 *>(p.xq + r * p.k);
+#pragma unroll 4
+            for (int i = threadIdx.x; i < p.k / 16; i += blockDim.x)
+                to[i] = __ldg(from + i);
+            if (threadIdx.x == 0)
+                p.xq_scales[r] = __ldg(p.x_scales + row);
+        } else {
+            quant_row<T>(static_cast<const uint8_t *>(p.x) + row * p.k * int64_t(sizeof(T)), p.xq + r * p.k, p.xq_scales + r, p.k / 8, part[turn]);
+            turn ^= 1;
+        }
+    }
 }
 
 template <class T>
@@ -189,7 +220,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     extern __shared__ __align__(1024) uint8_t i8_smem[];
     __shared__ int start[kI8MaxExperts + 1], first[kI8MaxExperts + 1];
     __shared__ uint64_t bar_mem[2 * kI8MaxStages + 4];
-    __shared__ float row_scale[4][kI8MaxTokens];
+    __shared__ __align__(16) float row_scale[kI8EpilogueWarps][kI8MaxTokens / 2];
     __shared__ uint32_t slots[2];
     const uint32_t ring = (ptx::smem_addr(i8_smem) + 1023u) & ~1023u;
     const uint32_t bars = ptx::smem_addr(bar_mem);
@@ -208,7 +239,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         }
         for (int a = 0; a < 2; ++a) {
             ptx::mbar_init(tfull(a), 1);
-            ptx::mbar_init(tempty(a), 8);  // the epilogue warps of both CTAs
+            ptx::mbar_init(tempty(a), 2 * kI8EpilogueWarps);  // the epilogue warps of both CTAs
         }
         *abort_flag = 0u;
         ptx::fence_mbar_init();
@@ -220,7 +251,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         ptx::tmem_alloc<2>(ptx::smem_addr(slots), 512);
         ptx::tmem_relinquish<2>();
     }
-    if (!p.after_quant)
+    if (!p.after_rows)
         ptx::griddep_wait();
     ptx::fence_proxy_async_global();
     ptx::griddep_launch_dependents();
@@ -231,40 +262,36 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     ptx::tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(slots);
     const Abort ab{p.status + 2, abort_flag, p.timeout_ns};
-    const I8Plan plan(work.items, p.steps, pairs, pair);
+    const I8Plan plan(work.items, p.steps, p.min_steps, pairs, pair);
 
     if (warp == 0) {
         const uint32_t issue = ptx::elect_one_sync();
         const uint32_t full_leader = ptx::mapa(full(0), 0);
         int s = 0;
         uint32_t ph = 0;
-        bool ok = true, waited = !p.after_quant;
+        bool ok = true, waited = !p.after_rows;
         plan.pieces([&](int64_t item, int k0, int n, int, int) {
             const I8Item it = work.at(p, item);
-            const int half = it.width / 2;  // tokens of this CTA
-            // lane l gathers tokens 4 l to 4 l + 3 of them; a missing one is read as row 0, its sums go nowhere
-            int row[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = int(rank) * half + 4 * lane + i;
-                row[i] = 4 * lane < half && j < it.count ? max(0, i8_row(p, it.r0 + j, it.n0 == 0 && k0 == 0)) : 0;
-            }
-            const int4 rows = make_int4(row[0], row[1], row[2], row[3]);
-            const uint32_t gathers = 4 * lane < half ? 1u : 0u;
+            // loads of this CTA's half of the tokens, and of both; what of a half no load covers goes into sums that nothing reads
+            const int half = it.width / 2, box_bytes = p.box * kI8StepK;
+            auto boxes = [&](int r) { return (min(half, max(0, it.count - r * half)) + p.box - 1) / p.box; };
+            const int mine = boxes(int(rank)), row = it.r0 + int(rank) * half;
+            const uint32_t bytes = 2u * kI8WeightBytes + uint32_t((boxes(0) + boxes(1)) * box_bytes);
             for (int j = 0; ok && j < n; ++j) {
                 ok = wait_all(empty(s), ph ^ 1u, ab, kStatusTimeout | kRoleProducer | uint32_t(s));
                 if (!ok)
                     break;
                 const uint32_t a = ring + uint32_t(s * p.stage_bytes);
                 const int c = (k0 + j) * kI8StepK;
-                ptx::mbar_arrive_expect_tx(full(s), 2u * (kI8WeightBytes + uint32_t(half) * kI8StepK), rank == 0 ? issue : 0u);
+                ptx::mbar_arrive_expect_tx(full(s), bytes, rank == 0 ? issue : 0u);
                 ptx::tma_load_3d_pair(a, &tmap_w, full_leader + 8u * s, c, it.n0 + int(rank) * 128, it.e, issue);
-                if (!waited) {  // quant_rows' output is read from here on
+                if (!waited) {  // i8_rows' output is read from here on
                     ptx::griddep_wait();
                     ptx::fence_proxy_async_global();
                     waited = true;
                 }
-                tma_gather4_pair(a + kI8WeightBytes + uint32_t(lane) * 512u, &tmap_x, full_leader + 8u * s, c, rows, gathers);
+                for (int i = 0; i < mine; ++i)
+                    ptx::tma_load_2d_pair(a + kI8WeightBytes + uint32_t(i * box_bytes), &tmap_x, full_leader + 8u * s, c, row + i * p.box, issue);
                 if (++s == p.stages) {
                     s = 0;
                     ph ^= 1u;
@@ -280,7 +307,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             }
         }
         if (!waited)
-            ptx::griddep_wait();  // this launch ends after quant_rows even where it has no work
+            ptx::griddep_wait();  // this launch ends after i8_rows even where it has no work
     } else if (warp == 1) {
         if (rank == 0) {
             const uint32_t issue = ptx::elect_one_sync();
@@ -331,28 +358,39 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         {
             const int64_t low = work.falls ? 0 : start[0], high = work.falls ? 0 : start[p.experts];
             const int64_t pieces = p.n / 8, total = (low + p.rows - high) * pieces;
-            for (int64_t i = int64_t(blockIdx.x) * 128 + (threadIdx.x - 64); i < total; i += int64_t(gridDim.x) * 128) {
+            for (int64_t i = int64_t(blockIdx.x) * (32 * kI8EpilogueWarps) + (threadIdx.x - 64); i < total; i += int64_t(gridDim.x) * (32 * kI8EpilogueWarps)) {
                 const int64_t r = i / pieces, row = r < low ? r : r - low + high;
                 reinterpret_cast<uint4 *>(out + row * p.n)[i - r * pieces] = make_uint4(0, 0, 0, 0);
             }
         }
+        const int group = (warp - 2) >> 2;  // blocks of 32 tokens that this warp takes: group, group + 2, ...
+        float *my_scales = row_scale[warp - 2];
         uint32_t turn = 0;
         bool ok = true;
         plan.pieces([&](int64_t item, int, int, int first_pair, int pieces) {
             if (!ok)
                 return;
             const I8Item it = work.at(p, item);
-            const int col = it.n0 + int(rank) * 128 + quarter * 32 + lane;
-            if (p.after_quant && turn == 0)
-                ptx::griddep_wait();  // x_scales are quant_rows' output
-            // scales of the chunk's rows, each warp its own copy
-            __syncwarp();
-            for (int j = lane; j < it.width; j += 32) {
-                const int row = j < it.count ? i8_row(p, it.r0 + j, false) : -1;
-                row_scale[quarter][j] = row < 0 ? 0.0f : __ldg(p.x_scales + row);
-            }
+            const int col = it.n0 + int(rank) * 128 + quarter * 32 + lane, blocks = it.width / 32;
+            if (p.after_rows && turn == 0)
+                ptx::griddep_wait();  // xq_scales are i8_rows' output
+            // scales of the rows of this warp's blocks, and of this lane's weight row; whether all are far from the ends of fp32's range
             const float scale = col < p.n ? __ldg(p.scales + int64_t(it.e) * p.n + col) : 0.0f;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = 32 * (group + 2 * i) + lane;
+                x[i] = j < it.count ? __ldg(p.xq_scales + it.r0 + j) : 0.0f;
+            }
+            auto ordinary = [](float v) { return v == 0.0f || (fabsf(v) > 9.0949470e-13f && fabsf(v) < 1.0995116e12f); };  // 2^-40, 2^40
+            bool plain = ordinary(scale);
             __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                plain = plain && ordinary(x[i]);
+                my_scales[32 * i + lane] = x[i];
+            }
+            plain = __all_sync(0xffffffffu, plain) != 0;
             const int acc = int(turn & 1u);
             ok = wait_warp(tfull(acc), (turn >> 1) & 1u, ab, kStatusTimeout | kRoleEpilogue | uint32_t(acc));
             if (!ok)
@@ -360,18 +398,17 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             ++turn;
             ptx::tc_fence_after();
             const uint32_t from = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(acc * kI8MaxTokens);
-            const int blocks = it.width / 32;
             const int64_t most = p.chunk / 32;
-            // this warp's part of pair c's piece: slot 0 where the piece begins inside its item, 1 where it begins it
+            // this quarter's part of pair c's piece: slot 0 where the piece begins inside its item, 1 where it begins it
             auto slot = [&](int c) {
                 return reinterpret_cast<int4 *>(p.ws) + (((int64_t(2 * c + (c == first_pair ? 1 : 0)) * 2 + rank) * 4 + quarter) * most) * 256 + lane;
             };
             bool store = true;
-            if (pieces > 1) {
-                int32_t *counter = p.counters + (first_pair * 2 + int(rank)) * 4 + quarter;
+            if (pieces > 1 && group < blocks) {
+                int32_t *counter = p.counters + (first_pair * 2 + int(rank)) * kI8EpilogueWarps + warp - 2;
                 int4 *mine = slot(pair);
 #pragma unroll 1
-                for (int b = 0; b < blocks; ++b) {
+                for (int b = group; b < blocks; b += 2) {
                     uint32_t r[32];
                     ptx::tmem_ld_32x32b_x32(from + uint32_t(b * 32), r);
                     ptx::tmem_wait_ld(r);
@@ -393,34 +430,46 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             }
             if (store) {
 #pragma unroll 1
-                for (int b = 0; b < blocks; ++b) {
+                for (int b = group; b < blocks; b += 2) {
                     uint32_t r[32];
                     ptx::tmem_ld_32x32b_x32(from + uint32_t(b * 32), r);
                     ptx::tmem_wait_ld(r);
-                    for (int c = first_pair; c < first_pair + pieces; ++c)
-                        if (c != pair) {
-                            const int4 *theirs = slot(c) + b * 256;
+                    if (pieces > 1)
+                        for (int c = first_pair; c < first_pair + pieces; ++c)
+                            if (c != pair) {
+                                const int4 *theirs = slot(c) + b * 256;
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int4 v = __ldcg(theirs + j * 32);
-                                r[4 * j] += uint32_t(v.x);
-                                r[4 * j + 1] += uint32_t(v.y);
-                                r[4 * j + 2] += uint32_t(v.z);
-                                r[4 * j + 3] += uint32_t(v.w);
+                                for (int j = 0; j < 8; ++j) {
+                                    const int4 v = __ldcg(theirs + j * 32);
+                                    r[4 * j] += uint32_t(v.x);
+                                    r[4 * j + 1] += uint32_t(v.y);
+                                    r[4 * j + 2] += uint32_t(v.z);
+                                    r[4 * j + 3] += uint32_t(v.w);
+                                }
                             }
+                    // Two tokens of a lane become two weight rows of one token by an exchange with the lane beside it: even lanes
+                    // store token j, odd ones j + 1, four bytes each.
+                    const int rows = col < p.n ? it.count - b * 32 - (lane & 1) : 0;
+                    T *to = out + int64_t(it.r0 + b * 32 + (lane & 1)) * p.n + (col & ~1);
+                    const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
+                    const float4 *scales = reinterpret_cast<const float4 *>(my_scales + 16 * (b - group));
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 x4 = scales[j / 4];
+                        const float xs[4] = {x4.x, x4.y, x4.z, x4.w};
+                        float v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            // the smaller scale first: no product on the way leaves fp32's range unless the result does
+                            const bool less = !plain && !(fabsf(xs[i]) < fabsf(scale));
+                            v[i] = float(int(r[j + i])) * (less ? scale : xs[i]) * (less ? xs[i] : scale);
                         }
-                    if (col < p.n) {
-                        T *to = out + int64_t(it.r0 + b * 32) * p.n + col;
-                        const int rows = it.count - b * 32;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (j < rows) {
-                                // the smaller scale first: no product on the way leaves fp32's range unless the result does
-                                const float x = row_scale[quarter][b * 32 + j];
-                                const bool less = fabsf(x) < fabsf(scale);
-                                const float v = float(int(r[j])) * (less ? x : scale) * (less ? scale : x);
-                                to[int64_t(j) * p.n] = from_f32<T>(v);
-                            }
+                        for (int i = 0; i < 4; i += 2) {
+                            const uint32_t own = moe::pack2<T>(v[i], v[i + 1]), other = __shfl_xor_sync(0xffffffffu, own, 1);
+                            if (j + i < rows)
+                                __stcs(reinterpret_cast<uint32_t *>(to + int64_t(j + i) * p.n), __byte_perm(own, other, pick));
+                        }
                     }
                 }
             }

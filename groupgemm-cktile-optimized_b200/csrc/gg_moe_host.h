@@ -113,11 +113,11 @@ inline int encode_bytes_3d(gg_handle *h, CUtensorMap &map, const void *base, int
     const cuuint32_t box[3] = {box_cols, box_rows, 1};
     return encode_bytes(h, map, base, 3, dim, stride, box, swizzle);
 }
-// Over [rows, cols], for gathers of four rows: boxes one row high.
-inline int encode_bytes_rows(gg_handle *h, CUtensorMap &map, const void *base, int64_t cols, int64_t rows, uint32_t box_cols,
-                             CUtensorMapSwizzle swizzle) {
+// Over [rows, cols].
+inline int encode_bytes_2d(gg_handle *h, CUtensorMap &map, const void *base, int64_t cols, int64_t rows, uint32_t box_cols, uint32_t box_rows,
+                           CUtensorMapSwizzle swizzle) {
     const cuuint64_t dim[2] = {cuuint64_t(cols), cuuint64_t(rows)}, stride[1] = {cuuint64_t(cols)};
-    const cuuint32_t box[2] = {box_cols, 1};
+    const cuuint32_t box[2] = {box_cols, box_rows};
     return encode_bytes(h, map, base, 2, dim, stride, box, swizzle);
 }
 

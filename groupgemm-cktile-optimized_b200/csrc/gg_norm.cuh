@@ -154,67 +154,69 @@ struct QuantParams {
     int vecs;         // k / 8
 };
 
-// A block a row (and every gridDim.x-th after it): up to kQuantHeld vectors a thread stay in registers between the
-// largest magnitude and the rounding, what is longer is read again.
+// One row by a block: up to kQuantHeld vectors a thread stay in registers between the largest magnitude and the rounding, what is
+// longer is read again. part: 16 words of shared memory, other ones for the next row.
 constexpr int kQuantHeld = 4;
+template <class T> __device__ __forceinline__ void quant_row(const void *row, int8_t *to, float *scale_to, int vecs, uint32_t *part) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+    Vec8<T> v[kQuantHeld];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kQuantHeld; ++i) {
+        const int at = tid + i * int(blockDim.x);
+        if (at < vecs)
+            v[i].ldg(row, at);
+    }
+#pragma unroll
+    for (int i = 0; i < kQuantHeld; ++i)
+        if (tid + i * int(blockDim.x) < vecs) {
+            float f[8];
+            v[i].get(f);
+            top = top_of(top, f);
+        }
+    for (int at = tid + kQuantHeld * int(blockDim.x); at < vecs; at += blockDim.x) {
+        Vec8<T> u;
+        float f[8];
+        u.ldg(row, at);
+        u.get(f);
+        top = top_of(top, f);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0)
+        part[warp] = top;
+    __syncthreads();  // a warp writes these words again only after the next row's barrier
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? part[lane] : 0u);
+    float scale;
+    const Rounding by(top, scale);
+    if (tid == 0)
+        *scale_to = scale;
+    uint2 *q = reinterpret_cast<uint2 *>(to);
+#pragma unroll
+    for (int i = 0; i < kQuantHeld; ++i) {
+        const int at = tid + i * int(blockDim.x);
+        if (at < vecs) {
+            float f[8];
+            v[i].get(f);
+            q[at] = round8(by, f);
+        }
+    }
+    for (int at = tid + kQuantHeld * int(blockDim.x); at < vecs; at += blockDim.x) {
+        Vec8<T> u;
+        float f[8];
+        u.ldg(row, at);
+        u.get(f);
+        q[at] = round8(by, f);
+    }
+}
+
+// A block a row (and every gridDim.x-th after it).
 template <class T> __global__ void __launch_bounds__(512) quant_rows(const __grid_constant__ QuantParams p) {
     __shared__ uint32_t part[2][16];
     ptx::griddep_wait();
-    // A kernel that follows may start: one that reads q waits for this one, and what precedes this one is done (its blocks have waited).
     ptx::griddep_launch_dependents();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
     int turn = 0;
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
-        const uint8_t *row = static_cast<const uint8_t *>(p.x) + r * p.vecs * int64_t(8 * sizeof(T));
-        Vec8<T> v[kQuantHeld];
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < kQuantHeld; ++i) {
-            const int at = tid + i * int(blockDim.x);
-            if (at < p.vecs)
-                v[i].ldg(row, at);
-        }
-#pragma unroll
-        for (int i = 0; i < kQuantHeld; ++i)
-            if (tid + i * int(blockDim.x) < p.vecs) {
-                float f[8];
-                v[i].get(f);
-                top = top_of(top, f);
-            }
-        for (int at = tid + kQuantHeld * int(blockDim.x); at < p.vecs; at += blockDim.x) {
-            Vec8<T> u;
-            float f[8];
-            u.ldg(row, at);
-            u.get(f);
-            top = top_of(top, f);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0)
-            part[turn][warp] = top;
-        __syncthreads();  // a warp writes this half again only after the next row's barrier
-        top = __reduce_max_sync(0xffffffffu, lane < warps ? part[turn][lane] : 0u);
-        float scale;
-        const Rounding to(top, scale);
-        if (tid == 0)
-            p.scales[r] = scale;
-        uint2 *q = reinterpret_cast<uint2 *>(p.q) + r * p.vecs;
-#pragma unroll
-        for (int i = 0; i < kQuantHeld; ++i) {
-            const int at = tid + i * int(blockDim.x);
-            if (at < p.vecs) {
-                float f[8];
-                v[i].get(f);
-                q[at] = round8(to, f);
-            }
-        }
-        for (int at = tid + kQuantHeld * int(blockDim.x); at < p.vecs; at += blockDim.x) {
-            Vec8<T> u;
-            float f[8];
-            u.ldg(row, at);
-            u.get(f);
-            q[at] = round8(to, f);
-        }
-    }
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1)
+        quant_row<T>(static_cast<const uint8_t *>(p.x) + r * p.vecs * int64_t(8 * sizeof(T)), p.q + r * p.vecs * 8, p.scales + r, p.vecs, part[turn]);
 }
 
 // ---- rows through a ring in shared memory ----

@@ -170,10 +170,10 @@ const void *quant_fn(int dtype) {
                               : reinterpret_cast<const void *>(&gg::moe::quant_rows<__nv_bfloat16>);
 }
 
-MoeLaunch quant_launch(int dtype, int64_t rows, int64_t k, int num_sms) {
+// Threads of a block that rounds rows of k.
+unsigned quant_threads(int64_t rows, int64_t k, int num_sms) {
     const int64_t vecs = k / 8, each = rows > 4 * num_sms ? gg::moe::kQuantHeld : 1;
-    const int64_t threads = std::min<int64_t>(512, ((vecs + each - 1) / each + 31) / 32 * 32);
-    return MoeLaunch{quant_fn(dtype), unsigned(std::min<int64_t>(rows, 32 * num_sms)), unsigned(threads), 0};
+    return unsigned(std::min<int64_t>(512, ((vecs + each - 1) / each + 31) / 32 * 32));
 }
 
 int prepare_quant(gg_handle *h, const gg_quant_problem &q, gg_stream_t stream, char *why, size_t why_len) {
@@ -194,7 +194,8 @@ int prepare_quant(gg_handle *h, const gg_quant_problem &q, gg_stream_t stream, c
     set_params(h, p);
     char detail[160];
     std::snprintf(detail, sizeof(detail), "gg_quant<%s> k=%lld", type_name(q.dtype), static_cast<long long>(q.k));
-    return finish(h, stream, {quant_launch(q.dtype, q.rows, q.k, num_sms)}, detail);
+    const MoeLaunch rows{quant_fn(q.dtype), unsigned(std::min<int64_t>(q.rows, 32 * num_sms)), quant_threads(q.rows, q.k, num_sms), 0};
+    return finish(h, stream, {rows}, detail);
 }
 
 // ---- 8-bit products ----
@@ -221,8 +222,7 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
         return refuse(h, why, why_len, "x, weight and out must be 16-byte aligned, x_scales, scales, offsets and src 4-byte aligned");
     if (q.n * q.k >= int64_t(1) << 39)
         return refuse(h, why, why_len, "one expert's weights are too large for a TMA descriptor");
-    const int64_t x_rows = q.src ? q.tokens : q.rows;
-    const int64_t tiles = (q.n + kI8TileRows - 1) / kI8TileRows;
+    const int64_t tiles = (q.n + kI8TileRows - 1) / kI8TileRows, steps = (q.k + kI8StepK - 1) / kI8StepK;
     // Tokens of a chunk at most: a stage has place for half of them beside its 16 KB of weights.
     int chunk = kI8MaxTokens;
     while (chunk > 32 && q.rows <= chunk / 2)
@@ -233,23 +233,17 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
     const int pairs = num_sms / 2;
-    const size_t sums = 2 * size_t(pairs) * size_t(chunk) * 1024;
-    const size_t xq = q.x_scales ? 0 : size_t(x_rows) * size_t(q.k);
-    if (const int rc = reserve(h, sums + xq + (q.x_scales ? 0 : size_t(x_rows) * 4)))
+    const bool order = q.rows > 0 && (q.src || !q.x_scales);  // rows are put into expert order or rounded first
+    const size_t sums = 2 * size_t(pairs) * size_t(chunk) * 1024, rounded = order ? size_t(q.rows) * size_t(q.k) : 0;
+    if (const int rc = reserve(h, sums + rounded + (order ? size_t(q.rows) * 4 : 0)))
         return rc;
-    if (const int rc = reserve_counters(h, size_t(pairs) * 8 * 4, stream))
+    if (const int rc = reserve_counters(h, size_t(pairs) * 2 * kI8EpilogueWarps * 4, stream))
         return rc;
-    int8_t *rounded = reinterpret_cast<int8_t *>(h->d_ws) + sums;
-    float *rounded_scales = reinterpret_cast<float *>(rounded + xq);
-    if (q.rows > 0) {
-        if (const int rc = encode_bytes_3d(h, h->moe.map[0], q.weight, q.k, q.n, q.experts, kI8StepK, kI8TileRows / 2, CU_TENSOR_MAP_SWIZZLE_128B))
-            return rc;
-        if (const int rc = encode_bytes_rows(h, h->moe.map[1], q.x_scales ? q.x : rounded, q.k, x_rows, kI8StepK, CU_TENSOR_MAP_SWIZZLE_128B))
-            return rc;
-    }
     I8Params p{};
-    p.quant = QuantParams{q.x, rounded, rounded_scales, x_rows, int(q.k / 8)};
-    p.x_scales = q.x_scales ? q.x_scales : rounded_scales;
+    p.x = q.x;
+    p.x_scales = q.x_scales;
+    p.xq = order ? reinterpret_cast<int8_t *>(h->d_ws) + sums : static_cast<int8_t *>(const_cast<void *>(q.x));
+    p.xq_scales = order ? reinterpret_cast<float *>(p.xq + rounded) : const_cast<float *>(q.x_scales);
     p.scales = q.scales;
     p.offsets = q.offsets;
     p.src = q.src;
@@ -265,24 +259,31 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     p.experts = q.experts;
     p.top_k = q.src ? q.top_k : 1;
     p.tiles = int(tiles);
-    p.steps = int((q.k + kI8StepK - 1) / kI8StepK);
+    p.steps = int(steps);
     p.chunk = chunk;
+    p.box = std::min(kI8Box, chunk / 2);
     p.stage_bytes = kI8WeightBytes + chunk / 2 * kI8StepK;
     p.stages = std::min(kI8MaxStages, kI8Ring / p.stage_bytes);
-    p.after_quant = q.x_scales || q.rows == 0 ? 0 : 1;
+    p.min_steps = kI8MinSteps;
+    p.after_rows = order ? 1 : 0;
+    if (q.rows > 0) {
+        if (const int rc = encode_bytes_3d(h, h->moe.map[0], q.weight, q.k, q.n, q.experts, kI8StepK, kI8TileRows / 2, CU_TENSOR_MAP_SWIZZLE_128B))
+            return rc;
+        if (const int rc = encode_bytes_2d(h, h->moe.map[1], p.xq, q.k, q.rows, kI8StepK, unsigned(p.box), CU_TENSOR_MAP_SWIZZLE_128B))
+            return rc;
+    }
     set_params(h, p);
-    const void *fn = q.dtype == GG_FP16 ? reinterpret_cast<const void *>(&i8_products<__half>)
-                                        : reinterpret_cast<const void *>(&i8_products<__nv_bfloat16>);
+    const bool half = q.dtype == GG_FP16;
+    const void *fn = half ? reinterpret_cast<const void *>(&i8_products<__half>) : reinterpret_cast<const void *>(&i8_products<__nv_bfloat16>);
     GG_CUDA(h, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8Smem));
-    MoeLaunch quant = quant_launch(q.dtype, x_rows, q.k, num_sms);
-    if (!p.after_quant)
-        quant.grid = 0;
+    const MoeLaunch rows{half ? reinterpret_cast<const void *>(&i8_rows<__half>) : reinterpret_cast<const void *>(&i8_rows<__nv_bfloat16>),
+                         order ? unsigned(std::min<int64_t>(q.rows, 32 * num_sms)) : 0u, quant_threads(q.rows, q.x_scales ? q.k / 2 : q.k, num_sms), 0};
     MoeLaunch products{fn, q.rows > 0 ? unsigned(2 * pairs) : 0u, kI8Threads, size_t(kI8Smem), 2};
     products.cluster = 2;
     char detail[160];
     std::snprintf(detail, sizeof(detail), "gg_i8<%s> n=%lld k=%lld chunk=%d stages=%d pairs=%d", type_name(q.dtype), static_cast<long long>(q.n),
                   static_cast<long long>(q.k), chunk, p.stages, pairs);
-    return finish(h, stream, {quant, products}, detail);
+    return finish(h, stream, {rows, products}, detail);
 }
 
 }  // namespace

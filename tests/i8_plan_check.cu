@@ -35,13 +35,14 @@ int main(int argc, char **argv) {
     for (int l = 0; l < launches; ++l) {
         const int pairs = range(0, 3) ? 74 : range(1, 80), steps = range(1, range(0, 1) ? 8 : 120);
         const int64_t items = range(0, range(0, 1) ? 200 : 1000);
+        const int min_steps = range(1, 24);
         std::vector<std::vector<char>> done(items, std::vector<char>(steps, 0));
         std::map<int64_t, std::vector<int>> owners;  // of cut items: the pairs, as they come
         std::map<int64_t, std::pair<int, int>> told;
         std::set<int> slots;
         for (int c = 0; c < pairs; ++c) {
-            const I8Plan plan(items, steps, pairs, c);
-            CHECK(plan.cut >= 0 && plan.cut <= items && plan.cut < 2 * pairs);
+            const I8Plan plan(items, steps, min_steps, pairs, c);
+            CHECK(plan.cut >= 0 && plan.cut <= items && plan.cut < 2 * pairs && plan.ranges <= pairs && (plan.ranges >= plan.cut || plan.ranges == pairs));
             plan.pieces([&](int64_t item, int k0, int n, int first, int pieces) {
                 ++pieces_seen;
                 CHECK(item >= 0 && item < items && n > 0 && k0 >= 0 && k0 + n <= steps && pieces >= 1);
