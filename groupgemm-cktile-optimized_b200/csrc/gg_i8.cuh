@@ -51,7 +51,7 @@ struct I8Params {
     const int32_t *src;       // [rows] slots, or null: row r is x[r]
     void *out;                // [rows, n]
     uint32_t *status;         // [0] status word, [2] timeouts of this launch
-    int32_t *ws;              // [2 x pairs][2 CTAs][4 quarters][chunk / 32][8][32] int4
+    int32_t *ws;              // [2 x pairs][2 CTAs][4 quarters][chunk / 16][4][32] int4
     int32_t *counters;        // [pairs][2 CTAs][8 warps], 0 between launches
     int64_t rows, slots;      // slots: tokens * top_k
     uint64_t timeout_ns;
@@ -251,14 +251,15 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         ptx::tmem_alloc<2>(ptx::smem_addr(slots), 512);
         ptx::tmem_relinquish<2>();
     }
+    ptx::tc_fence_before();
+    __syncwarp();
+    ptx::cluster_arrive();  // this CTA's barriers are initialised
     if (!p.after_rows)
         ptx::griddep_wait();
     ptx::fence_proxy_async_global();
     ptx::griddep_launch_dependents();
     const I8Work work(p, start, first);
-    ptx::tc_fence_before();
-    __syncthreads();
-    ptx::cluster_sync();  // the peer's barriers are initialised before any remote arrive
+    ptx::cluster_wait();  // and so are the peer's, before any remote arrive
     ptx::tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(slots);
     const Abort ab{p.status + 2, abort_flag, p.timeout_ns};
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 reinterpret_cast<uint4 *>(out + row * p.n)[i - r * pieces] = make_uint4(0, 0, 0, 0);
             }
         }
-        const int group = (warp - 2) >> 2;  // blocks of 32 tokens that this warp takes: group, group + 2, ...
+        const int group = (warp - 2) >> 2;  // blocks of 16 tokens that this warp takes: group, group + 2, ...
         float *my_scales = row_scale[warp - 2];
         uint32_t turn = 0;
         bool ok = true;
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             if (!ok)
                 return;
             const I8Item it = work.at(p, item);
-            const int col = it.n0 + int(rank) * 128 + quarter * 32 + lane, blocks = it.width / 32;
+            const int col = it.n0 + int(rank) * 128 + quarter * 32 + lane, blocks = (it.count + 15) / 16;
             if (p.after_rows && turn == 0)
                 ptx::griddep_wait();  // xq_scales are i8_rows' output
             // scales of the rows of this warp's blocks, and of this lane's weight row; whether all are far from the ends of fp32's range
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int j = 32 * (group + 2 * i) + lane;
+                const int j = 16 * (group + 4 * i + 2 * (lane >> 4)) + (lane & 15);
                 x[i] = j < it.count ? __ldg(p.xq_scales + it.r0 + j) : 0.0f;
             }
             auto ordinary = [](float v) { return v == 0.0f || (fabsf(v) > 9.0949470e-13f && fabsf(v) < 1.0995116e12f); };  // 2^-40, 2^40
@@ -398,10 +399,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             ++turn;
             ptx::tc_fence_after();
             const uint32_t from = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(acc * kI8MaxTokens);
-            const int64_t most = p.chunk / 32;
+            const int64_t most = p.chunk / 16;
             // this quarter's part of pair c's piece: slot 0 where the piece begins inside its item, 1 where it begins it
             auto slot = [&](int c) {
-                return reinterpret_cast<int4 *>(p.ws) + (((int64_t(2 * c + (c == first_pair ? 1 : 0)) * 2 + rank) * 4 + quarter) * most) * 256 + lane;
+                return reinterpret_cast<int4 *>(p.ws) + (((int64_t(2 * c + (c == first_pair ? 1 : 0)) * 2 + rank) * 4 + quarter) * most) * 128 + lane;
             };
             bool store = true;
             if (pieces > 1 && group < blocks) {
@@ -409,12 +410,12 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 int4 *mine = slot(pair);
 #pragma unroll 1
                 for (int b = group; b < blocks; b += 2) {
-                    uint32_t r[32];
-                    ptx::tmem_ld_32x32b_x32(from + uint32_t(b * 32), r);
-                    ptx::tmem_wait_ld(r);
+                    uint32_t r[16];
+                    tmem_ld_x16(from + uint32_t(b * 16), r);
+                    tmem_wait_ld16(r);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        __stcg(mine + b * 256 + j * 32, make_int4(int(r[4 * j]), int(r[4 * j + 1]), int(r[4 * j + 2]), int(r[4 * j + 3])));
+                    for (int j = 0; j < 4; ++j)
+                        __stcg(mine + b * 128 + j * 32, make_int4(int(r[4 * j]), int(r[4 * j + 1]), int(r[4 * j + 2]), int(r[4 * j + 3])));
                 }
                 __threadfence();
                 __syncwarp();
@@ -429,17 +430,25 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 }
             }
             if (store) {
+                // Two tokens of a lane become two weight rows of one token by an exchange with the lane beside it: even lanes store
+                // token j, odd ones j + 1, four bytes each.
+                const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
+                const int64_t row_bytes = int64_t(p.n) * int64_t(sizeof(T));
+                uint8_t *to = reinterpret_cast<uint8_t *>(out) + (it.r0 + 16 * group + (lane & 1)) * row_bytes + (col & ~1) * int64_t(sizeof(T));
+                int rows = col < p.n ? it.count - 16 * group - (lane & 1) : 0;
+                const float *xs = my_scales;
 #pragma unroll 1
-                for (int b = group; b < blocks; b += 2) {
-                    uint32_t r[32];
-                    ptx::tmem_ld_32x32b_x32(from + uint32_t(b * 32), r);
-                    ptx::tmem_wait_ld(r);
+                for (int b = group; b < blocks; b += 2, to += 32 * row_bytes, rows -= 32, xs += 16) {
+                    uint32_t r[16];
+                    tmem_ld_x16(from + uint32_t(b * 16), r);
+                    tmem_wait_ld16(r);
                     if (pieces > 1)
+#pragma unroll 1
                         for (int c = first_pair; c < first_pair + pieces; ++c)
                             if (c != pair) {
-                                const int4 *theirs = slot(c) + b * 256;
+                                const int4 *theirs = slot(c) + b * 128;
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) {
+                                for (int j = 0; j < 4; ++j) {
                                     const int4 v = __ldcg(theirs + j * 32);
                                     r[4 * j] += uint32_t(v.x);
                                     r[4 * j + 1] += uint32_t(v.y);
@@ -447,29 +456,22 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                                     r[4 * j + 3] += uint32_t(v.w);
                                 }
                             }
-                    // Two tokens of a lane become two weight rows of one token by an exchange with the lane beside it: even lanes
-                    // store token j, odd ones j + 1, four bytes each.
-                    const int rows = col < p.n ? it.count - b * 32 - (lane & 1) : 0;
-                    T *to = out + int64_t(it.r0 + b * 32 + (lane & 1)) * p.n + (col & ~1);
-                    const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
-                    const float4 *scales = reinterpret_cast<const float4 *>(my_scales + 16 * (b - group));
+                    // scales near the ends of fp32's range: products that leave it on the way only, in 64 bits
+                    if (plain)
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 x4 = scales[j / 4];
-                        const float xs[4] = {x4.x, x4.y, x4.z, x4.w};
-                        float v[4];
+                        for (int j = 0; j < 16; ++j)
+                            r[j] = __float_as_uint(float(int(r[j])) * xs[j] * scale);
+                    else
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            // the smaller scale first: no product on the way leaves fp32's range unless the result does
-                            const bool less = !plain && !(fabsf(xs[i]) < fabsf(scale));
-                            v[i] = float(int(r[j + i])) * (less ? scale : xs[i]) * (less ? xs[i] : scale);
-                        }
+                        for (int j = 0; j < 16; ++j)
+                            r[j] = __float_as_uint(float(double(int(r[j])) * double(xs[j]) * double(scale)));
+                    uint8_t *at = to;
 #pragma unroll
-                        for (int i = 0; i < 4; i += 2) {
-                            const uint32_t own = moe::pack2<T>(v[i], v[i + 1]), other = __shfl_xor_sync(0xffffffffu, own, 1);
-                            if (j + i < rows)
-                                __stcs(reinterpret_cast<uint32_t *>(to + int64_t(j + i) * p.n), __byte_perm(own, other, pick));
-                        }
+                    for (int j = 0; j < 16; j += 2, at += 2 * row_bytes) {
+                        const uint32_t own = moe::pack2<T>(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+                        const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+                        if (j < rows)
+                            __stcs(reinterpret_cast<uint32_t *>(at), __byte_perm(own, other, pick));
                     }
                 }
             }
