@@ -3,9 +3,9 @@
 //   ds = r (d - mean d - c mean(d c)) + dsum   with c = (s - m) r, d = dy gamma;   dgamma = sum_t dy c, dbeta = sum_t dy
 //
 // What bounds them: each row is read once and written once. One block an SM stays for the whole launch; its warps form
-// groups that take a row each, a vector of 8 values or two a thread, held in registers between the sums and the result. Rows come through a
-// ring in shared memory, bulk copies a few rows ahead, so that the sums' latency (shuffles and a barrier a row) passes while
-// the next rows are on their way, and a thread's weight, bias and sums of gradients stay in registers from row to row.
+// groups that take a row each, one to four vectors of 8 values a thread. Rows come through a ring in shared memory, bulk copies a few rows
+// ahead, so that the sums' latency (shuffles and a barrier a row) passes while the next rows are on their way, and a thread's weight, bias
+// and sums of gradients stay in registers from row to row.
 #pragma once
 
 #include "gg_moe.cuh"
@@ -14,9 +14,11 @@ namespace gg {
 namespace moe {
 
 constexpr int kNormMaxHidden = 16384;
-constexpr int kNormSmem = 200 * 1024;  // of a block's ring
+constexpr int kNormThreads = 512;      // of a block at most
+constexpr int kNormSmem = 212 * 1024;  // of a block's ring and copies
 constexpr int kNormMaxSlots = 8;       // rows that a group's ring holds
-constexpr int kNormMaxGroups = 15;     // each has a named barrier beside the block's own
+constexpr int kNormMaxGroups = 14;     // each has a named barrier beside the block's own
+constexpr int kNormMaxWarps = 16;      // of a group
 
 struct NormParams {
     const void *x, *residual;   // [rows, hidden]
@@ -29,6 +31,7 @@ struct NormParams {
     int64_t rows;
     int vecs;                   // 8 values each, of a row
     int warps, groups, slots;   // a group's warps, a block's groups, a ring's rows
+    int params_at;              // the parameters' copy in shared memory, 0: none
     float eps;
     uint64_t timeout_ns;
 };
@@ -43,7 +46,7 @@ struct NormGradParams {
     uint32_t *status;
     int64_t rows;
     int vecs;
-    int warps, groups, slots;
+    int warps, groups, slots, params_at;
     int blocks;
     uint64_t timeout_ns;
 };
@@ -59,19 +62,61 @@ __device__ __forceinline__ uint4 lds_row(uint32_t addr) {
     return v;
 }
 
-// Eight values of a row in the words that hold them.
+// Two fp32 values in a 64-bit register pair, and the operations that take both at once (each rounded as the single one).
+using pair_t = uint64_t;
+__device__ __forceinline__ pair_t pair(float a, float b) {
+    pair_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float2 split(pair_t p) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+    pair_t p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+    pair_t p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+__device__ __forceinline__ pair_t fma2(pair_t a, pair_t b, pair_t c) {
+    pair_t p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
+    return p;
+}
+__device__ __forceinline__ float both(pair_t p) {
+    const float2 v = split(p);
+    return v.x + v.y;
+}
+
+// Eight values of a row in the words that hold them: of 16 bits columns 8 vec to 8 vec + 7, of 32 bits four in the row's first half and
+// four in its second (4 vec on, 4 (vecs + vec) on), so that a warp's accesses are 16 bytes a lane side by side.
 template <class T> struct Vec8 {
     uint4 w;
-    __device__ __forceinline__ void lds(uint32_t row, int vec) { w = lds_row(row + uint32_t(vec) * 16u); }
-    __device__ __forceinline__ void ldg(const void *row, int vec) { w = __ldg(static_cast<const uint4 *>(row) + vec); }
+    __device__ __forceinline__ void lds(uint32_t row, int vec, int) { w = lds_row(row + uint32_t(vec) * 16u); }
+    __device__ __forceinline__ void ldg(const void *row, int vec, int) { w = __ldg(static_cast<const uint4 *>(row) + vec); }
     __device__ __forceinline__ void get(float (&f)[8]) const {
         const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y), c = unpack2<T>(w.z), d = unpack2<T>(w.w);
         f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = c.x, f[5] = c.y, f[6] = d.x, f[7] = d.y;
     }
+    __device__ __forceinline__ void get(pair_t (&f)[4]) const {
+        const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y), c = unpack2<T>(w.z), d = unpack2<T>(w.w);
+        f[0] = pair(a.x, a.y), f[1] = pair(b.x, b.y), f[2] = pair(c.x, c.y), f[3] = pair(d.x, d.y);
+    }
+    __device__ __forceinline__ void set(const pair_t (&f)[4]) {
+        const float2 a = split(f[0]), b = split(f[1]), c = split(f[2]), d = split(f[3]);
+        w = make_uint4(moe::pack2<T>(a.x, a.y), moe::pack2<T>(b.x, b.y), moe::pack2<T>(c.x, c.y), moe::pack2<T>(d.x, d.y));
+    }
     __device__ __forceinline__ void set(const float (&f)[8]) {
         w = make_uint4(moe::pack2<T>(f[0], f[1]), moe::pack2<T>(f[2], f[3]), moe::pack2<T>(f[4], f[5]), moe::pack2<T>(f[6], f[7]));
     }
-    __device__ __forceinline__ void stg(void *row, int vec) const { __stcs(static_cast<uint4 *>(row) + vec, w); }
+    __device__ __forceinline__ void stg(void *row, int vec, int) const { __stcs(static_cast<uint4 *>(row) + vec, w); }
+    static __device__ __forceinline__ void stg_q(int8_t *row, int vec, int, uint2 q) { reinterpret_cast<uint2 *>(row)[vec] = q; }
     // The largest magnitude's bits (NaN above all), of two columns at a time; bits(): as fp32's.
     __device__ __forceinline__ uint32_t top(uint32_t so_far) const {
         return __vimax3_s16x2(__vimax3_s16x2(so_far, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), w.z & 0x7fff7fffu, w.w & 0x7fff7fffu);
@@ -83,25 +128,37 @@ template <class T> struct Vec8 {
 };
 template <> struct Vec8<float> {
     float4 a, b;
-    __device__ __forceinline__ void lds(uint32_t row, int vec) {
-        const uint4 u = lds_row(row + uint32_t(vec) * 32u), v = lds_row(row + uint32_t(vec) * 32u + 16u);
+    __device__ __forceinline__ void lds(uint32_t row, int vec, int vecs) {
+        const uint4 u = lds_row(row + uint32_t(vec) * 16u), v = lds_row(row + uint32_t(vecs + vec) * 16u);
         a = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
         b = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
     }
-    __device__ __forceinline__ void ldg(const void *row, int vec) {
-        a = __ldg(static_cast<const float4 *>(row) + 2 * vec);
-        b = __ldg(static_cast<const float4 *>(row) + 2 * vec + 1);
+    __device__ __forceinline__ void ldg(const void *row, int vec, int vecs) {
+        a = __ldg(static_cast<const float4 *>(row) + vec);
+        b = __ldg(static_cast<const float4 *>(row) + vecs + vec);
     }
     __device__ __forceinline__ void get(float (&f)[8]) const {
         f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    }
+    __device__ __forceinline__ void get(pair_t (&f)[4]) const {
+        f[0] = pair(a.x, a.y), f[1] = pair(a.z, a.w), f[2] = pair(b.x, b.y), f[3] = pair(b.z, b.w);
+    }
+    __device__ __forceinline__ void set(const pair_t (&f)[4]) {
+        const float2 u = split(f[0]), v = split(f[1]), x = split(f[2]), y = split(f[3]);
+        a = make_float4(u.x, u.y, v.x, v.y);
+        b = make_float4(x.x, x.y, y.x, y.y);
     }
     __device__ __forceinline__ void set(const float (&f)[8]) {
         a = make_float4(f[0], f[1], f[2], f[3]);
         b = make_float4(f[4], f[5], f[6], f[7]);
     }
-    __device__ __forceinline__ void stg(void *row, int vec) const {
-        __stcs(static_cast<float4 *>(row) + 2 * vec, a);
-        __stcs(static_cast<float4 *>(row) + 2 * vec + 1, b);
+    __device__ __forceinline__ void stg(void *row, int vec, int vecs) const {
+        __stcs(static_cast<float4 *>(row) + vec, a);
+        __stcs(static_cast<float4 *>(row) + vecs + vec, b);
+    }
+    static __device__ __forceinline__ void stg_q(int8_t *row, int vec, int vecs, uint2 q) {
+        reinterpret_cast<uint32_t *>(row)[vec] = q.x;
+        reinterpret_cast<uint32_t *>(row)[vecs + vec] = q.y;
     }
     __device__ __forceinline__ uint32_t top(uint32_t so_far) const {
         const uint32_t m = 0x7fffffffu;
@@ -116,7 +173,7 @@ template <> struct Vec8<float> {
 // scale = top / 127 and q = the whole number nearest to 127 v / top, halves to the even one, for the row's largest magnitude top: of
 // the exact quotient, so that the result does not depend on how it is computed. v (127 / top) is off by at most 127 * 2^-24 = 7.6e-6 by
 // the division's rounding, and the sum with 1.5 * 2^23 that brings its nearest whole number into the low bits rounds once. Where
-// that leaves the choice open for one of eight values (within 2e-5 of a half), all eight are decided exactly, by the sign of
+// that leaves the choice open for one of eight values (within 3e-5 of a half), all eight are decided exactly, by the sign of
 // 254 v - (2 f + 1) top, f = floor: both products are split into a rounded part and its error by fma, and their difference is exact (it is small).
 // So are rows whose top is below 2^-60 or above 2^60, scaled by 2^80 or 2^-80 first so that nothing here leaves fp32's normal range.
 // A row of zeros has scale 0 and q 0; one that holds NaN or an infinity has scale NaN and q 0.
@@ -124,22 +181,23 @@ template <> struct Vec8<float> {
 struct Rounding {
     float top, inverse, up;
     bool zero, careful;  // all q are 0; all values the exact way
-    __device__ __forceinline__ Rounding(uint32_t top_bits, float &scale) {  // of the largest magnitude's bits (NaN above all)
+    static __device__ __forceinline__ float scale(uint32_t top_bits) {
+        return top_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(top_bits), 127.0f);
+    }
+    __device__ __forceinline__ explicit Rounding(uint32_t top_bits) {  // of the largest magnitude's bits (NaN above all)
         top = __uint_as_float(top_bits);
-        const bool odd = top_bits >= 0x7f800000u;
-        scale = odd ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 127.0f);
-        zero = odd || top_bits == 0u;
+        zero = top_bits >= 0x7f800000u || top_bits == 0u;
         up = top < 8.6736174e-19f ? 1.2089258e24f : top > 1.1529215e18f ? 8.2718061e-25f : 1.0f;  // 2^-60, 2^80; 2^60, 2^-80
         careful = zero || up != 1.0f;
         top = zero ? 1.0f : top * up;
-        inverse = __fdiv_rn(127.0f, top);
+        inverse = 127.0f * __frcp_rn(top);
     }
     __device__ __forceinline__ uint32_t exact(float v) const {
         if (zero)
             return 0u;
         const float a = fabsf(v) * up, t = a * inverse;
         float m = rintf(t);
-        if (fabsf(t - m) > 0.49998f) {
+        if (fabsf(t - m) > 0.49997f) {
             const float f = floorf(t), b = 2.0f * f + 1.0f, p = b * top;
             const float e = fmaf(b, top, -p), r = fmaf(254.0f, a, -p);
             m = r > e ? f + 1.0f : r < e ? f : 2.0f * rintf(0.5f * (f + 0.5f));
@@ -155,7 +213,7 @@ struct Rounding {
             worst = fmaxf(worst, fabsf(fmaf(v[i], inverse, 12582912.0f - s)));
             n[i] = __float_as_uint(s);
         }
-        if (worst > 0.49998f || careful)
+        if (worst > 0.49997f || careful)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 n[i] = exact(v[i]);
@@ -183,7 +241,7 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
     for (int i = 0; i < kQuantHeld; ++i) {
         const int at = tid + i * int(blockDim.x);
         if (at < vecs)
-            v[i].ldg(row, at);
+            v[i].ldg(row, at, vecs);
     }
 #pragma unroll
     for (int i = 0; i < kQuantHeld; ++i)
@@ -191,7 +249,7 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
             top = v[i].top(top);
     for (int at = tid + kQuantHeld * int(blockDim.x); at < vecs; at += blockDim.x) {
         Vec8<T> u;
-        u.ldg(row, at);
+        u.ldg(row, at, vecs);
         top = u.top(top);
     }
     top = __reduce_max_sync(0xffffffffu, Vec8<T>::bits(top));
@@ -199,26 +257,24 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
         part[warp] = top;
     __syncthreads();  // a warp writes these words again only after the next row's barrier
     top = __reduce_max_sync(0xffffffffu, lane < warps ? part[lane] : 0u);
-    float scale;
-    const Rounding by(top, scale);
+    const Rounding by(top);
     if (tid == 0)
-        *scale_to = scale;
-    uint2 *q = reinterpret_cast<uint2 *>(to);
+        *scale_to = Rounding::scale(top);
 #pragma unroll
     for (int i = 0; i < kQuantHeld; ++i) {
         const int at = tid + i * int(blockDim.x);
         if (at < vecs) {
             float f[8];
             v[i].get(f);
-            q[at] = by(f);
+            Vec8<T>::stg_q(to, at, vecs, by(f));
         }
     }
     for (int at = tid + kQuantHeld * int(blockDim.x); at < vecs; at += blockDim.x) {
         Vec8<T> u;
         float f[8];
-        u.ldg(row, at);
+        u.ldg(row, at, vecs);
         u.get(f);
-        q[at] = by(f);
+        Vec8<T>::stg_q(to, at, vecs, by(f));
     }
 }
 
@@ -230,6 +286,26 @@ template <class T> __global__ void __launch_bounds__(512) quant_rows(const __gri
     int turn = 0;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1)
         quant_row<T>(static_cast<const uint8_t *>(p.x) + r * p.vecs * int64_t(8 * sizeof(T)), p.q + r * p.vecs * 8, p.scales + r, p.vecs, part[turn]);
+}
+
+// ---- sums of two values at a time ----
+
+// Of a warp: lanes 0-15 get the sum of a, lanes 16-31 that of b.
+__device__ __forceinline__ float halves_sum(float a, float b) {
+    const bool low = (threadIdx.x & 16u) == 0;
+    float keep = low ? a : b;
+    keep += __shfl_xor_sync(0xffffffffu, low ? b : a, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+        keep += __shfl_xor_sync(0xffffffffu, keep, o);
+    return keep;
+}
+// Of each half warp's 16 values, both sums for all lanes.
+__device__ __forceinline__ float2 each_half_sum(float v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
 }
 
 // ---- rows through a ring in shared memory ----
@@ -312,14 +388,65 @@ __device__ __forceinline__ void row_ring_end(uint32_t *status, volatile uint32_t
     }
 }
 
-// Mean and variance without cancellation: each warp its own mean and the squares around it, joined by
-//   sum (v - m)^2 = sum over warps of (squares_w + n_w (m_w - m)^2).
-template <class T, class W, int V, int kMax>
-__global__ void __launch_bounds__(kMax, 1) norm_rows(const __grid_constant__ NormParams p) {
+// A thread's weights or biases, 8 a vector: held in registers for all rows where it has one or two vectors, else read for each row from
+// the block's copy in shared memory (or, where there is no place for that, from global memory), since they would cost the registers
+// that hold the row or the sums.
+template <class T, class W, int V> struct NormParam {
+    static constexpr bool kHeld = V <= 2;
+    const uint8_t *from;  // null: 1 or 0 throughout
+    float otherwise;
+    int vecs;
+    Vec8<W> held[kHeld ? V : 1];
+    // copy: place in shared memory, or null. By all threads of the block, which have to be together before the first use.
+    __device__ __forceinline__ NormParam(const void *array, float otherwise_, int first, int step, int vecs_, uint8_t *copy)
+        : from(static_cast<const uint8_t *>(array)), otherwise(otherwise_), vecs(vecs_) {
+        if constexpr (kHeld) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (first + v * step < vecs)
+                    read(held[v], first + v * step);
+        } else if (array && copy) {
+            for (int i = threadIdx.x; i < vecs * int(sizeof(W)) / 2; i += blockDim.x)
+                reinterpret_cast<uint4 *>(copy)[i] = __ldg(static_cast<const uint4 *>(array) + i);
+            from = copy;
+        }
+    }
+    __device__ __forceinline__ void read(Vec8<W> &v, int at) const {
+        if (!from) {
+            const pair_t both = pair(otherwise, otherwise), all[4] = {both, both, both, both};
+            v.set(all);
+            return;
+        }
+        const uint4 *words = reinterpret_cast<const uint4 *>(from);
+        if constexpr (std::is_same<W, float>::value) {
+            constexpr bool near = !std::is_same<T, float>::value;  // the columns of a 16-bit row's vector
+            const uint4 a = words[near ? 2 * at : at], b = words[near ? 2 * at + 1 : vecs + at];
+            v.a = make_float4(__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z), __uint_as_float(a.w));
+            v.b = make_float4(__uint_as_float(b.x), __uint_as_float(b.y), __uint_as_float(b.z), __uint_as_float(b.w));
+        } else {
+            v.w = words[at];
+        }
+    }
+    __device__ __forceinline__ void get(int v, int at, pair_t (&f)[4]) const {
+        if constexpr (kHeld) {
+            held[v].get(f);
+        } else {
+            Vec8<W> w;
+            read(w, at);
+            w.get(f);
+        }
+    }
+};
+
+// Mean and variance without cancellation: each warp its own mean m_w and the squares S_w around it, joined around the first warp's mean, t_w = m_w - m_0:
+//   mean = m_0 + sum n_w t_w / n     sum (v - mean)^2 = sum (S_w + n_w t_w^2) - n (mean - m_0)^2
+// where what is taken off is at most the sum of the others' n_w t_w^2, so that no more than a factor of the number of warps is lost.
+template <class T, class W, int V>
+__global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_constant__ NormParams p) {
     extern __shared__ __align__(1024) uint8_t norm_smem[];
     __shared__ uint64_t bars[kNormMaxGroups * kNormMaxSlots];
-    __shared__ float2 part[kNormMaxGroups * 2 * 32];
-    __shared__ uint32_t tops[kNormMaxGroups * 2 * 32];
+    __shared__ float part[kNormMaxGroups][2][2 * kNormMaxWarps];
+    __shared__ uint32_t tops[kNormMaxGroups][2][kNormMaxWarps];
     __shared__ volatile uint32_t flag;
     RowRing<2> g = row_ring<2>(p, p.residual ? 2 : 1, ptx::smem_addr(norm_smem), bars, &flag, p.vecs * int(8 * sizeof(T)));
     g.from[0] = static_cast<const uint8_t *>(p.x);
@@ -327,7 +454,7 @@ __global__ void __launch_bounds__(kMax, 1) norm_rows(const __grid_constant__ Nor
     const int warp = g.tid >> 5, lane = g.tid & 31;
     for (int s = 0; s < g.slots; ++s)
         g.load(s, g.first + s * g.stride);
-    // values of warp w (and of this one)
+    // values of warp w
     auto count = [&](int w) {
         int n = 0;
 #pragma unroll
@@ -335,74 +462,70 @@ __global__ void __launch_bounds__(kMax, 1) norm_rows(const __grid_constant__ Nor
             n += min(32, max(0, p.vecs - v * g.threads - w * 32));
         return float(8 * n);
     };
-    const float mine = count(warp), inv_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
-    const float theirs = lane < p.warps ? count(lane) : 0.0f, inv_theirs = theirs > 0.0f ? 1.0f / theirs : 0.0f;
-    const float inv_hidden = 1.0f / float(8 * p.vecs);
-    Vec8<W> gamma[V], beta[V];
-    {
-        const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1}, none[8] = {};
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int at = g.tid + v * g.threads;
-            gamma[v].set(one);
-            beta[v].set(none);
-            if (p.gamma && at < p.vecs)
-                gamma[v].ldg(p.gamma, at);
-            if (p.beta && at < p.vecs)
-                beta[v].ldg(p.beta, at);
-        }
-    }
+    const float inv_mine = 1.0f / fmaxf(8.0f, count(warp)), hidden = float(8 * p.vecs), inv_hidden = 1.0f / hidden;
+    const int other = lane & 15;  // the warp whose sums this lane joins
+    const float theirs = other < p.warps ? count(other) : 0.0f;
+    const int param_bytes = p.vecs * int(8 * sizeof(W));
+    uint8_t *copy = p.params_at ? norm_smem + p.params_at : nullptr;
+    const NormParam<T, W, V> gamma(p.gamma, 1.0f, g.tid, g.threads, p.vecs, copy),
+        beta(p.beta, 0.0f, g.tid, g.threads, p.vecs, copy ? copy + param_bytes : nullptr);
+    __syncthreads();
     int slot = 0, turn = 0;
     uint32_t phase = 0;
     for (int64_t r = g.first; r < p.rows; r += g.stride) {
         g.wait(slot, phase);
-        const int64_t row = r * p.vecs;  // in vectors
-        float f[V][8];
-        float sum = 0.0f;
+        const int64_t row = r * g.row_bytes;
+        pair_t f[V][4];
+        pair_t sum = 0;  // of even and of odd columns
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
             if (at < p.vecs) {
                 Vec8<T> x;
-                x.lds(g.at(slot, 0), at);
+                x.lds(g.at(slot, 0), at, p.vecs);
                 x.get(f[v]);
                 if (p.residual) {
-                    float a[8];
-                    x.lds(g.at(slot, 1), at);
+                    pair_t a[4];
+                    x.lds(g.at(slot, 1), at, p.vecs);
                     x.get(a);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        f[v][i] += a[i];
+                    for (int i = 0; i < 4; ++i)
+                        f[v][i] = add2(f[v][i], a[i]);
                     x.set(f[v]);
                     x.get(f[v]);
                     if (p.sum && g.ok)
-                        x.stg(static_cast<uint8_t *>(p.sum) + row * int64_t(8 * sizeof(T)), at);
+                        x.stg(static_cast<uint8_t *>(p.sum) + row, at, p.vecs);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    sum += f[v][i];
+                for (int i = 0; i < 4; ++i)
+                    sum = add2(sum, f[v][i]);
             }
         }
-        sum = warp_sum(sum);
-        float squares = 0.0f;
-        const float m_warp = sum * inv_mine;
+        const float m_warp = warp_sum(both(sum)) * inv_mine;
+        const pair_t minus_warp = pair(-m_warp, -m_warp);
+        pair_t squared = 0;
 #pragma unroll
         for (int v = 0; v < V; ++v)
             if (g.tid + v * g.threads < p.vecs)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    squares = fmaf(f[v][i] - m_warp, f[v][i] - m_warp, squares);
-        squares = warp_sum(squares);
-        float2 *mailbox = part + (g.group * 2 + turn) * 32;
-        if (lane == 0)
-            mailbox[warp] = make_float2(sum, squares);
+                for (int i = 0; i < 4; ++i) {
+                    const pair_t d = add2(f[v][i], minus_warp);
+                    squared = fma2(d, d, squared);
+                }
+        const float squares = warp_sum(both(squared));
+        float *box = part[g.group][turn];
+        if (lane == 0) {
+            box[warp] = m_warp;
+            box[kNormMaxWarps + warp] = squares;
+        }
         g.sync();  // the slot has been read, too
         g.load(slot, r + g.slots * g.stride);
-        const float2 w = lane < p.warps ? mailbox[lane] : make_float2(0.0f, 0.0f);
-        const float mean = warp_sum(w.x) * inv_hidden;
-        const float off = w.x * inv_theirs - mean;
-        const float var = warp_sum(fmaf(theirs * off, off, w.y)) * inv_hidden;
-        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(var + p.eps));
+        const float m_first = box[0];
+        const float t = other < p.warps ? box[other] - m_first : 0.0f;
+        const float2 joined = each_half_sum(lane < 16 ? theirs * t : other < p.warps ? fmaf(theirs * t, t, box[kNormMaxWarps + other]) : 0.0f);
+        const float off = joined.x * inv_hidden, mean = m_first + off;
+        const float var = fmaxf(0.0f, joined.y * inv_hidden - off * off);
+        const float rstd = rsqrtf(isnan(joined.y) ? joined.y : var + p.eps);
         if (g.tid == 0 && g.ok) {
             if (p.mean)
                 p.mean[r] = mean;
@@ -410,42 +533,43 @@ __global__ void __launch_bounds__(kMax, 1) norm_rows(const __grid_constant__ Nor
                 p.rstd[r] = rstd;
         }
         uint32_t top = 0;
+        Vec8<T> y[V];
+        const pair_t minus_mean = pair(-mean, -mean), both_rstd = pair(rstd, rstd);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
             if (at < p.vecs) {
-                float a[8], b[8];
-                gamma[v].get(a);
-                beta[v].get(b);
+                pair_t a[4], b[4];
+                gamma.get(v, at, a);
+                beta.get(v, at, b);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    f[v][i] = fmaf((f[v][i] - mean) * rstd, a[i], b[i]);
-                Vec8<T> y;
-                y.set(f[v]);
+                for (int i = 0; i < 4; ++i)
+                    f[v][i] = fma2(mul2(add2(f[v][i], minus_mean), both_rstd), a[i], b[i]);
+                y[v].set(f[v]);
                 if (p.y && g.ok)
-                    y.stg(static_cast<uint8_t *>(p.y) + row * int64_t(8 * sizeof(T)), at);
-                if (p.q) {
-                    top = y.top(top);
-                    y.get(f[v]);  // the integers are of y as it is written
-                }
+                    y[v].stg(static_cast<uint8_t *>(p.y) + row, at, p.vecs);
+                if (p.q)
+                    top = y[v].top(top);
             }
         }
         if (p.q) {
-            uint32_t *box = tops + (g.group * 2 + turn) * 32;
+            uint32_t *most = tops[g.group][turn];
             top = __reduce_max_sync(0xffffffffu, Vec8<T>::bits(top));
             if (lane == 0)
-                box[warp] = top;
+                most[warp] = top;
             g.sync();
-            top = __reduce_max_sync(0xffffffffu, lane < p.warps ? box[lane] : 0u);
-            float scale;
-            const Rounding by(top, scale);
+            top = __reduce_max_sync(0xffffffffu, lane < p.warps ? most[lane] : 0u);
+            const Rounding by(top);
             if (g.tid == 0 && g.ok)
-                p.q_scales[r] = scale;
+                p.q_scales[r] = Rounding::scale(top);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const int at = g.tid + v * g.threads;
-                if (at < p.vecs && g.ok)
-                    reinterpret_cast<uint2 *>(p.q)[row + at] = by(f[v]);
+                if (at < p.vecs && g.ok) {
+                    float a[8];
+                    y[v].get(a);  // the integers are of y as it is written
+                    Vec8<T>::stg_q(p.q + r * p.vecs * 8, at, p.vecs, by(a));
+                }
             }
         }
         turn ^= 1;
@@ -458,12 +582,13 @@ __global__ void __launch_bounds__(kMax, 1) norm_rows(const __grid_constant__ Nor
 }
 
 // The gradients: a block's sums of dgamma and dbeta stay in registers over its rows, its groups' are added in order, and each block
-// leaves its sums for norm_grad_sum.
-template <class T, class W, int V, int kMax>
-__global__ void __launch_bounds__(kMax, 1) norm_grad_rows(const __grid_constant__ NormGradParams p) {
+// leaves its sums for norm_grad_sum. A row is read from its slot twice, before and after the sums along it, so that the registers hold
+// those sums only; so a slot is loaded again one row later, when the next row's barrier shows that all are past it.
+template <class T, class W, int V>
+__global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_constant__ NormGradParams p) {
     extern __shared__ __align__(1024) uint8_t norm_smem[];
     __shared__ uint64_t bars[kNormMaxGroups * kNormMaxSlots];
-    __shared__ float2 part[kNormMaxGroups * 2 * 32];
+    __shared__ float part[kNormMaxGroups][2][2 * kNormMaxWarps];
     __shared__ volatile uint32_t flag;
     RowRing<3> g = row_ring<3>(p, p.dsum ? 3 : 2, ptx::smem_addr(norm_smem), bars, &flag, p.vecs * int(8 * sizeof(T)));
     g.from[0] = static_cast<const uint8_t *>(p.x);
@@ -473,91 +598,86 @@ __global__ void __launch_bounds__(kMax, 1) norm_grad_rows(const __grid_constant_
     for (int s = 0; s < g.slots; ++s)
         g.load(s, g.first + s * g.stride);
     const float inv_hidden = 1.0f / float(8 * p.vecs);
-    Vec8<W> gamma[V];
-    float dgamma[V][8] = {}, dbeta[V][8] = {};
-    {
-        const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1};
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            gamma[v].set(one);
-            if (p.gamma && g.tid + v * g.threads < p.vecs)
-                gamma[v].ldg(p.gamma, g.tid + v * g.threads);
-        }
-    }
-    float mean = 0.0f, rstd = 0.0f;
+    const NormParam<T, W, V> gamma(p.gamma, 1.0f, g.tid, g.threads, p.vecs, p.params_at ? norm_smem + p.params_at : nullptr);
+    __syncthreads();
+    pair_t dgamma[V][4] = {}, dbeta[V][4] = {};
+    float next_mean = 0.0f, next_rstd = 0.0f;
     if (g.first < p.rows) {
-        mean = __ldg(p.mean + g.first);
-        rstd = __ldg(p.rstd + g.first);
+        next_mean = __ldg(p.mean + g.first);
+        next_rstd = __ldg(p.rstd + g.first);
     }
     int slot = 0, turn = 0;
     uint32_t phase = 0;
     for (int64_t r = g.first; r < p.rows; r += g.stride) {
-        float next_mean = 0.0f, next_rstd = 0.0f;
+        const float rstd = next_rstd;
+        const pair_t minus_mean = pair(-next_mean, -next_mean), both_rstd = pair(rstd, rstd);
         if (r + g.stride < p.rows) {
             next_mean = __ldg(p.mean + r + g.stride);
             next_rstd = __ldg(p.rstd + r + g.stride);
         }
         g.wait(slot, phase);
-        Vec8<T> x[V], dy[V], more[V];
-        float along = 0.0f, level = 0.0f;  // sums of d c and of d
+        pair_t along = 0, level = 0;  // sums of d (x - mean) and of d, of even and of odd columns
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
             if (at < p.vecs) {
-                x[v].lds(g.at(slot, 0), at);
-                dy[v].lds(g.at(slot, 1), at);
-                if (p.dsum)
-                    more[v].lds(g.at(slot, 2), at);
-                float a[8], b[8], w[8];
-                x[v].get(a);
-                dy[v].get(b);
-                gamma[v].get(w);
+                Vec8<T> x, dy;
+                pair_t a[4], b[4], w[4];
+                x.lds(g.at(slot, 0), at, p.vecs);
+                dy.lds(g.at(slot, 1), at, p.vecs);
+                x.get(a);
+                dy.get(b);
+                gamma.get(v, at, w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float c = (a[i] - mean) * rstd, d = b[i] * w[i];
-                    level += d;
-                    along = fmaf(d, c, along);
-                    dgamma[v][i] = fmaf(b[i], c, dgamma[v][i]);
-                    dbeta[v][i] += b[i];
+                for (int i = 0; i < 4; ++i) {
+                    const pair_t c = add2(a[i], minus_mean), d = mul2(b[i], w[i]);
+                    level = add2(level, d);
+                    along = fma2(d, c, along);
+                    dgamma[v][i] = fma2(mul2(b[i], both_rstd), c, dgamma[v][i]);
+                    dbeta[v][i] = add2(dbeta[v][i], b[i]);
                 }
             }
         }
-        along = warp_sum(along);
-        level = warp_sum(level);
-        float2 *mailbox = part + (g.group * 2 + turn) * 32;
-        if (lane == 0)
-            mailbox[warp] = make_float2(along, level);
-        g.sync();  // the slot has been read, too
-        g.load(slot, r + g.slots * g.stride);
-        const float2 s = lane < p.warps ? mailbox[lane] : make_float2(0.0f, 0.0f);
-        along = warp_sum(s.x) * inv_hidden;
-        level = warp_sum(s.y) * inv_hidden;
+        const float mine = halves_sum(both(along), both(level));
+        float *box = part[g.group][turn];
+        if ((lane & 15) == 0)
+            box[(lane & 16) + warp] = mine;  // kNormMaxWarps of each
+        g.sync();  // all are past the row before
+        if (g.slots > 1 && r != g.first)
+            g.load(slot ? slot - 1 : g.slots - 1, r + (g.slots - 1) * g.stride);
+        const float2 sums = each_half_sum((lane & 15) < p.warps ? box[lane] : 0.0f);
+        const float less = -rstd * (sums.y * inv_hidden), tilt = -(rstd * (sums.x * inv_hidden)) * rstd * rstd;
+        const pair_t both_less = pair(less, less), slope = pair(tilt, tilt);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
             if (at < p.vecs) {
-                float a[8], b[8], w[8];
-                x[v].get(a);
-                dy[v].get(b);
-                gamma[v].get(w);
+                Vec8<T> x, dy;
+                pair_t a[4], b[4], w[4];
+                x.lds(g.at(slot, 0), at, p.vecs);
+                dy.lds(g.at(slot, 1), at, p.vecs);
+                x.get(a);
+                dy.get(b);
+                gamma.get(v, at, w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float c = (a[i] - mean) * rstd;
-                    a[i] = rstd * (fmaf(b[i], w[i], -level) - c * along);
-                }
+                for (int i = 0; i < 4; ++i)
+                    a[i] = fma2(add2(a[i], minus_mean), slope, fma2(mul2(b[i], w[i]), both_rstd, both_less));
                 if (p.dsum) {
-                    more[v].get(b);
+                    x.lds(g.at(slot, 2), at, p.vecs);
+                    x.get(b);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        a[i] += b[i];
+                    for (int i = 0; i < 4; ++i)
+                        a[i] = add2(a[i], b[i]);
                 }
-                x[v].set(a);
+                x.set(a);
                 if (g.ok)
-                    x[v].stg(static_cast<uint8_t *>(p.dx) + r * p.vecs * int64_t(8 * sizeof(T)), at);
+                    x.stg(static_cast<uint8_t *>(p.dx) + r * g.row_bytes, at, p.vecs);
             }
         }
-        mean = next_mean;
-        rstd = next_rstd;
+        if (g.slots == 1) {
+            g.sync();
+            g.load(0, r + g.stride);
+        }
         turn ^= 1;
         if (++slot == g.slots) {
             slot = 0;
@@ -570,15 +690,16 @@ __global__ void __launch_bounds__(kMax, 1) norm_grad_rows(const __grid_constant_
     // The rings are done with: group 0 adds the other groups' sums, in order. [group - 1][2][hidden]
     float *sums = reinterpret_cast<float *>(norm_smem);
     const int hidden = 8 * p.vecs;
+    auto of_group = [&](int o, int which, int vec) { return reinterpret_cast<ulonglong2 *>(sums + (2 * o + which) * hidden + 8 * vec); };
     if (g.group > 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
             if (at < p.vecs)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sums[(g.group - 1) * 2 * hidden + 8 * at + i] = dgamma[v][i];
-                    sums[((g.group - 1) * 2 + 1) * hidden + 8 * at + i] = dbeta[v][i];
+                for (int i = 0; i < 2; ++i) {
+                    of_group(g.group - 1, 0, at)[i] = make_ulonglong2(dgamma[v][2 * i], dgamma[v][2 * i + 1]);
+                    of_group(g.group - 1, 1, at)[i] = make_ulonglong2(dbeta[v][2 * i], dbeta[v][2 * i + 1]);
                 }
         }
     }
@@ -592,16 +713,21 @@ __global__ void __launch_bounds__(kMax, 1) norm_grad_rows(const __grid_constant_
             continue;
         for (int o = 0; o < p.groups - 1; ++o)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                dgamma[v][i] += sums[o * 2 * hidden + 8 * at + i];
-                dbeta[v][i] += sums[(o * 2 + 1) * hidden + 8 * at + i];
+            for (int i = 0; i < 2; ++i) {
+                const ulonglong2 a = of_group(o, 0, at)[i], b = of_group(o, 1, at)[i];
+                dgamma[v][2 * i] = add2(dgamma[v][2 * i], a.x);
+                dgamma[v][2 * i + 1] = add2(dgamma[v][2 * i + 1], a.y);
+                dbeta[v][2 * i] = add2(dbeta[v][2 * i], b.x);
+                dbeta[v][2 * i + 1] = add2(dbeta[v][2 * i + 1], b.y);
             }
-        float4 *to = reinterpret_cast<float4 *>(p.parts + int64_t(blockIdx.x) * 2 * hidden + 8 * at);
-        to[0] = make_float4(dgamma[v][0], dgamma[v][1], dgamma[v][2], dgamma[v][3]);
-        to[1] = make_float4(dgamma[v][4], dgamma[v][5], dgamma[v][6], dgamma[v][7]);
-        to += hidden / 4;
-        to[0] = make_float4(dbeta[v][0], dbeta[v][1], dbeta[v][2], dbeta[v][3]);
-        to[1] = make_float4(dbeta[v][4], dbeta[v][5], dbeta[v][6], dbeta[v][7]);
+        ulonglong2 *to = reinterpret_cast<ulonglong2 *>(p.parts + int64_t(blockIdx.x) * 2 * hidden);
+        constexpr bool split_row = std::is_same<T, float>::value;  // see Vec8
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int four = split_row ? at + i * p.vecs : 2 * at + i;
+            to[four] = make_ulonglong2(dgamma[v][2 * i], dgamma[v][2 * i + 1]);
+            to[hidden / 4 + four] = make_ulonglong2(dbeta[v][2 * i], dbeta[v][2 * i + 1]);
+        }
     }
 }
 

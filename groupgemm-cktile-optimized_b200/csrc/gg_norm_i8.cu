@@ -17,40 +17,46 @@ using gg::moe::kNormMaxGroups;
 using gg::moe::kNormMaxHidden;
 using gg::moe::kNormMaxSlots;
 using gg::moe::kNormSmem;
+using gg::moe::kNormThreads;
 
 // ---- layer norm ----
 
 struct NormShape {
-    int v, most;                // vectors a thread, threads a block at most: the kernel's V and kMax
-    int warps, groups, slots;
+    int v;  // vectors a thread
+    int warps, groups, slots, params_at;
     unsigned blocks;
     size_t smem;
 };
 
-NormShape norm_shape(int64_t rows, int vecs, int tensors, int elem, int num_sms) {
+#ifndef NORMV
+#define NORMV(vecs) ((vecs) <= 64 ? 1 : (vecs) <= 1024 ? 2 : 4)
+#endif
+NormShape norm_shape(int64_t rows, int vecs, int tensors, int elem, int params, int param_size, int num_sms) {
     NormShape s{};
-    s.v = vecs <= 512 ? 1 : 2;
-    s.most = vecs <= 512 || vecs > 1024 ? 1024 : 512;
+    s.v = NORMV(vecs);
     s.warps = (vecs + 32 * s.v - 1) / (32 * s.v);
     const int64_t each = (rows + num_sms - 1) / num_sms;  // rows of a block
-    s.groups = int(std::max<int64_t>(1, std::min<int64_t>({each, s.most / (32 * s.warps), kNormMaxGroups})));
+    s.groups = int(std::max<int64_t>(1, std::min<int64_t>({each, kNormThreads / (32 * s.warps), kNormMaxGroups})));
     const size_t row = size_t(vecs) * 8 * size_t(elem) * size_t(tensors);
-    while (s.groups > 1 && size_t(s.groups) * 2 * row > size_t(kNormSmem))
+    size_t copy = s.v > 2 ? size_t(params) * size_t(vecs) * 8 * size_t(param_size) : 0;
+    if (2 * row + copy > size_t(kNormSmem))
+        copy = 0;  // read from global memory
+    while (s.groups > 1 && size_t(s.groups) * 2 * row + copy > size_t(kNormSmem))
         --s.groups;
     s.blocks = unsigned(std::min<int64_t>(num_sms, (rows + s.groups - 1) / s.groups));
     const int64_t turns = (each + s.groups - 1) / s.groups;  // rows of a group
-    s.slots = int(std::max<int64_t>(1, std::min<int64_t>({int64_t(kNormSmem / (size_t(s.groups) * row)), turns, kNormMaxSlots})));
+    s.slots = int(std::max<int64_t>(1, std::min<int64_t>({int64_t((kNormSmem - copy) / (size_t(s.groups) * row)), turns, kNormMaxSlots})));
     s.smem = size_t(s.groups) * size_t(s.slots) * row;
+    s.params_at = copy ? int(s.smem) : 0;
+    s.smem += copy;
     return s;
 }
 
+template <class T, class W, int V> const void *norm_fn(bool grad) {
+    return grad ? reinterpret_cast<const void *>(&gg::moe::norm_grad_rows<T, W, V>) : reinterpret_cast<const void *>(&gg::moe::norm_rows<T, W, V>);
+}
 template <class T, class W> const void *norm_fn(const NormShape &s, bool grad) {
-    using namespace gg::moe;
-    if (s.v == 1)
-        return grad ? reinterpret_cast<const void *>(&norm_grad_rows<T, W, 1, 1024>) : reinterpret_cast<const void *>(&norm_rows<T, W, 1, 1024>);
-    if (s.most == 512)
-        return grad ? reinterpret_cast<const void *>(&norm_grad_rows<T, W, 2, 512>) : reinterpret_cast<const void *>(&norm_rows<T, W, 2, 512>);
-    return grad ? reinterpret_cast<const void *>(&norm_grad_rows<T, W, 2, 1024>) : reinterpret_cast<const void *>(&norm_rows<T, W, 2, 1024>);
+    return s.v == 1 ? norm_fn<T, W, 1>(grad) : s.v == 2 ? norm_fn<T, W, 2>(grad) : norm_fn<T, W, 4>(grad);
 }
 const void *norm_fn(const NormShape &s, int dtype, int param_type, bool grad) {
     if (dtype == GG_F32)
@@ -88,7 +94,8 @@ int prepare_norm(gg_handle *h, const gg_norm_problem &q, gg_stream_t stream, cha
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
-    const NormShape s = norm_shape(q.tokens, int(q.hidden / 8), q.residual ? 2 : 1, q.dtype == GG_F32 ? 4 : 2, num_sms);
+    const NormShape s = norm_shape(q.tokens, int(q.hidden / 8), q.residual ? 2 : 1, q.dtype == GG_F32 ? 4 : 2, 2,
+                                   q.param_type == GG_F32 ? 4 : 2, num_sms);
     gg::moe::NormParams p{};
     p.x = q.x;
     p.residual = q.residual;
@@ -106,6 +113,7 @@ int prepare_norm(gg_handle *h, const gg_norm_problem &q, gg_stream_t stream, cha
     p.warps = s.warps;
     p.groups = s.groups;
     p.slots = s.slots;
+    p.params_at = s.params_at;
     p.eps = q.eps;
     p.timeout_ns = uint64_t(h->opt_timeout_ms) * 1000000u;
     set_params(h, p);
@@ -127,7 +135,8 @@ int prepare_norm_grad(gg_handle *h, const gg_norm_grad_problem &q, gg_stream_t s
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
-    const NormShape s = norm_shape(q.tokens, int(q.hidden / 8), q.dsum ? 3 : 2, q.dtype == GG_F32 ? 4 : 2, num_sms);
+    const NormShape s = norm_shape(q.tokens, int(q.hidden / 8), q.dsum ? 3 : 2, q.dtype == GG_F32 ? 4 : 2, 1,
+                                   q.param_type == GG_F32 ? 4 : 2, num_sms);
     const size_t sums = 2 * size_t(q.hidden) * 4;  // dgamma and dbeta of a block or group
     if (const int rc = reserve(h, std::max<size_t>(1, s.blocks) * sums))
         return rc;
@@ -148,6 +157,7 @@ int prepare_norm_grad(gg_handle *h, const gg_norm_grad_problem &q, gg_stream_t s
     p.warps = s.warps;
     p.groups = s.groups;
     p.slots = s.slots;
+    p.params_at = s.params_at;
     p.blocks = int(s.blocks);
     p.timeout_ns = uint64_t(h->opt_timeout_ms) * 1000000u;
     set_params(h, p);
