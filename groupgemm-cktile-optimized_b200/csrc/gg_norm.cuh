@@ -15,7 +15,7 @@ namespace moe {
 
 constexpr int kNormMaxHidden = 16384;
 constexpr int kNormThreads = 512;      // of a block at most
-constexpr int kNormSmem = 212 * 1024;  // of a block's ring and copies
+constexpr int kNormSmem = 212 * 1024;  // of a block's ring and copies at most
 constexpr int kNormMaxSlots = 8;       // rows that a group's ring holds
 constexpr int kNormMaxGroups = 14;     // each has a named barrier beside the block's own
 constexpr int kNormMaxWarps = 16;      // of a group
@@ -94,16 +94,23 @@ __device__ __forceinline__ float both(pair_t p) {
     return v.x + v.y;
 }
 
+// Sums of the two 16-bit values of a word.
+template <class T> __device__ __forceinline__ uint32_t plus2(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t plus2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 v = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t plus2<__half>(uint32_t a, uint32_t b) {
+    const __half2 v = __hadd2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
 // Eight values of a row in the words that hold them: of 16 bits columns 8 vec to 8 vec + 7, of 32 bits four in the row's first half and
 // four in its second (4 vec on, 4 (vecs + vec) on), so that a warp's accesses are 16 bytes a lane side by side.
 template <class T> struct Vec8 {
     uint4 w;
     __device__ __forceinline__ void lds(uint32_t row, int vec, int) { w = lds_row(row + uint32_t(vec) * 16u); }
     __device__ __forceinline__ void ldg(const void *row, int vec, int) { w = __ldg(static_cast<const uint4 *>(row) + vec); }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y), c = unpack2<T>(w.z), d = unpack2<T>(w.w);
-        f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = c.x, f[5] = c.y, f[6] = d.x, f[7] = d.y;
-    }
     __device__ __forceinline__ void get(pair_t (&f)[4]) const {
         const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y), c = unpack2<T>(w.z), d = unpack2<T>(w.w);
         f[0] = pair(a.x, a.y), f[1] = pair(b.x, b.y), f[2] = pair(c.x, c.y), f[3] = pair(d.x, d.y);
@@ -112,10 +119,12 @@ template <class T> struct Vec8 {
         const float2 a = split(f[0]), b = split(f[1]), c = split(f[2]), d = split(f[3]);
         w = make_uint4(moe::pack2<T>(a.x, a.y), moe::pack2<T>(b.x, b.y), moe::pack2<T>(c.x, c.y), moe::pack2<T>(d.x, d.y));
     }
-    __device__ __forceinline__ void set(const float (&f)[8]) {
-        w = make_uint4(moe::pack2<T>(f[0], f[1]), moe::pack2<T>(f[2], f[3]), moe::pack2<T>(f[4], f[5]), moe::pack2<T>(f[6], f[7]));
-    }
     __device__ __forceinline__ void stg(void *row, int vec, int) const { __stcs(static_cast<uint4 *>(row) + vec, w); }
+    // Rounded once, and alike, whether the sums are formed in 16 or in 32 bits: where 32 bits do not hold a sum exactly, the smaller term is
+    // below a quarter of the larger one's last place.
+    __device__ __forceinline__ void add(const Vec8 &o) {
+        w = make_uint4(plus2<T>(w.x, o.w.x), plus2<T>(w.y, o.w.y), plus2<T>(w.z, o.w.z), plus2<T>(w.w, o.w.w));
+    }
     static __device__ __forceinline__ void stg_q(int8_t *row, int vec, int, uint2 q) { reinterpret_cast<uint2 *>(row)[vec] = q; }
     // The largest magnitude's bits (NaN above all), of two columns at a time; bits(): as fp32's.
     __device__ __forceinline__ uint32_t top(uint32_t so_far) const {
@@ -137,9 +146,6 @@ template <> struct Vec8<float> {
         a = __ldg(static_cast<const float4 *>(row) + vec);
         b = __ldg(static_cast<const float4 *>(row) + vecs + vec);
     }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    }
     __device__ __forceinline__ void get(pair_t (&f)[4]) const {
         f[0] = pair(a.x, a.y), f[1] = pair(a.z, a.w), f[2] = pair(b.x, b.y), f[3] = pair(b.z, b.w);
     }
@@ -148,10 +154,6 @@ template <> struct Vec8<float> {
         a = make_float4(u.x, u.y, v.x, v.y);
         b = make_float4(x.x, x.y, y.x, y.y);
     }
-    __device__ __forceinline__ void set(const float (&f)[8]) {
-        a = make_float4(f[0], f[1], f[2], f[3]);
-        b = make_float4(f[4], f[5], f[6], f[7]);
-    }
     __device__ __forceinline__ void stg(void *row, int vec, int vecs) const {
         __stcs(static_cast<float4 *>(row) + vec, a);
         __stcs(static_cast<float4 *>(row) + vecs + vec, b);
@@ -159,6 +161,10 @@ template <> struct Vec8<float> {
     static __device__ __forceinline__ void stg_q(int8_t *row, int vec, int vecs, uint2 q) {
         reinterpret_cast<uint32_t *>(row)[vec] = q.x;
         reinterpret_cast<uint32_t *>(row)[vecs + vec] = q.y;
+    }
+    __device__ __forceinline__ void add(const Vec8 &o) {
+        a = make_float4(a.x + o.a.x, a.y + o.a.y, a.z + o.a.z, a.w + o.a.w);
+        b = make_float4(b.x + o.b.x, b.y + o.b.y, b.z + o.b.z, b.w + o.b.w);
     }
     __device__ __forceinline__ uint32_t top(uint32_t so_far) const {
         const uint32_t m = 0x7fffffffu;
@@ -204,19 +210,25 @@ struct Rounding {
         }
         return uint32_t(v < 0.0f ? -int(m) : int(m));
     }
-    __device__ __forceinline__ uint2 operator()(const float (&v)[8]) const {
+    __device__ __forceinline__ uint2 operator()(const pair_t (&v)[4]) const {
         uint32_t n[8];
         float worst = 0.0f;
+        const pair_t by = pair(inverse, inverse), to_low = pair(12582912.0f, 12582912.0f), minus = pair(-1.0f, -1.0f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float s = fmaf(v[i], inverse, 12582912.0f);  // its low byte is the number's
-            worst = fmaxf(worst, fabsf(fmaf(v[i], inverse, 12582912.0f - s)));
-            n[i] = __float_as_uint(s);
+        for (int i = 0; i < 4; ++i) {
+            const pair_t s = fma2(v[i], by, to_low);  // the low bytes are the numbers'
+            const float2 off = split(fma2(v[i], by, fma2(s, minus, to_low))), bits = split(s);
+            worst = fmaxf(worst, fmaxf(fabsf(off.x), fabsf(off.y)));
+            n[2 * i] = __float_as_uint(bits.x);
+            n[2 * i + 1] = __float_as_uint(bits.y);
         }
         if (worst > 0.49997f || careful)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                n[i] = exact(v[i]);
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = split(v[i]);
+                n[2 * i] = exact(f.x);
+                n[2 * i + 1] = exact(f.y);
+            }
         return make_uint2(__byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410),
                           __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410));
     }
@@ -264,14 +276,14 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
     for (int i = 0; i < kQuantHeld; ++i) {
         const int at = tid + i * int(blockDim.x);
         if (at < vecs) {
-            float f[8];
+            pair_t f[4];
             v[i].get(f);
             Vec8<T>::stg_q(to, at, vecs, by(f));
         }
     }
     for (int at = tid + kQuantHeld * int(blockDim.x); at < vecs; at += blockDim.x) {
         Vec8<T> u;
-        float f[8];
+        pair_t f[4];
         u.ldg(row, at, vecs);
         u.get(f);
         Vec8<T>::stg_q(to, at, vecs, by(f));
@@ -483,19 +495,14 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
             if (at < p.vecs) {
                 Vec8<T> x;
                 x.lds(g.at(slot, 0), at, p.vecs);
-                x.get(f[v]);
                 if (p.residual) {
-                    pair_t a[4];
-                    x.lds(g.at(slot, 1), at, p.vecs);
-                    x.get(a);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        f[v][i] = add2(f[v][i], a[i]);
-                    x.set(f[v]);
-                    x.get(f[v]);
+                    Vec8<T> more;
+                    more.lds(g.at(slot, 1), at, p.vecs);
+                    x.add(more);
                     if (p.sum && g.ok)
                         x.stg(static_cast<uint8_t *>(p.sum) + row, at, p.vecs);
                 }
+                x.get(f[v]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     sum = add2(sum, f[v][i]);
@@ -534,7 +541,8 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
         }
         uint32_t top = 0;
         Vec8<T> y[V];
-        const pair_t minus_mean = pair(-mean, -mean), both_rstd = pair(rstd, rstd);
+        // (s - mean) rstd as s rstd - mean rstd: off by a rounding of mean rstd, as the mean's own rounding makes it
+        const pair_t minus = pair(-mean * rstd, -mean * rstd), both_rstd = pair(rstd, rstd);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
@@ -544,7 +552,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
                 beta.get(v, at, b);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    f[v][i] = fma2(mul2(add2(f[v][i], minus_mean), both_rstd), a[i], b[i]);
+                    f[v][i] = fma2(fma2(f[v][i], both_rstd, minus), a[i], b[i]);
                 y[v].set(f[v]);
                 if (p.y && g.ok)
                     y[v].stg(static_cast<uint8_t *>(p.y) + row, at, p.vecs);
@@ -566,7 +574,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
             for (int v = 0; v < V; ++v) {
                 const int at = g.tid + v * g.threads;
                 if (at < p.vecs && g.ok) {
-                    float a[8];
+                    pair_t a[4];
                     y[v].get(a);  // the integers are of y as it is written
                     Vec8<T>::stg_q(p.q + r * p.vecs * 8, at, p.vecs, by(a));
                 }

@@ -28,12 +28,10 @@ struct NormShape {
     size_t smem;
 };
 
-#ifndef NORMV
-#define NORMV(vecs) ((vecs) <= 64 ? 1 : (vecs) <= 1024 ? 2 : 4)
-#endif
-NormShape norm_shape(int64_t rows, int vecs, int tensors, int elem, int params, int param_size, int num_sms) {
+// ahead: bytes of rows that a block keeps on their way or in use, beyond the two that a group needs at least.
+NormShape norm_shape(int64_t rows, int vecs, int v, int tensors, int elem, int params, int param_size, size_t ahead, int num_sms) {
     NormShape s{};
-    s.v = NORMV(vecs);
+    s.v = v;
     s.warps = (vecs + 32 * s.v - 1) / (32 * s.v);
     const int64_t each = (rows + num_sms - 1) / num_sms;  // rows of a block
     s.groups = int(std::max<int64_t>(1, std::min<int64_t>({each, kNormThreads / (32 * s.warps), kNormMaxGroups})));
@@ -45,7 +43,8 @@ NormShape norm_shape(int64_t rows, int vecs, int tensors, int elem, int params, 
         --s.groups;
     s.blocks = unsigned(std::min<int64_t>(num_sms, (rows + s.groups - 1) / s.groups));
     const int64_t turns = (each + s.groups - 1) / s.groups;  // rows of a group
-    s.slots = int(std::max<int64_t>(1, std::min<int64_t>({int64_t((kNormSmem - copy) / (size_t(s.groups) * row)), turns, kNormMaxSlots})));
+    const int64_t fit = int64_t((kNormSmem - copy) / (size_t(s.groups) * row)), wanted = std::max<int64_t>(2, int64_t(ahead / (size_t(s.groups) * row)));
+    s.slots = int(std::max<int64_t>(1, std::min<int64_t>({fit, wanted, turns, kNormMaxSlots})));
     s.smem = size_t(s.groups) * size_t(s.slots) * row;
     s.params_at = copy ? int(s.smem) : 0;
     s.smem += copy;
@@ -94,8 +93,10 @@ int prepare_norm(gg_handle *h, const gg_norm_problem &q, gg_stream_t stream, cha
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
-    const NormShape s = norm_shape(q.tokens, int(q.hidden / 8), q.residual ? 2 : 1, q.dtype == GG_F32 ? 4 : 2, 2,
-                                   q.param_type == GG_F32 ? 4 : 2, num_sms);
+    // Vectors a thread: as few warps a row as registers allow, which is two vectors, since the sums between lanes cost the same for any number; with
+    // 8-bit rows, whose longer way wants two rows at a time, four.
+    const int vecs = int(q.hidden / 8), v = vecs <= 64 ? 1 : vecs <= (q.q ? 96 : 1024) ? 2 : 4;
+    const NormShape s = norm_shape(q.tokens, vecs, v, q.residual ? 2 : 1, q.dtype == GG_F32 ? 4 : 2, 2, q.param_type == GG_F32 ? 4 : 2, 88 << 10, num_sms);
     gg::moe::NormParams p{};
     p.x = q.x;
     p.residual = q.residual;
@@ -109,7 +110,7 @@ int prepare_norm(gg_handle *h, const gg_norm_problem &q, gg_stream_t stream, cha
     p.q_scales = q.q_scales;
     p.status = h->d_status;
     p.rows = q.tokens;
-    p.vecs = int(q.hidden / 8);
+    p.vecs = vecs;
     p.warps = s.warps;
     p.groups = s.groups;
     p.slots = s.slots;
@@ -135,8 +136,8 @@ int prepare_norm_grad(gg_handle *h, const gg_norm_grad_problem &q, gg_stream_t s
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
-    const NormShape s = norm_shape(q.tokens, int(q.hidden / 8), q.dsum ? 3 : 2, q.dtype == GG_F32 ? 4 : 2, 1,
-                                   q.param_type == GG_F32 ? 4 : 2, num_sms);
+    const int vecs = int(q.hidden / 8), v = vecs <= 64 ? 1 : vecs <= 1024 ? 2 : 4;
+    const NormShape s = norm_shape(q.tokens, vecs, v, q.dsum ? 3 : 2, q.dtype == GG_F32 ? 4 : 2, 1, q.param_type == GG_F32 ? 4 : 2, 160 << 10, num_sms);
     const size_t sums = 2 * size_t(q.hidden) * 4;  // dgamma and dbeta of a block or group
     if (const int rc = reserve(h, std::max<size_t>(1, s.blocks) * sums))
         return rc;
@@ -153,7 +154,7 @@ int prepare_norm_grad(gg_handle *h, const gg_norm_grad_problem &q, gg_stream_t s
     p.parts = h->d_ws;
     p.status = h->d_status;
     p.rows = q.tokens;
-    p.vecs = int(q.hidden / 8);
+    p.vecs = vecs;
     p.warps = s.warps;
     p.groups = s.groups;
     p.slots = s.slots;
