@@ -77,14 +77,13 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, ui
 // How the items of a launch are dealt out (host-callable, so that a CPU test can walk it): the first `cut` items by ranges of steps,
 // pair c's being [cut steps c / ranges, cut steps (c + 1) / ranges); then items cut + c, cut + c + pairs, ...
 struct I8Plan {
-    int64_t items;
-    int cut, ranges, pairs, steps;
+    int items, cut, ranges, pairs, steps;
     int64_t begin, end;  // this pair's range
     int c;
-    __host__ __device__ __forceinline__ I8Plan(int64_t items_, int steps_, int min_steps, int pairs_, int c_)
+    __host__ __device__ __forceinline__ I8Plan(int items_, int steps_, int min_steps, int pairs_, int c_)
         : items(items_), pairs(pairs_), steps(steps_), c(c_) {
-        const int64_t over = items % pairs;
-        cut = over == 0 ? 0 : int(items < pairs ? items : pairs + over);
+        const int over = items % pairs;
+        cut = over == 0 ? 0 : items < pairs ? items : pairs + over;
         const int64_t total = int64_t(cut) * steps, pieces = total / min_steps > cut ? total / min_steps : cut;
         ranges = int(pieces < 1 ? 1 : pieces < pairs ? pieces : pairs);
         begin = c < ranges ? total * c / ranges : 0;
@@ -95,14 +94,15 @@ struct I8Plan {
     // f(item, first step, steps, first pair of the item, pieces) for each of this pair's pieces, in order.
     template <class F> __host__ __device__ __forceinline__ void pieces(F &&f) const {
         for (int64_t s = begin; s < end;) {
-            const int64_t item = s / steps;
-            const int k0 = int(s - item * steps);
+            const int item = int(s / steps);
+            const int64_t at = int64_t(item) * steps;
+            const int k0 = int(s - at);
             const int n = int(end - s < steps - k0 ? end - s : steps - k0);
-            const int first = pair_of(item * steps);
-            f(item, k0, n, first, pair_of(item * steps + steps - 1) - first + 1);
+            const int first = pair_of(at);
+            f(item, k0, n, first, pair_of(at + steps - 1) - first + 1);
             s += n;
         }
-        for (int64_t item = cut + c; item < items; item += pairs)
+        for (int item = cut + c; item < items; item += pairs)
             f(item, 0, steps, c, 1);
     }
 };
@@ -113,18 +113,56 @@ struct I8Item {
 // Token chunks of `count` rows, and their size: as equal as steps of 32 allow.
 __host__ __device__ __forceinline__ int i8_chunks(int count, int most) { return (count + most - 1) / most; }
 __host__ __device__ __forceinline__ int i8_chunk_size(int count, int chunks) { return ((count + chunks - 1) / chunks + 31) & ~31; }
-// Item `in` of an expert's tiles x chunks: bands of kI8Band tiles, in each the chunks one after the other, each over the band's tiles, so that
-// the pairs at work at one time share a band's weights and a few chunks' tokens in L2.
-__host__ __device__ __forceinline__ void i8_place(int in, int tiles, int chunks, int &tile, int &chunk) {
-    const int band = in / (kI8Band * chunks), rest = in - band * (kI8Band * chunks);
-    const int wide = tiles - band * kI8Band < kI8Band ? tiles - band * kI8Band : kI8Band;
-    chunk = rest / wide;
-    tile = band * kI8Band + rest - chunk * wide;
-}
+// Where an item lies. A role's items only rise, so the expert and the band of the last one are kept: looked up anew for each item, the
+// divisions and the search had cost the products 1100 cycles an item, where one of 2048 k takes 8200.
+//   Order of an expert's tiles x chunks: bands of kI8Band tiles, in each the chunks one after the other, each over the band's tiles, so
+//   that the pairs at work at one time share a band's weights and a few chunks' tokens in L2.
+struct I8Cursor {
+    int e = 0, begin = 0, end = 0;      // the expert and its items
+    int row = 0, rows = 0, chunks = 0, size = 0;
+    int band = 0, band_begin = 0, wide = 0, shift = 0;  // its tiles from kI8Band band on, `wide` of them (2^shift, or shift -1)
+    __host__ __device__ __forceinline__ void to_band(int band_, int begin_, int tiles) {
+        band = band_;
+        band_begin = begin_;
+        wide = tiles - band * kI8Band < kI8Band ? tiles - band * kI8Band : kI8Band;
+        shift = wide == 8 ? 3 : wide == 4 ? 2 : wide == 2 ? 1 : wide == 1 ? 0 : -1;
+    }
+    // start: first row of each expert; first: token chunks of the experts before
+    __host__ __device__ __forceinline__ I8Item at(int item, int tiles, int experts, const int *start, const int *first) {
+        if (item >= end) {
+            const int run = item / tiles;
+            int lo = e, hi = experts - 1;
+            for (int i = 0; i < 4 && lo < hi && first[lo + 1] <= run; ++i)
+                ++lo;
+            while (lo < hi) {  // the last expert whose first chunk is at or before it
+                if (first[lo + 1] > run)
+                    break;
+                const int mid = (lo + hi + 1) >> 1;
+                if (first[mid] <= run)
+                    lo = mid;
+                else
+                    hi = mid - 1;
+            }
+            e = lo;
+            begin = first[e] * tiles;
+            end = first[e + 1] * tiles;
+            row = start[e];
+            rows = start[e + 1] - row;
+            chunks = first[e + 1] - first[e];
+            size = i8_chunk_size(rows, chunks);
+            to_band(0, begin, tiles);
+        }
+        while (item >= band_begin + wide * chunks)
+            to_band(band + 1, band_begin + wide * chunks, tiles);
+        const int rest = item - band_begin, chunk = shift >= 0 ? rest >> shift : rest / wide;
+        const int left = rows - chunk * size, count = left < size ? left : size;
+        return {e, (band * kI8Band + rest - chunk * wide) * kI8TileRows, row + chunk * size, count, (count + 31) & ~31};
+    }
+};
 
 struct I8Work {
     const int *start, *first;  // shared: first row of each expert (checked), token chunks of the experts before
-    int64_t items;
+    int items;
     bool falls;
 
     // offsets come from the device: each is held to the range that the rows allow, and where they fall no expert gets rows. By all threads
@@ -155,23 +193,10 @@ struct I8Work {
         if (tid == 0)
             first_[E] = chunks;
         __syncthreads();
-        items = int64_t(chunks) * p.tiles;
+        items = chunks * p.tiles;
     }
-    __device__ __forceinline__ I8Item at(const I8Params &p, int64_t item) const {
-        const int run = int(item / p.tiles);
-        int lo = 0, hi = p.experts - 1;  // the last expert whose first chunk is at or before it
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (first[mid] <= run)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        const int chunks = first[lo + 1] - first[lo], rows = start[lo + 1] - start[lo], size = i8_chunk_size(rows, chunks);
-        int tile, chunk;
-        i8_place(int(item - int64_t(first[lo]) * p.tiles), p.tiles, chunks, tile, chunk);
-        const int count = min(size, rows - chunk * size);
-        return {lo, tile * kI8TileRows, start[lo] + chunk * size, count, (count + 31) & ~31};
+    __device__ __forceinline__ I8Item at(const I8Params &p, int item, I8Cursor &cursor) const {
+        return cursor.at(item, p.tiles, p.experts, start, first);
     }
 };
 
@@ -271,8 +296,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         int s = 0;
         uint32_t ph = 0;
         bool ok = true, waited = !p.after_rows;
-        plan.pieces([&](int64_t item, int k0, int n, int, int) {
-            const I8Item it = work.at(p, item);
+        I8Cursor cursor;
+        plan.pieces([&](int item, int k0, int n, int, int) {
+            const I8Item it = work.at(p, item, cursor);
             // loads of this CTA's half of the tokens, and of both; what of a half no load covers goes into sums that nothing reads
             const int half = it.width / 2, box_bytes = p.box * kI8StepK;
             auto boxes = [&](int r) { return (min(half, max(0, it.count - r * half)) + p.box - 1) / p.box; };
@@ -315,10 +341,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             int s = 0;
             uint32_t ph = 0, turn = 0;
             bool ok = true;
-            plan.pieces([&](int64_t item, int, int n, int, int) {
+            I8Cursor cursor;
+            plan.pieces([&](int item, int, int n, int, int) {
                 if (!ok)
                     return;
-                const I8Item it = work.at(p, item);
+                const I8Item it = work.at(p, item, cursor);
                 const uint32_t idesc = i8_idesc(kI8TileRows, it.width);
                 const int acc = int(turn & 1u);
                 ok = wait_all(tempty(acc), ((turn >> 1) & 1u) ^ 1u, ab, kStatusTimeout | kRoleMma | 0x40u | uint32_t(acc));
@@ -368,10 +395,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         float *my_scales = row_scale[warp - 2];
         uint32_t turn = 0;
         bool ok = true;
-        plan.pieces([&](int64_t item, int, int, int first_pair, int pieces) {
+        I8Cursor cursor;
+        plan.pieces([&](int item, int, int, int first_pair, int pieces) {
             if (!ok)
                 return;
-            const I8Item it = work.at(p, item);
+            const I8Item it = work.at(p, item, cursor);
             const int col = it.n0 + int(rank) * 128 + quarter * 32 + lane, blocks = (it.count + 15) / 16;
             if (p.after_rows && turn == 0)
                 ptx::griddep_wait();  // xq_scales are i8_rows' output

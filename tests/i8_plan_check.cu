@@ -2,7 +2,8 @@
 // and item order (gg_i8.cuh, host-callable), for every pair of random launches.
 //   * every (item, step) is covered by exactly one piece, no piece is empty, and pieces of an item agree on its first pair and their number;
 //   * a cut item's pieces are its first pair's and the pairs' after it, one each, with workspace slots and counters of their own;
-//   * chunks cover an expert's rows, none is empty or larger than the limit, and items map onto every (tile, chunk) once.
+//   * chunks are not empty or larger than the limit, and the items of experts with and without rows, as a role's cursor finds them one after
+//     the other, cover every (row, tile) once.
 // Prints "ok <launches> <pieces>" and exits 0, or prints the first violation and exits 1.
 #include <cstdio>
 #include <cstdlib>
@@ -17,7 +18,7 @@ using namespace gg::moe;
 #define CHECK(cond)                                                    \
     do {                                                               \
         if (!(cond)) {                                                 \
-            std::printf("line %d: %s (items %lld steps %d pairs %d)\n", __LINE__, #cond, (long long)items, steps, pairs); \
+            std::printf("line %d: %s (items %d steps %d pairs %d)\n", __LINE__, #cond, items, steps, pairs); \
             std::exit(1);                                              \
         }                                                              \
     } while (0)
@@ -34,16 +35,16 @@ int main(int argc, char **argv) {
     long long pieces_seen = 0;
     for (int l = 0; l < launches; ++l) {
         const int pairs = range(0, 3) ? 74 : range(1, 80), steps = range(1, range(0, 1) ? 8 : 120);
-        const int64_t items = range(0, range(0, 1) ? 200 : 1000);
+        const int items = range(0, range(0, 1) ? 200 : 1000);
         const int min_steps = range(1, 24);
         std::vector<std::vector<char>> done(items, std::vector<char>(steps, 0));
-        std::map<int64_t, std::vector<int>> owners;  // of cut items: the pairs, as they come
-        std::map<int64_t, std::pair<int, int>> told;
+        std::map<int, std::vector<int>> owners;  // of cut items: the pairs, as they come
+        std::map<int, std::pair<int, int>> told;
         std::set<int> slots;
         for (int c = 0; c < pairs; ++c) {
             const I8Plan plan(items, steps, min_steps, pairs, c);
             CHECK(plan.cut >= 0 && plan.cut <= items && plan.cut < 2 * pairs && plan.ranges <= pairs && (plan.ranges >= plan.cut || plan.ranges == pairs));
-            plan.pieces([&](int64_t item, int k0, int n, int first, int pieces) {
+            plan.pieces([&](int item, int k0, int n, int first, int pieces) {
                 ++pieces_seen;
                 CHECK(item >= 0 && item < items && n > 0 && k0 >= 0 && k0 + n <= steps && pieces >= 1);
                 for (int k = k0; k < k0 + n; ++k) {
@@ -71,17 +72,35 @@ int main(int argc, char **argv) {
         for (auto &d : done)
             for (char c : d)
                 CHECK(c);
-        // chunks and item order of one expert
-        const int most = 32 << range(0, 3), count = range(1, 3000), tiles = range(1, 40);
-        const int chunks = i8_chunks(count, most), size = i8_chunk_size(count, chunks);
-        CHECK(size <= most && size % 32 == 0 && (chunks - 1) * size < count && chunks * size >= count);
-        std::vector<char> seen(size_t(tiles) * chunks, 0);
-        for (int in = 0; in < tiles * chunks; ++in) {
-            int tile, chunk;
-            i8_place(in, tiles, chunks, tile, chunk);
-            CHECK(tile >= 0 && tile < tiles && chunk >= 0 && chunk < chunks && !seen[tile * chunks + chunk]);
-            seen[tile * chunks + chunk] = 1;
+        // chunks and item order of experts, some without rows, as a role with a stride sees them
+        const int most = 32 << range(0, 3), tiles = range(1, 40), experts = range(1, range(0, 1) ? 4 : 200), stride = range(1, 80);
+        std::vector<int> start(experts + 1), first(experts + 1);
+        for (int e = 0; e < experts; ++e) {
+            const int count = range(0, 2) ? range(0, range(0, 1) ? 40 : 1500) : 0, chunks = i8_chunks(count, most);
+            start[e + 1] = start[e] + count;
+            first[e + 1] = first[e] + chunks;
+            if (chunks) {
+                const int size = i8_chunk_size(count, chunks);
+                CHECK(size <= most && size % 32 == 0 && (chunks - 1) * size < count && chunks * size >= count);
+            }
         }
+        std::vector<char> rows_seen(size_t(start[experts]) * tiles, 0);
+        for (int c = 0; c < stride; ++c) {
+            I8Cursor cursor;
+            for (int item = c; item < first[experts] * tiles; item += stride) {
+                const I8Item it = cursor.at(item, tiles, experts, start.data(), first.data());
+                CHECK(it.e >= 0 && it.e < experts && it.count > 0 && it.width >= it.count && it.width % 32 == 0 && it.width <= most);
+                CHECK(it.r0 >= start[it.e] && it.r0 + it.count <= start[it.e + 1]);
+                CHECK(it.n0 % kI8TileRows == 0 && it.n0 >= 0 && it.n0 / kI8TileRows < tiles);
+                for (int r = it.r0; r < it.r0 + it.count; ++r) {
+                    char &seen = rows_seen[size_t(r) * tiles + it.n0 / kI8TileRows];
+                    CHECK(!seen);
+                    seen = 1;
+                }
+            }
+        }
+        for (char c : rows_seen)
+            CHECK(c);
     }
     std::printf("ok %d %lld\n", launches, pieces_seen);
     return 0;
