@@ -35,7 +35,7 @@ constexpr int kI8Threads = (2 + kI8EpilogueWarps) * 32;
 constexpr int kI8Smem = kI8Ring + 1024;
 #ifndef I8BOX
 #define I8BOX 32
-#define I8MIN 8
+#define I8MIN 16
 #endif
 constexpr int kI8Box = I8BOX;         // rows of a token load at most
 constexpr int kI8MinSteps = I8MIN;     // of a cut piece
@@ -239,7 +239,8 @@ template <class T> __global__ void __launch_bounds__(512) i8_rows(const __grid_c
     }
 }
 
-template <class T>
+// kOnce: weights are read once, as a rule, and leave L2 first.
+template <class T, bool kOnce>
 __global__ void __launch_bounds__(kI8Threads, 1)
     i8_products(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ I8Params p) {
     extern __shared__ __align__(1024) uint8_t i8_smem[];
@@ -296,6 +297,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         int s = 0;
         uint32_t ph = 0;
         bool ok = true, waited = !p.after_rows;
+        [[maybe_unused]] const uint64_t once = ptx::l2_policy_evict_first();
         I8Cursor cursor;
         plan.pieces([&](int item, int k0, int n, int, int) {
             const I8Item it = work.at(p, item, cursor);
@@ -311,7 +313,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 const uint32_t a = ring + uint32_t(s * p.stage_bytes);
                 const int c = (k0 + j) * kI8StepK;
                 ptx::mbar_arrive_expect_tx(full(s), bytes, rank == 0 ? issue : 0u);
-                ptx::tma_load_3d_pair(a, &tmap_w, full_leader + 8u * s, c, it.n0 + int(rank) * 128, it.e, issue);
+                if constexpr (kOnce)
+                    ptx::tma_load_3d_pair_hint(a, &tmap_w, full_leader + 8u * s, c, it.n0 + int(rank) * 128, it.e, once, issue);
+                else
+                    ptx::tma_load_3d_pair(a, &tmap_w, full_leader + 8u * s, c, it.n0 + int(rank) * 128, it.e, issue);
                 if (!waited) {  // i8_rows' output is read from here on
                     ptx::griddep_wait();
                     ptx::fence_proxy_async_global();

@@ -211,6 +211,10 @@ int prepare_quant(gg_handle *h, const gg_quant_problem &q, gg_stream_t stream, c
 
 // ---- 8-bit products ----
 
+template <class T> const void *i8_products_fn(bool once) {
+    return once ? reinterpret_cast<const void *>(&gg::moe::i8_products<T, true>) : reinterpret_cast<const void *>(&gg::moe::i8_products<T, false>);
+}
+
 int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *why, size_t why_len) {
     using namespace gg::moe;
     if (q.dtype != GG_BF16 && q.dtype != GG_FP16)
@@ -234,16 +238,21 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     if (q.n * q.k >= int64_t(1) << 39)
         return refuse(h, why, why_len, "one expert's weights are too large for a TMA descriptor");
     const int64_t tiles = (q.n + kI8TileRows - 1) / kI8TileRows, steps = (q.k + kI8StepK - 1) / kI8StepK;
-    // Tokens of a chunk at most: a stage has place for half of them beside its 16 KB of weights.
-    int chunk = kI8MaxTokens;
-    while (chunk > 32 && q.rows <= chunk / 2)
-        chunk /= 2;
-    if (std::min(q.rows, q.experts + q.rows / chunk) * tiles >= kMaxIndex)
+    if (std::min(q.rows, q.experts + q.rows / 32) * tiles >= kMaxIndex)
         return refuse(h, why, why_len, "too many weight rows and experts for one launch");
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
     const int pairs = num_sms / 2;
+    // Tokens of a chunk at most: a stage has place for half of them beside its 16 KB of weights, so that small chunks keep more weights on
+    // their way, but an expert with more rows than that has its weights loaded again. And chunks small enough that there are about as many
+    // items as pairs, before any are cut along k. `once`: weights leave L2 first. Us with chunks of 64 / 128 / 256, and in brackets once, of
+    // 32 experts of 4096 x 4096 by their mean rows: 8 90 (86) / 90 (86) / 93 (88); 32 95 (91) / 94 (91) / 97 (93); 48 104 (103) / 101 (98) / 101 (98);
+    // 64 116 / 102 (101) / 103 (101); 96 154 / 111 (112) / 115 (110); 128 189 / 138 / 119 (119); 256 336 / 228 / 170 (174).
+    const int64_t mean = q.rows / q.experts;
+    int chunk = mean <= 32 ? 64 : mean <= 64 ? 128 : kI8MaxTokens;
+    while (chunk > 32 && (q.rows + chunk / 2 - 1) / (chunk / 2) * tiles <= pairs)
+        chunk /= 2;
     const bool order = q.rows > 0 && (q.src || !q.x_scales);  // rows are put into expert order or rounded first
     const size_t sums = 2 * size_t(pairs) * size_t(chunk) * 1024, rounded = order ? size_t(q.rows) * size_t(q.k) : 0;
     if (const int rc = reserve(h, sums + rounded + (order ? size_t(q.rows) * 4 : 0)))
@@ -285,7 +294,7 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     }
     set_params(h, p);
     const bool half = q.dtype == GG_FP16;
-    const void *fn = half ? reinterpret_cast<const void *>(&i8_products<__half>) : reinterpret_cast<const void *>(&i8_products<__nv_bfloat16>);
+    const void *fn = half ? i8_products_fn<__half>(mean <= 128) : i8_products_fn<__nv_bfloat16>(mean <= 128);
     GG_CUDA(h, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8Smem));
     const MoeLaunch rows{half ? reinterpret_cast<const void *>(&i8_rows<__half>) : reinterpret_cast<const void *>(&i8_rows<__nv_bfloat16>),
                          order ? unsigned(std::min<int64_t>(q.rows, 32 * num_sms)) : 0u, quant_threads(q.rows, q.x_scales ? q.k / 2 : q.k, num_sms), 0};
