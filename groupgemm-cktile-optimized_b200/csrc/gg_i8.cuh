@@ -49,6 +49,7 @@ struct I8Params {
     const float *scales;      // [experts, n]
     const int32_t *offsets;   // [experts + 1]
     const int32_t *src;       // [rows] slots, or null: row r is x[r]
+    int32_t *inv;             // [slots] places (i8_token_rows)
     void *out;                // [rows, n]
     uint32_t *status;         // [0] status word, [2] timeouts of this launch
     int32_t *ws;              // [2 x pairs][2 CTAs][4 quarters][chunk / 16][4][32] int4
@@ -236,6 +237,118 @@ template <class T> __global__ void __launch_bounds__(512) i8_rows(const __grid_c
             quant_row<T>(static_cast<const uint8_t *>(p.x) + row * p.k * int64_t(sizeof(T)), p.xq + r * p.k, p.xq_scales + r, p.k / 8, part[turn]);
             turn ^= 1;
         }
+    }
+}
+
+// The same by tokens, where one goes to several places: each row of x is read and rounded once. i8_places finds each slot's place, inv[src[r]] =
+// r, for i8_token_rows. What inv holds from other runs or of slots without a place is known by src, which does not point back; and of places
+// that name one slot twice all but one are done by themselves at the end. 16384 tokens of 7168 at 2 places: 140 us by places, XXX by tokens.
+constexpr int kI8PlaceThreads = 256, kI8TokenPlaces = 32;
+__device__ __forceinline__ int2 i8_live(const I8Params &p) {
+    return make_int2(max(0, p.offsets[0]), int(min(p.rows, int64_t(p.offsets[p.experts]))));
+}
+__global__ void __launch_bounds__(kI8PlaceThreads) i8_places(const __grid_constant__ I8Params p) {
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const int2 live = i8_live(p);
+    if (threadIdx.x == 0 && (p.offsets[0] < 0 || p.offsets[p.experts] > p.rows))
+        report(p.status, kSiteOffsets);  // before the src that such offsets reach
+    for (int64_t r = live.x + int64_t(blockIdx.x) * kI8PlaceThreads + threadIdx.x; r < live.y; r += int64_t(gridDim.x) * kI8PlaceThreads) {
+        const int s = p.src[r];
+        if (s >= 0 && s < p.slots) {
+            p.inv[s] = int(r);
+        } else {
+            report(p.status, kSiteSrc);
+            p.xq_scales[r] = 0.0f;
+        }
+    }
+}
+template <class T> __global__ void __launch_bounds__(512) i8_token_rows(const __grid_constant__ I8Params p) {
+    __shared__ uint32_t part[2][16];
+    __shared__ int places[2][kI8TokenPlaces + 1];  // and their number
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();  // as i8_rows
+    const int2 live = i8_live(p);
+    const int tid = threadIdx.x;
+    int turn = 0;
+    auto row = [&](int64_t t, auto &&find) {
+        int *place = places[turn];
+        if (p.x_scales) {
+            const uint4 *from = reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(p.x) + t * p.k);
+            const int pieces = p.k / 16;
+            uint4 v[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (tid + i * int(blockDim.x) < pieces)
+                    v[i] = __ldg(from + tid + i * int(blockDim.x));
+            find(place);
+            __syncthreads();
+            const int n = place[kI8TokenPlaces];
+            for (int j = 0; j < n; ++j) {
+                uint4 *to = reinterpret_cast<uint4 *>(p.xq + int64_t(place[j]) * p.k);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (tid + i * int(blockDim.x) < pieces)
+                        to[tid + i * int(blockDim.x)] = v[i];
+                for (int i = tid + 2 * int(blockDim.x); i < pieces; i += blockDim.x)
+                    to[i] = __ldg(from + i);
+                if (tid == 0)
+                    p.xq_scales[place[j]] = __ldg(p.x_scales + t);
+            }
+        } else {
+            quant_row<T>(static_cast<const uint8_t *>(p.x) + t * p.k * int64_t(sizeof(T)), p.k / 8, part[turn], [&] { find(place); }, [&](float scale) {
+                const int n = place[kI8TokenPlaces];
+                if (tid == 0)
+                    for (int j = 0; j < n; ++j)
+                        p.xq_scales[place[j]] = scale;
+                return [&p, place, n](int at, int vecs, uint2 v) {
+                    for (int j = 0; j < n; ++j)
+                        Vec8<T>::stg_q(p.xq + int64_t(place[j]) * p.k, at, vecs, v);
+                };
+            });
+        }
+        turn ^= 1;
+    };
+    const int64_t tokens = p.slots / p.top_k;
+    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x)
+        row(t, [&](int *place) {
+            if (tid >= 32)
+                return;
+            bool there = false;
+            int r = 0;
+            if (tid < p.top_k) {
+                const int s = int(t) * p.top_k + tid;
+                r = p.inv[s];
+                there = r >= live.x && r < live.y && p.src[r] == s;
+            }
+            const unsigned all = __ballot_sync(0xffffffffu, there);
+            if (there)
+                place[__popc(all & ((1u << tid) - 1u))] = r;
+            if (tid == 0)
+                place[kI8TokenPlaces] = __popc(all);
+        });
+    // places whose slot another one has, too
+    for (int64_t base = live.x + int64_t(blockIdx.x) * blockDim.x; base < live.y; base += int64_t(gridDim.x) * blockDim.x) {
+        const int64_t mine = base + tid;
+        bool alone = true;
+        if (mine < live.y) {
+            const int s = p.src[mine];
+            alone = s < 0 || s >= p.slots || p.inv[s] == int(mine);
+        }
+        if (!__syncthreads_or(!alone))
+            continue;
+        for (int64_t r = base; r < min(base + blockDim.x, int64_t(live.y)); ++r) {
+            const int s = p.src[r];
+            if (s < 0 || s >= p.slots || p.inv[s] == int(r))
+                continue;
+            row(s / p.top_k, [&](int *place) {
+                if (tid == 0) {
+                    place[0] = int(r);
+                    place[kI8TokenPlaces] = 1;
+                }
+            });
+        }
+        __syncthreads();
     }
 }
 

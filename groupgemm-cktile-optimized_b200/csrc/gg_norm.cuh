@@ -243,9 +243,10 @@ struct QuantParams {
 };
 
 // One row by a block: up to kQuantHeld vectors a thread stay in registers between the largest magnitude and the rounding, what is
-// longer is read again. part: 16 words of shared memory, other ones for the next row.
+// longer is read again. part: 16 words of shared memory, other ones for the next row. before() runs before the block's one barrier, then
+// to(scale) says where rows go: what it returns takes (vec, vecs, eight integers).
 constexpr int kQuantHeld = 4;
-template <class T> __device__ __forceinline__ void quant_row(const void *row, int8_t *to, float *scale_to, int vecs, uint32_t *part) {
+template <class T, class B, class S> __device__ __forceinline__ void quant_row(const void *row, int vecs, uint32_t *part, B &&before, S &&to) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
     Vec8<T> v[kQuantHeld];
     uint32_t top = 0;
@@ -255,6 +256,7 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
         if (at < vecs)
             v[i].ldg(row, at, vecs);
     }
+    before();
 #pragma unroll
     for (int i = 0; i < kQuantHeld; ++i)
         if (tid + i * int(blockDim.x) < vecs)
@@ -270,15 +272,14 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
     __syncthreads();  // a warp writes these words again only after the next row's barrier
     top = __reduce_max_sync(0xffffffffu, lane < warps ? part[lane] : 0u);
     const Rounding by(top);
-    if (tid == 0)
-        *scale_to = Rounding::scale(top);
+    auto store = to(tid == 0 ? Rounding::scale(top) : 0.0f);
 #pragma unroll
     for (int i = 0; i < kQuantHeld; ++i) {
         const int at = tid + i * int(blockDim.x);
         if (at < vecs) {
             pair_t f[4];
             v[i].get(f);
-            Vec8<T>::stg_q(to, at, vecs, by(f));
+            store(at, vecs, by(f));
         }
     }
     for (int at = tid + kQuantHeld * int(blockDim.x); at < vecs; at += blockDim.x) {
@@ -286,8 +287,16 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
         pair_t f[4];
         u.ldg(row, at, vecs);
         u.get(f);
-        Vec8<T>::stg_q(to, at, vecs, by(f));
+        store(at, vecs, by(f));
     }
+}
+// To one place.
+template <class T> __device__ __forceinline__ void quant_row(const void *row, int8_t *q, float *scale_to, int vecs, uint32_t *part) {
+    quant_row<T>(row, vecs, part, [] {}, [&](float scale) {
+        if (threadIdx.x == 0)
+            *scale_to = scale;
+        return [=](int at, int n, uint2 v) { Vec8<T>::stg_q(q, at, n, v); };
+    });
 }
 
 // A block a row (and every gridDim.x-th after it).

@@ -255,7 +255,10 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
         chunk /= 2;
     const bool order = q.rows > 0 && (q.src || !q.x_scales);  // rows are put into expert order or rounded first
     const size_t sums = 2 * size_t(pairs) * size_t(chunk) * 1024, rounded = order ? size_t(q.rows) * size_t(q.k) : 0;
-    if (const int rc = reserve(h, sums + rounded + (order ? size_t(q.rows) * 4 : 0)))
+    // By tokens where a token has several places and there is more to move than the launch before costs: us by places / by tokens, 1024 x 8 rows
+    // of 7168 291 / 293, 2048 x 8 of 4096 97.5 / 96.8, 16384 x 2 of 7168 777 / 734 (with the products).
+    const bool by_token = order && q.src && q.top_k >= 2 && q.top_k <= kI8TokenPlaces && q.rows * q.k >= int64_t(1) << 23;
+    if (const int rc = reserve(h, sums + rounded + (order ? size_t(q.rows) * 4 : 0) + (by_token ? size_t(q.tokens) * size_t(q.top_k) * 4 : 0)))
         return rc;
     if (const int rc = reserve_counters(h, size_t(pairs) * 2 * kI8EpilogueWarps * 4, stream))
         return rc;
@@ -264,6 +267,7 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     p.x_scales = q.x_scales;
     p.xq = order ? reinterpret_cast<int8_t *>(h->d_ws) + sums : static_cast<int8_t *>(const_cast<void *>(q.x));
     p.xq_scales = order ? reinterpret_cast<float *>(p.xq + rounded) : const_cast<float *>(q.x_scales);
+    p.inv = by_token ? reinterpret_cast<int32_t *>(p.xq_scales + q.rows) : nullptr;
     p.scales = q.scales;
     p.offsets = q.offsets;
     p.src = q.src;
@@ -296,14 +300,19 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     const bool half = q.dtype == GG_FP16;
     const void *fn = half ? i8_products_fn<__half>(mean <= 128) : i8_products_fn<__nv_bfloat16>(mean <= 128);
     GG_CUDA(h, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8Smem));
-    const MoeLaunch rows{half ? reinterpret_cast<const void *>(&i8_rows<__half>) : reinterpret_cast<const void *>(&i8_rows<__nv_bfloat16>),
-                         order ? unsigned(std::min<int64_t>(q.rows, 32 * num_sms)) : 0u, quant_threads(q.rows, q.x_scales ? q.k / 2 : q.k, num_sms), 0};
+    const void *rows_fn = by_token ? (half ? reinterpret_cast<const void *>(&i8_token_rows<__half>) : reinterpret_cast<const void *>(&i8_token_rows<__nv_bfloat16>))
+                                   : (half ? reinterpret_cast<const void *>(&i8_rows<__half>) : reinterpret_cast<const void *>(&i8_rows<__nv_bfloat16>));
+    const int64_t sources = by_token ? q.tokens : q.rows;
+    const MoeLaunch places{reinterpret_cast<const void *>(&i8_places),
+                           by_token ? unsigned(std::min<int64_t>((q.rows + kI8PlaceThreads - 1) / kI8PlaceThreads, 8 * num_sms)) : 0u, kI8PlaceThreads, 0};
+    const MoeLaunch rows{rows_fn, order ? unsigned(std::min<int64_t>(sources, 32 * num_sms)) : 0u,
+                         quant_threads(sources, q.x_scales ? q.k / 2 : q.k, num_sms), 0};
     MoeLaunch products{fn, q.rows > 0 ? unsigned(2 * pairs) : 0u, kI8Threads, size_t(kI8Smem), 2};
     products.cluster = 2;
     char detail[160];
     std::snprintf(detail, sizeof(detail), "gg_i8<%s> n=%lld k=%lld chunk=%d stages=%d pairs=%d", type_name(q.dtype), static_cast<long long>(q.n),
                   static_cast<long long>(q.k), chunk, p.stages, pairs);
-    return finish(h, stream, {rows, products}, detail);
+    return finish(h, stream, {places, rows, products}, detail);
 }
 
 }  // namespace

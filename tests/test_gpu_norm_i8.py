@@ -437,6 +437,50 @@ def test_i8(gg, counts, n, k, kind, top_k, extra, eight):
     assert torch.equal(first.view(torch.int16), out.t.view(torch.int16))
 
 
+@pytest.mark.parametrize("kind,top_k,eight", [("bf16", 2, False), ("fp16", 2, True), ("bf16", 7, True), ("fp16", 32, False), ("bf16", 1, False)])
+def test_i8_rows_by_tokens(gg, kind, top_k, eight):
+    """Enough rows that each token is rounded once for all its places: with tokens that have none or some of them, and in further runs, whose
+    routing the places of the run before do not fit: one that names slots twice, one with entries that are no slots."""
+    torch = _torch()
+    counts = [3000, 0, 1100, 77]
+    c = i8_case(torch, counts, 264, 2064, kind, top_k, 300, eight)
+    assert c["rows"] * c["k"] >= 1 << 23
+    out, b = run_i8(gg, torch, c)
+    check_i8(torch, c, out.t)
+    stream = torch.cuda.current_stream().cuda_stream
+    src = c["src"].clone()
+    for change in ("other", "fewer", "twice", "bad"):
+        if change == "other":
+            c["src"].copy_(torch.randperm(c["tokens"] * top_k, device="cuda")[: c["rows"]].int())
+        elif change == "fewer":
+            c["counts"] = [500, 40, 0, 0]
+            c["offsets"].copy_(torch.tensor([0, 500, 540, 540, 540], dtype=torch.int32))
+            c["src"][540:] = -1
+        elif change == "twice":
+            c["counts"] = counts
+            c["offsets"].copy_(torch.tensor(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)))
+            c["src"].copy_(src)
+            c["src"][5:4000:7] = c["src"][4:3999:7]
+            c["src"][100:140] = c["src"][99]
+        else:
+            c["src"].copy_(src)
+            c["src"][17], c["src"][3100] = -9, c["tokens"] * top_k
+        out.t.fill_(3)
+        b.run(stream)
+        assert b.device_status(stream) == (0x2011 if change == "bad" else 0)
+        if change == "bad":
+            assert (out.t[17] == 0).all() and (out.t[3100] == 0).all()
+            c["src"][17] = c["src"][3100] = 0  # what the reference takes for them is not compared
+            keep = out.t.clone()
+            ref_rows = torch.ones(c["rows"], dtype=torch.bool, device="cuda")
+            ref_rows[17] = ref_rows[3100] = False
+            c["src"].copy_(src)
+            b.run(stream)
+            torch.cuda.synchronize()
+            assert torch.equal(out.t[ref_rows], keep[ref_rows])
+        check_i8(torch, c, out.t)
+
+
 def test_i8_largest_sums(gg):
     """All factors -128 at the longest k: the sum is 2^31 less one factor's share, and still exact."""
     torch = _torch()
