@@ -10,7 +10,12 @@ and wgrad -> dispatch's gradient, router's gradient. The grouped GEMM takes its 
 ServingLayer: route -> 4-bit products (which gather the tokens themselves) -> combine. Nothing comes
 back to the host and nothing is allocated, so a step can be captured in a CUDA graph.
 
-quantize_w4() makes the 4-bit weights that gg_prepare_w4 reads from 16- or 32-bit ones.
+ServingLayerI8: the same over 8-bit experts, for any number of tokens: norm (its 8-bit rows are the products' input) -> route -> 8-bit
+products -> combine.
+
+Norm: the layer norm in front of a TrainingLayer, forward and backward, with the residual that it is added to.
+
+quantize_w4() and quantize_i8() make the 4- and 8-bit weights that gg_prepare_w4 and gg_prepare_i8 read from 16- or 32-bit ones.
 
     python moe_layer.py        one training step and one serving step on the GPU, checked against plain torch
 """
@@ -93,6 +98,99 @@ def quantize_w4(w: torch.Tensor, group: int, symmetric: bool = True):
     q = q.view(e, n, groups * group)[:, :, :k]
     packed = (q[:, :, 0::2] | (q[:, :, 1::2] << 4)).contiguous()
     return packed, scales.contiguous(), None if symmetric else zero.to(torch.uint8).contiguous()
+
+
+def quantize_i8(w: torch.Tensor):
+    """w [experts, n, k] in 16 or 32 bits, on the GPU -> (weight int8 of the same shape, scales [experts, n] in fp32): each row rounded to
+    the nearest of 255 values (gg_prepare_quant)."""
+    e, n, k = w.shape
+    w = _check("w", w, (e, n, k), *LOGITS).contiguous()
+    weight = torch.empty(e, n, k, dtype=torch.int8, device=w.device)
+    scales = torch.empty(e, n, dtype=torch.float32, device=w.device)
+    gg = load_package()
+    b = gg.make_b200_backend()
+    _ready(b.prepare_quant(_dtype(gg, w.dtype), e * n, k, _ptr(w), _ptr(weight), _ptr(scales), stream=_stream()))
+    b.run(_stream())
+    torch.cuda.current_stream().synchronize()  # the handle goes
+    return weight, scales
+
+
+class Norm:
+    """The layer norm in front of a layer, forward and backward, with weight and bias `gamma` and `beta` [hidden] (None: 1 and 0), in the
+    tokens' type or fp32. The tensors of a step may have any strides: what is not contiguous is copied first. check() as TrainingLayer's."""
+
+    def __init__(self, gamma: torch.Tensor | None, beta: torch.Tensor | None, eps: float = 1e-5):
+        types = set()
+        for name, v in (("gamma", gamma), ("beta", beta)):
+            if v is not None:
+                if not _check(name, v, tuple(getattr(v, "shape", ()))[:1], *LOGITS).is_contiguous():
+                    raise ValueError(f"{name} must be contiguous")
+                types.add(v.dtype)
+        if len(types) > 1:
+            raise ValueError("gamma and beta must be of one type")
+        self.gg = load_package()
+        self.gamma, self.beta, self.eps, self.params = gamma, beta, eps, next(iter(types), None)
+        self.backends = {name: self.gg.make_b200_backend() for name in ("norm", "norm_grad")}
+        self.sum = None
+
+    def check(self) -> None:
+        """Waits for the current stream and raises if a kernel of the last forward or backward reported an error."""
+        s = _stream()
+        bad = [f"{name}: {b.last_error()}" for name, b in self.backends.items() if b.device_status(s)]
+        if bad:
+            raise RuntimeError("; ".join(bad))
+
+    def _run(self, name: str, prepare: str, *args, **kw) -> None:
+        b, s = self.backends[name], _stream()
+        _ready(getattr(b, prepare)(*args, stream=s, **kw))
+        b.run(s)
+
+    def _types(self, x: torch.Tensor) -> tuple[int, int]:
+        t = _dtype(self.gg, x.dtype)
+        if self.params not in (None, x.dtype, torch.float32):
+            raise ValueError(f"gamma and beta must be {x.dtype} or torch.float32, not {self.params}")
+        return t, _dtype(self.gg, self.params or x.dtype)
+
+    def _hidden(self, x: torch.Tensor) -> tuple[int, int]:
+        t, h = x.shape
+        for name, v in (("gamma", self.gamma), ("beta", self.beta)):
+            if v is not None:
+                _check(name, v, (h,), self.params)
+        return t, h
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """x [tokens, hidden] -> (y, x + residual): y is the norm of the second, which goes past the layer (x itself without a residual)."""
+        t, h = self._hidden(x)
+        x = _check("x", x, (t, h), *LOGITS).contiguous()
+        dt, pt = self._types(x)
+        total = x
+        if residual is not None:
+            residual = _check("residual", residual, (t, h), x.dtype).contiguous()
+            total = torch.empty_like(x)
+        y = torch.empty_like(x)
+        self.mean, self.rstd = (torch.empty(t, dtype=torch.float32, device=x.device) for _ in range(2))
+        self._run("norm", "prepare_norm", dt, t, h, _ptr(x), _ptr(y), gamma_ptr=_ptr(self.gamma), beta_ptr=_ptr(self.beta), param_type=pt,
+                  residual_ptr=_ptr(residual), sum_ptr=_ptr(total) if residual is not None else 0, mean_ptr=_ptr(self.mean),
+                  rstd_ptr=_ptr(self.rstd), eps=self.eps)
+        self.sum = total
+        return y, total
+
+    def backward(self, dy: torch.Tensor, dsum: torch.Tensor | None = None):
+        """(dx, dgamma, dbeta) of the last forward, for dy [tokens, hidden] and the gradient that reaches the sum past the layer. dx is the
+        residual's gradient, too; dgamma and dbeta [hidden] are fp32."""
+        if self.sum is None:
+            raise ValueError("backward needs a forward before it")
+        x = self.sum
+        t, h = x.shape
+        dy = _check("dy", dy, (t, h), x.dtype).contiguous()
+        if dsum is not None:
+            dsum = _check("dsum", dsum, (t, h), x.dtype).contiguous()
+        dx = torch.empty_like(x)
+        dgamma, dbeta = (torch.empty(h, dtype=torch.float32, device=x.device) for _ in range(2))
+        dt, pt = self._types(x)
+        self._run("norm_grad", "prepare_norm_grad", dt, t, h, _ptr(x), _ptr(self.mean), _ptr(self.rstd), _ptr(dy), _ptr(dx),
+                  gamma_ptr=_ptr(self.gamma), param_type=pt, dsum_ptr=_ptr(dsum), dgamma_ptr=_ptr(dgamma), dbeta_ptr=_ptr(dbeta))
+        return dx, dgamma, dbeta
 
 
 class Router:
@@ -249,6 +347,70 @@ class ServingLayer:
         return self.y
 
 
+class ServingLayerI8:
+    """One layer for up to a fixed number of tokens a step, over 8-bit experts `weight` [experts, n, k] with `scales` [experts, n]; all buffers
+    and handles are made here. With gamma and beta [k] the layer norm is a part of it: norm() makes `normed` (and the products' 8-bit rows) of
+    `x`, and of x + `residual` in `sum`; the caller forms `logits` of it; then run(). Without them, run() rounds x itself."""
+
+    def __init__(self, weight: torch.Tensor, scales: torch.Tensor, tokens: int, top_k: int, dtype: torch.dtype = torch.bfloat16,
+                 gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None, eps: float = 1e-5, residual: bool = False,
+                 logits_dtype: torch.dtype = torch.float32, normalize: bool = True):
+        gg = load_package()
+        e, n, k = weight.shape
+        dev = weight.device
+        _check("weight", weight, (e, n, k), torch.int8)
+        _check("scales", scales, (e, n), torch.float32)
+        if dtype not in HALF:
+            raise ValueError(f"dtype must be {HALF[0]} or {HALF[1]}, not {dtype}")
+        if (gamma is None) != (beta is None):
+            raise ValueError("gamma and beta go together")
+        if residual and gamma is None:
+            raise ValueError("a residual needs gamma and beta")
+        self.keep = (weight, scales, gamma, beta)
+        self.x = torch.zeros(tokens, k, dtype=dtype, device=dev)
+        self.residual = torch.zeros_like(self.x) if residual else None
+        self.mask = torch.zeros(tokens, dtype=torch.uint8, device=dev)  # places without a token
+        self.logits = torch.zeros(tokens, e, dtype=logits_dtype, device=dev)
+        self.rows = torch.empty(tokens * top_k, n, dtype=dtype, device=dev)
+        self.y = torch.empty(tokens, n, dtype=dtype, device=dev)
+        self.router = r = Router(self.logits, top_k, self.mask, normalize, losses=False)
+        dt, s = _dtype(gg, dtype), _stream()
+        self.norms = self.normed = self.sum = None
+        rows_in, rows_scales = self.x, None
+        if gamma is not None:
+            for name, v in (("gamma", gamma), ("beta", beta)):
+                if not _check(name, v, (k,), dtype, torch.float32).is_contiguous() or v.dtype != gamma.dtype:
+                    raise ValueError("gamma and beta must be contiguous and of one type")
+            self.norms, self.normed = gg.make_b200_backend(), torch.empty_like(self.x)
+            self.sum = torch.empty_like(self.x) if residual else self.x
+            rows_in, rows_scales = torch.empty(tokens, k, dtype=torch.int8, device=dev), torch.empty(tokens, dtype=torch.float32, device=dev)
+            self.rounded = (rows_in, rows_scales)
+            _ready(self.norms.prepare_norm(dt, tokens, k, _ptr(self.x), _ptr(self.normed), gamma_ptr=_ptr(gamma), beta_ptr=_ptr(beta),
+                                           param_type=_dtype(gg, gamma.dtype), residual_ptr=_ptr(self.residual),
+                                           sum_ptr=_ptr(self.sum) if residual else 0, q_ptr=_ptr(rows_in), q_scales_ptr=_ptr(rows_scales),
+                                           eps=eps, stream=s))
+        self.products, self.combine = gg.make_b200_backend(), gg.make_b200_backend()
+        _ready(self.products.prepare_i8(dt, e, n, k, tokens * top_k, _ptr(rows_in), _ptr(weight), _ptr(scales), _ptr(r.offsets), _ptr(self.rows),
+                                        x_scales_ptr=_ptr(rows_scales), src_ptr=_ptr(r.src), tokens=tokens, top_k=top_k, stream=s))
+        _ready(self.combine.prepare_combine(dt, tokens, top_k, e, n, _ptr(self.rows), _ptr(r.dest), _ptr(self.y),
+                                            weights_ptr=_ptr(r.weights), stream=s))
+
+    def norm(self) -> torch.Tensor:
+        """The norm of what x and residual hold, [tokens, k]."""
+        if self.norms is None:
+            raise ValueError("this layer has no norm")
+        self.norms.run(_stream())
+        return self.normed
+
+    def run(self) -> torch.Tensor:
+        """One step on what x (or the last norm), mask and logits hold; y [tokens, n], zero where mask is."""
+        s = _stream()
+        self.router.backend.run(s)
+        self.products.run(s)
+        self.combine.run(s)
+        return self.y
+
+
 def plain_layer(x, w, logits, top_k, mask=None):
     """The layer in elementary operations with autograd: (y, losses) in x's type and fp32, for normalised weights."""
     t, e = logits.shape
@@ -275,20 +437,31 @@ def main() -> None:
     dy = torch.randn(tokens, n, device="cuda").bfloat16()
     dlosses = torch.tensor([0.01, 0.001], device="cuda")
 
-    layer = TrainingLayer(w, top_k)
-    y, losses = layer.forward(x, logits, mask)
-    dx, dw, dlogits = layer.backward(dy, dlosses)
+    residual = torch.randn(tokens, k, device="cuda").bfloat16()
+    gamma, beta = 1 + 0.1 * torch.randn(k, device="cuda"), 0.1 * torch.randn(k, device="cuda")
+
+    layer, norm = TrainingLayer(w, top_k), Norm(gamma, beta)
+    normed, past = norm.forward(x, residual)
+    y, losses = layer.forward(normed, logits, mask)
+    dnormed, dw, dlogits = layer.backward(dy, dlosses)
+    dpast = torch.randn(tokens, k, device="cuda").bfloat16()
+    dx, dgamma, dbeta = norm.backward(dnormed, dpast)
     layer.check()
-    leaves = [v.double().requires_grad_() for v in (x, w)] + [logits.double().requires_grad_()]
-    py, pl = plain_layer(leaves[0], leaves[1], leaves[2], top_k, mask)
-    (torch.sum(py * dy.double()) + torch.sum(pl * dlosses.double())).backward()
+    norm.check()
+    leaves = [v.double().requires_grad_() for v in (x, w, logits, gamma, beta)]
+    total = leaves[0] + residual.double()
+    c = total - total.mean(1, keepdim=True)
+    pn = c * torch.rsqrt(c.square().mean(1, keepdim=True) + norm.eps) * leaves[3] + leaves[4]
+    py, pl = plain_layer(pn, leaves[1], leaves[2], top_k, mask)
+    (torch.sum(py * dy.double()) + torch.sum(pl * dlosses.double()) + torch.sum(total * dpast.double())).backward()
     def far(a, b):
         d = ((a.double() - b.double()).norm() / b.double().norm()).item()
-        assert d < 2e-2, d  # five roundings to bf16
+        assert d < 2e-2, d  # seven roundings to bf16
         return d
 
-    print("training: y %.2g losses %.2g dx %.2g dw %.2g dlogits %.2g (relative to 64 bits)" % (
-        far(y, py), far(losses, pl), far(dx, leaves[0].grad), far(dw, leaves[1].grad), far(dlogits, leaves[2].grad)))
+    print("training: y %.2g losses %.2g dx %.2g dw %.2g dlogits %.2g dgamma %.2g dbeta %.2g (relative to 64 bits)" % (
+        far(y, py), far(losses, pl), far(dx, leaves[0].grad), far(dw, leaves[1].grad), far(dlogits, leaves[2].grad),
+        far(dgamma, leaves[3].grad), far(dbeta, leaves[4].grad)))
 
     q, scales, zeros = quantize_w4(w, group)
     serve = ServingLayer(q, scales, zeros, group, 16, top_k)
@@ -298,6 +471,13 @@ def main() -> None:
     nibbles = torch.stack([q & 15, q >> 4], 3).view(e, n, k).double() - 8
     py, _ = plain_layer(x[:16].double(), nibbles * scales.double().repeat_interleave(group, 2), logits[:16].double(), top_k)
     print("serving: y %.2g (relative to 64 bits on the same 4-bit weights)" % far(serve.run(), py))
+
+    weight, scales = quantize_i8(w)
+    serve = ServingLayerI8(weight, scales, tokens, top_k, gamma=gamma, beta=beta, residual=True)
+    for to, v in ((serve.x, x), (serve.residual, residual), (serve.mask, mask), (serve.logits, logits)):
+        to.copy_(v)
+    py, _ = plain_layer(serve.norm().double(), weight.double() * scales.double()[..., None], logits.double(), top_k, mask)
+    print("serving: y %.2g (relative to 64 bits on the same 8-bit weights)" % far(serve.run(), py))
 
 
 if __name__ == "__main__":
