@@ -332,7 +332,7 @@ __device__ __forceinline__ float2 each_half_sum(float v) {
 // ---- rows through a ring in shared memory ----
 
 // A group of warps of a block, its ring of rows and its barrier. All threads of a group take the same steps; a wait that gives up is
-// recorded and the group goes on without waiting or storing, so that its barriers stay matched.
+// recorded and the group goes on without waiting, so that its barriers stay matched.
 template <int kTensors> struct RowRing {
     uint32_t base, bars;
     uint32_t row_bytes;
@@ -459,10 +459,11 @@ template <class T, class W, int V> struct NormParam {
     }
 };
 
+// kFull: every thread has V vectors, so that none asks for each.
 // Mean and variance without cancellation: each warp its own mean m_w and the squares S_w around it, joined around the first warp's mean, t_w = m_w - m_0:
 //   mean = m_0 + sum n_w t_w / n     sum (v - mean)^2 = sum (S_w + n_w t_w^2) - n (mean - m_0)^2
 // where what is taken off is at most the sum of the others' n_w t_w^2, so that no more than a factor of the number of warps is lost.
-template <class T, class W, int V>
+template <class T, class W, int V, bool kFull>
 __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_constant__ NormParams p) {
     extern __shared__ __align__(1024) uint8_t norm_smem[];
     __shared__ uint64_t bars[kNormMaxGroups * kNormMaxSlots];
@@ -501,14 +502,14 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
-            if (at < p.vecs) {
+            if (kFull || at < p.vecs) {
                 Vec8<T> x;
                 x.lds(g.at(slot, 0), at, p.vecs);
                 if (p.residual) {
                     Vec8<T> more;
                     more.lds(g.at(slot, 1), at, p.vecs);
                     x.add(more);
-                    if (p.sum && g.ok)
+                    if (p.sum)
                         x.stg(static_cast<uint8_t *>(p.sum) + row, at, p.vecs);
                 }
                 x.get(f[v]);
@@ -522,7 +523,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
         pair_t squared = 0;
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            if (g.tid + v * g.threads < p.vecs)
+            if (kFull || g.tid + v * g.threads < p.vecs)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const pair_t d = add2(f[v][i], minus_warp);
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
-            if (at < p.vecs) {
+            if (kFull || at < p.vecs) {
                 pair_t a[4], b[4];
                 gamma.get(v, at, a);
                 beta.get(v, at, b);
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
                 for (int i = 0; i < 4; ++i)
                     f[v][i] = fma2(fma2(f[v][i], both_rstd, minus), a[i], b[i]);
                 y[v].set(f[v]);
-                if (p.y && g.ok)
+                if (p.y)
                     y[v].stg(static_cast<uint8_t *>(p.y) + row, at, p.vecs);
                 if (p.q)
                     top = y[v].top(top);
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const int at = g.tid + v * g.threads;
-                if (at < p.vecs && g.ok) {
+                if (kFull || at < p.vecs) {
                     pair_t a[4];
                     y[v].get(a);  // the integers are of y as it is written
                     Vec8<T>::stg_q(p.q + r * p.vecs * 8, at, p.vecs, by(a));
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
 // The gradients: a block's sums of dgamma and dbeta stay in registers over its rows, its groups' are added in order, and each block
 // leaves its sums for norm_grad_sum. A row is read from its slot twice, before and after the sums along it, so that the registers hold
 // those sums only; so a slot is loaded again one row later, when the next row's barrier shows that all are past it.
-template <class T, class W, int V>
+template <class T, class W, int V, bool kFull>
 __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_constant__ NormGradParams p) {
     extern __shared__ __align__(1024) uint8_t norm_smem[];
     __shared__ uint64_t bars[kNormMaxGroups * kNormMaxSlots];
@@ -637,7 +638,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
-            if (at < p.vecs) {
+            if (kFull || at < p.vecs) {
                 Vec8<T> x, dy;
                 pair_t a[4], b[4], w[4];
                 x.lds(g.at(slot, 0), at, p.vecs);
@@ -668,7 +669,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
-            if (at < p.vecs) {
+            if (kFull || at < p.vecs) {
                 Vec8<T> x, dy;
                 pair_t a[4], b[4], w[4];
                 x.lds(g.at(slot, 0), at, p.vecs);
@@ -687,8 +688,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
                         a[i] = add2(a[i], b[i]);
                 }
                 x.set(a);
-                if (g.ok)
-                    x.stg(static_cast<uint8_t *>(p.dx) + r * g.row_bytes, at, p.vecs);
+                x.stg(static_cast<uint8_t *>(p.dx) + r * g.row_bytes, at, p.vecs);
             }
         }
         if (g.slots == 1) {
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
-            if (at < p.vecs)
+            if (kFull || at < p.vecs)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     of_group(g.group - 1, 0, at)[i] = make_ulonglong2(dgamma[v][2 * i], dgamma[v][2 * i + 1]);
@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int at = g.tid + v * g.threads;
-        if (at >= p.vecs)
+        if (!kFull && at >= p.vecs)
             continue;
         for (int o = 0; o < p.groups - 1; ++o)
 #pragma unroll

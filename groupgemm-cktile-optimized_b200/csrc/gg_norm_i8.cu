@@ -23,6 +23,7 @@ using gg::moe::kNormThreads;
 
 struct NormShape {
     int v;  // vectors a thread
+    bool full;
     int warps, groups, slots, params_at;
     unsigned blocks;
     size_t smem;
@@ -33,6 +34,7 @@ NormShape norm_shape(int64_t rows, int vecs, int v, int tensors, int elem, int p
     NormShape s{};
     s.v = v;
     s.warps = (vecs + 32 * s.v - 1) / (32 * s.v);
+    s.full = vecs == 32 * s.v * s.warps;
     const int64_t each = (rows + num_sms - 1) / num_sms;  // rows of a block
     s.groups = int(std::max<int64_t>(1, std::min<int64_t>({each, kNormThreads / (32 * s.warps), kNormMaxGroups})));
     const size_t row = size_t(vecs) * 8 * size_t(elem) * size_t(tensors);
@@ -51,11 +53,16 @@ NormShape norm_shape(int64_t rows, int vecs, int v, int tensors, int elem, int p
     return s;
 }
 
-template <class T, class W, int V> const void *norm_fn(bool grad) {
-    return grad ? reinterpret_cast<const void *>(&gg::moe::norm_grad_rows<T, W, V>) : reinterpret_cast<const void *>(&gg::moe::norm_rows<T, W, V>);
+template <class T, class W, int V, bool kFull> const void *norm_fn(bool grad) {
+    return grad ? reinterpret_cast<const void *>(&gg::moe::norm_grad_rows<T, W, V, kFull>)
+                : reinterpret_cast<const void *>(&gg::moe::norm_rows<T, W, V, kFull>);
 }
 template <class T, class W> const void *norm_fn(const NormShape &s, bool grad) {
-    return s.v == 1 ? norm_fn<T, W, 1>(grad) : s.v == 2 ? norm_fn<T, W, 2>(grad) : norm_fn<T, W, 4>(grad);
+    if (s.v == 1)
+        return norm_fn<T, W, 1, false>(grad);
+    if (s.v == 2)
+        return s.full ? norm_fn<T, W, 2, true>(grad) : norm_fn<T, W, 2, false>(grad);
+    return s.full ? norm_fn<T, W, 4, true>(grad) : norm_fn<T, W, 4, false>(grad);
 }
 const void *norm_fn(const NormShape &s, int dtype, int param_type, bool grad) {
     if (dtype == GG_F32)
