@@ -34,7 +34,7 @@ NormShape norm_shape(int64_t rows, int vecs, int v, int tensors, int elem, int p
     NormShape s{};
     s.v = v;
     s.warps = (vecs + 32 * s.v - 1) / (32 * s.v);
-    s.full = vecs == 32 * s.v * s.warps;
+    s.full = s.v > 2 && vecs == 32 * s.v * s.warps;
     const int64_t each = (rows + num_sms - 1) / num_sms;  // rows of a block
     s.groups = int(std::max<int64_t>(1, std::min<int64_t>({each, kNormThreads / (32 * s.warps), kNormMaxGroups})));
     const size_t row = size_t(vecs) * 8 * size_t(elem) * size_t(tensors);
@@ -61,7 +61,7 @@ template <class T, class W> const void *norm_fn(const NormShape &s, bool grad) {
     if (s.v == 1)
         return norm_fn<T, W, 1, false>(grad);
     if (s.v == 2)
-        return s.full ? norm_fn<T, W, 2, true>(grad) : norm_fn<T, W, 2, false>(grad);
+        return norm_fn<T, W, 2, false>(grad);
     return s.full ? norm_fn<T, W, 4, true>(grad) : norm_fn<T, W, 4, false>(grad);
 }
 const void *norm_fn(const NormShape &s, int dtype, int param_type, bool grad) {
@@ -143,7 +143,7 @@ int prepare_norm_grad(gg_handle *h, const gg_norm_grad_problem &q, gg_stream_t s
     int num_sms = 0;
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
-    const int vecs = int(q.hidden / 8), v = vecs <= 64 ? 1 : vecs <= 1024 ? 2 : 4;
+    const int vecs = int(q.hidden / 8), v = vecs <= 64 ? 1 : vecs <= 512 ? 2 : 4;
     const NormShape s = norm_shape(q.tokens, vecs, v, q.dsum ? 3 : 2, q.dtype == GG_F32 ? 4 : 2, 1, q.param_type == GG_F32 ? 4 : 2, 160 << 10, num_sms);
     const size_t sums = 2 * size_t(q.hidden) * 4;  // dgamma and dbeta of a block or group
     if (const int rc = reserve(h, std::max<size_t>(1, s.blocks) * sums))
