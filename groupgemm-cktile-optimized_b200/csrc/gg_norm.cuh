@@ -552,8 +552,8 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
         }
         uint32_t top = 0;
         Vec8<T> y[V];
-        // (s - mean) rstd as s rstd - mean rstd: off by a rounding of mean rstd, as the mean's own rounding makes it
-        const pair_t minus = pair(-mean * rstd, -mean * rstd), both_rstd = pair(rstd, rstd);
+        // (s rstd - mean rstd would be one operation less, but off by a rounding of mean rstd: rows of one value would not give beta)
+        const pair_t minus_mean = pair(-mean, -mean), both_rstd = pair(rstd, rstd);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
                 beta.get(v, at, b);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    f[v][i] = fma2(fma2(f[v][i], both_rstd, minus), a[i], b[i]);
+                    f[v][i] = fma2(mul2(add2(f[v][i], minus_mean), both_rstd), a[i], b[i]);
                 y[v].set(f[v]);
                 if (p.y)
                     y[v].stg(static_cast<uint8_t *>(p.y) + row, at, p.vecs);
@@ -749,7 +749,8 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
     }
 }
 
-// Adds the blocks' sums in a fixed order: a block 32 columns, each warp every eighth part, ten of them on their way at once.
+// Adds the blocks' sums in a fixed order: a block 32 columns, each warp every eighth part. (With 10 or 19 parts on
+// their way at once it takes 0.8 to 1.7 us longer: its registers no longer fit beside the blocks whose end it waits for.)
 constexpr int kNormSumWarps = 8;
 __global__ void __launch_bounds__(kNormSumWarps * 32) norm_grad_sum(const __grid_constant__ NormGradParams p) {
     __shared__ float part[kNormSumWarps][32];
@@ -759,7 +760,7 @@ __global__ void __launch_bounds__(kNormSumWarps * 32) norm_grad_sum(const __grid
     const int col = int(blockIdx.x) * 32 + lane;  // of [2, hidden]
     float sum = 0.0f;
     if (col < 2 * hidden)
-#pragma unroll 10
+#pragma unroll 4
         for (int b = warp; b < p.blocks; b += kNormSumWarps)
             sum += __ldcg(p.parts + int64_t(b) * 2 * hidden + col);
     part[warp][lane] = sum;

@@ -7,7 +7,7 @@ Whole numbers have to be equal. Tolerances for computed values, u = 2^-24 (one f
   rstd               half of var's relative error: 48 u of the sum of squares, and 2 * 48 u A / sigma from the means' errors
   y                  |gamma| rstd (mean's error + u |s - mean|) + |y - beta| (rstd's error + 4 u) + 2 u |y|
   dx                 rstd (48 u mean|d| + |c| 48 u mean|d c| + 6 u (|d| + |level| + |c along|)) + 2 u |dx|
-  sums over tokens   a group's rows one after the other, up to 15 groups, 19 of a block's eighth, 8 warps, 4 of a term:
+  sums over tokens   a group's rows one after the other, up to 14 groups, 19 of a block's eighth, 8 warps, 4 of a term:
                      (tokens / 148 + 48) u of the sum of magnitudes
   8-bit products     the whole sum exact, then its rounding and two products: 3 u
 and half a unit in the last place where the output has 16 bits (u where it has 32).
@@ -166,6 +166,34 @@ def test_norm_in_place(gg, into):
     assert torch.equal(target, want) and torch.equal(y, y0)
     run(gg, torch, "norm", gg.BF16, 1500, 1024, want.data_ptr(), want.data_ptr())
     assert torch.equal(want, y0)
+
+
+@pytest.mark.parametrize("hidden", [64, 520, 7168])
+def test_norm_of_rows_of_one_value_is_beta(gg, hidden):
+    """Whatever the value (small whole numbers: their sums are exact), to the last bit."""
+    torch = _torch()
+    x = torch.arange(-40, 40, device="cuda").float()[:, None].expand(80, hidden).bfloat16().contiguous()
+    beta = torch.randn(hidden, device="cuda").bfloat16()
+    y, mean = torch.empty_like(x), torch.empty(80, device="cuda")
+    run(gg, torch, "norm", gg.BF16, 80, hidden, x.data_ptr(), y.data_ptr(), beta_ptr=beta.data_ptr(), mean_ptr=mean.data_ptr())
+    assert torch.equal(mean, x[:, 0].float()) and torch.equal(y, beta.expand(80, hidden))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_norm_residual_sums_of_any_values(gg, kind):
+    """The sum is the terms' sum in 32 bits, rounded, for every pair of exponents, subnormal, infinite and NaN values among them."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(17)
+    dt = _dtype(torch, kind)
+    bits = lambda: torch.randint(-2 ** 15, 2 ** 15, (700, 2880), generator=g, device="cuda").to(torch.int16).view(dt)  # noqa: E731
+    x, res = bits(), bits()
+    res[350:] = (-x[350:].float() * (1 + 2.0 ** -9 * torch.randn(350, 2880, generator=g, device="cuda"))).to(dt)  # near cancellation
+    total, y = torch.empty_like(x), torch.empty_like(x)
+    run(gg, torch, "norm", _type(gg, kind), 700, 2880, x.data_ptr(), y.data_ptr(), residual_ptr=res.data_ptr(), sum_ptr=total.data_ptr())
+    want = (x.float() + res.float()).to(dt)
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(total), nan)
+    assert torch.equal(total[~nan].view(torch.int16), want[~nan].view(torch.int16))
 
 
 def test_no_tokens(gg):
