@@ -551,22 +551,27 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             bool store = true;
             if (pieces > 1 && group < blocks) {
                 int32_t *counter = p.counters + (first_pair * 2 + int(rank)) * kI8EpilogueWarps + warp - 2;
-                int4 *mine = slot(pair);
-#pragma unroll 1
-                for (int b = group; b < blocks; b += 2) {
-                    uint32_t r[16];
-                    tmem_ld_x16(from + uint32_t(b * 16), r);
-                    tmem_wait_ld16(r);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        __stcg(mine + b * 128 + j * 32, make_int4(int(r[4 * j]), int(r[4 * j + 1]), int(r[4 * j + 2]), int(r[4 * j + 3])));
-                }
-                __threadfence();
-                __syncwarp();
+                // Where all the others have left theirs, this warp's own sums need not leave Tensor Memory.
                 int before = 0;
                 if (lane == 0)
-                    before = atomicAdd(counter, 1);
-                store = __shfl_sync(0xffffffffu, before, 0) == pieces - 1;
+                    before = *reinterpret_cast<volatile int32_t *>(counter);
+                if (__shfl_sync(0xffffffffu, before, 0) != pieces - 1) {
+                    int4 *mine = slot(pair);
+#pragma unroll 1
+                    for (int b = group; b < blocks; b += 2) {
+                        uint32_t r[16];
+                        tmem_ld_x16(from + uint32_t(b * 16), r);
+                        tmem_wait_ld16(r);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            __stcg(mine + b * 128 + j * 32, make_int4(int(r[4 * j]), int(r[4 * j + 1]), int(r[4 * j + 2]), int(r[4 * j + 3])));
+                    }
+                    __threadfence();
+                    __syncwarp();
+                    if (lane == 0)
+                        before = atomicAdd(counter, 1);
+                    store = __shfl_sync(0xffffffffu, before, 0) == pieces - 1;
+                }
                 if (store) {
                     __threadfence();
                     if (lane == 0)
