@@ -9,8 +9,8 @@
 //
 //   i8_rows: the rows of x in expert order, rounded to 8 bits where they come in 16. (TMA gathers of four rows in the product kernel
 //   would spare it, but take 44 cycles each: a stage of 128 rows a CTA 1400 cycles, of which the products need 512.)
-//   i8_products. Work split: items (expert, token chunk, 256 weight rows). Each pair takes whole items in turn; the items that would leave
-//   pairs idle at the end (or all, where there are few) are cut along k into equal ranges of steps, one a pair, taken first. What is cut
+//   i8_products. Work split: items (expert, token chunk, 256 weight rows). Each pair takes whole items in turn; where it pays (i8_cuts), the
+//   items that would leave pairs idle at the end (or all, where there are few) are cut along k into equal ranges of steps, one a pair, taken first. What is cut
 //   leaves its sums in the workspace, and the last warp to arrive adds them up (no order to keep).
 //   Warps: 0 loads (weights and tokens, a ring of stages), 1 issues the products (of the pair's first CTA), 2-9 take the sums out of
 //   Tensor Memory, two accumulators in turn.
@@ -58,7 +58,6 @@ struct I8Params {
     int chunk;                // most tokens of a chunk, a multiple of 32
     int box;                  // rows of a token load
     int stages, stage_bytes;
-    int min_steps;            // of a cut piece
     int after_rows;           // 1: i8_rows precedes, and everything before it is done when this kernel starts
 };
 
@@ -73,17 +72,29 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, ui
                  : "memory");
 }
 
+// Whether the items that do not fill a last round of the pairs are cut along k. What it saves: of wide chunks, which the products bind, the part
+// of a round that pairs would be idle; of narrow ones, which memory binds, the part below about half, since fewer pairs at work load faster. What
+// it costs, in steps, grows with the sums that leave and come back. Us cut / whole, one token through e of 4096 x 7168 (16 e items for 74 pairs):
+// e = 5 31 / 39, 6 35 / 40, 7 39 / 40, 8 44 / 41, 9 48 / 45, 10 51 / 59, 12 59 / 60, 14 68 / 76; 256 c rows of 4096 x 4096 (16 c items): c = 5 35 / 33, 8
+// 43 / 36, 10 44 / 46, 14 56 / 58, 18 69 / 64, 20 74 / 75; of 4096 x 1024 5 26 / 17, 10 30 / 21, 20 38 / 30.
+__host__ __device__ __forceinline__ bool i8_cuts(int over, int pairs, int steps, int chunk) {
+    if (over == 0)
+        return false;
+    const int64_t cost = 4 + chunk / 8, saved = chunk <= 64 ? 55 * int64_t(pairs) - 100 * int64_t(over) : 100 * int64_t(pairs - over);
+    return saved * steps > 100 * cost * pairs;
+}
+
 // How the items of a launch are dealt out (host-callable, so that a CPU test can walk it): the first `cut` items by ranges of steps,
 // pair c's being [cut steps c / ranges, cut steps (c + 1) / ranges); then items cut + c, cut + c + pairs, ...
 struct I8Plan {
     int items, cut, ranges, pairs, steps;
     int64_t begin, end;  // this pair's range
     int c;
-    __host__ __device__ __forceinline__ I8Plan(int items_, int steps_, int min_steps, int pairs_, int c_)
+    __host__ __device__ __forceinline__ I8Plan(int items_, int steps_, int chunk, int pairs_, int c_)
         : items(items_), pairs(pairs_), steps(steps_), c(c_) {
         const int over = items % pairs;
-        cut = over == 0 ? 0 : items < pairs ? items : pairs + over;
-        const int64_t total = int64_t(cut) * steps, pieces = total / min_steps > cut ? total / min_steps : cut;
+        cut = !i8_cuts(over, pairs, steps, chunk) ? 0 : items < pairs ? items : pairs + over;
+        const int64_t total = int64_t(cut) * steps, pieces = total / kI8MinSteps > cut ? total / kI8MinSteps : cut;
         ranges = int(pieces < 1 ? 1 : pieces < pairs ? pieces : pairs);
         begin = c < ranges ? total * c / ranges : 0;
         end = c < ranges ? total * (c + 1) / ranges : 0;
@@ -400,7 +411,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     ptx::tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(slots);
     const Abort ab{p.status + 2, abort_flag, p.timeout_ns};
-    const I8Plan plan(work.items, p.steps, p.min_steps, pairs, pair);
+    const I8Plan plan(work.items, p.steps, p.chunk, pairs, pair);
 
     if (warp == 0) {
         const uint32_t issue = ptx::elect_one_sync();

@@ -295,7 +295,6 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     p.box = std::min(kI8Box, chunk / 2);
     p.stage_bytes = kI8WeightBytes + chunk / 2 * kI8StepK;
     p.stages = std::min(kI8MaxStages, kI8Ring / p.stage_bytes);
-    p.min_steps = kI8MinSteps;
     p.after_rows = order ? 1 : 0;
     if (q.rows > 0) {
         if (const int rc = encode_bytes_3d(h, h->moe.map[0], q.weight, q.k, q.n, q.experts, kI8StepK, kI8TileRows / 2, CU_TENSOR_MAP_SWIZZLE_128B))

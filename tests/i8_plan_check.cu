@@ -32,17 +32,18 @@ int main(int argc, char **argv) {
         s ^= s << 17;
         return lo + int(s % uint64_t(hi - lo + 1));
     };
-    long long pieces_seen = 0;
+    long long pieces_seen = 0, cut_seen = 0;
     for (int l = 0; l < launches; ++l) {
         const int pairs = range(0, 3) ? 74 : range(1, 80), steps = range(1, range(0, 1) ? 8 : 120);
         const int items = range(0, range(0, 1) ? 200 : 1000);
-        const int min_steps = range(1, 24);
+        const int most = 32 << range(0, 3);
         std::vector<std::vector<char>> done(items, std::vector<char>(steps, 0));
         std::map<int, std::vector<int>> owners;  // of cut items: the pairs, as they come
         std::map<int, std::pair<int, int>> told;
         std::set<int> slots;
         for (int c = 0; c < pairs; ++c) {
-            const I8Plan plan(items, steps, min_steps, pairs, c);
+            const I8Plan plan(items, steps, most, pairs, c);
+            cut_seen += plan.cut > 0 && plan.ranges > plan.cut;
             CHECK(plan.cut >= 0 && plan.cut <= items && plan.cut < 2 * pairs && plan.ranges <= pairs && (plan.ranges >= plan.cut || plan.ranges == pairs));
             plan.pieces([&](int item, int k0, int n, int first, int pieces) {
                 ++pieces_seen;
@@ -73,7 +74,7 @@ int main(int argc, char **argv) {
             for (char c : d)
                 CHECK(c);
         // chunks and item order of experts, some without rows, as a role with a stride sees them
-        const int most = 32 << range(0, 3), tiles = range(1, 40), experts = range(1, range(0, 1) ? 4 : 200), stride = range(1, 80);
+        const int tiles = range(1, 40), experts = range(1, range(0, 1) ? 4 : 200), stride = range(1, 80);
         std::vector<int> start(experts + 1), first(experts + 1);
         for (int e = 0; e < experts; ++e) {
             const int count = range(0, 2) ? range(0, range(0, 1) ? 40 : 1500) : 0, chunks = i8_chunks(count, most);
@@ -102,6 +103,8 @@ int main(int argc, char **argv) {
         for (char c : rows_seen)
             CHECK(c);
     }
+    if (cut_seen < launches)  // launches whose items are really cut are among them
+        return std::printf("too few cut launches\n"), 1;
     std::printf("ok %d %lld\n", launches, pieces_seen);
     return 0;
 }

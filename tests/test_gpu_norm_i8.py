@@ -390,6 +390,12 @@ I8 = [
     ([1000, 513, 40, 770], 2880, 2880, "bf16", 2, 7, False),
     ([4096, 100, 3000], 512, 384, "bf16", 0, 0, True),
     ([20, 30], 256, 131056, "bf16", 0, 0, True),
+    # items that are cut along k: narrow and wide chunks, all items and those of the last rounds, experts of uneven rows
+    ([1] * 5, 4096, 7168, "fp16", 5, 0, False),
+    ([1280], 4096, 7168, "bf16", 0, 0, True),
+    ([1, 30, 0, 7, 64], 1032, 8192, "fp16", 1, 2, True),
+    ([900, 0, 1300], 2056, 9216, "bf16", 2, 1, False),
+    ([40], 8, 16384, "bf16", 0, 0, False),
 ]
 
 
