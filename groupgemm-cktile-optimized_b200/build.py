@@ -103,11 +103,13 @@ def _kernel_name(mangled: str) -> str:
         if not m:
             return re.sub(r"^_ZN.*?\d+([a-z_]+)E.*$", r"\1", mangled)
         name, rest = m.group(2)[: int(m.group(1))], m.group(2)[int(m.group(1)):]
-        args = re.match(r"I(f|6__half|13__nv_bfloat16|)((?:L[ib]\d+E)*)E", rest)
+        args = re.match(r"I((?:f|6__half|13__nv_bfloat16|S\d*_)*)((?:L[ib]\d+E)*)E", rest)
         if not args:
             return name
-        kind = [_TYPE[args.group(1)]] if args.group(1) else []
-        return name + "<" + ", ".join(kind + re.findall(r"L[ib](\d+)E", args.group(2))) + ">"
+        kinds = []
+        for kind in re.findall(r"f|6__half|13__nv_bfloat16|S\d*_", args.group(1)):
+            kinds.append(kinds[0] if kind.startswith("S") else _TYPE[kind])  # S: the first type again
+        return name + "<" + ", ".join(kinds + re.findall(r"L[ib](\d+)E", args.group(2))) + ">"
     dt = "fp16" if m.group(1) == "6__half" else "bf16"
     return f"grouped_gemm_sm100<{dt}, cta_group={m.group(2)}, BN={m.group(3)}, atoms={m.group(4)}, {_OP[m.group(5)]}>"
 

@@ -14,6 +14,9 @@
 //   leaves its sums in the workspace, and the last warp to arrive adds them up (no order to keep).
 //   Warps: 0 loads (weights and tokens, a ring of stages), 1 issues the products (of the pair's first CTA), 2-9 take the sums out of
 //   Tensor Memory, two accumulators in turn.
+// What bounds it: few rows, the weights' bytes (64 experts of 4096 x 7168, 16 rows each on average: 271 us alone, 6.9 TB/s; one token through 8 of
+// them 43 us with the rows before, of which 36 are bytes); many, the tensor pipe (8 experts of 4096 rows: 557 us, 3.45 POPS, 93% of its cycles) and, where
+// calls follow one another, the power cap.
 #pragma once
 
 #include "gg_moe.cuh"
@@ -37,7 +40,7 @@ constexpr int kI8Smem = kI8Ring + 1024;
 // (8 experts of 4096 rows, 4096 x 7168) and 962 / 818 / 812 / 757 (65536 rows of 32 of 7168 x 2048).
 constexpr int kI8Box = 128;
 constexpr int kI8MinSteps = 16;     // of a cut piece: with 8, 300 rows of 1000 x 2048 took 15.7 us in place of 11.9
-constexpr int kI8Band = 8;          // tiles whose weights are visited together (see item)
+constexpr int kI8Band = 8;          // tiles whose weights are visited together (see I8Cursor)
 
 struct I8Params {
     const void *x;            // [tokens or rows, k], as the caller has them (i8_rows)
@@ -251,7 +254,7 @@ template <class T> __global__ void __launch_bounds__(512) i8_rows(const __grid_c
 
 // The same by tokens, where one goes to several places: each row of x is read and rounded once. i8_places finds each slot's place, inv[src[r]] =
 // r, for i8_token_rows. What inv holds from other runs or of slots without a place is known by src, which does not point back; and of places
-// that name one slot twice all but one are done by themselves at the end. 16384 tokens of 7168 at 2 places: 140 us by places, XXX by tokens.
+// that name one slot twice all but one are done by themselves at the end. 16384 tokens of 7168 at 2 places: 150 us by places, 104 by tokens, of which 4 are i8_places.
 constexpr int kI8PlaceThreads = 256, kI8TokenPlaces = 32;
 __device__ __forceinline__ int2 i8_live(const I8Params &p) {
     return make_int2(max(0, p.offsets[0]), int(min(p.rows, int64_t(p.offsets[p.experts]))));

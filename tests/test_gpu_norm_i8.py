@@ -349,6 +349,24 @@ def test_quant_halves_and_their_neighbours(gg, kind):
     assert np.array_equal(q.cpu().numpy(), want) and np.array_equal(scales.cpu().numpy(), want_scales)
 
 
+@pytest.mark.parametrize("kind,bits,below", [("bf16", 7, 10), ("fp16", 10, 9)])
+def test_quant_every_pair_of_mantissas(gg, kind, bits, below):
+    """A row for each mantissa of its largest value, with every mantissa of smaller ones, from its own exponent down to what rounds to zero."""
+    torch = _torch()
+    m = torch.arange(1 << bits, 2 << bits, device="cuda").double()
+    v = torch.cat([m * 2.0 ** -(bits + e) for e in range(below)])
+    v = torch.where(torch.arange(v.numel(), device="cuda") % 2 == 0, v, -v)
+    for scale in (1.0, 0.25):
+        x = torch.where(v[None, :].abs() <= m[:, None] * 2.0 ** -bits, v[None, :], 0.0)
+        x[:, 0] = m * 2.0 ** -bits
+        x = (x * scale).to(_dtype(torch, kind))
+        rows, k = x.shape
+        q, scales = torch.empty(rows, k, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+        run(gg, torch, "quant", _type(gg, kind), rows, k, x.data_ptr(), q.data_ptr(), scales.data_ptr())
+        want, want_scales = quant_ref(x.float().cpu().numpy())
+        assert np.array_equal(q.cpu().numpy(), want) and np.array_equal(scales.cpu().numpy(), want_scales)
+
+
 @pytest.mark.parametrize("kind,small", [("bf16", 2.0 ** -133), ("fp16", 2.0 ** -24), ("f32", 2.0 ** -149)])
 def test_quant_extreme_rows(gg, kind, small):
     """Zeros, the type's smallest and largest values, NaN and infinities (in any place of a long row)."""
