@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = 16 * (group + 4 * i + 2 * (lane >> 4)) + (lane & 15);
-                x[i] = j < it.count ? __ldg(p.xq_scales + it.r0 + j) : 0.0f;
+                x[i] = j < it.count ? __ldcg(p.xq_scales + it.r0 + j) : 0.0f;  // from L2: written while this kernel runs
             }
             auto ordinary = [](float v) { return v == 0.0f || (fabsf(v) > 9.0949470e-13f && fabsf(v) < 1.0995116e12f); };  // 2^-40, 2^40
             bool plain = ordinary(scale);

@@ -383,7 +383,7 @@ class ServingLayerI8:
                     raise ValueError("gamma and beta must be contiguous and of one type")
             self.norms, self.normed = gg.make_b200_backend(), torch.empty_like(self.x)
             self.sum = torch.empty_like(self.x) if residual else self.x
-            rows_in, rows_scales = torch.empty(tokens, k, dtype=torch.int8, device=dev), torch.empty(tokens, dtype=torch.float32, device=dev)
+            rows_in, rows_scales = torch.zeros(tokens, k, dtype=torch.int8, device=dev), torch.zeros(tokens, dtype=torch.float32, device=dev)
             self.rounded = (rows_in, rows_scales)
             _ready(self.norms.prepare_norm(dt, tokens, k, _ptr(self.x), _ptr(self.normed), gamma_ptr=_ptr(gamma), beta_ptr=_ptr(beta),
                                            param_type=_dtype(gg, gamma.dtype), residual_ptr=_ptr(self.residual),
@@ -403,7 +403,7 @@ class ServingLayerI8:
         return self.normed
 
     def run(self) -> torch.Tensor:
-        """One step on what x (or the last norm), mask and logits hold; y [tokens, n], zero where mask is."""
+        """One step on what x (or the last norm; before the first, rows of zeros), mask and logits hold; y [tokens, n], zero where mask is."""
         s = _stream()
         self.router.backend.run(s)
         self.products.run(s)

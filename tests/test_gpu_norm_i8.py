@@ -129,6 +129,24 @@ def test_norm_without_parameters_and_only_8_bit_rows(gg):
     assert np.array_equal(q.cpu().numpy(), want) and np.array_equal(scales.cpu().numpy(), want_scales)
 
 
+@pytest.mark.parametrize("hidden,kind,params,q", [(64, "bf16", "bf16", False), (4096, "fp16", "f32", True), (16384, "bf16", "bf16", False),
+                                                  (16384, "f32", "f32", True), (8200, "bf16", "f32", False)])
+@pytest.mark.parametrize("which", ["gamma", "beta"])
+def test_norm_with_one_parameter(gg, hidden, kind, params, q, which):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(hidden)
+    x = rows_of(torch, g, 150, hidden, kind)
+    v = (1 + 0.3 * torch.randn(hidden, generator=g, device="cuda")).to(_dtype(torch, params))
+    y, rows, scales = torch.empty_like(x), torch.empty(150, hidden, dtype=torch.int8, device="cuda"), torch.empty(150, device="cuda")
+    run(gg, torch, "norm", _type(gg, kind), 150, hidden, x.data_ptr(), y.data_ptr(), param_type=_type(gg, params), q_ptr=rows.data_ptr() if q else 0,
+        q_scales_ptr=scales.data_ptr() if q else 0, **{which + "_ptr": v.data_ptr()})
+    ref, _, _, t_y, _, _ = norm_ref(_np(x), _np(v) if which == "gamma" else f64(1.0), _np(v) if which == "beta" else f64(0.0), 1e-5)
+    close(_np(y), ref, t_y + HALF_ULP[kind] * (np.abs(ref) + t_y) + TINY[kind])
+    if q:
+        want, want_scales = quant_ref(y.float().cpu().numpy())
+        assert np.array_equal(rows.cpu().numpy(), want) and np.array_equal(scales.cpu().numpy(), want_scales)
+
+
 def test_norm_far_mean_equal_rows_and_special_values(gg):
     """A mean far above the spread costs no more than its own rounding; rows of one value give beta; NaN and infinities stay in their row."""
     torch = _torch()
@@ -414,6 +432,7 @@ I8 = [
     ([1, 30, 0, 7, 64], 1032, 8192, "fp16", 1, 2, True),
     ([900, 0, 1300], 2056, 9216, "bf16", 2, 1, False),
     ([40], 8, 16384, "bf16", 0, 0, False),
+    ([4000, 300], 136, 2064, "bf16", 33, 0, False),  # more places a token than are put in order by tokens
 ]
 
 
