@@ -321,7 +321,7 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
     });
 }
 
-// A block a row (and every gridDim.x-th after it). 32768 rows of 7168, bf16: 160 us (4.4 TB.
+// A block a row (and every gridDim.x-th after it). 32768 rows of 7168, bf16: 116 us (6.1 TB/s).
 template <class T> __global__ void __launch_bounds__(512) quant_rows(const __grid_constant__ QuantParams p) {
     __shared__ uint32_t part[2][16];
     ptx::griddep_wait();

@@ -263,8 +263,12 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     const bool order = q.rows > 0 && (q.src || !q.x_scales);  // rows are put into expert order or rounded first
     const size_t sums = 2 * size_t(pairs) * size_t(chunk) * 1024, rounded = order ? size_t(q.rows) * size_t(q.k) : 0;
     // By tokens where a token has several places and there is more to move than the launch before costs: us by places / by tokens, 1024 x 8 rows
-    // of 7168 291 / 293, 2048 x 8 of 4096 97.5 / 96.8, 16384 x 2 of 7168 777 / 734 (with the products).
-    const bool by_token = order && q.src && q.top_k >= 2 && q.top_k <= kI8TokenPlaces && q.rows * q.k >= int64_t(1) << 23;
+    // of 7168 291 / 293, 2048 x 8 of 4096 97.5 / 96.8, 16384 x 2 of 7168 777 / 734 (with the products). Where there are fewer rows than slots
+    // (other experts' are elsewhere), tokens without a place are read for nothing: 65536 tokens of 2880 in 16 bits with 1/8, 1, 1.25, 1.5 and 2
+    // rows a token 31 / 127, 169 / 191, 209 / 208, 248 / 224 and 320 / 253, 16384 of 4096 in 8 bits with 1, 1.5 and 2 40 / 47, 60 / 64 and 72 / 73
+    // (both with 8 weight rows only).
+    const bool by_token = order && q.src && q.top_k >= 2 && q.top_k <= kI8TokenPlaces && q.rows * q.k >= int64_t(1) << 23 &&
+                          8 * q.rows >= (q.x_scales ? 15 : 10) * q.tokens;
     if (const int rc = reserve(h, sums + rounded + (order ? size_t(q.rows) * 4 : 0) + (by_token ? size_t(q.tokens) * size_t(q.top_k) * 4 : 0)))
         return rc;
     if (const int rc = reserve_counters(h, size_t(pairs) * 2 * kI8EpilogueWarps * 4, stream))

@@ -552,6 +552,23 @@ def test_i8_rows_by_tokens(gg, kind, top_k, eight):
         check_i8(torch, c, out.t)
 
 
+@pytest.mark.parametrize("kind,eight", [("bf16", False), ("fp16", True)])
+@pytest.mark.parametrize("more", [0.9, 2.3, 8])
+def test_i8_rows_of_few_tokens(gg, kind, eight, more):
+    """Rows of some of the slots only, as where other experts' rows are elsewhere: from more than two rows a token to a fraction of one."""
+    torch = _torch()
+    c = i8_case(torch, [2900, 0, 1201], 136, 2064, kind, 4, 33, eight)
+    tokens, g = int(c["tokens"] * 2 * more), torch.Generator(device="cuda").manual_seed(11)
+    pick = torch.randint(0, c["tokens"], (tokens,), generator=g, device="cuda")
+    c["x"], c["q"], c["qs"] = c["x"][pick].contiguous(), c["q"][pick], c["qs"][pick].contiguous()
+    c["x_scales"] = c["qs"] if eight else None
+    c["tokens"] = tokens
+    c["src"] = torch.randperm(4 * tokens, generator=g, device="cuda")[: c["rows"]].int()
+    c["src"][-33:] = -1
+    out, _ = run_i8(gg, torch, c)
+    check_i8(torch, c, out.t)
+
+
 def test_i8_largest_sums(gg):
     """All factors -128 at the longest k: the sum is 2^31 less one factor's share, and still exact."""
     torch = _torch()
