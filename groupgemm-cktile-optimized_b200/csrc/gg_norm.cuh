@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_consta
         const float2 joined = each_half_sum(lane < 16 ? theirs * t : other < p.warps ? fmaf(theirs * t, t, box[kNormMaxWarps + other]) : 0.0f);
         const float off = joined.x * inv_hidden, mean = m_first + off;
         const float var = fmaxf(0.0f, joined.y * inv_hidden - off * off);
-        const float rstd = rsqrtf(isnan(joined.y) ? joined.y : var + p.eps);
+        const float rstd = rsqrtf(joined.y < INFINITY ? var + p.eps : joined.y);  // infinite squares: 0, and NaN stays
         if (g.tid == 0 && g.ok) {
             if (p.mean)
                 p.mean[r] = mean;

@@ -129,6 +129,25 @@ def test_norm_without_parameters_and_only_8_bit_rows(gg):
     assert np.array_equal(q.cpu().numpy(), want) and np.array_equal(scales.cpu().numpy(), want_scales)
 
 
+@pytest.mark.parametrize("hidden,kind", [(1024, "bf16"), (7168, "f32"), (16384, "bf16"), (2880, "f32")])
+def test_norm_of_rows_whose_squares_pass_fp32(gg, hidden, kind):
+    """Squares around the mean beyond fp32's largest value count as infinite wherever in the row they are: rstd is 0 and y the bias."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(hidden)
+    dt = _dtype(torch, kind)
+    x = rows_of(torch, g, 6, hidden, kind)
+    x[1, hidden // 2:] = 1e25
+    x[2, : hidden // 2] = -1e25
+    x[3, hidden // 3] = 1e30
+    x[4, 256:512] = torch.tensor([1e25, -1e25], device="cuda").repeat(128).to(dt)
+    beta = torch.randn(hidden, generator=g, device="cuda").to(dt)
+    y, rstd = torch.empty_like(x), torch.empty(6, device="cuda")
+    run(gg, torch, "norm", _type(gg, kind), 6, hidden, x.data_ptr(), y.data_ptr(), beta_ptr=beta.data_ptr(), param_type=_type(gg, kind),
+        rstd_ptr=rstd.data_ptr())
+    assert (rstd[1:5] == 0).all() and (rstd[[0, 5]] > 0).all()
+    assert torch.equal(y[1:5], beta.expand(4, hidden))
+
+
 @pytest.mark.parametrize("hidden,kind,params,q", [(64, "bf16", "bf16", False), (4096, "fp16", "f32", True), (16384, "bf16", "bf16", False),
                                                   (16384, "f32", "f32", True), (8200, "bf16", "f32", False)])
 @pytest.mark.parametrize("which", ["gamma", "beta"])
