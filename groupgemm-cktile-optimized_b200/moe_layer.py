@@ -160,6 +160,7 @@ class Norm:
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         """x [tokens, hidden] -> (y, x + residual): y is the norm of the second, which goes past the layer (x itself without a residual)."""
+        self.sum = None  # until this forward has run
         t, h = self._hidden(x)
         x = _check("x", x, (t, h), *LOGITS).contiguous()
         dt, pt = self._types(x)

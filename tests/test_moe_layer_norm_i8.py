@@ -61,6 +61,18 @@ def test_norm_backward(layer):
             norm.backward(dy, dsum)
 
 
+def test_norm_backward_after_a_refused_forward(layer):
+    """It would pair the tokens of one forward with the statistics of another."""
+    import torch
+
+    norm = layer.Norm(None, None)
+    norm.sum, norm.mean, norm.rstd = torch.zeros(T, K), torch.zeros(T), torch.zeros(T)
+    with pytest.raises(ValueError, match="not on the current CUDA device"):
+        norm.forward(torch.zeros(1, K))
+    with pytest.raises(ValueError, match="forward before it"):
+        norm.backward(torch.zeros(T, K))
+
+
 @pytest.mark.parametrize("change,reason", [
     (dict(weight=lambda t: t.zeros(E, N, K)), "weight must be torch.int8"),
     (dict(scales=lambda t: t.zeros(E, N, dtype=t.bfloat16)), "scales must be torch.float32"),
