@@ -16,6 +16,7 @@ namespace moe {
 
 constexpr int kNormMaxHidden = 16384;
 constexpr int kNormThreads = 512;      // of a block at most
+constexpr int kNormFullThreads = 768;  // of norm_rows' check-free form, which fits 80 registers without spills (the others do not, by 80 to 180 bytes)
 constexpr int kNormSmem = 212 * 1024;  // of a block's ring and copies at most
 constexpr int kNormMaxSlots = 8;       // rows that a group's ring holds
 constexpr int kNormMaxGroups = 14;     // each has a named barrier beside the block's own
@@ -483,11 +484,15 @@ template <class T, class W, int V> struct NormParam {
 
 // kFull: every thread has V vectors, so that none asks for each (only with four: with two it saved the forward pass instructions but took
 // 157 us in place of 145 for 16384 x 7168 with a residual, its reads and writes closer together).
+// Forward it takes more groups of warps at once (kNormFullThreads): with 8-bit rows, whose way is long and has two barriers, 16384 rows of 7168
+// take 123 us with three groups of seven warps (136 with two), of 12288 191 with two of twelve (240 with one), of 4096 67 (71). Where the groups
+// stay as many, the fewer registers cost up to 4% (16384 columns 290 against 280). Four groups in 72 registers won nothing at 7168 and lost 5% at
+// 5120 and 8192.
 // Mean and variance without cancellation: each warp its own mean m_w and the squares S_w around it, joined around the first warp's mean, t_w = m_w - m_0:
 //   mean = m_0 + sum n_w t_w / n     sum (v - mean)^2 = sum (S_w + n_w t_w^2) - n (mean - m_0)^2
 // where what is taken off is at most the sum of the others' n_w t_w^2, so that no more than a factor of the number of warps is lost.
 template <class T, class W, int V, bool kFull>
-__global__ void __launch_bounds__(kNormThreads, 1) norm_rows(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kFull ? kNormFullThreads : kNormThreads, 1) norm_rows(const __grid_constant__ NormParams p) {
     extern __shared__ __align__(1024) uint8_t norm_smem[];
     __shared__ uint64_t bars[kNormMaxGroups * kNormMaxSlots];
     __shared__ float part[kNormMaxGroups][2][2 * kNormMaxWarps];

@@ -13,6 +13,7 @@ using namespace gg::host;
 using gg::fail;
 using gg::MoeLaunch;
 using gg::refuse;
+using gg::moe::kNormFullThreads;
 using gg::moe::kNormMaxGroups;
 using gg::moe::kNormMaxHidden;
 using gg::moe::kNormMaxSlots;
@@ -29,15 +30,20 @@ struct NormShape {
     size_t smem;
 };
 
-// ahead: bytes of rows that a block keeps on their way or in use, beyond the two that a group needs at least.
-NormShape norm_shape(int64_t rows, int vecs, int v, int tensors, int elem, int params, int param_size, size_t ahead, int num_sms) {
+// full_threads: of a block of the check-free form, at most. ahead: bytes of rows that a block keeps on their way or in use, beyond the two that a
+// group needs at least.
+NormShape norm_shape(int64_t rows, int vecs, int v, int full_threads, int tensors, int elem, int params, int param_size, size_t ahead, int num_sms) {
     NormShape s{};
     s.v = v;
     s.warps = (vecs + 32 * s.v - 1) / (32 * s.v);
     s.full = s.v > 2 && vecs == 32 * s.v * s.warps;
     const int64_t each = (rows + num_sms - 1) / num_sms;  // rows of a block
-    s.groups = int(std::max<int64_t>(1, std::min<int64_t>({each, kNormThreads / (32 * s.warps), kNormMaxGroups})));
     const size_t row = size_t(vecs) * 8 * size_t(elem) * size_t(tensors);
+    int most = (s.full ? full_threads : kNormThreads) / (32 * s.warps);
+    // what 768 threads add keeps to about `ahead` (7168 columns with a residual and 8-bit rows 191 us with a third group, 185 without)
+    while (most > kNormThreads / (32 * s.warps) && size_t(most) * 2 * row > (100 << 10))
+        --most;
+    s.groups = int(std::max<int64_t>(1, std::min<int64_t>({each, most, kNormMaxGroups})));
     size_t copy = s.v > 2 ? size_t(params) * size_t(vecs) * 8 * size_t(param_size) : 0;
     if (2 * row + copy > size_t(kNormSmem))
         copy = 0;  // read from global memory
@@ -103,7 +109,7 @@ int prepare_norm(gg_handle *h, const gg_norm_problem &q, gg_stream_t stream, cha
     // Vectors a thread: as few warps a row as registers allow, which is two vectors, since the sums between lanes cost the same for any number; with
     // 8-bit rows, whose longer way wants two rows at a time, four.
     const int vecs = int(q.hidden / 8), v = vecs <= 64 ? 1 : vecs <= (q.q ? 96 : 1024) ? 2 : 4;
-    const NormShape s = norm_shape(q.tokens, vecs, v, q.residual ? 2 : 1, q.dtype == GG_F32 ? 4 : 2, 2, q.param_type == GG_F32 ? 4 : 2, 88 << 10, num_sms);
+    const NormShape s = norm_shape(q.tokens, vecs, v, kNormFullThreads, q.residual ? 2 : 1, q.dtype == GG_F32 ? 4 : 2, 2, q.param_type == GG_F32 ? 4 : 2, 88 << 10, num_sms);
     gg::moe::NormParams p{};
     p.x = q.x;
     p.residual = q.residual;
@@ -144,7 +150,7 @@ int prepare_norm_grad(gg_handle *h, const gg_norm_grad_problem &q, gg_stream_t s
     if (const int rc = bind_device(h, stream, num_sms, why, why_len))
         return rc;
     const int vecs = int(q.hidden / 8), v = vecs <= 64 ? 1 : vecs <= 512 ? 2 : 4;
-    const NormShape s = norm_shape(q.tokens, vecs, v, q.dsum ? 3 : 2, q.dtype == GG_F32 ? 4 : 2, 1, q.param_type == GG_F32 ? 4 : 2, 160 << 10, num_sms);
+    const NormShape s = norm_shape(q.tokens, vecs, v, kNormThreads, q.dsum ? 3 : 2, q.dtype == GG_F32 ? 4 : 2, 1, q.param_type == GG_F32 ? 4 : 2, 160 << 10, num_sms);
     const size_t sums = 2 * size_t(q.hidden) * 4;  // dgamma and dbeta of a block or group
     if (const int rc = reserve(h, std::max<size_t>(1, s.blocks) * sums))
         return rc;

@@ -78,6 +78,10 @@ NORM = [
     (310, 8200, "fp16", "f32", True, True),
     (160, 16384, "bf16", "bf16", False, False),
     (160, 16384, "f32", "f32", True, True),
+    (1100, 7168, "bf16", "bf16", True, True),
+    (900, 5120, "fp16", "f32", False, True),
+    (400, 9216, "bf16", "f32", False, True),
+    (3000, 1024, "f32", "f32", False, True),
 ]
 
 
