@@ -16,7 +16,7 @@ namespace moe {
 
 constexpr int kNormMaxHidden = 16384;
 constexpr int kNormThreads = 512;      // of a block at most
-constexpr int kNormFullThreads = 768;  // of norm_rows' check-free form, which fits 80 registers without spills (the others do not, by 80 to 180 bytes)
+constexpr int kNormFullThreads = 768;  // of norm_rows' check-free form, which fits 80 registers (fp32 spills 4 bytes; the others 80 to 180)
 constexpr int kNormSmem = 212 * 1024;  // of a block's ring and copies at most
 constexpr int kNormMaxSlots = 8;       // rows that a group's ring holds
 constexpr int kNormMaxGroups = 14;     // each has a named barrier beside the block's own
