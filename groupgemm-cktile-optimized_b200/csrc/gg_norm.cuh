@@ -482,6 +482,9 @@ template <class T, class W, int V> struct NormParam {
     }
 };
 
+// What a row's values are moved by: where their squares pass fp32 (rstd 0) their distance to the mean can pass it, too, and 0 times that would not be 0.
+__device__ __forceinline__ float minus_mean_of(float mean, float rstd) { return rstd == 0.0f && fabsf(mean) < INFINITY ? 0.0f : -mean; }
+
 // kFull: every thread has V vectors, so that none asks for each (only with four: with two it saved the forward pass instructions but took
 // 157 us in place of 145 for 16384 x 7168 with a residual, its reads and writes closer together).
 // Forward it takes more groups of warps at once (kNormFullThreads): with 8-bit rows, whose way is long and has two barriers, 16384 rows of 7168
@@ -491,6 +494,8 @@ template <class T, class W, int V> struct NormParam {
 // Mean and variance without cancellation: each warp its own mean m_w and the squares S_w around it, joined around the first warp's mean, t_w = m_w - m_0:
 //   mean = m_0 + sum n_w t_w / n     sum (v - mean)^2 = sum (S_w + n_w t_w^2) - n (mean - m_0)^2
 // where what is taken off is at most the sum of the others' n_w t_w^2, so that no more than a factor of the number of warps is lost.
+// Where one of these sums passes fp32, the row is joined once more by the warps' shares n_w / n, which pass it only where the row's own squares do:
+// means of 8 values or more are far from fp32's end, and where a t_w^2 passes it, the squares around the row's mean, 4 t_w^2 at least, do too.
 template <class T, class W, int V, bool kFull>
 __global__ void __launch_bounds__(kFull ? kNormFullThreads : kNormThreads, 1) norm_rows(const __grid_constant__ NormParams p) {
     extern __shared__ __align__(1024) uint8_t norm_smem[];
@@ -568,9 +573,16 @@ __global__ void __launch_bounds__(kFull ? kNormFullThreads : kNormThreads, 1) no
         const float m_first = box[0];
         const float t = other < p.warps ? box[other] - m_first : 0.0f;
         const float2 joined = each_half_sum(lane < 16 ? theirs * t : other < p.warps ? fmaf(theirs * t, t, box[kNormMaxWarps + other]) : 0.0f);
-        const float off = joined.x * inv_hidden, mean = m_first + off;
-        const float var = fmaxf(0.0f, joined.y * inv_hidden - off * off);
-        const float rstd = rsqrtf(joined.y < INFINITY ? var + p.eps : joined.y);  // infinite squares: 0, and NaN stays
+        const float off = joined.x * inv_hidden;
+        float mean = m_first + off, minus = -mean, rstd = rsqrtf(fmaxf(0.0f, joined.y * inv_hidden - off * off) + p.eps);
+        if (!(joined.y < INFINITY)) {  // (joined.x passes fp32 only where joined.y does) alike in all of a group's threads
+            const float share = theirs * inv_hidden, of_warp = other < p.warps ? box[kNormMaxWarps + other] : 0.0f;
+            const float2 far = each_half_sum(lane < 16 ? share * t : fmaf(share * t, t, of_warp * inv_hidden));
+            mean = box[0] + far.x;
+            const float var = fmaxf(0.0f, far.y - far.x * far.x), squares = far.y < INFINITY ? var * hidden : far.y;
+            rstd = rsqrtf(squares < INFINITY ? var + p.eps : squares);  // infinite squares: 0, and NaN stays
+            minus = minus_mean_of(mean, rstd);
+        }
         if (g.tid == 0 && g.ok) {
             if (p.mean)
                 p.mean[r] = mean;
@@ -580,7 +592,7 @@ __global__ void __launch_bounds__(kFull ? kNormFullThreads : kNormThreads, 1) no
         uint32_t top = 0;
         Vec8<T> y[V];
         // (s rstd - mean rstd would be one operation less, but off by a rounding of mean rstd: rows of one value would not give beta)
-        const pair_t minus_mean = pair(-mean, -mean), both_rstd = pair(rstd, rstd);
+        const pair_t minus_mean = pair(minus, minus), both_rstd = pair(rstd, rstd);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;

@@ -265,8 +265,8 @@ int gg_prepare_w4(gg_handle *h, const gg_w4_problem *p, gg_stream_t stream, char
  *   q, q_scales: y rounded to 8-bit integers as gg_prepare_quant does, in the same pass (for gg_prepare_i8)
  *
  * dtype bf16, fp16 or fp32 (x, residual, sum, y); param_type that or GG_F32 (gamma, beta). Statistics are fp32, of the squares
- * around the mean: a row whose squares pass fp32's largest value has rstd 0, one whose sum does NaN. sum may be the
- * same array as x or residual, y the same as x where sum is not asked for. hidden a multiple of 8 up to 16384; x, residual, gamma, beta,
+ * around the mean: a row whose squares pass fp32's largest value has rstd 0 and y = beta, one whose sum (or that of a part of its columns)
+ * does NaN. sum may be the same array as x or residual, y the same as x where sum is not asked for. hidden a multiple of 8 up to 16384; x, residual, gamma, beta,
  * sum, y and q 16-byte aligned. */
 typedef struct gg_norm_problem {
     int32_t dtype;
