@@ -668,13 +668,14 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
     uint32_t phase = 0;
     for (int64_t r = g.first; r < p.rows; r += g.stride) {
         const float rstd = next_rstd;
-        const pair_t minus_mean = pair(-next_mean, -next_mean), both_rstd = pair(rstd, rstd);
+        const float minus = minus_mean_of(next_mean, rstd);
+        const pair_t minus_mean = pair(minus, minus), both_rstd = pair(rstd, rstd);
         if (r + g.stride < p.rows) {
             next_mean = __ldg(p.mean + r + g.stride);
             next_rstd = __ldg(p.rstd + r + g.stride);
         }
         g.wait(slot, phase);
-        pair_t along = 0, level = 0;  // sums of d (x - mean) and of d, of even and of odd columns
+        pair_t along = 0, level = 0;  // sums of d c and of d, of even and of odd columns
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int at = g.tid + v * g.threads;
@@ -688,10 +689,10 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
                 gamma.get(v, at, w);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const pair_t c = add2(a[i], minus_mean), d = mul2(b[i], w[i]);
+                    const pair_t c = mul2(add2(a[i], minus_mean), both_rstd), d = mul2(b[i], w[i]);
                     level = add2(level, d);
                     along = fma2(d, c, along);
-                    dgamma[v][i] = fma2(mul2(b[i], both_rstd), c, dgamma[v][i]);
+                    dgamma[v][i] = fma2(b[i], c, dgamma[v][i]);
                     dbeta[v][i] = add2(dbeta[v][i], b[i]);
                 }
             }
@@ -704,7 +705,8 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
         if (g.slots > 1 && r != g.first)
             g.load(slot ? slot - 1 : g.slots - 1, r + (g.slots - 1) * g.stride);
         const float2 sums = each_half_sum((lane & 15) < p.warps ? box[lane] : 0.0f);
-        const float less = -rstd * (sums.y * inv_hidden), tilt = -(rstd * (sums.x * inv_hidden)) * rstd * rstd;
+        // dx = rstd (d + (x - mean) tilt) + less: no factor of it is the square of rstd or of a value
+        const float less = -rstd * (sums.y * inv_hidden), tilt = -rstd * (sums.x * inv_hidden);
         const pair_t both_less = pair(less, less), slope = pair(tilt, tilt);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -719,7 +721,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
                 gamma.get(v, at, w);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    a[i] = fma2(add2(a[i], minus_mean), slope, fma2(mul2(b[i], w[i]), both_rstd, both_less));
+                    a[i] = fma2(fma2(add2(a[i], minus_mean), slope, mul2(b[i], w[i])), both_rstd, both_less);
                 if (p.dsum) {
                     x.lds(g.at(slot, 2), at, p.vecs);
                     x.get(b);

@@ -294,7 +294,7 @@ int gg_prepare_norm(gg_handle *h, const gg_norm_problem *p, gg_stream_t stream, 
  *
  * x is the norm's input: sum where there was a residual, whose gradient is dx, too. dsum is the gradient that reaches the
  * sum by its other way (past the layer), or NULL. dgamma and dbeta are fp32, either may be NULL; the same inputs give the same bits. dx may be
- * the same array as dy or dsum. Limits as gg_prepare_norm's. */
+ * the same array as dy or dsum. A row whose squares pass fp32 (rstd 0) has dx = dsum and adds nothing to dgamma. Limits as gg_prepare_norm's. */
 typedef struct gg_norm_grad_problem {
     int32_t dtype;
     int32_t param_type;      /* of gamma */

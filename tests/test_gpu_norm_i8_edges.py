@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from test_gpu_moe_ops import HALF_ULP, TINY, U, _dtype, _torch, _type, close
-from test_gpu_norm_i8 import _np, norm_ref, quant_ref, rows_of, run
+from test_gpu_norm_i8 import _np, grad_ref, norm_ref, quant_ref, rows_of, run
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,55 @@ def test_norm_of_rows_whose_squares_are_just_in_range(gg, hidden, kind):
     close(_np(rstd), r, 200 * U * r)
     t_y = t_y + 200 * U * np.abs(ref)
     close(_np(y), ref, t_y + HALF_ULP[kind] * (np.abs(ref) + t_y) + TINY[kind])
+
+
+@pytest.mark.parametrize("dsum", [False, True])
+@pytest.mark.parametrize("hidden,kind,_", RANGE)
+def test_norm_grad_of_rows_without_spread(gg, hidden, kind, _, dsum):
+    """Rows whose squares pass fp32 have rstd 0: their dx is dsum to the last bit, they add nothing to dgamma, and the rows beside them are as ever."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(hidden + 1)
+    dt = _dtype(torch, kind)
+    x = far_rows(torch, g, hidden, kind)
+    t = x.shape[0]
+    dy, more = (torch.randn(t, hidden, generator=g, device="cuda").to(dt) for _ in range(2))
+    gamma = (1 + 0.3 * torch.randn(hidden, generator=g, device="cuda")).to(dt)
+    y, mean, rstd = torch.empty_like(x), torch.empty(t, device="cuda"), torch.empty(t, device="cuda")
+    run(gg, torch, "norm", _type(gg, kind), t, hidden, x.data_ptr(), y.data_ptr(), gamma_ptr=gamma.data_ptr(), mean_ptr=mean.data_ptr(),
+        rstd_ptr=rstd.data_ptr())
+    assert (rstd[1:-1] == 0).all() and torch.isfinite(mean).all()
+    check_grad(gg, torch, kind, x, mean, rstd, gamma, dy, more if dsum else None)
+    dx = torch.empty_like(x)
+    run(gg, torch, "norm_grad", _type(gg, kind), t, hidden, x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr(),
+        gamma_ptr=gamma.data_ptr(), dsum_ptr=more.data_ptr() if dsum else 0)
+    assert torch.equal(dx[1:-1], more[1:-1] if dsum else torch.zeros_like(dx[1:-1]))
+
+
+def check_grad(gg, torch, kind, x, mean, rstd, gamma, dy, more):
+    t, hidden = x.shape
+    dx = torch.empty_like(x)
+    dgamma, dbeta = torch.empty(hidden, device="cuda"), torch.empty(hidden, device="cuda")
+    run(gg, torch, "norm_grad", _type(gg, kind), t, hidden, x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr(),
+        gamma_ptr=gamma.data_ptr(), dsum_ptr=more.data_ptr() if more is not None else 0, dgamma_ptr=dgamma.data_ptr(), dbeta_ptr=dbeta.data_ptr())
+    ref, tol, dg, a_dg, db, a_db = grad_ref(_np(x), _np(dy), _np(mean), _np(rstd), _np(gamma), _np(more) if more is not None else 0.0)
+    close(_np(dx), ref, tol + HALF_ULP[kind] * (np.abs(ref) + tol) + TINY[kind])
+    many = (t // 148 + 48) * U
+    close(_np(dgamma), dg, many * a_dg + 1e-37)
+    close(_np(dbeta), db, many * a_db + 1e-37)
+
+
+@pytest.mark.parametrize("hidden,kind", [(64, "bf16"), (1024, "f32"), (7168, "bf16"), (8200, "f32"), (16384, "bf16")])
+def test_norm_grad_of_large_values_and_gradients(gg, hidden, kind):
+    """Rows and gradients whose products pass fp32, which the gradient's own terms do not: rstd times a value is about 1."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(hidden + 2)
+    dt = _dtype(torch, kind)
+    x = (torch.randn(20, hidden, generator=g, device="cuda") * 1e14).to(dt)
+    dy = (torch.randn(20, hidden, generator=g, device="cuda") * 1e28).to(dt)
+    x[::2], dy[1::2] = rows_of(torch, g, 10, hidden, kind), torch.randn(10, hidden, generator=g, device="cuda").to(dt)
+    x[::3], dy[::3] = (x[::3].float() * 1e-12).to(dt), (dy[::3].float() * 1e-12).to(dt)
+    gamma = (1 + 0.3 * torch.randn(hidden, generator=g, device="cuda")).to(dt)
+    x[5], dy[5] = (torch.randn(hidden, generator=g, device="cuda") * 1e14).to(dt), (torch.randn(hidden, generator=g, device="cuda") * 1e28).to(dt)
+    mean = x.double().mean(1).float()
+    rstd = (x.double().var(1, unbiased=False) + 1e-5).rsqrt().float()
+    check_grad(gg, torch, kind, x, mean, rstd, gamma, dy, None)
