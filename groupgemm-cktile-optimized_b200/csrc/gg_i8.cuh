@@ -61,7 +61,9 @@ struct I8Params {
     int chunk;                // most tokens of a chunk, a multiple of 32
     int box;                  // rows of a token load
     int stages, stage_bytes;
-    int after_rows;           // 1: i8_rows precedes, and everything before it is done when this kernel starts
+    // 1: i8_rows precedes. Everything before that is done when this kernel starts, for i8_rows' blocks have waited for it, but this kernel has not
+    // itself: what it reads before its own wait (offsets; weights, by TMA) comes from L2, not from what an SM may still hold of an earlier run.
+    int after_rows;
 };
 
 // Instruction descriptor of kind::i8: D s32 (2 at bit 4), A and B signed (1 at bits 7 and 10), both K-major, N >> 3, M >> 4.
@@ -179,12 +181,12 @@ struct I8Work {
     bool falls;
 
     // offsets come from the device: each is held to the range that the rows allow, and where they fall no expert gets rows. By all threads
-    // of the block, which are together after it.
+    // of the block, which are together after it. Read from L2, since they are read before the wait where the rows' kernel precedes (I8Params).
     __device__ __forceinline__ I8Work(const I8Params &p, int *start_, int *first_) : start(start_), first(first_) {
         const int E = p.experts, tid = threadIdx.x;
         bool bad = false;
         for (int e = tid; e <= E; e += blockDim.x) {
-            const int64_t v = p.offsets[e], before = e ? p.offsets[e - 1] : 0;
+            const int64_t v = __ldcg(p.offsets + e), before = e ? __ldcg(p.offsets + e - 1) : 0;
             bad |= v < before;
             if (v < before || v > p.rows)
                 report(p.status, kSiteOffsets);
