@@ -242,11 +242,21 @@ template <class T> __global__ void __launch_bounds__(512) i8_rows(const __grid_c
         if (p.x_scales) {
             const uint4 *from = reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(p.x) + row * p.k);
             uint4 *to = reinterpret_cast<uint4 *>(p.xq + r * p.k);
-#pragma unroll 4
-            for (int i = threadIdx.x; i < p.k / 16; i += blockDim.x)
-                to[i] = __ldg(from + i);
+            const int pieces = p.k / 16, threads = int(blockDim.x);  // four on their way: a load does not pass the stores before it
+#pragma unroll 1
+            for (int i = threadIdx.x; i < pieces; i += 4 * threads) {
+                uint4 v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j * threads < pieces)
+                        v[j] = from[i + j * threads];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j * threads < pieces)
+                        to[i + j * threads] = v[j];
+            }
             if (threadIdx.x == 0)
-                p.xq_scales[r] = __ldg(p.x_scales + row);
+                p.xq_scales[r] = __ldcg(p.x_scales + row);
         } else {
             quant_row<T>(static_cast<const uint8_t *>(p.x) + row * p.k * int64_t(sizeof(T)), p.xq + r * p.k, p.xq_scales + r, p.k / 8, part[turn]);
             turn ^= 1;
@@ -294,7 +304,7 @@ template <class T> __global__ void __launch_bounds__(512) i8_token_rows(const __
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (tid + i * int(blockDim.x) < pieces)
-                    v[i] = __ldg(from + tid + i * int(blockDim.x));
+                    v[i] = from[tid + i * int(blockDim.x)];
             find(place);
             __syncthreads();
             const int n = place[kI8TokenPlaces];
@@ -305,9 +315,9 @@ template <class T> __global__ void __launch_bounds__(512) i8_token_rows(const __
                     if (tid + i * int(blockDim.x) < pieces)
                         to[tid + i * int(blockDim.x)] = v[i];
                 for (int i = tid + 2 * int(blockDim.x); i < pieces; i += blockDim.x)
-                    to[i] = __ldg(from + i);
+                    to[i] = from[i];
                 if (tid == 0)
-                    p.xq_scales[place[j]] = __ldg(p.x_scales + t);
+                    p.xq_scales[place[j]] = __ldcg(p.x_scales + t);
             }
         } else {
             quant_row<T>(static_cast<const uint8_t *>(p.x) + t * p.k * int64_t(sizeof(T)), p.k / 8, part[turn], [&] { find(place); }, [&](float scale) {
@@ -536,12 +546,12 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             if (p.after_rows && turn == 0)
                 ptx::griddep_wait();  // xq_scales are i8_rows' output
             // scales of the rows of this warp's blocks, and of this lane's weight row; whether all are far from the ends of fp32's range
-            const float scale = col < p.n ? __ldg(p.scales + int64_t(it.e) * p.n + col) : 0.0f;
+            const float scale = col < p.n ? __ldcg(p.scales + int64_t(it.e) * p.n + col) : 0.0f;
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = 16 * (group + 4 * i + 2 * (lane >> 4)) + (lane & 15);
-                x[i] = j < it.count ? __ldcg(p.xq_scales + it.r0 + j) : 0.0f;  // from L2: written while this kernel runs
+                x[i] = j < it.count ? __ldcg(p.xq_scales + it.r0 + j) : 0.0f;
             }
             auto ordinary = [](float v) { return v == 0.0f || (fabsf(v) > 9.0949470e-13f && fabsf(v) < 1.0995116e12f); };  // 2^-40, 2^40
             bool plain = ordinary(scale);

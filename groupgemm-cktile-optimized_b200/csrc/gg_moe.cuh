@@ -14,6 +14,9 @@
 namespace gg {
 namespace moe {
 
+// Each kernel starts while the one before it in the stream ends. What that one may still write (rows, scales, statistics, offsets) is read after
+// the kernel's wait and never by the read-only path (__ldg, ld.global.nc), which asks that it be unchanged for the whole of the kernel's life.
+
 // Sites of the index checks (status word kStatusBounds | site): these indices come from device
 // memory that the host never sees, so a kernel checks each before it uses it as an address; one
 // that is out of range is recorded (the first wins) and its access skipped.

@@ -112,7 +112,7 @@ template <> __device__ __forceinline__ uint32_t plus2<__half>(uint32_t a, uint32
 template <class T> struct Vec8 {
     uint4 w;
     __device__ __forceinline__ void lds(uint32_t row, int vec, int) { w = lds_row(row + uint32_t(vec) * 16u); }
-    __device__ __forceinline__ void ldg(const void *row, int vec, int) { w = __ldg(static_cast<const uint4 *>(row) + vec); }
+    __device__ __forceinline__ void load(const void *row, int vec, int) { w = static_cast<const uint4 *>(row)[vec]; }
     __device__ __forceinline__ void get(pair_t (&f)[4]) const {
         const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y), c = unpack2<T>(w.z), d = unpack2<T>(w.w);
         f[0] = pair(a.x, a.y), f[1] = pair(b.x, b.y), f[2] = pair(c.x, c.y), f[3] = pair(d.x, d.y);
@@ -144,9 +144,9 @@ template <> struct Vec8<float> {
         a = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
         b = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
     }
-    __device__ __forceinline__ void ldg(const void *row, int vec, int vecs) {
-        a = __ldg(static_cast<const float4 *>(row) + vec);
-        b = __ldg(static_cast<const float4 *>(row) + vecs + vec);
+    __device__ __forceinline__ void load(const void *row, int vec, int vecs) {
+        a = static_cast<const float4 *>(row)[vec];
+        b = static_cast<const float4 *>(row)[vecs + vec];
     }
     __device__ __forceinline__ void get(pair_t (&f)[4]) const {
         f[0] = pair(a.x, a.y), f[1] = pair(a.z, a.w), f[2] = pair(b.x, b.y), f[3] = pair(b.z, b.w);
@@ -277,7 +277,7 @@ template <class T, class B, class S> __device__ __forceinline__ void quant_row(c
     for (int i = 0; i < kQuantHeld; ++i) {
         const int at = tid + i * int(blockDim.x);
         if (at < vecs)
-            v[i].ldg(row, at, vecs);
+            v[i].load(row, at, vecs);
     }
     before();
 #pragma unroll
@@ -286,7 +286,7 @@ template <class T, class B, class S> __device__ __forceinline__ void quant_row(c
             top = v[i].top(top);
     for (int at = tid + kQuantHeld * int(blockDim.x); at < vecs; at += blockDim.x) {
         Vec8<T> u;
-        u.ldg(row, at, vecs);
+        u.load(row, at, vecs);
         top = u.top(top);
     }
     top = __reduce_max_sync(0xffffffffu, Vec8<T>::bits(top));
@@ -308,7 +308,7 @@ template <class T, class B, class S> __device__ __forceinline__ void quant_row(c
     for (int at = tid + kQuantHeld * int(blockDim.x); at < vecs; at += blockDim.x) {
         Vec8<T> u;
         pair_t f[4];
-        u.ldg(row, at, vecs);
+        u.load(row, at, vecs);
         u.get(f);
         store(at, vecs, by(f));
     }
@@ -451,7 +451,7 @@ template <class T, class W, int V> struct NormParam {
                     read(held[v], first + v * step);
         } else if (array && copy) {
             for (int i = threadIdx.x; i < vecs * int(sizeof(W)) / 2; i += blockDim.x)
-                reinterpret_cast<uint4 *>(copy)[i] = __ldg(static_cast<const uint4 *>(array) + i);
+                reinterpret_cast<uint4 *>(copy)[i] = __ldcg(static_cast<const uint4 *>(array) + i);
             from = copy;
         }
     }
@@ -661,8 +661,8 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
     pair_t dgamma[V][4] = {}, dbeta[V][4] = {};
     float next_mean = 0.0f, next_rstd = 0.0f;
     if (g.first < p.rows) {
-        next_mean = __ldg(p.mean + g.first);
-        next_rstd = __ldg(p.rstd + g.first);
+        next_mean = __ldcg(p.mean + g.first);
+        next_rstd = __ldcg(p.rstd + g.first);
     }
     int slot = 0, turn = 0;
     uint32_t phase = 0;
@@ -671,8 +671,8 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_grad_rows(const __grid_c
         const float minus = minus_mean_of(next_mean, rstd);
         const pair_t minus_mean = pair(minus, minus), both_rstd = pair(rstd, rstd);
         if (r + g.stride < p.rows) {
-            next_mean = __ldg(p.mean + r + g.stride);
-            next_rstd = __ldg(p.rstd + r + g.stride);
+            next_mean = __ldcg(p.mean + r + g.stride);
+            next_rstd = __ldcg(p.rstd + r + g.stride);
         }
         g.wait(slot, phase);
         pair_t along = 0, level = 0;  // sums of d c and of d, of even and of odd columns

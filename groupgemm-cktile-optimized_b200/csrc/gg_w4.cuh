@@ -268,7 +268,7 @@ template <class T, bool kFragments> __global__ void __launch_bounds__(kW4GatherT
             const int step = piece >> 4, c = piece & 15;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (row >= 0 && piece * 8 < p.k)
-                v = __ldg(reinterpret_cast<const uint4 *>(from + piece * 8));
+                v = __ldcg(reinterpret_cast<const uint4 *>(from + piece * 8));
             const int at = kFragments ? (((i >> 3) * 4 + (c >> 2)) * 32 + (i & 7) * 4 + (c & 3)) * 16
                                       : ((c >> 3) * count + i) * 128 + (((c & 7) ^ (i & 7)) << 4);
             *reinterpret_cast<uint4 *>(to + int64_t(step) * count * kW4TokenBytes + at) =

@@ -64,3 +64,56 @@ def test_serving_steps_whose_routing_changes(layer, tokens, top_k, k, norm):
         assert torch.equal(fast.router.offsets, plain.router.offsets)
         assert torch.equal(fast.y.view(torch.int16), plain.y.view(torch.int16)), i
     assert fast.products.device_status() == 0 and plain.products.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_each_operator_behind_the_one_that_writes_its_input(gg, kind):
+    """Norm -> its gradients -> rounding -> 8-bit products, and norm -> 4-bit products, in one graph, with contents that change."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    t, h, n, group = 37, 1024, 264, 64
+    dt, half = dict(bf16=torch.bfloat16, f32=torch.float32)[kind], torch.bfloat16
+    kt = dict(bf16=gg.BF16, f32=gg.F32)[kind]
+    x, dy, w = rand(t, h).to(dt), rand(t, h).to(dt), rand(n, h).to(dt)
+    offsets = torch.tensor([0, t], dtype=torch.int32, device="cuda")
+    qweight = torch.randint(0, 256, (1, n, h // 2), dtype=torch.uint8, generator=g, device="cuda")
+    w4_scales = (0.01 * torch.rand(1, n, h // group, generator=g, device="cuda")).to(half)
+
+    def chain(pdl):
+        f32 = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+        o = dict(y=torch.zeros_like(x), mean=f32(t), rstd=f32(t), dx=torch.zeros_like(x), dgamma=f32(h), dbeta=f32(h), q=torch.zeros(t, h, dtype=torch.int8, device="cuda"),
+                 qs=f32(t), wq=torch.zeros(1, n, h, dtype=torch.int8, device="cuda"), ws=f32(1, n), out=torch.zeros(t, n, dtype=half, device="cuda"),
+                 out4=torch.zeros(t, n, dtype=half, device="cuda"))
+        p = {k: v.data_ptr() for k, v in o.items()}
+        b = [gg.make_b200_backend() for _ in range(6)]
+        whys = [b[0].prepare_norm(kt, t, h, x.data_ptr(), p["y"], mean_ptr=p["mean"], rstd_ptr=p["rstd"]),
+                b[1].prepare_norm_grad(kt, t, h, x.data_ptr(), p["mean"], p["rstd"], dy.data_ptr(), p["dx"], dgamma_ptr=p["dgamma"], dbeta_ptr=p["dbeta"]),
+                b[2].prepare_quant(kt, t, h, p["dx"], p["q"], p["qs"]),
+                b[3].prepare_quant(kt, n, h, w.data_ptr(), p["wq"], p["ws"]),
+                b[4].prepare_i8(gg.BF16, 1, n, h, t, p["q"], p["wq"], p["ws"], offsets.data_ptr(), p["out"], x_scales_ptr=p["qs"])]
+        if kind == "bf16":
+            whys.append(b[5].prepare_w4(gg.BF16, 1, n, h, group, t, p["y"], qweight.data_ptr(), w4_scales.data_ptr(), offsets.data_ptr(), p["out4"]))
+        assert not any(whys), whys
+        for v in b:
+            v.set_option("pdl", pdl)
+        order = [0, 1, 2, 3, 4] + ([0, 5] if kind == "bf16" else [])
+
+        def step():
+            s = torch.cuda.current_stream().cuda_stream
+            for i in order:
+                b[i].run(s)
+
+        return o, step, b
+
+    fast, run_fast, backends = chain(1)
+    plain, run_plain, _ = chain(0)
+    graph = captured(torch, run_fast, 2)
+    for i in range(30):
+        for v in (x, dy, w):
+            v.copy_(rand(*v.shape).mul_(1 + i).to(dt))
+        graph.replay()
+        run_plain()
+        for k in fast:
+            assert torch.equal(fast[k].view(torch.uint8), plain[k].view(torch.uint8)), (k, i)
+    assert not any(v.device_status() for v in backends[:5])
