@@ -36,9 +36,6 @@ constexpr int kI8Ring = 192 * 1024;
 constexpr int kI8EpilogueWarps = 8;
 constexpr int kI8Threads = (2 + kI8EpilogueWarps) * 32;
 constexpr int kI8Smem = kI8Ring + 1024;
-// Rows of a token load at most: one load a stage, as for the weights. With 16 / 32 / 64 / 128 rows the large products took 892 / 826 / 859 / 700 us
-// (8 experts of 4096 rows, 4096 x 7168) and 962 / 818 / 812 / 757 (65536 rows of 32 of 7168 x 2048).
-constexpr int kI8Box = 128;
 constexpr int kI8MinSteps = 16;     // of a cut piece: with 8, 300 rows of 1000 x 2048 took 15.7 us in place of 11.9
 constexpr int kI8Band = 8;          // tiles whose weights are visited together (see I8Cursor)
 
@@ -59,7 +56,6 @@ struct I8Params {
     uint64_t timeout_ns;
     int n, k, experts, top_k, tiles, steps;
     int chunk;                // most tokens of a chunk, a multiple of 32
-    int box;                  // rows of a token load
     int stages, stage_bytes;
     // 1: i8_rows precedes. Everything before that is done when this kernel starts, for i8_rows' blocks have waited for it, but this kernel has not
     // itself: what it reads before its own wait (offsets; weights, by TMA) comes from L2, not from what an SM may still hold of an earlier run.
@@ -438,11 +434,12 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         I8Cursor cursor;
         plan.pieces([&](int item, int k0, int n, int, int) {
             const I8Item it = work.at(p, item, cursor);
-            // loads of this CTA's half of the tokens, and of both; what of a half no load covers goes into sums that nothing reads
-            const int half = it.width / 2, box_bytes = p.box * kI8StepK;
-            auto boxes = [&](int r) { return (min(half, max(0, it.count - r * half)) + p.box - 1) / p.box; };
-            const int mine = boxes(int(rank)), row = it.r0 + int(rank) * half;
-            const uint32_t bytes = 2u * kI8WeightBytes + uint32_t((boxes(0) + boxes(1)) * box_bytes);
+            // A CTA's half of the tokens is one load, of half a chunk's rows whatever the item has (16, 32 or 64 rows a load took 892, 826 and
+            // 859 us in place of 700: 8 experts of 4096 rows, 4096 x 7168); where no row of the half is there, none. What is loaded beyond the
+            // item's rows, or not at all, goes into sums that nothing reads.
+            const int half = it.width / 2, row = it.r0 + int(rank) * half;
+            const bool mine = it.count > int(rank) * half;
+            const uint32_t bytes = 2u * kI8WeightBytes + (it.count > half ? 2u : 1u) * uint32_t(p.stage_bytes - kI8WeightBytes);
             for (int j = 0; ok && j < n; ++j) {
                 ok = wait_all(empty(s), ph ^ 1u, ab, kStatusTimeout | kRoleProducer | uint32_t(s));
                 if (!ok)
@@ -459,8 +456,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                     ptx::fence_proxy_async_global();
                     waited = true;
                 }
-                for (int i = 0; i < mine; ++i)
-                    ptx::tma_load_2d_pair(a + kI8WeightBytes + uint32_t(i * box_bytes), &tmap_x, full_leader + 8u * s, c, row + i * p.box, issue);
+                if (mine)
+                    ptx::tma_load_2d_pair(a + kI8WeightBytes, &tmap_x, full_leader + 8u * s, c, row, issue);
                 if (++s == p.stages) {
                     s = 0;
                     ph ^= 1u;

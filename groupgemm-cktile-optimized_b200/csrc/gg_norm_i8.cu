@@ -302,14 +302,13 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     p.tiles = int(tiles);
     p.steps = int(steps);
     p.chunk = chunk;
-    p.box = std::min(kI8Box, chunk / 2);
     p.stage_bytes = kI8WeightBytes + chunk / 2 * kI8StepK;
     p.stages = std::min(kI8MaxStages, kI8Ring / p.stage_bytes);
     p.after_rows = order ? 1 : 0;
     if (q.rows > 0) {
         if (const int rc = encode_bytes_3d(h, h->moe.map[0], q.weight, q.k, q.n, q.experts, kI8StepK, kI8TileRows / 2, CU_TENSOR_MAP_SWIZZLE_128B))
             return rc;
-        if (const int rc = encode_bytes_2d(h, h->moe.map[1], p.xq, q.k, q.rows, kI8StepK, unsigned(p.box), CU_TENSOR_MAP_SWIZZLE_128B))
+        if (const int rc = encode_bytes_2d(h, h->moe.map[1], p.xq, q.k, q.rows, kI8StepK, unsigned(chunk / 2), CU_TENSOR_MAP_SWIZZLE_128B))
             return rc;
     }
     set_params(h, p);
