@@ -56,6 +56,7 @@ struct I8Params {
     uint64_t timeout_ns;
     int n, k, experts, top_k, tiles, steps;
     int chunk;                // most tokens of a chunk, a multiple of 32
+    int test_stall;           // test only: 1 = the first pair's first stage waits for an arrival that never comes
     int stages, stage_bytes;
     // 1: i8_rows precedes. Everything before that is done when this kernel starts, for i8_rows' blocks have waited for it, but this kernel has not
     // itself: what it reads before its own wait (offsets; weights, by TMA) comes from L2, not from what an SM may still hold of an earlier run.
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            ptx::mbar_init(full(s), 1);
+            ptx::mbar_init(full(s), p.test_stall && blockIdx.x == 0 && s == 0 ? 2 : 1);
             ptx::mbar_init(empty(s), 1);
         }
         for (int a = 0; a < 2; ++a) {

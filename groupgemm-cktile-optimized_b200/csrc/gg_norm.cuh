@@ -34,6 +34,7 @@ struct NormParams {
     int vecs;                   // 8 values each, of a row
     int warps, groups, slots;   // a group's warps, a block's groups, a ring's rows
     int params_at;              // the parameters' copy in shared memory, 0: none
+    int test_stall;             // test only: 1 = the first slot's barrier waits for an arrival that never comes
     float eps;
     uint64_t timeout_ns;
 };
@@ -50,6 +51,7 @@ struct NormGradParams {
     int vecs;
     int warps, groups, slots, params_at;
     int blocks;
+    int test_stall;
     uint64_t timeout_ns;
 };
 
@@ -407,7 +409,7 @@ __device__ __forceinline__ RowRing<kTensors> row_ring(const P &p, int tensors, u
     g.ab = Abort{p.status + 2, flag, p.timeout_ns};
     if (g.tid == 0)
         for (int s = 0; s < p.slots; ++s)
-            ptx::mbar_init(g.bars + 8u * s, 1);
+            ptx::mbar_init(g.bars + 8u * s, p.test_stall && blockIdx.x == 0 && g.group == 0 && s == 0 ? 2 : 1);
     if (threadIdx.x == 0)
         *flag = 0u;
     ptx::fence_mbar_init();

@@ -130,6 +130,7 @@ int prepare_norm(gg_handle *h, const gg_norm_problem &q, gg_stream_t stream, cha
     p.params_at = s.params_at;
     p.eps = q.eps;
     p.timeout_ns = uint64_t(h->opt_timeout_ms) * 1000000u;
+    p.test_stall = h->opt_test_stall;
     set_params(h, p);
     const void *fn = norm_fn(s, q.dtype, q.param_type, false);
     GG_CUDA(h, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem));
@@ -174,6 +175,7 @@ int prepare_norm_grad(gg_handle *h, const gg_norm_grad_problem &q, gg_stream_t s
     p.params_at = s.params_at;
     p.blocks = int(s.blocks);
     p.timeout_ns = uint64_t(h->opt_timeout_ms) * 1000000u;
+    p.test_stall = h->opt_test_stall;
     set_params(h, p);
     const void *fn = norm_fn(s, q.dtype, q.param_type, true);
     GG_CUDA(h, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormSmem));
@@ -295,6 +297,7 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     p.rows = q.rows;
     p.slots = q.src ? q.tokens * q.top_k : 0;
     p.timeout_ns = uint64_t(h->opt_timeout_ms) * 1000000u;
+    p.test_stall = h->opt_test_stall;
     p.n = int(q.n);
     p.k = int(q.k);
     p.experts = q.experts;

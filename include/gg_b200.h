@@ -451,8 +451,9 @@ int gg_device_status(gg_handle *h, gg_stream_t stream, uint32_t *status);
  *                row's stores out of bounds, skips them and reports 0x2002 in the status word (the
  *                release build has no checks and stores every row); used to test the checks
  *   "test_stall" test only: 1 = the kernel never loads the first stage of its first CTA (pair),
- *                so that wait runs out after timeout_ms and gg_device_status() reports it;
- *                used to test failure detection without faulting the GPU
+ *                so that wait runs out after timeout_ms and gg_device_status() reports it (the norm, its
+ *                gradients and the 8-bit products: that stage's barrier waits for an arrival that never
+ *                comes); used to test failure detection without faulting the GPU
  * Returns GG_OK or GG_ERR_ARG for an unknown key. The knobs are the analogue of the compile-time
  * CkTileConfig (ck_kernel/ck_grouped_gemm_config.hpp:26-86) that the reference edits to tune. */
 int gg_set_option(gg_handle *h, const char *key, int64_t value);
