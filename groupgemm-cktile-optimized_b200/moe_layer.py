@@ -117,7 +117,11 @@ def quantize_i8(w: torch.Tensor):
 
 class Norm:
     """The layer norm in front of a layer, forward and backward, with weight and bias `gamma` and `beta` [hidden] (None: 1 and 0), in the
-    tokens' type or fp32. The tensors of a step may have any strides: what is not contiguous is copied first. check() as TrainingLayer's."""
+    tokens' type or fp32. The tensors of a step may have any strides: what is not contiguous is copied first. check() as TrainingLayer's.
+
+    Backward reads the forward's sum (x itself without a residual, if it is contiguous) and gamma again: one that was changed in place since then
+    is refused. Each call prepares its handle for the tensors that it is given, and so waits for the current stream; it cannot be captured in a CUDA
+    graph (gg_prepare_norm and gg_prepare_norm_grad with buffers that stay can: only their preparation waits)."""
 
     def __init__(self, gamma: torch.Tensor | None, beta: torch.Tensor | None, eps: float = 1e-5):
         types = set()
@@ -131,7 +135,7 @@ class Norm:
         self.gg = load_package()
         self.gamma, self.beta, self.eps, self.params = gamma, beta, eps, next(iter(types), None)
         self.backends = {name: self.gg.make_b200_backend() for name in ("norm", "norm_grad")}
-        self.sum = None
+        self.sum = self.versions = None
 
     def check(self) -> None:
         """Waits for the current stream and raises if a kernel of the last forward or backward reported an error."""
@@ -144,6 +148,10 @@ class Norm:
         b, s = self.backends[name], _stream()
         _ready(getattr(b, prepare)(*args, stream=s, **kw))
         b.run(s)
+
+    def _versions(self) -> tuple:
+        """Torch's counts of the changes in place of what backward reads again (tensors of inference mode have none)."""
+        return tuple(None if v is None or v.is_inference() else v._version for v in (self.sum, self.gamma))
 
     def _types(self, x: torch.Tensor) -> tuple[int, int]:
         t = _dtype(self.gg, x.dtype)
@@ -160,7 +168,7 @@ class Norm:
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         """x [tokens, hidden] -> (y, x + residual): y is the norm of the second, which goes past the layer (x itself without a residual)."""
-        self.sum = None  # until this forward has run
+        self.sum = self.versions = None  # until this forward has run
         t, h = self._hidden(x)
         x = _check("x", x, (t, h), *LOGITS).contiguous()
         dt, pt = self._types(x)
@@ -174,6 +182,7 @@ class Norm:
                   residual_ptr=_ptr(residual), sum_ptr=_ptr(total) if residual is not None else 0, mean_ptr=_ptr(self.mean),
                   rstd_ptr=_ptr(self.rstd), eps=self.eps)
         self.sum = total
+        self.versions = self._versions()
         return y, total
 
     def backward(self, dy: torch.Tensor, dsum: torch.Tensor | None = None):
@@ -181,6 +190,8 @@ class Norm:
         residual's gradient, too; dgamma and dbeta [hidden] are fp32."""
         if self.sum is None:
             raise ValueError("backward needs a forward before it")
+        if self.versions not in (None, self._versions()):
+            raise ValueError("the forward's sum (its x without a residual) or gamma was changed in place before backward")
         x = self.sum
         t, h = x.shape
         dy = _check("dy", dy, (t, h), x.dtype).contiguous()
