@@ -15,8 +15,8 @@
 //   Warps: 0 loads (weights and tokens, a ring of stages), 1 issues the products (of the pair's first CTA), 2-9 take the sums out of
 //   Tensor Memory, two accumulators in turn.
 // What bounds it: few rows, the weights' bytes (64 experts of 4096 x 7168, 16 rows each on average: 271 us alone, 6.9 TB/s; one token through 8 of
-// them 43 us with the rows before, of which 36 are bytes); many, the tensor pipe (8 experts of 4096 rows: 557 us, 3.45 POPS, 93% of its cycles) and, where
-// calls follow one another, the power cap.
+// them 42 us with the rows before, of which 36 are bytes); many, the tensor pipe (8 experts of 4096 rows: 557-573 us, 3.4 POPS, 93-95% of its cycles) and,
+// where calls follow one another, the power cap.
 #pragma once
 
 #include "gg_moe.cuh"
@@ -36,7 +36,9 @@ constexpr int kI8Ring = 192 * 1024;
 constexpr int kI8EpilogueWarps = 8;
 constexpr int kI8Threads = (2 + kI8EpilogueWarps) * 32;
 constexpr int kI8Smem = kI8Ring + 1024;
-constexpr int kI8MinSteps = 16;     // of a cut piece: with 8, 300 rows of 1000 x 2048 took 15.7 us in place of 11.9
+// Of a cut piece, at least. It counts where cut items have fewer steps than 16 for each pair; us with 4 / 8 / 16 / 32 for 20 rows of one expert of
+// 2048 x 4096 13.1 / 12.1 / 13.0 / 13.9, 1000 x 8192 15.5 / 13.5 / 13.8 / 16.1, 512 x 7168 14.1 / 12.7 / 14.0 / 17.0, 1024 x 16384 19.1 / 16.8 / 15.3 / 17.0.
+constexpr int kI8MinSteps = 16;
 constexpr int kI8Band = 8;          // tiles whose weights are visited together (see I8Cursor)
 
 struct I8Params {
@@ -77,8 +79,8 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t adesc, ui
 // Whether the items that do not fill a last round of the pairs are cut along k. What it saves: of wide chunks, which the products bind, the part
 // of a round that pairs would be idle; of narrow ones, which memory binds, the part below about half, since fewer pairs at work load faster. What
 // it costs, in steps, grows with the sums that leave and come back. Us cut / whole, one token through e of 4096 x 7168 (16 e items for 74 pairs):
-// e = 5 31 / 39, 6 35 / 40, 7 39 / 40, 8 44 / 41, 9 48 / 45, 10 51 / 59, 12 59 / 60, 14 68 / 76; 256 c rows of 4096 x 4096 (16 c items): c = 5 35 / 33, 8
-// 43 / 36, 10 44 / 46, 14 56 / 58, 18 69 / 64, 20 74 / 75; of 4096 x 1024 5 26 / 17, 10 30 / 21, 20 38 / 30.
+// e = 5 32 / 37, 6 36 / 38, 7 40 / 39, 8 44 / 42, 9 49 / 45, 10 51 / 56, 12 60 / 58, 14 69 / 74; 256 c rows of 4096 x 4096 (16 c items): c = 5 35 / 32, 8
+// 43 / 36, 10 44 / 45, 14 56 / 57, 18 69 / 65, 20 75 / 74; of 4096 x 1024 5 25 / 16, 10 29 / 19, 20 38 / 29.
 __host__ __device__ __forceinline__ bool i8_cuts(int over, int pairs, int steps, int chunk) {
     if (over == 0)
         return false;

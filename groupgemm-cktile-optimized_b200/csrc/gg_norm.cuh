@@ -5,8 +5,9 @@
 // What bounds them: each row is read once and written once. One block an SM stays for the whole launch; its warps form
 // groups that take a row each, one to four vectors of 8 values a thread. Rows come through a ring in shared memory, bulk copies a few rows
 // ahead, so that the sums' latency (shuffles and a barrier a row) passes while the next rows are on their way, and a thread's weight, bias
-// and sums of gradients stay in registers from row to row. Measured, bf16, with a residual (or its gradient): 16384 x 7168 norm_rows 148-151 us
-// (6.3 TB/s, 96% of the measured copy rate), norm_grad_rows 160-170 (5.5-5.9 TB/s); 16384 x 4096 85 and 89; 2048 x 4096 fp32 gradients 23.
+// and sums of gradients stay in registers from row to row. Measured, bf16, with a residual (or its gradient): 16384 x 7168 norm_rows 145-151 us
+// (6.2-6.5 TB/s, 95-99% of the measured copy rate), the gradients 161-175 (5.4-5.8 TB/s); 16384 x 4096 85 and 88; fp32 8192 x 4096 90 (forward),
+// 2048 x 4096 28 (gradients, of which norm_grad_rows 24).
 #pragma once
 
 #include "gg_moe.cuh"
@@ -16,7 +17,7 @@ namespace moe {
 
 constexpr int kNormMaxHidden = 16384;
 constexpr int kNormThreads = 512;      // of a block at most
-constexpr int kNormFullThreads = 768;  // of norm_rows' check-free form, which fits 80 registers (fp32 spills 4 bytes; the others 80 to 180)
+constexpr int kNormFullThreads = 768;  // of norm_rows' check-free form, which fits 80 registers (fp32 spills 8 bytes; the others 80 to 180)
 constexpr int kNormSmem = 212 * 1024;  // of a block's ring and copies at most
 constexpr int kNormMaxSlots = 8;       // rows that a group's ring holds
 constexpr int kNormMaxGroups = 14;     // each has a named barrier beside the block's own
@@ -324,7 +325,7 @@ template <class T> __device__ __forceinline__ void quant_row(const void *row, in
     });
 }
 
-// A block a row (and every gridDim.x-th after it). 32768 rows of 7168, bf16: 116 us (6.1 TB/s).
+// A block a row (and every gridDim.x-th after it). 32768 rows of 7168, bf16: 116-124 us (5.7-6.1 TB/s).
 template <class T> __global__ void __launch_bounds__(512) quant_rows(const __grid_constant__ QuantParams p) {
     __shared__ uint32_t part[2][16];
     ptx::griddep_wait();
@@ -490,7 +491,7 @@ __device__ __forceinline__ float minus_mean_of(float mean, float rstd) { return 
 // kFull: every thread has V vectors, so that none asks for each (only with four: with two it saved the forward pass instructions but took
 // 157 us in place of 145 for 16384 x 7168 with a residual, its reads and writes closer together).
 // Forward it takes more groups of warps at once (kNormFullThreads): with 8-bit rows, whose way is long and has two barriers, 16384 rows of 7168
-// take 123 us with three groups of seven warps (136 with two), of 12288 191 with two of twelve (240 with one), of 4096 67 (71). Where the groups
+// take 123-125 us with three groups of seven warps (136 with two), of 12288 191 with two of twelve (240 with one), of 4096 68 (71). Where the groups
 // stay as many, the fewer registers cost up to 4% (16384 columns 290 against 280). Four groups in 72 registers won nothing at 7168 and lost 5% at
 // 5120 and 8192.
 // Mean and variance without cancellation: each warp its own mean m_w and the squares S_w around it, joined around the first warp's mean, t_w = m_w - m_0:

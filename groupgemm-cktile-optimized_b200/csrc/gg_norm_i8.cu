@@ -262,8 +262,10 @@ int prepare_i8(gg_handle *h, const gg_i8_problem &q, gg_stream_t stream, char *w
     // Tokens of a chunk at most: a stage has place for half of them beside its 16 KB of weights, so that small chunks keep more weights on
     // their way, but an expert with more rows than that has its weights loaded again. And chunks small enough that there are about as many
     // items as pairs, before any are cut along k. `once`: weights leave L2 first. Us with chunks of 64 / 128 / 256, and in brackets once, of
-    // 32 experts of 4096 x 4096 by their mean rows: 8 90 (86) / 90 (86) / 93 (88); 32 95 (91) / 94 (91) / 97 (93); 48 104 (103) / 101 (98) / 101 (98);
-    // 64 116 / 102 (101) / 103 (101); 96 154 / 111 (112) / 115 (110); 128 189 / 138 / 119 (119); 256 336 / 228 / 170 (174).
+    // 32 experts of 4096 x 4096 by their mean rows: 8 87 (83) / 87 (83) / 87 (84); 32 91 (86) / 91 (88) / 94 (90); 48 100 (97) / 97 (94) / 97 (93);
+    // 64 100 (99) / 96 (93) / 99 (95); 96 119 (121) / 102 (103) / 103 (101); 128 142 (149) / 116 (118) / 111 (111); 256 234 (241) / 173 (177) / 147 (151).
+    // All for even loads: the host does not see the counts, so rows that all go to few of many experts take the chunks of their mean (1024 rows of
+    // one of 64 experts of 4096 x 7168 56 us, with chunks of 256 32; 900 of one and 2 of each other 316 and 309).
     const int64_t mean = q.rows / q.experts;
     int chunk = mean <= 32 ? 64 : mean <= 64 ? 128 : kI8MaxTokens;
     while (chunk > 32 && (q.rows + chunk / 2 - 1) / (chunk / 2) * tiles <= pairs)
