@@ -152,13 +152,13 @@ struct W4Work {
     int64_t total, begin, end;  // steps: of the launch, this CTA's range
     int ctas;
 
-    // offsets come from the device: each is held to the range that the rows allow. Returns whether they fall anywhere; then no expert gets
+    // offsets come from the device, and from L2, since all but w4_gather read them before their own wait: each is held to the range that the rows allow. Returns whether they fall anywhere; then no expert gets
     // rows: what is sized by the rows (items, workspace, 32-bit indices) holds for rising offsets. By all threads of the block, which are
     // together after it. (Setting start to 0 here in place of a flag cost one token's products 0.6 us of 36.)
     static __device__ __forceinline__ bool starts(const W4Params &p, int *start) {
         bool falls = false;
         for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) {
-            const int64_t v = p.offsets[e], before = e ? p.offsets[e - 1] : 0;
+            const int64_t v = __ldcg(p.offsets + e), before = e ? __ldcg(p.offsets + e - 1) : 0;
             falls |= v < before;
             if (v < before || v > p.rows)
                 report(p.status, kSiteOffsets);

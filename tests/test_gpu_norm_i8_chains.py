@@ -66,6 +66,31 @@ def test_serving_steps_whose_routing_changes(layer, tokens, top_k, k, norm):
     assert fast.products.device_status() == 0 and plain.products.device_status() == 0
 
 
+@pytest.mark.parametrize("tokens,top_k,k", [(1, 8, 1024), (40, 4, 512), (300, 4, 512)])
+def test_4_bit_serving_steps_whose_routing_changes(layer, tokens, top_k, k):
+    """The same over 4-bit experts, for few rows an expert and for many."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(tokens + k)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    e, n = 64, 520
+    q, scales, zeros = layer.quantize_w4((rand(e, n, k) / k ** 0.5).bfloat16(), 64)
+    fast, plain = (layer.ServingLayer(q, scales, zeros, 64, tokens, top_k) for _ in range(2))
+    for b in (plain.router.backend, plain.products, plain.combine):
+        b.set_option("pdl", 0)
+    fast.mask.fill_(1)
+    plain.mask.fill_(1)
+    graph = captured(torch, fast.run, 3)
+    for i in range(40):
+        for a, b, v in ((fast.x, plain.x, rand(tokens, k).bfloat16()), (fast.logits, plain.logits, rand(tokens, e))):
+            a.copy_(v)
+            b.copy_(v)
+        graph.replay()
+        plain.run()
+        assert torch.equal(fast.router.offsets, plain.router.offsets)
+        assert torch.equal(fast.y.view(torch.int16), plain.y.view(torch.int16)), i
+    assert fast.products.device_status() == 0 and plain.products.device_status() == 0
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_each_operator_behind_the_one_that_writes_its_input(gg, kind):
     """Norm -> its gradients -> rounding -> 8-bit products, and norm -> 4-bit products, in one graph, with contents that change."""
