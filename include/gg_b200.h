@@ -111,13 +111,14 @@ int gg_prepare_grad(gg_handle *h, const gg_grad_problem *p, int32_t op, gg_strea
 
 /* ---- The layer around the grouped GEMM ----
  *
- * Router, token movement and 4-bit products of the same mixture-of-experts layer. The reference
+ * Router, token movement, norm, and 4- and 8-bit products of the same mixture-of-experts layer. The reference
  * benchmarks the grouped GEMM alone, on rows that are in expert order already; these calls produce
  * that order, take the rows there and back, and serve few tokens from small weights. Each prepare
  * call below is used as gg_prepare: it validates (GG_NOT_SUPPORTED with a reason in `why`), allocates
  * what the handle needs and waits for `stream`; then gg_run() enqueues the operator on any stream
- * without waiting and allocates nothing (it can be captured in a CUDA graph). A handle holds one
- * prepared operator at a time and its launches must not overlap on the GPU. Operands are device
+ * without waiting and allocates nothing (it can be captured in a CUDA graph; what was captured is good
+ * until the handle is prepared again or released, either of which may free memory that it uses). A
+ * handle holds one prepared operator at a time and its launches must not overlap on the GPU. Operands are device
  * pointers to contiguous arrays that the caller owns; the contents may change between runs.
  *
  * Indices that come from device memory (dest, src, ids, offsets) are checked by the kernels: one
