@@ -120,7 +120,7 @@ class Norm:
     tokens' type or fp32. The tensors of a step may have any strides: what is not contiguous is copied first. check() as TrainingLayer's.
 
     Backward reads the forward's sum (x itself without a residual, if it is contiguous) and gamma again: one that was changed in place since then
-    is refused. Each call prepares its handle for the tensors that it is given, and so waits for the current stream; it cannot be captured in a CUDA
+    is refused (unless it is a part of a larger tensor, where torch does not tell). Each call prepares its handle for the tensors that it is given, and so waits for the current stream; it cannot be captured in a CUDA
     graph (gg_prepare_norm and gg_prepare_norm_grad with buffers that stay can: only their preparation waits)."""
 
     def __init__(self, gamma: torch.Tensor | None, beta: torch.Tensor | None, eps: float = 1e-5):
@@ -150,8 +150,14 @@ class Norm:
         b.run(s)
 
     def _versions(self) -> tuple:
-        """Torch's counts of the changes in place of what backward reads again (tensors of inference mode have none)."""
-        return tuple(None if v is None or v.is_inference() else v._version for v in (self.sum, self.gamma))
+        """Torch's counts of the changes in place of what backward reads again. A part of a larger tensor is left out, since it is counted with
+        the others, and so are tensors of inference mode, which have no count."""
+        def count(v):
+            if v is None or v.is_inference() or v.untyped_storage().nbytes() != v.numel() * v.element_size():
+                return None
+            return v._version
+
+        return count(self.sum), count(self.gamma)
 
     def _types(self, x: torch.Tensor) -> tuple[int, int]:
         t = _dtype(self.gg, x.dtype)

@@ -65,3 +65,18 @@ def test_changes_of_what_backward_does_not_read(layer):
         y, past = norm.forward(x)
         norm.backward(dy)
     norm.check()
+
+
+def test_changes_beside_a_part_of_a_larger_tensor(layer):
+    """One buffer for the activations of many layers, whose changes torch counts together, and a parameter of a flat one."""
+    import torch
+
+    acts, params = torch.randn(3, 40, 64, device="cuda").bfloat16(), torch.randn(4, 64, device="cuda")
+    dy = torch.randn(40, 64, device="cuda").bfloat16()
+    for x, gamma in ((acts[0], params[1]), (acts[0].detach(), params[1].detach())):
+        norm = layer.Norm(gamma, None)
+        norm.forward(x)
+        want = norm.backward(dy)
+        acts[1].mul_(2)
+        params[2].mul_(2)
+        assert all(torch.equal(a, b) for a, b in zip(norm.backward(dy), want))
